@@ -376,6 +376,63 @@ int sl8_kv_write_paged_rotated(const void* k_new, const void* v_new, const int32
                                int64_t block_size, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Rotary positions of Q and K, one launch. No counterpart in the reference (its callers rotate).
+ *   q [B,Hq,S,D], k [B,Hkv,S,D] (f16 / bf16 / f32; either may have no heads) in any strides of
+ *   b, h, s (elements; the last dimension dense) -> q_out, k_out contiguous, not q or k themselves.
+ *   Pair p of the first R elements, (p, p + R/2) or, interleaved, (2p, 2p+1), turns by the angle of
+ *   table [table_rows][R] fp32 (16-byte aligned; cos of R/2 pairs, then sin) at its axis' position:
+ *     x_i' = x_i cos - x_j sin, x_j' = x_j cos + x_i sin (inverse: -sin, the gradient), in fp32.
+ *   positions int32 or int64 [axes][B][S]: axis a of token (b, s) is at a * pos_axis + b * pos_b + s
+ *   (pos_b 0: shared by the batch); outside the table: its nearest end. sections int32[axes] (host):
+ *   how many consecutive pairs each axis turns (axes = 1: ignored). D even, at most 512; R even.
+ * ---------------------------------------------------------------------- */
+int sl8_rope(const void* q, const void* k, int dtype, const int64_t* q_strides,
+             const int64_t* k_strides, const void* positions, int positions_i64, int64_t pos_axis,
+             int64_t pos_b, const float* table, int64_t table_rows, const int32_t* sections, int axes,
+             int interleaved, int inverse, void* q_out, void* k_out, int64_t B, int64_t Hq,
+             int64_t Hkv, int64_t S, int64_t D, int64_t R, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Block-scaled paged int8 KV cache: codes int8 [num_blocks, Hkv, block_size, D] with one fp32
+ * scale per block and head [num_blocks, Hkv], for K and for V; D 64 / 128 / 256, block_size a
+ * multiple of 16 up to 128. New tokens are rows of one list [T, H, D]: sequence b's are rows
+ * cu_lens[b] .. cu_lens[b+1] - 1 (cu_lens int32 [B+1] on the device, not falling, from 0; NULL:
+ * row b, T = B) and the last of its context_lens[b] tokens; block_table int32
+ * [B, max_blocks_per_seq] as in the paged cache above. Block ids outside the pool are skipped.
+ * No counterpart in the reference, whose paged cache has a scale per token.
+ *
+ * sl8_kv_append_block8: k_new, v_new [T,Hkv,D] and (Hq > 0) q [T,Hq,D], f16 or bf16, strides of
+ *   token and head (elements, multiples of 8; rows 16-byte aligned). K, and Q into q_out
+ *   [T,Hq,D], are turned as sl8_rope does (positions [axes][T]; NULL: not at all, then no Q; R a
+ *   multiple of 16); rotate != 0: K's rows then pass through the normalised Hadamard matrix. In fp32,
+ *   a block and head with new rows gets scale' = max(scale of the rows it keeps, amax|new| *
+ *   fp32(1/127), 2^-60), its new rows codes rint(x / scale'), kept codes c become rint(c * (scale /
+ *   scale')). Rows past a sequence's last token are left as they were. A block is written by one
+ *   sequence of a call. Values must be finite.
+ * ---------------------------------------------------------------------- */
+int sl8_kv_append_block8(const void* k_new, const void* v_new, const void* q, int dtype,
+                         const int64_t* k_strides, const int64_t* v_strides, const int64_t* q_strides,
+                         const void* positions, int positions_i64, const float* table,
+                         int64_t table_rows, const int32_t* sections, int axes, int interleaved,
+                         int rotate, const int32_t* cu_lens, const int32_t* context_lens,
+                         const int32_t* block_table, int8_t* k_cache, float* k_scale, int8_t* v_cache,
+                         float* v_scale, void* q_out, int64_t T, int64_t B, int64_t Hq, int64_t Hkv,
+                         int64_t D, int64_t R, int64_t num_blocks, int64_t block_size,
+                         int64_t max_blocks_per_seq, void* stream);
+
+/* Attention of the new tokens (already in the cache) over that cache: q [T,Hq,D] f16 or bf16
+ * (rotate != 0: times the normalised Hadamard matrix first, as the keys), each row quantised to int8
+ * with one scale times q_scale_mul (softmax_scale * log2 e) -> out [T,Hq,D] of q's type. Row i of a
+ * sequence's n sees keys <= context_lens - n + i, and with window_left >= 0 keys > that -
+ * window_left; zeros where it sees none and in rows behind the last sequence. All 16-byte aligned. */
+int sl8_attn_paged_block8(const void* q, int dtype, int rotate, float q_scale_mul,
+                          const int8_t* k_cache, const float* k_scale, const int8_t* v_cache,
+                          const float* v_scale, const int32_t* cu_lens, const int32_t* context_lens,
+                          const int32_t* block_table, void* out, int64_t T, int64_t B, int64_t Hq,
+                          int64_t Hkv, int64_t D, int64_t num_blocks, int64_t block_size,
+                          int64_t max_blocks_per_seq, int64_t window_left, void* stream);
+
+/* ------------------------------------------------------------------------
  * Q4_K GEMM/GEMV over native GGUF super-blocks (144 B per 256 weights:
  * fp16 d, fp16 dmin, 12 B packed 6-bit sub-scales/mins, 128 B nibbles).
  *   y[m,n] = x_scale[m] * sum_j (d*sc_j*<x_j,q_j> - dmin*m_j*sum(x_j))

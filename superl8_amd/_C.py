@@ -12,6 +12,7 @@ reference's "must be CUDA tensors" checks.
 """
 from __future__ import annotations
 
+import ctypes
 import math
 
 import torch
@@ -767,6 +768,205 @@ def kv_write_paged(k_new, v_new, slot_mapping, k_cache, k_scale, v_cache, v_scal
         call("sl8_kv_write_paged_rotated" if rotate else "sl8_kv_write_paged", k_new.data_ptr(),
              v_new.data_ptr(), slot_mapping.data_ptr(), k_cache.data_ptr(), k_scale.data_ptr(),
              v_cache.data_ptr(), v_scale.data_ptr(), B, Hkv, D, k_cache.shape[0], k_cache.shape[2], stream_of(k_new))
+
+
+# ---------------------------------------------------------------------------
+# rotary positions and the block-scaled paged int8 cache (no counterpart in the reference)
+# ---------------------------------------------------------------------------
+_HEAD_DIMS_BLOCK8 = (64, 128, 256)
+_BLOCK8_MAX = 128
+
+
+def _rope_checks(tag, positions, table, sections, want, D):
+    """The checks on the positions, the table and the sections of a rotation: positions of one of
+    the shapes `want` (an axis for each section in front). Returns (axes, sections as int32[axes],
+    positions, table)."""
+    if positions.dtype not in (torch.int32, torch.int64):
+        _fail(f"{tag}: positions must be int32 or int64")
+    if table.dtype != torch.float32 or table.dim() != 2 or table.shape[0] < 1:
+        _fail(f"{tag}: table must be float32 [positions, rotary dim]")
+    R = table.shape[1]
+    if R < 2 or R % 2 or R > D:
+        _fail(f"{tag}: rotary dim must be even and at most the head dim, got {R}")
+    axes, cs = 1, None
+    shape = tuple(positions.shape)
+    if sections is not None:
+        axes = len(sections)
+        if not 1 <= axes <= 4 or any(int(n) < 1 for n in sections) or sum(sections) != R // 2:
+            _fail(f"{tag}: sections must be 1 to 4 positive counts of pairs that add up to {R // 2}, "
+                  f"got {list(sections)}")
+        cs = (ctypes.c_int32 * axes)(*(int(n) for n in sections))
+        shape = shape[1:] if shape[:1] == (axes,) else None
+    if shape not in want:
+        _fail(f"{tag}: positions must be {' or '.join(str(list(w)) for w in want)}"
+              f"{f' behind an axis of {axes}' if sections is not None else ''}, got "
+              f"{list(positions.shape)}")
+    table = table.contiguous()
+    if table.data_ptr() % 16:
+        table = table.clone()
+    return axes, cs, positions.contiguous(), table
+
+
+def _strides(t, *dims):
+    """Strides of t's dimensions as the entry points take them (a dimension of one has none)."""
+    return (ctypes.c_int64 * len(dims))(*(t.stride(d) if t.shape[d] != 1 else 0 for d in dims))
+
+
+def rope(q, k, positions, table, sections=None, interleaved=False, inverse=False):
+    """Rotary positions of q [B,Hq,S,D] and k [B,Hkv,S,D] (or None), fp16/bf16/fp32, any strides:
+    (q', k') contiguous. positions int32/int64 [S] or [B,S], with sections [A,S] or [A,B,S];
+    table fp32 [P,R]: cos of R/2 pairs, then sin."""
+    _on_gpu(q, positions, table)
+    _check(q.dtype in (torch.float16, torch.bfloat16, torch.float32),
+           "rope: q/k must be float16/bfloat16/float32")
+    _check(q.dim() == 4, "rope: expect q[B,Hq,S,D]")
+    B, Hq, S, D = q.shape
+    if D < 2 or D % 2 or D > 512:
+        _fail(f"rope: head dim must be even, 2..512, got {D}")
+    if k is not None:
+        _on_gpu(q, k)
+        _check(k.dtype == q.dtype, "rope: q and k must have one dtype")
+        _check(k.dim() == 4 and k.shape[0] == B and k.shape[2] == S and k.shape[3] == D,
+               "rope: expect k[B,Hkv,S,D] like q")
+    axes, cs, positions, table = _rope_checks("rope", positions, table, sections, ((S,), (B, S)), D)
+    per_batch = positions.dim() - (sections is not None) == 2
+    q = q if q.stride(-1) == 1 else q.contiguous()
+    q_out = q.new_empty((B, Hq, S, D))
+    Hkv, k_out, k_ptr, ks = 0, None, None, None
+    if k is not None:
+        k = k if k.stride(-1) == 1 else k.contiguous()
+        Hkv, k_out = k.shape[1], k.new_empty(k.shape)
+        k_ptr, ks = k.data_ptr(), _strides(k, 0, 1, 2)
+    if B and S and Hq + Hkv:
+        with on_device(q):
+            call("sl8_rope", q.data_ptr(), k_ptr, dtype_code(q.dtype), _strides(q, 0, 1, 2), ks,
+                 positions.data_ptr(), int(positions.dtype == torch.int64), positions.numel() // axes,
+                 S if per_batch else 0, table.data_ptr(), table.shape[0], cs, axes,
+                 int(bool(interleaved)), int(bool(inverse)), q_out.data_ptr(), _lib.ptr(k_out), B, Hq,
+                 Hkv, S, D, table.shape[1], stream_of(q))
+    return q_out, k_out
+
+
+def _block8_checks(tag, k_cache, k_scale, v_cache, v_scale, block_table, context_lens, cu_lens, T, Hkv,
+                   D):
+    """The checks on a block-scaled paged cache and its sequences; (B, num_blocks, block_size,
+    max_blocks_per_seq)."""
+    if k_cache.dtype != torch.int8 or v_cache.dtype != torch.int8:
+        _fail(f"{tag}: k_cache/v_cache must be int8")
+    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+        _fail(f"{tag}: scales must be float32")
+    if k_cache.dim() != 4 or k_cache.shape[1] != Hkv or k_cache.shape[3] != D:
+        _fail(f"{tag}: k_cache must be [num_blocks,H_kv,block_size,D]")
+    if v_cache.shape != k_cache.shape:
+        _fail(f"{tag}: v_cache shape must match k_cache")
+    nblk, _, bs, _ = k_cache.shape
+    if tuple(k_scale.shape) != (nblk, Hkv) or tuple(v_scale.shape) != (nblk, Hkv):
+        _fail(f"{tag}: k_scale/v_scale must be [num_blocks,H_kv]")
+    _contig(k_cache, k_scale, v_cache, v_scale, block_table, context_lens)
+    if block_table.dtype != torch.int32 or context_lens.dtype != torch.int32:
+        _fail(f"{tag}: block_table/context_lens must be int32")
+    if context_lens.dim() != 1:
+        _fail(f"{tag}: context_lens must be [B]")
+    B = context_lens.shape[0]
+    if block_table.dim() != 2 or block_table.shape[0] != B:
+        _fail(f"{tag}: block_table must be [B, max_blocks_per_seq]")
+    if cu_lens is None:
+        if T != B:
+            _fail(f"{tag}: without cu_lens there is one row per sequence, got {T} for {B}")
+    else:
+        _contig(cu_lens)
+        if cu_lens.dtype != torch.int32 or tuple(cu_lens.shape) != (B + 1,):
+            _fail(f"{tag}: cu_lens must be int32 [B + 1]")
+    if D not in _HEAD_DIMS_BLOCK8:
+        _fail(f"{tag}: head dim must be {_dims_msg(_HEAD_DIMS_BLOCK8)}, got {D}")
+    if bs < 16 or bs > _BLOCK8_MAX or bs % 16:
+        _fail(f"{tag}: block_size must be a multiple of 16, 16..{_BLOCK8_MAX}, got {bs}")
+    return B, nblk, bs, block_table.shape[1]
+
+
+def _rows16(t):
+    """t [T, H, D], copied where its rows are not 16-byte aligned."""
+    if t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(
+            t.shape[d] == 1 or t.stride(d) % 8 == 0 for d in (0, 1)):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def kv_append_block8(k_new, v_new, k_cache, k_scale, v_cache, v_scale, block_table, context_lens,
+                     cu_lens=None, q=None, positions=None, table=None, sections=None,
+                     interleaved=False, rotate=False):
+    """Append of new tokens k_new, v_new [T,Hkv,D] (fp16/bf16) to a block-scaled paged int8 cache,
+    in place; K turned by position (positions not None) and then, with rotate, multiplied by the
+    Hadamard matrix. Returns the turned q [T,Hq,D], None without one."""
+    tag = "kv_append_block8"
+    _on_gpu(k_new, v_new, k_cache, k_scale, v_cache, v_scale, block_table, context_lens,
+            *(t for t in (cu_lens, q, positions, table) if t is not None))
+    dt = k_new.dtype
+    if dt not in (torch.float16, torch.bfloat16) or v_new.dtype != dt:
+        _fail(f"{tag}: k_new/v_new must both be float16 or bfloat16")
+    if k_new.dim() != 3 or v_new.shape != k_new.shape:
+        _fail(f"{tag}: k_new/v_new must be [T,H_kv,D]")
+    T, Hkv, D = k_new.shape
+    if Hkv < 1:
+        _fail(f"{tag}: k_new/v_new must be [T,H_kv,D]")
+    B, nblk, bs, maxb = _block8_checks(tag, k_cache, k_scale, v_cache, v_scale, block_table,
+                                       context_lens, cu_lens, T, Hkv, D)
+    axes, cs, rows, R, Hq = 1, None, 0, 0, 0
+    if (positions is None) != (table is None):
+        _fail(f"{tag}: positions and table come together")
+    if positions is not None:
+        axes, cs, positions, table = _rope_checks(tag, positions, table, sections, ((T,),), D)
+        rows, R = table.shape
+        if R % 16:
+            _fail(f"{tag}: rotary dim must be a multiple of 16, got {R}")
+    q_out = qs = None
+    if q is not None:
+        if positions is None:
+            _fail(f"{tag}: q needs positions")
+        if q.dtype != dt or q.dim() != 3 or q.shape[0] != T or q.shape[2] != D:
+            _fail(f"{tag}: q must be [T,H_q,D] of k_new's dtype")
+        q, Hq = _rows16(q), q.shape[1]
+        q_out, qs = q.new_empty((T, Hq, D)), _strides(q, 0, 1)
+    if T:
+        k_new, v_new = _rows16(k_new), _rows16(v_new)
+        with on_device(k_new):
+            call("sl8_kv_append_block8", k_new.data_ptr(), v_new.data_ptr(), _lib.ptr(q),
+                 dtype_code(dt), _strides(k_new, 0, 1), _strides(v_new, 0, 1), qs,
+                 _lib.ptr(positions), int(positions is not None and positions.dtype == torch.int64),
+                 _lib.ptr(table), rows, cs, axes, int(bool(interleaved)), int(bool(rotate)),
+                 _lib.ptr(cu_lens), context_lens.data_ptr(), block_table.data_ptr(),
+                 k_cache.data_ptr(), k_scale.data_ptr(), v_cache.data_ptr(), v_scale.data_ptr(),
+                 _lib.ptr(q_out), T, B, Hq, Hkv, D, R, nblk, bs, maxb, stream_of(k_new))
+    return q_out
+
+
+def attn_paged_block8(q, q_mul, rotate, k_cache, k_scale, v_cache, v_scale, block_table,
+                      context_lens, cu_lens=None, window_left=-1):
+    """Attention of the new tokens q [T,Hq,D] (fp16/bf16) over a block-scaled paged int8 cache that
+    holds them already -> [T,Hq,D] of q's dtype; q_mul is softmax_scale * log2(e)."""
+    tag = "attn_paged_block8"
+    _on_gpu(q, k_cache, k_scale, v_cache, v_scale, block_table, context_lens,
+            *(() if cu_lens is None else (cu_lens,)))
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        _fail(f"{tag}: q must be float16 or bfloat16")
+    if q.dim() != 3 or k_cache.dim() != 4:
+        _fail(f"{tag}: q must be [T,H_q,D], k_cache [num_blocks,H_kv,block_size,D]")
+    _contig(q)
+    T, Hq, D = q.shape
+    Hkv = k_cache.shape[1]
+    if Hkv < 1 or Hq % Hkv:
+        _fail(f"{tag}: H_q must be divisible by H_kv (GQA)")
+    B, nblk, bs, maxb = _block8_checks(tag, k_cache, k_scale, v_cache, v_scale, block_table,
+                                       context_lens, cu_lens, T, Hkv, D)
+    out = q.new_empty((T, Hq, D))
+    if T and Hq:
+        with on_device(q):
+            call("sl8_attn_paged_block8", q.data_ptr(), dtype_code(q.dtype), int(bool(rotate)),
+                 float(q_mul), k_cache.data_ptr(), k_scale.data_ptr(), v_cache.data_ptr(),
+                 v_scale.data_ptr(), _lib.ptr(cu_lens), context_lens.data_ptr(),
+                 block_table.data_ptr(), out.data_ptr(), T, B, Hq, Hkv, D, nblk, bs, maxb,
+                 int(window_left), stream_of(q))
+    return out
 
 
 # ---------------------------------------------------------------------------

@@ -75,6 +75,11 @@ SIGNATURES = {
     "sl8_kv_write_paged": (_I, [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P]),
     "sl8_kv_write_paged_rotated": (_I, [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64,
                                         _P]),
+    "sl8_rope": (_I, [_P, _P, _I, _P, _P, _P, _I, _I64, _I64, _P, _I64, _P, _I, _I, _I, _P, _P]
+                 + [_I64] * 6 + [_P]),
+    "sl8_kv_append_block8": (_I, [_P, _P, _P, _I, _P, _P, _P, _P, _I, _P, _I64, _P, _I, _I, _I]
+                             + [_P] * 8 + [_I64] * 9 + [_P]),
+    "sl8_attn_paged_block8": (_I, [_P, _I, _I, _F] + [_P] * 8 + [_I64] * 9 + [_P]),
     "sl8_gemm_decode_q4k": (_I, [_P, _P, _P, _P, _I, _I64, _I64, _I64, _P]),
     "sl8_gemm_decode_q4k_xblock": (_I, [_P, _P, _P, _P, _I, _I64, _I64, _I64, _P]),
     "sl8_gemm_q4k": (_I, [_P, _P, _P, _P, _I, _I64, _I64, _I64, _P]),

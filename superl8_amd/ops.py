@@ -306,6 +306,88 @@ def quantize_kv_write_paged_k8v3(k_new: torch.Tensor, v_new: torch.Tensor,
     return cb
 
 
+def rope_table(max_positions: int, rotary_dim: int, *, base: float = 10000.0, sections=None,
+               device="cuda") -> torch.Tensor:
+    """The table of `rope`: fp32 [max_positions, rotary_dim], cos of the rotary_dim / 2 pairs, then
+    sin, of position * base^(-pair / pairs), from 64 bits. With sections (pairs per axis) the
+    frequencies start again at each axis, as positions in images have it; leave them out for one
+    axis and for axes that share one row of frequencies (video)."""
+    if rotary_dim < 2 or rotary_dim % 2 or max_positions < 1:
+        raise ValueError(f"rope_table needs an even rotary dim and at least one position, got "
+                         f"{rotary_dim} and {max_positions}")
+    half = rotary_dim // 2
+    if sections is not None and (min(sections, default=0) < 1 or sum(sections) != half):
+        raise ValueError(f"sections must be positive and add up to {half}, got {list(sections)}")
+    f = torch.cat([torch.arange(n, dtype=torch.float64) / n for n in (sections or (half,))])
+    pos = torch.arange(max_positions, dtype=torch.float64, device=device)
+    angle = pos[:, None] * (float(base) ** -f).to(pos.device)
+    return torch.cat([angle.cos(), angle.sin()], 1).float()
+
+
+def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, table: torch.Tensor, *,
+         sections=None, interleaved: bool = False, inverse: bool = False):
+    """Rotary positions of q [B,Hq,S,D] and k [B,Hkv,S,D] (or None) in one launch, fp16/bf16/fp32:
+    contiguous (q', k'), ready for attn_int8_fwd. Views of a fused projection are read in place.
+
+    Pair p of the first R elements turns by the angle of table[position, p] (fp32 [P, R]: cos, then
+    sin; see rope_table); (p, p + R/2) is a pair, or (2p, 2p+1) with `interleaved`. positions
+    int32/int64 [S] or [B,S]; with `sections` (up to 4 counts of consecutive pairs, in order)
+    [A,S] or [A,B,S], an axis for each. Positions outside the table count as its nearest end.
+    `inverse` turns back: the gradient of q and k from that of q' and k'."""
+    return _C.rope(q, k, positions, table, sections, interleaved, inverse)
+
+
+def quantize_kv_append_block8(k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Tensor,
+                              k_scale: torch.Tensor, v_cache: torch.Tensor, v_scale: torch.Tensor,
+                              block_table: torch.Tensor, context_lens: torch.Tensor, *,
+                              cu_lens: torch.Tensor | None = None, q: torch.Tensor | None = None,
+                              positions: torch.Tensor | None = None,
+                              table: torch.Tensor | None = None, sections=None,
+                              interleaved: bool = False,
+                              rotate: bool = True) -> torch.Tensor | None:
+    """Append a step's new tokens to a paged int8 cache with one scale per block and head, in place,
+    K (and q) turned by position on the way; returns the turned q [T,Hq,D] (None without q).
+
+    k_new, v_new [T,Hkv,D] and q [T,Hq,D] fp16/bf16 (views of a fused projection are read in place);
+    k_cache, v_cache int8 [num_blocks,Hkv,block_size,D] (D 64/128/256, block_size a multiple of 16,
+    16..128); k_scale, v_scale fp32 [num_blocks,Hkv]. cu_lens int32 [B+1]: sequence b's new tokens
+    are rows cu_lens[b]..cu_lens[b+1]-1 (None: one each); context_lens int32 [B]: its length with
+    them; block_table int32 [B,max_blocks]. positions int32/int64 [T] (with `sections` [A,T]) and
+    table as in `rope` (rotary dim a multiple of 16); without them K is taken as turned already.
+    `rotate` as in quantize_kv_write_paged. A block that new tokens enter is requantised where its
+    scale grows; sequences of one call must not write into the same block. Values must be finite."""
+    if rotate:
+        hadamard_dim(k_new.shape[-1])
+    return _C.kv_append_block8(k_new, v_new, k_cache, k_scale, v_cache, v_scale,
+                               block_table.contiguous(), context_lens.contiguous(),
+                               None if cu_lens is None else cu_lens.contiguous(), q, positions,
+                               table, sections, interleaved, rotate)
+
+
+def attn_paged_block8(q: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.Tensor,
+                      v_cache: torch.Tensor, v_scale: torch.Tensor, block_table: torch.Tensor,
+                      context_lens: torch.Tensor, *, cu_lens: torch.Tensor | None = None,
+                      scale: float | None = None, rotate: bool = True,
+                      window_left: int = -1) -> torch.Tensor:
+    """Attention over a paged int8 cache with one scale per block and head, written by
+    quantize_kv_append_block8 (the same `rotate`): one to thousands of new tokens per sequence,
+    mixed in one call, nothing read on the host.
+
+    q [T,Hq,D] fp16/bf16 -> [T,Hq,D] of its dtype: sequence b's rows are cu_lens[b]..cu_lens[b+1]-1
+    (None: row b), the last of its context_lens[b] tokens, which the cache holds already. Each sees
+    the keys up to itself and, with window_left >= 0, only the last window_left of them; a row
+    that sees none and rows behind the last sequence are zeros."""
+    softmax_scale = (1.0 / (q.shape[-1] ** 0.5)) if scale is None else scale
+    q = q.contiguous()
+    if q.data_ptr() % 16:
+        q = q.clone()
+    from .quant import LOG2E
+
+    return _C.attn_paged_block8(q, softmax_scale * LOG2E, rotate, k_cache, k_scale, v_cache, v_scale,
+                                block_table.contiguous(), context_lens.contiguous(),
+                                None if cu_lens is None else cu_lens.contiguous(), window_left)
+
+
 def quantize_kv_cache_3bit(k: torch.Tensor, v: torch.Tensor, *, rotate: bool = True,
                            fit: bool = True, block_size: int = 128) -> dict:
     """3-bit Lloyd-Max storage codec of a whole K/V cache (reference ops.py:590-655):
