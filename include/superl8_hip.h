@@ -424,13 +424,16 @@ int sl8_kv_append_block8(const void* k_new, const void* v_new, const void* q, in
  * (rotate != 0: times the normalised Hadamard matrix first, as the keys), each row quantised to int8
  * with one scale times q_scale_mul (softmax_scale * log2 e) -> out [T,Hq,D] of q's type. Row i of a
  * sequence's n sees keys <= context_lens - n + i, and with window_left >= 0 keys > that -
- * window_left; zeros where it sees none and in rows behind the last sequence. All 16-byte aligned. */
+ * window_left; zeros where it sees none and in rows behind the last sequence. All 16-byte aligned.
+ * workspace: sl8_attn_paged_block8_workspace() bytes (current device), uninitialised. */
+size_t sl8_attn_paged_block8_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D);
 int sl8_attn_paged_block8(const void* q, int dtype, int rotate, float q_scale_mul,
                           const int8_t* k_cache, const float* k_scale, const int8_t* v_cache,
                           const float* v_scale, const int32_t* cu_lens, const int32_t* context_lens,
                           const int32_t* block_table, void* out, int64_t T, int64_t B, int64_t Hq,
                           int64_t Hkv, int64_t D, int64_t num_blocks, int64_t block_size,
-                          int64_t max_blocks_per_seq, int64_t window_left, void* stream);
+                          int64_t max_blocks_per_seq, int64_t window_left, void* workspace,
+                          size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------
  * Q4_K GEMM/GEMV over native GGUF super-blocks (144 B per 256 weights:

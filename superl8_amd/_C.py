@@ -961,11 +961,13 @@ def attn_paged_block8(q, q_mul, rotate, k_cache, k_scale, v_cache, v_scale, bloc
     out = q.new_empty((T, Hq, D))
     if T and Hq:
         with on_device(q):
+            ws_bytes = _lib.load().sl8_attn_paged_block8_workspace(T, B, Hq, Hkv, D)
+            ws = q.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
             call("sl8_attn_paged_block8", q.data_ptr(), dtype_code(q.dtype), int(bool(rotate)),
                  float(q_mul), k_cache.data_ptr(), k_scale.data_ptr(), v_cache.data_ptr(),
                  v_scale.data_ptr(), _lib.ptr(cu_lens), context_lens.data_ptr(),
                  block_table.data_ptr(), out.data_ptr(), T, B, Hq, Hkv, D, nblk, bs, maxb,
-                 int(window_left), stream_of(q))
+                 int(window_left), _lib.ptr(ws), ws_bytes, stream_of(q))
     return out
 
 

@@ -5,13 +5,33 @@
 // with a window j > p - window too. Its row (rotated by the Hadamard matrix as the keys were, in
 // 32 bits) is quantised to int8 with one scale qs; then
 //   s_j = qs * scale * log2(e) * ks[block(j)] * <q, k_j> (exact integers inside),
-//   out = sum_j 2^(s_j - m) vs[block(j)] v_j / sum_j 2^(s_j - m);
-// a row that sees nothing gives zeros.
+//   out = sum_j 2^s_j vs[block(j)] v_j / sum_j 2^s_j;
+// a row that sees nothing gives zeros. The scale of V goes into the exponent: with
+//   t_j = s_j + log2 vs, m = max t_j, w_j = 2^(t_j - m):  out = sum w_j v_j / sum w_j / vs,
+// so that the weights that meet the codes v_j in 16 bits are at most 1 whatever the scales, the
+// largest contribution has full precision, and a block's scale costs one fma that the product s_j
+// needs anyway. (Least scale 2^-60: the sum of w / vs stays within 32 bits.)
+//
+// Rows of a sequence and KV head are (token, query head of the group), G = Hq / Hkv to a token; a
+// unit is ROWS of them that share every byte of K and V.
+#include <climits>
+
+#include "attn_common.hpp"
 #include "block8.hpp"
 #include "rowquant.hpp"
 
 namespace sl8 {
 namespace {
+
+constexpr int A8_THREADS = 256, A8_WAVES = 4;
+constexpr int A8_TILE = 64;       // keys: what splits and units' first keys are multiples of
+constexpr int A8_MIN_TILES = 4;   // least keys of a split: a tile for each wave
+constexpr float A8_NONE = -1e30f; // maximum of nothing
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef int v2i __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
 
 struct AttnArgs {
   Block8Seqs s;
@@ -19,83 +39,568 @@ struct AttnArgs {
   const int8_t *k, *v;
   const float *ks, *vs;
   void* out;
-  int Hq, Hkv;
+  int Hq, Hkv, G;
   float q_mul;
-  int64_t window;
+  int window;  // below 0: none
+  int slots;   // workgroups to split the keys over, 0: no splits
+  // splits only: partial sums [grid][ROWS][D], (m, l) [grid][ROWS], what to join of each pair
+  float* part;
+  float2* ml;
+  int4* pairs;  // [2 * pairs]: (first item, splits, items between, KV head), (first row, unit's first, rows)
+  int* count;   // pairs
 };
 
-// One wave per query row and head: a lane is a key in the scores, D / 64 channels in the sum.
-template <int DT, int D, bool ROT>
-__global__ void __launch_bounds__(64) attn_block8_row_kernel(const AttnArgs p) {
-  constexpr int LPR = row_lanes(D), C = D / 64;
-  __shared__ __attribute__((aligned(16))) int q_s[D / 4];
-  __shared__ float w_s[64];
-  const Block8Seqs& s = p.s;
-  const int lane = threadIdx.x;
-  const int64_t t = blockIdx.x / p.Hq;
-  const int h = blockIdx.x % p.Hq, kvh = h / (p.Hq / p.Hkv);
-  const int64_t to = (t * p.Hq + h) * D;
+// ---------------------------------------------------------------------------
+// The work list. Every workgroup makes it for itself from the lengths: what is on the device is not
+// known to the host, and a launch to make it costs more than these few hundred cycles (a wave
+// counts 64 sequences at once).
+//
+// Items of a sequence: units x Hkv x splits. A split has at most L tiles, L the least for which
+// the items fit the slots that are resident at once, so that a batch of mixed lengths gives every
+// slot about the same number of keys. KV heads are next to each other: item % 8 is the XCD, and
+// the units that read a head's keys meet in its L2.
+// ---------------------------------------------------------------------------
+struct SeqWork {
+  int units, tiles;
+};
 
-  const int b = seq_of(s.B, lane, t, [&](int i) { return s.row(i); });
-  int64_t lo = 0, hi = 0;
-  if (b >= 0 && t < s.row(b + 1)) {
-    const int64_t len = s.lens[b], pos = len - (s.row(b + 1) - s.row(b)) + (t - s.row(b));
-    hi = min(min(pos + 1, len), (int64_t)s.maxb * s.bs);
-    if (p.window >= 0) lo = max((int64_t)0, pos - p.window + 1);
+struct Item {
+  int b, unit, kvh, split, splits, units, pair;
+  bool live;
+};
+
+template <int ROWS>
+__device__ __forceinline__ SeqWork seq_work(const AttnArgs& p, int b) {
+  SeqWork w{0, 1};
+  if (b < p.s.B) {
+    const int n = max(0, (int)(p.s.row(b + 1) - p.s.row(b)));
+    const int cap = p.s.maxb * p.s.bs;
+    int span = min(max(p.s.lens[b], 0), cap);
+    if (p.window >= 0) span = (int)min((int64_t)span, (int64_t)p.window + ROWS / p.G + A8_TILE);
+    w.units = (n * p.G + ROWS - 1) / ROWS;
+    w.tiles = max(1, (span + A8_TILE - 1) / A8_TILE);
   }
+  return w;
+}
 
-  float f[8] = {};
-  if (lane < LPR) VecIO<DT>::unpack(reinterpret_cast<const uint4*>(p.q + to)[lane], f);
-  if constexpr (ROT) hadamard_row<D, DT != SL8_DTYPE_F16>(f, lane);
-  float amax = 0.f;
+template <int ROWS>
+__device__ __forceinline__ Item find_item(const AttnArgs& p, int lane, int id) {
+  const SeqWork mine = seq_work<ROWS>(p, lane);
+  auto work = [&](int b0) { return b0 == 0 ? mine : seq_work<ROWS>(p, b0 + lane); };
+  int L = INT_MAX / 2;
+  if (p.slots) {
+    int most = 1, pairs = 0;
+    float all = 0.f;
+    for (int b0 = 0; b0 < p.s.B; b0 += 64) {
+      const SeqWork w = work(b0);
+      most = max(most, w.units ? w.tiles : 1);
+      pairs += w.units;
+      all += (float)w.units * (float)w.tiles;
+    }
+    most = (int)lane_group_reduce<64>((uint32_t)most, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+    pairs = lane_group_sum<64>(pairs) * p.Hkv;
+    all = wave_sum(all) * (float)p.Hkv;
+    // the least L with items(L) <= slots
+    int lo = max(A8_MIN_TILES, (int)(all / (float)p.slots * 0.999f)), hi = most;
+    if (pairs < p.slots) hi = min(hi, (int)(all / (float)(p.slots - pairs)) + 2);
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      int n = 0;
+      for (int b0 = 0; b0 < p.s.B; b0 += 64) {
+        const SeqWork w = work(b0);
+        n += w.units * ((w.tiles + mid - 1) / mid);
+      }
+      n = __builtin_amdgcn_readfirstlane(lane_group_sum<64>(n)) * p.Hkv;
+      if (n <= p.slots) hi = mid;
+      else lo = mid + 1;
+    }
+    L = max(lo, 1);
+  }
+  Item it{};
+  int items = 0, pairs = 0;
+  for (int b0 = 0; b0 < p.s.B; b0 += 64) {
+    const SeqWork w = work(b0);
+    const int s = (w.tiles + L - 1) / L;
+    const int np = w.units * p.Hkv, ni = np * s;
+    int ii = ni, pp = np;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(f[e]));
-  amax = lane_group_max<LPR>(amax);
-  const float sc = amax * (1.0f / 127.0f), safe = sc == 0.f ? 1.f : sc;
-  if (lane < LPR) reinterpret_cast<uint2*>(q_s)[lane] = row_codes8<DT>(f, safe);
-  const float qs = __shfl(safe, 0, 64) * p.q_mul;
-  __syncthreads();
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(ii, o, 64), y = __shfl_up(pp, o, 64);
+      if (lane >= o) ii += x, pp += y;
+    }
+    const uint64_t past = __builtin_amdgcn_ballot_w64(items + ii > id);
+    if (past && !it.live) {
+      const int at = __builtin_ctzll(past);
+      it.live = true;
+      it.b = b0 + at;
+      it.splits = __builtin_amdgcn_readlane(s, at);
+      it.units = __builtin_amdgcn_readlane(w.units, at);
+      const int r = id - (items + __builtin_amdgcn_readlane(ii - ni, at));
+      it.kvh = r % p.Hkv;
+      it.unit = r / p.Hkv % it.units;
+      it.split = r / p.Hkv / it.units;
+      it.pair = pairs + __builtin_amdgcn_readlane(pp - np, at) + it.unit * p.Hkv + it.kvh;
+      if (id) break;  // (the first workgroup counts all pairs)
+    }
+    items += __builtin_amdgcn_readlane(ii, 63);
+    pairs += __builtin_amdgcn_readlane(pp, 63);
+  }
+  if (p.slots && id == 0 && threadIdx.x == 0) *p.count = pairs;
+  return it;
+}
 
-  float m = -1e30f, l = 0.f, o[C] = {};
-  for (int64_t j0 = lo; j0 < hi; j0 += 64) {
-    const int64_t j = j0 + lane;
-    const int id = j < hi ? s.block(b, (int)(j / s.bs)) : -1;
-    float x = -INFINITY, v = 0.f;
+// The rows and keys of an item.
+struct Span {
+  int64_t row0;   // first row (token) of the sequence
+  int r0, cnt;    // the unit's first of its rows, and how many
+  int pos0;       // position of the sequence's first new token
+  int hi, cap;    // keys that there are, and that the table holds
+  int k0, k1;     // keys of the item: from a multiple of a tile
+};
+
+template <int ROWS>
+__device__ __forceinline__ Span item_span(const AttnArgs& p, const Item& it) {
+  Span w;
+  w.row0 = p.s.row(it.b);
+  const int n = (int)(p.s.row(it.b + 1) - w.row0);
+  const int64_t len = p.s.lens[it.b];
+  w.r0 = it.unit * ROWS;
+  w.cnt = min(ROWS, n * p.G - w.r0);
+  // (contexts below the new tokens: positions below 0, which see nothing)
+  const int64_t pos0 = max(len - n, (int64_t)-(1 << 28));
+  w.pos0 = (int)min(pos0, (int64_t)INT_MAX - (1 << 29));
+  w.hi = (int)max((int64_t)0, min(len, (int64_t)p.s.maxb * p.s.bs));
+  const int last = min(w.hi, w.pos0 + (w.r0 + w.cnt - 1) / p.G + 1);
+  int first = 0;
+  if (p.window >= 0) {
+    first = (int)max((int64_t)0, (int64_t)w.pos0 + w.r0 / p.G - p.window + 1);
+    first &= ~(A8_TILE - 1);
+  }
+  const int tiles = max(0, last - first + A8_TILE - 1) / A8_TILE;
+  const int per = (tiles + it.splits - 1) / it.splits * A8_TILE;
+  w.k0 = first + it.split * per;
+  w.k1 = min(last, w.k0 + per);
+  return w;
+}
+
+// Rows behind the last sequence are zeros.
+__device__ __forceinline__ void zero_tail(const AttnArgs& p, int D) {
+  if (!p.s.cu) return;
+  const int64_t chunks = (int64_t)p.Hq * D / 8;
+  uint4* o = static_cast<uint4*>(p.out);
+  for (int64_t t = p.s.row(p.s.B) + blockIdx.x; t < p.s.T; t += gridDim.x)
+    for (int64_t i = threadIdx.x; i < chunks; i += A8_THREADS) o[t * chunks + i] = make_uint4(0, 0, 0, 0);
+}
+
+// Row r of a unit: its offset in q and out.
+__device__ __forceinline__ int64_t row_at(const AttnArgs& p, const Span& w, int kvh, int r, int D) {
+  const int i = w.r0 + r;
+  return ((w.row0 + i / p.G) * p.Hq + kvh * p.G + i % p.G) * D;
+}
+
+// The unit's rows as int8 codes [ROWS][D] in LDS with their scales (times q_mul); rows past the last
+// are zeros.
+template <int DT, int D, int ROWS, bool ROT>
+__device__ __forceinline__ void quant_rows(const AttnArgs& p, const Span& w, int kvh, int8_t* q_s, float* qs_s) {
+  constexpr int LPR = row_lanes(D), RPB = A8_THREADS / LPR;
+  const int lane = threadIdx.x % LPR;
+#pragma unroll
+  for (int r1 = 0; r1 < ROWS; r1 += RPB) {
+    const int r = r1 + threadIdx.x / LPR;
+    if (ROWS % RPB && r >= ROWS) break;
+    const bool live = r < w.cnt;
+    float f[8];
+    VecIO<DT>::unpack(reinterpret_cast<const uint4*>(p.q + row_at(p, w, kvh, live ? r : 0, D))[lane], f);
+    if constexpr (ROT) hadamard_row<D, DT != SL8_DTYPE_F16>(f, lane);
+    float amax = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(f[e]));
+    amax = lane_group_max<LPR>(amax);
+    const float s = amax * (1.0f / 127.0f), safe = s == 0.f ? 1.f : s;
+    const uint2 c = row_codes8<DT>(f, safe);
+    reinterpret_cast<uint2*>(q_s + r * D)[lane] = live ? c : make_uint2(0, 0);
+    if (lane == 0) qs_s[r] = live ? safe * p.q_mul : 0.f;
+  }
+}
+
+// 16 consecutive keys lie in one block: their first row's offset in the caches and the block's
+// scales, none (log2 vs = -inf: weight 0) where there is no block or no key.
+struct Group {
+  int64_t at;  // bytes
+  float ks, lv, iv;
+};
+template <int D>
+__device__ __forceinline__ Group key_group(const AttnArgs& p, int b, int kvh, int key, int end) {
+  Group g{0, 0.f, -INFINITY, 0.f};
+  if (key < end) {
+    const int j = key / p.s.bs, off = key - j * p.s.bs;
+    const int id = p.s.block(b, j);
     if (id >= 0) {
       const int64_t bh = (int64_t)id * p.Hkv + kvh;
-      const int* kr = reinterpret_cast<const int*>(p.k + (bh * s.bs + j % s.bs) * D);
-      int acc = 0;
-#pragma unroll
-      for (int c = 0; c < D / 4; ++c) acc = __builtin_amdgcn_sdot4(kr[c], q_s[c], acc, false);
-      x = (float)acc * (qs * p.ks[bh]);
-      v = p.vs[bh];
+      const float vs = p.vs[bh];
+      g = Group{(bh * p.s.bs + off) * D, p.ks[bh], __builtin_amdgcn_logf(vs), 1.f / vs};
     }
-    const float mn = fmaxf(m, wave_max(x));
-    const float w = exp2f(x - mn), r = exp2f(m - mn);
-    m = mn;
-    l = l * r + wave_sum(w);
-#pragma unroll
-    for (int c = 0; c < C; ++c) o[c] *= r;
-    w_s[lane] = id >= 0 ? w * v : 0.f;
-    __syncthreads();
-    for (int i = 0; i < 64 && j0 + i < hi; ++i) {
-      const int ib = s.block(b, (int)((j0 + i) / s.bs));
-      if (ib < 0) continue;
-      const int8_t* vr = p.v + (((int64_t)ib * p.Hkv + kvh) * s.bs + (j0 + i) % s.bs) * D;
-#pragma unroll
-      for (int c = 0; c < C; ++c) o[c] = fmaf(w_s[i], (float)vr[lane + 64 * c], o[c]);
-    }
-    __syncthreads();
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  return g;
+}
+
+__device__ __forceinline__ float lane_value(float x, int lane) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
+}
+
+// 8 int8 codes as fp16: byte v xor 0x80 is v + 128, under the exponent byte 0x64 it is 1024 + that.
+__device__ __forceinline__ v8h codes_f16(v2i c) {
+  h2 o[4];
 #pragma unroll
-  for (int c = 0; c < C; ++c) st_out<DT>(p.out, to + lane + 64 * c, o[c] * inv);
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t x = (uint32_t)c[i] ^ 0x80808080u;
+    const h2 bias = {(_Float16)1152.f, (_Float16)1152.f};
+    o[2 * i] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u)) - bias;
+    o[2 * i + 1] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u)) - bias;
+  }
+  return __builtin_bit_cast(v8h, o);
+}
+
+__device__ __forceinline__ float max_xor16(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// ---------------------------------------------------------------------------
+// Few rows (a decode step, drafted tokens): each wave streams tiles of its own keys for all ROWS
+// rows, the 4 waves' states are joined in LDS. Bound by the bytes of K and V.
+//   * S^T = K Q^T on v_mfma_i32_16x16x64_i8, K straight from global memory into the A operand
+//     (lane (g4, col): 16 bytes of key col), the next tile's loads going out as soon as the
+//     products have read this one's;
+//   * lane (g4, col) then holds keys 4 g4 + i of each 16 for row col: the softmax needs two
+//     exchanges across the wave for the maximum, the weights are the B operand as they are;
+//   * V comes by direct copies into a ring of two tiles in LDS and is read transposed
+//     (ds_read_b64_tr_b8: 8 keys of a channel), in the order of keys that the weights have, and
+//     turned into fp16: O^T += V^T W on v_mfma_f32_16x16x32_f16. 16-byte chunks of a row are
+//     placed by an xor of its key, so that the 16 rows of half a wave lie in different banks.
+// ---------------------------------------------------------------------------
+template <int D> constexpr int stream_keys() { return D == 256 ? 32 : 64; }
+template <int D> __device__ __forceinline__ int v_swizzle(int key) {
+  if constexpr (D == 64) return ((key >> 2) & 1) | ((key >> 4) & 1) << 1;
+  else if constexpr (D == 128) return ((key >> 1) & 3) | ((key >> 4) & 1) << 2;
+  else return (key & 7) | ((key >> 4) & 1) << 3;
+}
+
+template <int DT, int D, int RT, bool ROT>
+__global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const AttnArgs p) {
+  constexpr int ROWS = 16 * RT, KT = stream_keys<D>(), NG = KT / 16, KS = D / 64, DTL = D / 16;
+  constexpr int TPM = 64 / NG;  // tiles whose groups the lanes hold
+  // Two arrays, not one of two stages: the compiler sees that the reads of one tile are not of the
+  // copies in flight, and waits for none of those. The waves' sums are joined in them (o_place).
+  __shared__ __attribute__((aligned(16))) int8_t v0_s[A8_WAVES * KT * D], v1_s[A8_WAVES * KT * D];
+  __shared__ __attribute__((aligned(16))) int8_t q_s[ROWS * D];
+  __shared__ float qs_s[ROWS], m_s[A8_WAVES][ROWS], l_s[A8_WAVES][ROWS];
+  static_assert(ROWS * D * 4 * A8_WAVES <= 2 * A8_WAVES * KT * D, "the sums fit the ring");
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, g4 = lane >> 4;
+
+  zero_tail(p, D);
+  const Item it = find_item<ROWS>(p, lane, blockIdx.x);
+  if (!it.live) return;
+  const Span w = item_span<ROWS>(p, it);
+  quant_rows<DT, D, ROWS, ROT>(p, w, it.kvh, q_s, qs_s);
+  __syncthreads();
+
+  v4i qb[RT][KS];
+  float qs[RT];
+  int lim[RT], low[RT];  // row sees keys [low, lim)
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = 16 * rt + col;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qb[rt][s] = *reinterpret_cast<const v4i*>(q_s + r * D + 64 * s + 16 * g4);
+    qs[rt] = qs_s[r];
+    const int pos = w.pos0 + (w.r0 + min(r, w.cnt - 1)) / p.G;
+    lim[rt] = min(pos + 1, w.k1);
+    low[rt] = p.window >= 0 ? (int)max((int64_t)pos - p.window + 1, (int64_t)0) : 0;
+  }
+  // keys that every row sees: [in0, in1)
+  const int in1 = min(w.pos0 + w.r0 / p.G + 1, w.k1);
+  const int in0 = p.window >= 0 ? w.pos0 + (w.r0 + w.cnt - 1) / p.G - p.window + 1 : 0;
+
+  float m[RT], l[RT];
+  v4f o[RT][DTL];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    m[rt] = A8_NONE;
+    l[rt] = 0.f;
+#pragma unroll
+    for (int t = 0; t < DTL; ++t) o[rt][t] = v4f{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // places: K's lane in a group, the copies' lanes (16-byte chunk of the row that goes to the
+  // lane's place) for even and odd groups, the transposed reads' rows
+  const int k_off = col * D + 16 * g4;
+  constexpr int CPR = D / 16, CPG = D / 64;  // chunks a row, copies a group
+  int v_off[2][CPG];
+#pragma unroll
+  for (int c = 0; c < CPG; ++c) {
+    const int ci = 64 * c + lane, r = ci / CPR, ch = ci % CPR;
+#pragma unroll
+    for (int odd = 0; odd < 2; ++odd) v_off[odd][c] = r * D + 16 * (ch ^ v_swizzle<D>(16 * odd + r));
+  }
+  const int vkey = (col >> 1) < 4 ? 4 * g4 + (col >> 1) : 12 + 4 * g4 + (col >> 1);
+  const int vt_off = vkey * D + 8 * (col & 1), vt_swz = 16 * v_swizzle<D>(vkey);
+
+  const int first = w.k0 + wave * KT, step = A8_WAVES * KT;
+  const int ntiles = first < w.k1 ? (w.k1 - first + step - 1) / step : 0;
+  // lane i: group i % NG of the wave's tile i / NG (of each TPM)
+  auto groups = [&](int tile) {
+    return key_group<D>(p, it.b, it.kvh, first + (tile + lane / NG) * step + 16 * (lane % NG), w.k1);
+  };
+  Group cur = groups(0), nxt = cur;
+  v4i ka[NG][KS];
+  auto base = [&](const Group& g, int i) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)g.at, i);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(g.at >> 32), i);
+    return (int64_t)(((uint64_t)hi << 32) | lo);
+  };
+  auto load = [&](const Group& g, int i0, int8_t* ring) {
+    int8_t* const to = ring + wave * KT * D;
+#pragma unroll
+    for (int g1 = 0; g1 < NG; ++g1) {
+      const int64_t at = base(g, i0 + g1);
+      const int8_t* kp = p.k + at;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) ka[g1][s] = *reinterpret_cast<const v4i*>(kp + k_off + 64 * s);
+    }
+#pragma unroll
+    for (int g1 = 0; g1 < NG; ++g1) {
+      const brsrc_t vr = make_rsrc(p.v + base(g, i0 + g1), 16 * D);
+#pragma unroll
+      for (int c = 0; c < CPG; ++c) buf16_to_lds(vr, to + g1 * 16 * D + c * 1024, v_off[g1 & 1][c], 0);
+    }
+  };
+  if (ntiles) load(cur, 0, v0_s);
+
+  auto tile = [&](int j, const int8_t* ring, int8_t* next) __attribute__((always_inline)) {
+    const int i0 = j % TPM * NG;  // the tile's groups are in lanes i0 .. i0 + NG - 1 of cur
+    const int key0 = first + j * step;
+    if (i0 == 0) nxt = groups(j + TPM);
+    v4i sc[RT][NG];
+#pragma unroll
+    for (int g1 = 0; g1 < NG; ++g1)
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        v4i acc = {0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(ka[g1][s], qb[rt][s], acc, 0, 0, 0);
+        sc[rt][g1] = acc;
+      }
+    float gks[NG], glv[NG], giv[NG];
+#pragma unroll
+    for (int g1 = 0; g1 < NG; ++g1) {
+      gks[g1] = lane_value(cur.ks, i0 + g1);
+      glv[g1] = lane_value(cur.lv, i0 + g1);
+      giv[g1] = lane_value(cur.iv, i0 + g1);
+    }
+    // (past the last tile: groups without a block, whose copies read the pool's first rows)
+    if (i0 + NG == 64) cur = nxt;
+    load(cur, (i0 + NG) & 63, next);
+
+    v8h wb[RT][NG / 2];
+    const bool inside = key0 >= in0 && key0 + KT <= in1;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      float t[NG][4];
+      float mt = -INFINITY;
+#pragma unroll
+      for (int g1 = 0; g1 < NG; ++g1) {
+        const float a = qs[rt] * gks[g1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[g1][i] = fmaf((float)sc[rt][g1][i], a, glv[g1]);
+      }
+      if (!inside) {
+#pragma unroll
+        for (int g1 = 0; g1 < NG; ++g1)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = key0 + 16 * g1 + 4 * g4 + i;
+            if (key >= lim[rt] || key < low[rt]) t[g1][i] = -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int g1 = 0; g1 < NG; ++g1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mt = fmaxf(mt, t[g1][i]);
+      mt = max_xor32(max_xor16(mt));
+      const float mn = fmaxf(m[rt], mt);
+      if (__builtin_amdgcn_ballot_w64(mn > m[rt])) {
+        const float r = __builtin_amdgcn_exp2f(m[rt] - mn);
+        l[rt] *= r;
+#pragma unroll
+        for (int d = 0; d < DTL; ++d) o[rt][d] *= r;
+        m[rt] = mn;
+      }
+#pragma unroll
+      for (int g1 = 0; g1 < NG; ++g1)
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          const float a = __builtin_amdgcn_exp2f(t[g1][i] - mn), b = __builtin_amdgcn_exp2f(t[g1][i + 1] - mn);
+          l[rt] = fmaf(a, giv[g1], fmaf(b, giv[g1], l[rt]));
+          const h2 ab = __builtin_convertvector((v2f{a, b}), h2);
+          wb[rt][g1 / 2][4 * (g1 & 1) + i] = ab[0];
+          wb[rt][g1 / 2][4 * (g1 & 1) + i + 1] = ab[1];
+        }
+    }
+
+    // V(j): copied before the NG * KS loads and NG * CPG copies of the next tile
+    __builtin_amdgcn_s_waitcnt((((NG * (KS + CPG)) & 15) | ((NG * (KS + CPG)) >> 4) << 14) | 0x0F70);
+    __builtin_amdgcn_sched_barrier(0);
+    const int8_t* vt = ring + wave * KT * D + vt_off;
+#pragma unroll
+    for (int kk = 0; kk < NG / 2; ++kk)
+#pragma unroll
+      for (int d = 0; d < DTL; ++d) {
+        const v8h a = codes_f16(__builtin_amdgcn_ds_read_tr8_b64_v2i32(
+            (__attribute__((address_space(3))) v2i*)(vt + 32 * kk * D + ((16 * d) ^ vt_swz))));
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+          o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wb[rt][kk], o[rt][d], 0, 0, 0);
+      }
+  };
+  for (int j = 0; j < ntiles;) {
+    tile(j++, v0_s, v1_s);
+    if (j >= ntiles) break;
+    tile(j++, v1_s, v0_s);
+  }
+
+  // ---- join the waves ----
+  // 4 channels (chunk c) of a wave's row r: placed by an xor of the row, as a column of rows is written
+  constexpr int O_WAVE = ROWS * D * 4, O_FIT = A8_WAVES * KT * D / O_WAVE;  // sums in the first array
+  auto o_place = [&](int x, int r, int c) {
+    int8_t* a = x < O_FIT ? v0_s + x * O_WAVE : v1_s + (x - O_FIT) * O_WAVE;
+    return a + (r * (D / 4) + (c ^ (r & 15))) * 16;
+  };
+  wait_dma();  // (the copies past the last tile land in the ring that is written below)
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    l[rt] += __shfl_xor(l[rt], 16, 64);
+    l[rt] += __shfl_xor(l[rt], 32, 64);
+    if (g4 == 0) {
+      m_s[wave][16 * rt + col] = m[rt];
+      l_s[wave][16 * rt + col] = l[rt];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = 16 * rt + col;
+    float mm = m[rt];
+#pragma unroll
+    for (int x = 0; x < A8_WAVES; ++x) mm = fmaxf(mm, m_s[x][r]);
+    const float f = __builtin_amdgcn_exp2f(m[rt] - mm);
+#pragma unroll
+    for (int d = 0; d < DTL; ++d) *reinterpret_cast<v4f*>(o_place(wave, r, 4 * d + g4)) = o[rt][d] * f;
+  }
+  __syncthreads();
+  for (int i = tid; i < ROWS * D / 4; i += A8_THREADS) {
+    const int r = i / (D / 4), d = 4 * (i % (D / 4));
+    if (r >= w.cnt) break;
+    v4f a = *reinterpret_cast<const v4f*>(o_place(0, r, d / 4));
+    float mm = m_s[0][r], den = 0.f;
+#pragma unroll
+    for (int x = 1; x < A8_WAVES; ++x) {
+      a += *reinterpret_cast<const v4f*>(o_place(x, r, d / 4));
+      mm = fmaxf(mm, m_s[x][r]);
+    }
+#pragma unroll
+    for (int x = 0; x < A8_WAVES; ++x) den += l_s[x][r] * __builtin_amdgcn_exp2f(m_s[x][r] - mm);
+    if (it.splits == 1) {
+      a *= den > 0.f ? 1.f / den : 0.f;
+      const int64_t to = row_at(p, w, it.kvh, r, D) + d;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) st_out<DT>(p.out, to + e, a[e]);
+    } else {
+      const int64_t row = (int64_t)blockIdx.x * ROWS + r;
+      *reinterpret_cast<v4f*>(p.part + row * D + d) = a;
+      if (d == 0) p.ml[row] = make_float2(mm, den);
+    }
+  }
+  if (p.slots && it.split == 0 && tid == 0) {
+    p.pairs[2 * it.pair] = make_int4(blockIdx.x, it.splits, it.units * p.Hkv, it.kvh);
+    p.pairs[2 * it.pair + 1] = make_int4((int)w.row0, w.r0, w.cnt, 0);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The splits of a pair (unit, KV head) joined: a wave per row, D / 64 channels a lane; sums in
+// the order of the splits.
+// ---------------------------------------------------------------------------
+template <int DT, int D, int ROWS>
+__global__ void __launch_bounds__(64) attn_block8_join_kernel(const AttnArgs p) {
+  constexpr int C = D / 64;
+  const int lane = threadIdx.x, r = blockIdx.y;
+  if ((int)blockIdx.x >= *p.count) return;
+  const int4 a = p.pairs[2 * blockIdx.x], u = p.pairs[2 * blockIdx.x + 1];
+  if (a.y == 1 || r >= u.z) return;
+  const int64_t row0 = (int64_t)a.x * ROWS + r, step = (int64_t)a.z * ROWS;
+  float mm = A8_NONE;
+  for (int s = lane; s < a.y; s += 64) mm = fmaxf(mm, p.ml[row0 + s * step].x);
+  mm = wave_max(mm);
+  float den = 0.f, o[C] = {};
+  for (int s0 = 0; s0 < a.y; s0 += 64) {
+    float f = 0.f, l = 0.f;
+    if (s0 + lane < a.y) {
+      const float2 x = p.ml[row0 + (s0 + lane) * step];
+      f = __builtin_amdgcn_exp2f(x.x - mm);
+      l = x.y * f;
+    }
+    den += wave_sum(l);
+    const int n = min(64, a.y - s0);
+#pragma unroll 8
+    for (int s = 0; s < n; ++s) {
+      const float* x = p.part + (row0 + (s0 + s) * step) * D + C * lane;
+      const float fs = lane_value(f, s);
+#pragma unroll
+      for (int c = 0; c < C; ++c) o[c] = fmaf(x[c], fs, o[c]);
+    }
+  }
+  const float inv = den > 0.f ? 1.f / den : 0.f;
+  const int i = u.y + r;
+  const int64_t to = (((int64_t)u.x + i / p.G) * p.Hq + a.w * p.G + i % p.G) * D + C * lane;
+#pragma unroll
+  for (int c = 0; c < C; ++c) st_out<DT>(p.out, to + c, o[c] * inv);
+}
+
+// How a call runs: rows of a unit, a bound on its pairs, whether keys are split over workgroups,
+// and the bytes that that takes.
+struct AttnPlan {
+  int rows;
+  int64_t pairs;
+  int slots;
+  int64_t grid;
+  size_t bytes;
+};
+
+AttnPlan attn_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D) {
+  AttnPlan a{};
+  if (T == 0 || B == 0 || Hq == 0) return a;
+  const int64_t G = Hq / Hkv;
+  // rows of a sequence on average: 32-row units read K and V half as often where 16 do not hold them
+  a.rows = D < 256 && T * G > 16 * B ? 32 : 16;
+  a.pairs = Hkv * (T * G / a.rows + B);
+  const int64_t slots = 2 * (int64_t)cu_count();  // two workgroups a CU (LDS)
+  a.slots = a.pairs < slots ? (int)slots : 0;
+  a.grid = a.slots ? slots : a.pairs;
+  if (a.slots) a.bytes = (size_t)a.grid * a.rows * (D + 2) * 4 + (size_t)a.pairs * 32 + 16;
+  return a;
 }
 
 }  // namespace
 }  // namespace sl8
 
 using namespace sl8;
+
+extern "C" size_t sl8_attn_paged_block8_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D) {
+  if (T <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || T >= (1LL << 28) || B >= (1 << 24) || Hq >= (1 << 16)) return 0;
+  return attn_plan(T, B, Hq, Hkv, D).bytes;
+}
 
 extern "C" int sl8_attn_paged_block8(const void* q, int dtype, int rotate, float q_scale_mul,
                                      const int8_t* k_cache, const float* k_scale,
@@ -104,7 +609,8 @@ extern "C" int sl8_attn_paged_block8(const void* q, int dtype, int rotate, float
                                      const int32_t* block_table, void* out, int64_t T, int64_t B,
                                      int64_t Hq, int64_t Hkv, int64_t D, int64_t num_blocks,
                                      int64_t block_size, int64_t max_blocks_per_seq,
-                                     int64_t window_left, void* stream) {
+                                     int64_t window_left, void* workspace, size_t workspace_bytes,
+                                     void* stream) {
   clear_error();
   const char* tag = "attn_paged_block8";
   SL8_CHECK_ARG(dtype == SL8_DTYPE_F16 || dtype == SL8_DTYPE_BF16, "fni8 %s: q must be float16 or bfloat16", tag);
@@ -112,30 +618,55 @@ extern "C" int sl8_attn_paged_block8(const void* q, int dtype, int rotate, float
                     num_blocks >= 0 && num_blocks < (1LL << 31) && max_blocks_per_seq >= 0 &&
                     max_blocks_per_seq < (1LL << 31) && block_size >= 0 && block_size < (1 << 16),
                 "fni8 %s: shape too large", tag);
-  AttnArgs p{Block8Seqs{cu_lens, context_lens, block_table, T, (int)B, (int)max_blocks_per_seq,
-                        (int)num_blocks, (int)block_size},
-             static_cast<const uint16_t*>(q), k_cache, v_cache, k_scale, v_scale, out, (int)Hq, (int)Hkv,
-             q_scale_mul, window_left};
+  AttnArgs p{};
+  p.s = Block8Seqs{cu_lens, context_lens, block_table, T, (int)B, (int)max_blocks_per_seq, (int)num_blocks,
+                   (int)block_size};
   if (const int rc = block8_check(tag, p.s, Hkv, D)) return rc;
   SL8_CHECK_ARG(Hq % Hkv == 0, "fni8 %s: H_q must be divisible by H_kv (GQA)", tag);
+  SL8_CHECK_ARG(T * Hq < (1LL << 30) && T * (Hq / Hkv) + B < (1LL << 30) / Hkv, "fni8 %s: shape too large", tag);
   if (T == 0 || Hq == 0) return SL8_OK;
   SL8_CHECK_ARG(q && out && (B == 0 || (context_lens && (max_blocks_per_seq == 0 || block_table))) &&
                     (num_blocks == 0 || (k_cache && k_scale && v_cache && v_scale)),
                 "fni8 %s: null pointer", tag);
   SL8_CHECK_ARG(aligned(q, 16) && aligned(out, 16) && aligned(k_cache, 16) && aligned(v_cache, 16),
                 "fni8 %s: q/k_cache/v_cache must be 16-byte aligned", tag);
-  SL8_CHECK_ARG(T * Hq < (1LL << 31), "fni8 %s: shape too large", tag);
+  const AttnPlan plan = attn_plan(T, B, Hq, Hkv, D);
+  SL8_CHECK_ARG(plan.bytes == 0 || (workspace && workspace_bytes >= plan.bytes && aligned(workspace, 16)),
+                "fni8 %s: workspace needs %zu bytes", tag, plan.bytes);
+  p.q = static_cast<const uint16_t*>(q);
+  p.k = k_cache; p.v = v_cache; p.ks = k_scale; p.vs = v_scale;
+  p.out = out;
+  p.Hq = (int)Hq; p.Hkv = (int)Hkv; p.G = (int)(Hq / Hkv);
+  p.q_mul = q_scale_mul;
+  p.window = window_left < 0 ? -1 : (int)(window_left < (1 << 30) ? window_left : (1 << 30));
+  p.slots = plan.slots;
+  if (num_blocks == 0) p.s.maxb = 0;  // nothing to read: no key is there
+  if (plan.slots) {
+    p.part = static_cast<float*>(workspace);
+    p.pairs = reinterpret_cast<int4*>(p.part + (size_t)plan.grid * plan.rows * D);
+    p.count = reinterpret_cast<int*>(p.pairs + 2 * plan.pairs);
+    p.ml = reinterpret_cast<float2*>(p.count + 4);
+  }
   const hipStream_t st = static_cast<hipStream_t>(stream);
+  const unsigned grid = (unsigned)(plan.grid > 0 ? plan.grid : 1);
   using std::integral_constant;
-  auto go = [&](auto dt, auto d) {
-    constexpr int DT = decltype(dt)::value, DD = decltype(d)::value;
-    if (rotate) attn_block8_row_kernel<DT, DD, true><<<(unsigned)(T * Hq), 64, 0, st>>>(p);
-    else attn_block8_row_kernel<DT, DD, false><<<(unsigned)(T * Hq), 64, 0, st>>>(p);
+  auto go = [&](auto dt, auto d, auto rt) {
+    constexpr int DT = decltype(dt)::value, DD = decltype(d)::value, RT = decltype(rt)::value;
+    if (rotate) attn_block8_stream_kernel<DT, DD, RT, true><<<grid, A8_THREADS, 0, st>>>(p);
+    else attn_block8_stream_kernel<DT, DD, RT, false><<<grid, A8_THREADS, 0, st>>>(p);
+    if (plan.slots)
+      attn_block8_join_kernel<DT, DD, 16 * RT><<<dim3((unsigned)plan.pairs, 16 * RT), 64, 0, st>>>(p);
+  };
+  auto by_rows = [&](auto dt, auto d) {
+    if constexpr (decltype(d)::value < 256) {
+      if (plan.rows == 32) return go(dt, d, integral_constant<int, 2>{});
+    }
+    go(dt, d, integral_constant<int, 1>{});
   };
   auto by_d = [&](auto dt) {
-    if (D == 64) go(dt, integral_constant<int, 64>{});
-    else if (D == 128) go(dt, integral_constant<int, 128>{});
-    else go(dt, integral_constant<int, 256>{});
+    if (D == 64) by_rows(dt, integral_constant<int, 64>{});
+    else if (D == 128) by_rows(dt, integral_constant<int, 128>{});
+    else by_rows(dt, integral_constant<int, 256>{});
   };
   if (dtype == SL8_DTYPE_F16) by_d(integral_constant<int, SL8_DTYPE_F16>{});
   else by_d(integral_constant<int, SL8_DTYPE_BF16>{});

@@ -53,7 +53,7 @@ inline int block8_check(const char* tag, const Block8Seqs& s, int64_t Hkv, int64
   SL8_CHECK_ARG(s.B >= 0 && s.T >= 0 && s.maxb >= 0 && s.num_blocks >= 0 && Hkv > 0 && Hkv < (1 << 16),
                 "fni8 %s: bad shape", tag);
   SL8_CHECK_ARG(s.cu || s.T == s.B, "fni8 %s: without cu_lens there is one row per sequence", tag);
-  SL8_CHECK_ARG(s.T < (1LL << 28) && s.B < (1 << 24) && (int64_t)s.maxb * s.bs < (1LL << 31),
+  SL8_CHECK_ARG(s.T < (1LL << 28) && s.B < (1 << 24) && (int64_t)s.maxb * s.bs < (1LL << 30),
                 "fni8 %s: shape too large", tag);
   return SL8_OK;
 }

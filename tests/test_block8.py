@@ -26,7 +26,8 @@ def append(**c):
 
 def attn(**c):
     a = dict(q=16, dtype=0, rot=0, mul=1.0, k=16, ks=16, v=16, vs=16, cu=None, lens=16, bt=16, out=16, T=2,
-             B=2, Hq=2, Hkv=1, D=64, nb=4, bs=16, maxb=2, window=-1)
+             B=2, Hq=2, Hkv=1, D=64, nb=4, bs=16, maxb=2, window=-1,
+             ws=16, ws_bytes=1 << 40)
     return _lib.load().sl8_attn_paged_block8(*(a | c).values(), None)
 
 
@@ -46,7 +47,8 @@ def attn(**c):
     (attn, dict(dtype=2), b"float16"), (attn, dict(D=32), b"head dim"), (attn, dict(bs=8), b"block_size"),
     (attn, dict(Hq=3, Hkv=2), b"divisible"), (attn, dict(T=3), b"one row"), (attn, dict(q=None), b"null"),
     (attn, dict(lens=None), b"null"), (attn, dict(vs=None), b"null"), (attn, dict(q=24), b"aligned"),
-    (attn, dict(k=8), b"aligned"), (attn, dict(maxb=1 << 31), b"large"),
+    (attn, dict(k=8), b"aligned"), (attn, dict(maxb=1 << 31), b"large"), (attn, dict(maxb=1 << 26), b"large"),
+    (attn, dict(ws=None), b"workspace"), (attn, dict(ws_bytes=100), b"workspace"), (attn, dict(ws=24), b"workspace"),
 ])
 def test_refused(call, change, word):
     assert call(**change) == -1
