@@ -18,7 +18,7 @@
 
 #include "attn_common.hpp"
 #include "block8.hpp"
-#include "rowquant.hpp"
+#include "rope.hpp"
 
 namespace sl8 {
 namespace {
@@ -26,7 +26,8 @@ namespace {
 constexpr int A8_THREADS = 256, A8_WAVES = 4;
 constexpr int A8_TILE = 64;       // keys: what splits and units' first keys are multiples of
 constexpr int A8_MIN_TILES = 4;   // least keys of a split: a tile for each wave
-constexpr float A8_NONE = -1e30f; // maximum of nothing
+constexpr float A8_NONE = -1e30f; // reference of nothing
+constexpr float A8_LAG = 12.f;    // log2 of the largest weight (fp16 holds 2^15)
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -42,6 +43,7 @@ struct AttnArgs {
   int Hq, Hkv, G;
   float q_mul;
   int window;  // below 0: none
+  bool rotate;
   int slots;   // workgroups to split the keys over, 0: no splits
   // splits only: partial sums [grid][ROWS][D], (m, l) [grid][ROWS], what to join of each pair
   float* part;
@@ -137,7 +139,7 @@ __device__ __forceinline__ Item find_item(const AttnArgs& p, int lane, int id) {
       it.units = __builtin_amdgcn_readlane(w.units, at);
       const int r = id - (items + __builtin_amdgcn_readlane(ii - ni, at));
       it.kvh = r % p.Hkv;
-      it.unit = r / p.Hkv % it.units;
+      it.unit = it.units - 1 - r / p.Hkv % it.units;  // (those that see the most keys first)
       it.split = r / p.Hkv / it.units;
       it.pair = pairs + __builtin_amdgcn_readlane(pp - np, at) + it.unit * p.Hkv + it.kvh;
       if (id) break;  // (the first workgroup counts all pairs)
@@ -183,13 +185,19 @@ __device__ __forceinline__ Span item_span(const AttnArgs& p, const Item& it) {
   return w;
 }
 
+// What the joining kernel needs of a pair (unit, KV head); from its first item.
+__device__ __forceinline__ void note_pair(const AttnArgs& p, const Span& w, const Item& it) {
+  p.pairs[2 * it.pair] = make_int4(blockIdx.x, it.splits, it.units * p.Hkv, it.kvh);
+  p.pairs[2 * it.pair + 1] = make_int4((int)w.row0, w.r0, w.cnt, 0);
+}
+
 // Rows behind the last sequence are zeros.
 __device__ __forceinline__ void zero_tail(const AttnArgs& p, int D) {
   if (!p.s.cu) return;
   const int64_t chunks = (int64_t)p.Hq * D / 8;
   uint4* o = static_cast<uint4*>(p.out);
   for (int64_t t = p.s.row(p.s.B) + blockIdx.x; t < p.s.T; t += gridDim.x)
-    for (int64_t i = threadIdx.x; i < chunks; i += A8_THREADS) o[t * chunks + i] = make_uint4(0, 0, 0, 0);
+    for (int64_t i = threadIdx.x; i < chunks; i += blockDim.x) o[t * chunks + i] = make_uint4(0, 0, 0, 0);
 }
 
 // Row r of a unit: its offset in q and out.
@@ -198,11 +206,11 @@ __device__ __forceinline__ int64_t row_at(const AttnArgs& p, const Span& w, int 
   return ((w.row0 + i / p.G) * p.Hq + kvh * p.G + i % p.G) * D;
 }
 
-// The unit's rows as int8 codes [ROWS][D] in LDS with their scales (times q_mul); rows past the last
-// are zeros.
-template <int DT, int D, int ROWS, bool ROT>
-__device__ __forceinline__ void quant_rows(const AttnArgs& p, const Span& w, int kvh, int8_t* q_s, float* qs_s) {
-  constexpr int LPR = row_lanes(D), RPB = A8_THREADS / LPR;
+// The unit's rows as int8 codes in LDS (row r at place(r)) with their scales (times q_mul); rows past
+// the last are zeros.
+template <int DT, int D, int ROWS, int THREADS, typename F>
+__device__ __forceinline__ void quant_rows(const AttnArgs& p, const Span& w, int kvh, F place, float* qs_s) {
+  constexpr int LPR = row_lanes(D), RPB = THREADS / LPR;
   const int lane = threadIdx.x % LPR;
 #pragma unroll
   for (int r1 = 0; r1 < ROWS; r1 += RPB) {
@@ -211,14 +219,14 @@ __device__ __forceinline__ void quant_rows(const AttnArgs& p, const Span& w, int
     const bool live = r < w.cnt;
     float f[8];
     VecIO<DT>::unpack(reinterpret_cast<const uint4*>(p.q + row_at(p, w, kvh, live ? r : 0, D))[lane], f);
-    if constexpr (ROT) hadamard_row<D, DT != SL8_DTYPE_F16>(f, lane);
+    if (p.rotate) hadamard_row<D, DT != SL8_DTYPE_F16>(f, lane);
     float amax = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(f[e]));
     amax = lane_group_max<LPR>(amax);
     const float s = amax * (1.0f / 127.0f), safe = s == 0.f ? 1.f : s;
     const uint2 c = row_codes8<DT>(f, safe);
-    reinterpret_cast<uint2*>(q_s + r * D)[lane] = live ? c : make_uint2(0, 0);
+    reinterpret_cast<uint2*>(place(r))[lane] = live ? c : make_uint2(0, 0);
     if (lane == 0) qs_s[r] = live ? safe * p.q_mul : 0.f;
   }
 }
@@ -266,6 +274,106 @@ __device__ __forceinline__ float max_xor16(float x) {
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
+// Softmax state of 16 RT rows in the layout of S^T: row 16 rt + col in the lanes of column col.
+template <int RT, int D>
+struct RowState {
+  float qs[RT];
+  int lim[RT], low[RT];  // the row sees keys [low, lim)
+  int in0, in1;          // keys that every row of the unit sees: [in0, in1)
+  float m[RT], l[RT];    // reference (log2) and sum of weights / vs
+  v4f o[RT][D / 16];
+
+  __device__ __forceinline__ void init(const AttnArgs& p, const Span& w, int r0, int col, const float* qs_s) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int r = r0 + 16 * rt + col;
+      qs[rt] = qs_s[r];
+      const int pos = w.pos0 + (w.r0 + min(r, w.cnt - 1)) / p.G;  // (rows past the last: as the last)
+      lim[rt] = min(pos + 1, w.k1);
+      low[rt] = p.window >= 0 ? (int)max((int64_t)pos - p.window + 1, (int64_t)0) : 0;
+      m[rt] = A8_NONE;
+      l[rt] = 0.f;
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t) o[rt][t] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+    in1 = min(w.pos0 + w.r0 / p.G + 1, w.k1);
+    in0 = p.window >= 0 ? w.pos0 + (w.r0 + w.cnt - 1) / p.G - p.window + 1 : 0;
+  }
+
+  // Weights of NG groups of 16 keys from their scores (lane (g4, col): keys 16 g + 4 g4 + i from
+  // key0): B operands of keys 32 kk + {4 g4 + i, 16 + 4 g4 + i}. The reference m lags behind the
+  // maximum by up to A8_LAG, so that most tiles need no exchange across lanes and no scaling: 16-bit
+  // weights reach 2^A8_LAG, and are as exact there as near 1. The sum takes them in 32 bits: in a
+  // block of small values a large weight may have no 16-bit form beside V's largest.
+  template <int NG>
+  __device__ __forceinline__ void weights(const v4i (&sc)[RT][NG], const float (&ks)[NG], const float (&lv)[NG],
+                                          const float (&iv)[NG], int key0, int keys_end, int g4,
+                                          v8h (&wb)[RT][NG / 2]) {
+    float x[RT][NG][4];
+    bool move = false;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const float ref = m[rt] == A8_NONE ? 0.f : m[rt];
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const float a = qs[rt] * ks[g], c = lv[g] - ref;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[rt][g][i] = fmaf((float)sc[rt][g][i], a, c);
+      }
+    }
+    if (!(key0 >= in0 && keys_end <= in1)) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = key0 + 16 * g + 4 * g4 + i;
+            if (key >= lim[rt] || key < low[rt]) x[rt][g][i] = -INFINITY;
+          }
+    }
+    float top[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      top[rt] = -INFINITY;
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top[rt] = fmaxf(top[rt], x[rt][g][i]);
+      move = move || top[rt] > (m[rt] == A8_NONE ? -INFINITY : A8_LAG);
+    }
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(move) != 0, 0)) {  // the maxima become the references
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const bool none = m[rt] == A8_NONE;
+        const float mt = max_xor32(max_xor16(top[rt]));
+        const float by = none ? (mt == -INFINITY ? 0.f : mt) : fmaxf(mt, 0.f);
+        m[rt] = none ? (mt == -INFINITY ? A8_NONE : mt) : m[rt] + by;
+        const float r = none ? 1.f : __builtin_amdgcn_exp2f(-by);
+        l[rt] *= r;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) o[rt][d] *= r;
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[rt][g][i] -= by;
+      }
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_exp2f(x[rt][g][i]);
+        l[rt] = fmaf((w[0] + w[1]) + (w[2] + w[3]), iv[g], l[rt]);
+        const h2 r[2] = {__builtin_convertvector((v2f{w[0], w[1]}), h2), __builtin_convertvector((v2f{w[2], w[3]}), h2)};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) wb[rt][g / 2][4 * (g & 1) + i] = r[i / 2][i & 1];
+      }
+  }
+};
+
 // ---------------------------------------------------------------------------
 // Few rows (a decode step, drafted tokens): each wave streams tiles of its own keys for all ROWS
 // rows, the 4 waves' states are joined in LDS. Bound by the bytes of K and V.
@@ -286,7 +394,7 @@ template <int D> __device__ __forceinline__ int v_swizzle(int key) {
   else return (key & 7) | ((key >> 4) & 1) << 3;
 }
 
-template <int DT, int D, int RT, bool ROT>
+template <int DT, int D, int RT>
 __global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const AttnArgs p) {
   constexpr int ROWS = 16 * RT, KT = stream_keys<D>(), NG = KT / 16, KS = D / 64, DTL = D / 16;
   constexpr int TPM = 64 / NG;  // tiles whose groups the lanes hold
@@ -303,35 +411,17 @@ __global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const
   const Item it = find_item<ROWS>(p, lane, blockIdx.x);
   if (!it.live) return;
   const Span w = item_span<ROWS>(p, it);
-  quant_rows<DT, D, ROWS, ROT>(p, w, it.kvh, q_s, qs_s);
+  quant_rows<DT, D, ROWS, A8_THREADS>(p, w, it.kvh, [&](int r) { return q_s + r * D; }, qs_s);
   __syncthreads();
 
   v4i qb[RT][KS];
-  float qs[RT];
-  int lim[RT], low[RT];  // row sees keys [low, lim)
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int r = 16 * rt + col;
+  for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-    for (int s = 0; s < KS; ++s) qb[rt][s] = *reinterpret_cast<const v4i*>(q_s + r * D + 64 * s + 16 * g4);
-    qs[rt] = qs_s[r];
-    const int pos = w.pos0 + (w.r0 + min(r, w.cnt - 1)) / p.G;
-    lim[rt] = min(pos + 1, w.k1);
-    low[rt] = p.window >= 0 ? (int)max((int64_t)pos - p.window + 1, (int64_t)0) : 0;
-  }
-  // keys that every row sees: [in0, in1)
-  const int in1 = min(w.pos0 + w.r0 / p.G + 1, w.k1);
-  const int in0 = p.window >= 0 ? w.pos0 + (w.r0 + w.cnt - 1) / p.G - p.window + 1 : 0;
-
-  float m[RT], l[RT];
-  v4f o[RT][DTL];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    m[rt] = A8_NONE;
-    l[rt] = 0.f;
-#pragma unroll
-    for (int t = 0; t < DTL; ++t) o[rt][t] = v4f{0.f, 0.f, 0.f, 0.f};
-  }
+    for (int s = 0; s < KS; ++s)
+      qb[rt][s] = *reinterpret_cast<const v4i*>(q_s + (16 * rt + col) * D + 64 * s + 16 * g4);
+  RowState<RT, D> st;
+  st.init(p, w, 0, col, qs_s);
 
   // places: K's lane in a group, the copies' lanes (16-byte chunk of the row that goes to the
   // lane's place) for even and odd groups, the transposed reads' rows
@@ -401,68 +491,43 @@ __global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const
     }
     // (past the last tile: groups without a block, whose copies read the pool's first rows)
     if (i0 + NG == 64) cur = nxt;
+    __builtin_amdgcn_sched_barrier(0);  // (K's registers are taken again, not others beside them)
     load(cur, (i0 + NG) & 63, next);
 
     v8h wb[RT][NG / 2];
-    const bool inside = key0 >= in0 && key0 + KT <= in1;
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      float t[NG][4];
-      float mt = -INFINITY;
-#pragma unroll
-      for (int g1 = 0; g1 < NG; ++g1) {
-        const float a = qs[rt] * gks[g1];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) t[g1][i] = fmaf((float)sc[rt][g1][i], a, glv[g1]);
-      }
-      if (!inside) {
-#pragma unroll
-        for (int g1 = 0; g1 < NG; ++g1)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = key0 + 16 * g1 + 4 * g4 + i;
-            if (key >= lim[rt] || key < low[rt]) t[g1][i] = -INFINITY;
-          }
-      }
-#pragma unroll
-      for (int g1 = 0; g1 < NG; ++g1)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mt = fmaxf(mt, t[g1][i]);
-      mt = max_xor32(max_xor16(mt));
-      const float mn = fmaxf(m[rt], mt);
-      if (__builtin_amdgcn_ballot_w64(mn > m[rt])) {
-        const float r = __builtin_amdgcn_exp2f(m[rt] - mn);
-        l[rt] *= r;
-#pragma unroll
-        for (int d = 0; d < DTL; ++d) o[rt][d] *= r;
-        m[rt] = mn;
-      }
-#pragma unroll
-      for (int g1 = 0; g1 < NG; ++g1)
-#pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-          const float a = __builtin_amdgcn_exp2f(t[g1][i] - mn), b = __builtin_amdgcn_exp2f(t[g1][i + 1] - mn);
-          l[rt] = fmaf(a, giv[g1], fmaf(b, giv[g1], l[rt]));
-          const h2 ab = __builtin_convertvector((v2f{a, b}), h2);
-          wb[rt][g1 / 2][4 * (g1 & 1) + i] = ab[0];
-          wb[rt][g1 / 2][4 * (g1 & 1) + i + 1] = ab[1];
-        }
-    }
+    st.weights(sc, gks, glv, giv, key0, key0 + KT, g4, wb);
 
     // V(j): copied before the NG * KS loads and NG * CPG copies of the next tile
     __builtin_amdgcn_s_waitcnt((((NG * (KS + CPG)) & 15) | ((NG * (KS + CPG)) >> 4) << 14) | 0x0F70);
     __builtin_amdgcn_sched_barrier(0);
     const int8_t* vt = ring + wave * KT * D + vt_off;
+    // operands 4 at a time, the next 4 being read under the products: more in flight spill, and so do
+    // the places of all, kept over the loop (the empty asm makes them the tile's own)
+    int swz = vt_swz;
+    asm volatile("" : "+v"(swz));
+    auto read = [&](int n) __attribute__((always_inline)) {
+      return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(
+          vt + 32 * (n / DTL) * D + ((16 * (n % DTL)) ^ swz)));
+    };
+    constexpr int N = NG / 2 * DTL;
+    v2i c[2][4];
 #pragma unroll
-    for (int kk = 0; kk < NG / 2; ++kk)
+    for (int i = 0; i < 4; ++i) c[0][i] = read(i);
 #pragma unroll
-      for (int d = 0; d < DTL; ++d) {
-        const v8h a = codes_f16(__builtin_amdgcn_ds_read_tr8_b64_v2i32(
-            (__attribute__((address_space(3))) v2i*)(vt + 32 * kk * D + ((16 * d) ^ vt_swz))));
+    for (int n0 = 0; n0 < N; n0 += 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n0 + 4 < N) c[(n0 / 4 + 1) & 1][i] = read(n0 + 4 + i);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const v8h a = codes_f16(c[n0 / 4 & 1][i]);
+        const int kk = (n0 + i) / DTL, d = (n0 + i) % DTL;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
-          o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wb[rt][kk], o[rt][d], 0, 0, 0);
+          st.o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wb[rt][kk], st.o[rt][d], 0, 0, 0);
       }
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
   for (int j = 0; j < ntiles;) {
     tile(j++, v0_s, v1_s);
@@ -480,23 +545,23 @@ __global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const
   wait_dma();  // (the copies past the last tile land in the ring that is written below)
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    l[rt] += __shfl_xor(l[rt], 16, 64);
-    l[rt] += __shfl_xor(l[rt], 32, 64);
+    st.l[rt] += __shfl_xor(st.l[rt], 16, 64);
+    st.l[rt] += __shfl_xor(st.l[rt], 32, 64);
     if (g4 == 0) {
-      m_s[wave][16 * rt + col] = m[rt];
-      l_s[wave][16 * rt + col] = l[rt];
+      m_s[wave][16 * rt + col] = st.m[rt];
+      l_s[wave][16 * rt + col] = st.l[rt];
     }
   }
   __syncthreads();
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int r = 16 * rt + col;
-    float mm = m[rt];
+    float mm = st.m[rt];
 #pragma unroll
     for (int x = 0; x < A8_WAVES; ++x) mm = fmaxf(mm, m_s[x][r]);
-    const float f = __builtin_amdgcn_exp2f(m[rt] - mm);
+    const float f = __builtin_amdgcn_exp2f(st.m[rt] - mm);
 #pragma unroll
-    for (int d = 0; d < DTL; ++d) *reinterpret_cast<v4f*>(o_place(wave, r, 4 * d + g4)) = o[rt][d] * f;
+    for (int d = 0; d < DTL; ++d) *reinterpret_cast<v4f*>(o_place(wave, r, 4 * d + g4)) = st.o[rt][d] * f;
   }
   __syncthreads();
   for (int i = tid; i < ROWS * D / 4; i += A8_THREADS) {
@@ -522,10 +587,191 @@ __global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const
       if (d == 0) p.ml[row] = make_float2(mm, den);
     }
   }
-  if (p.slots && it.split == 0 && tid == 0) {
-    p.pairs[2 * it.pair] = make_int4(blockIdx.x, it.splits, it.units * p.Hkv, it.kvh);
-    p.pairs[2 * it.pair + 1] = make_int4((int)w.row0, w.r0, w.cnt, 0);
+  if (p.slots && it.split == 0 && tid == 0) note_pair(p, w, it);
+}
+
+// ---------------------------------------------------------------------------
+// Many rows (prompts, drafts of wide groups): the NW waves of a workgroup have 16 RT rows each and
+// share every tile of keys through LDS, two tiles deep: K by direct copies, V turned into fp16
+// once on its way (10 instructions for 8 codes, which each wave for itself would spend again). The
+// products, the layouts and the softmax are the streaming kernel's; V is read transposed with
+// ds_read_b64_tr_b16. One barrier a tile; other workgroups of the CU run across it.
+// ---------------------------------------------------------------------------
+template <int D> constexpr int tile_keys() { return D == 256 ? 32 : 64; }
+template <int D> __device__ __forceinline__ int k_swizzle(int key) {  // 16-byte chunks, 16 keys apart
+  if constexpr (D == 64) return (key >> 2) & 3;
+  else if constexpr (D == 128) return (key >> 1) & 7;
+  else return key & 15;
+}
+template <int D> __device__ __forceinline__ int v16_swizzle(int key) {  // 32-byte chunks of fp16 rows
+  if constexpr (D == 64) return (key >> 1) & 3;
+  else return key & 7;
+}
+
+template <int DT, int D, int RT, int NW>
+__global__ void __launch_bounds__(64 * NW, 2) attn_block8_tile_kernel(const AttnArgs p) {
+  constexpr int THREADS = 64 * NW, ROWS = 16 * RT * NW, KT = tile_keys<D>(), NG = KT / 16;
+  constexpr int KS = D / 64, DTL = D / 16, CPR = D / 16;
+  constexpr int TPM = 64 / NG;
+  constexpr int COPIES = KT * D / (16 * THREADS);  // of 16 bytes a thread, for K and for V
+  static_assert(COPIES >= 1 && KT * D % (16 * THREADS) == 0, "a tile in whole copies");
+  __shared__ __attribute__((aligned(16))) int8_t k0_s[KT * D], k1_s[KT * D];
+  __shared__ __attribute__((aligned(16))) uint16_t v0_s[KT * D], v1_s[KT * D];
+  __shared__ float qs_s[ROWS];
+  static_assert(ROWS <= 4 * KT, "the rows' codes fit where V will be");
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, g4 = lane >> 4;
+  typedef short v4s __attribute__((ext_vector_type(4)));
+  typedef short v8s __attribute__((ext_vector_type(8)));
+
+  zero_tail(p, D);
+  const Item it = find_item<ROWS>(p, lane, blockIdx.x);
+  if (!it.live) return;
+  const Span w = item_span<ROWS>(p, it);
+
+  // a thread's copies: 16-byte chunk `ch` of key `key` of the tile (64 threads: one group of 16 keys)
+  int k_src[COPIES], v_src[COPIES], v_dst[COPIES];
+#pragma unroll
+  for (int c = 0; c < COPIES; ++c) {
+    const int ci = (c * NW + wave) * 64 + lane, key = ci / CPR, ch = ci % CPR;
+    k_src[c] = key % 16 * D + 16 * (ch ^ k_swizzle<D>(key % 16));
+    v_src[c] = key % 16 * D + 16 * ch;
+    v_dst[c] = key * D + 16 * (ch ^ v16_swizzle<D>(key));
   }
+  const int ntiles = w.k0 < w.k1 ? (w.k1 - w.k0 + KT - 1) / KT : 0;
+  auto groups = [&](int tile) {
+    return key_group<D>(p, it.b, it.kvh, w.k0 + (tile + lane / NG) * KT + 16 * (lane % NG), w.k1);
+  };
+  Group cur = groups(0), nxt = cur;
+  auto base = [&](int i) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)cur.at, i);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(cur.at >> 32), i);
+    return (int64_t)(((uint64_t)hi << 32) | lo);
+  };
+  uint4 vraw[COPIES];
+  auto load = [&](int i0, int8_t* kto) {
+#pragma unroll
+    for (int c = 0; c < COPIES; ++c) {
+      const int64_t at = base(i0 + (c * NW + wave) * 64 / CPR / 16);
+      vraw[c] = *reinterpret_cast<const uint4*>(p.v + at + v_src[c]);
+      buf16_to_lds(make_rsrc(p.k + at, 16 * D), kto + (c * NW + wave) * 1024, k_src[c], 0);
+    }
+  };
+  auto store_v = [&](uint16_t* vto) {
+#pragma unroll
+    for (int c = 0; c < COPIES; ++c) {
+      const v8h a = codes_f16(v2i{(int)vraw[c].x, (int)vraw[c].y}), b = codes_f16(v2i{(int)vraw[c].z, (int)vraw[c].w});
+      *reinterpret_cast<v8h*>(vto + v_dst[c]) = a;
+      *reinterpret_cast<v8h*>(vto + v_dst[c] + 8) = b;
+    }
+  };
+  if (ntiles) load(0, k0_s);
+
+  constexpr int FIT = 2 * KT;  // rows of codes in the first array of V
+  auto q_place = [&](int r) {
+    return r < FIT ? reinterpret_cast<int8_t*>(v0_s) + r * D : reinterpret_cast<int8_t*>(v1_s) + (r - FIT) * D;
+  };
+  quant_rows<DT, D, ROWS, THREADS>(p, w, it.kvh, q_place, qs_s);
+  __syncthreads();
+  v4i qb[RT][KS];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+      qb[rt][s] = *reinterpret_cast<const v4i*>(q_place(16 * (RT * wave + rt) + col) + 64 * s + 16 * g4);
+  RowState<RT, D> st;
+  st.init(p, w, 16 * RT * wave, col, qs_s);
+  __syncthreads();
+  if (ntiles) store_v(v0_s);
+  wait_dma();
+  __syncthreads();
+
+  const int k_swz = k_swizzle<D>(col);
+  const int vkey = 4 * g4 + (col >> 2);
+  const int vt_off = vkey * D + 4 * (col & 3);                           // (fp16 elements)
+  const int vt_swz = 16 * v16_swizzle<D>(vkey);
+  static_assert(D != 64 || tile_keys<D>() == 64, "");
+
+  auto tile = [&](int j, const int8_t* kt, const uint16_t* vt, int8_t* knext, uint16_t* vnext)
+      __attribute__((always_inline)) {
+    const int i0 = j % TPM * NG;
+    const int key0 = w.k0 + j * KT;
+    if (i0 == 0) nxt = groups(j + TPM);
+    float gks[NG], glv[NG], giv[NG];
+#pragma unroll
+    for (int g1 = 0; g1 < NG; ++g1) {
+      gks[g1] = lane_value(cur.ks, i0 + g1);
+      glv[g1] = lane_value(cur.lv, i0 + g1);
+      giv[g1] = lane_value(cur.iv, i0 + g1);
+    }
+    if (i0 + NG == 64) cur = nxt;
+    load((i0 + NG) & 63, knext);  // (past the last tile: the pool's first rows)
+
+    v4i sc[RT][NG];
+#pragma unroll
+    for (int g1 = 0; g1 < NG; ++g1) {
+      v4i ka[KS];
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+        ka[s] = *reinterpret_cast<const v4i*>(kt + (16 * g1 + col) * D + 16 * ((4 * s + g4) ^ k_swz));
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        v4i acc = {0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(ka[s], qb[rt][s], acc, 0, 0, 0);
+        sc[rt][g1] = acc;
+      }
+    }
+    v8h wb[RT][NG / 2];
+    st.weights(sc, gks, glv, giv, key0, key0 + KT, g4, wb);
+
+    int swz = vt_swz;
+    asm volatile("" : "+v"(swz));  // (the places are the tile's own: kept over the loop they spill)
+#pragma unroll
+    for (int kk = 0; kk < NG / 2; ++kk)
+#pragma unroll
+      for (int d = 0; d < DTL; ++d) {
+        const uint16_t* a0 = vt + vt_off + 32 * kk * D + ((16 * d) ^ swz);
+        const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(a0));
+        const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(a0 + 16 * D));
+        const v8h a = __builtin_bit_cast(v8h, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+          st.o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wb[rt][kk], st.o[rt][d], 0, 0, 0);
+      }
+    store_v(vnext);
+    wait_dma();
+    __syncthreads();
+  };
+  for (int j = 0; j < ntiles;) {
+    tile(j++, k0_s, v0_s, k1_s, v1_s);
+    if (j >= ntiles) break;
+    tile(j++, k1_s, v1_s, k0_s, v0_s);
+  }
+
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    float l = st.l[rt];
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    const int r = 16 * (RT * wave + rt) + col;
+    if (r >= w.cnt) continue;
+    if (it.splits == 1) {
+      const float inv = l > 0.f ? 1.f / l : 0.f;
+      uint16_t* to = static_cast<uint16_t*>(p.out) + row_at(p, w, it.kvh, r, D) + 4 * g4;
+#pragma unroll
+      for (int d = 0; d < DTL; ++d) {
+        const v4f a = st.o[rt][d] * inv;
+        *reinterpret_cast<uint2*>(to + 16 * d) = make_uint2(pack2<DT>(a[0], a[1]), pack2<DT>(a[2], a[3]));
+      }
+    } else {
+      const int64_t row = (int64_t)blockIdx.x * ROWS + r;
+#pragma unroll
+      for (int d = 0; d < DTL; ++d) *reinterpret_cast<v4f*>(p.part + row * D + 16 * d + 4 * g4) = st.o[rt][d];
+      if (g4 == 0) p.ml[row] = make_float2(st.m[rt], l);
+    }
+  }
+  if (p.slots && it.split == 0 && tid == 0) note_pair(p, w, it);
 }
 
 // ---------------------------------------------------------------------------
@@ -568,9 +814,10 @@ __global__ void __launch_bounds__(64) attn_block8_join_kernel(const AttnArgs p) 
   for (int c = 0; c < C; ++c) st_out<DT>(p.out, to + c, o[c] * inv);
 }
 
-// How a call runs: rows of a unit, a bound on its pairs, whether keys are split over workgroups,
-// and the bytes that that takes.
+// How a call runs: the kernel and its rows of a unit, a bound on the pairs, whether keys are split
+// over workgroups, and the bytes that that takes.
 struct AttnPlan {
+  int rt, nw;  // nw 0: streaming
   int rows;
   int64_t pairs;
   int slots;
@@ -580,12 +827,15 @@ struct AttnPlan {
 
 AttnPlan attn_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D) {
   AttnPlan a{};
+  a.rt = 1;
   if (T == 0 || B == 0 || Hq == 0) return a;
-  const int64_t G = Hq / Hkv;
-  // rows of a sequence on average: 32-row units read K and V half as often where 16 do not hold them
-  a.rows = D < 256 && T * G > 16 * B ? 32 : 16;
-  a.pairs = Hkv * (T * G / a.rows + B);
-  const int64_t slots = 2 * (int64_t)cu_count();  // two workgroups a CU (LDS)
+  const int64_t rows = (T * (Hq / Hkv) + B - 1) / B;  // of a sequence and KV head on average
+  if (rows <= 16) a.rt = 1;
+  else if (rows <= 32 && D < 256) a.rt = 2;
+  else a.nw = 4, a.rt = rows <= 64 ? 1 : 2;
+  a.rows = 16 * a.rt * (a.nw ? a.nw : 1);
+  a.pairs = Hkv * (T * (Hq / Hkv) / a.rows + B);
+  const int64_t slots = 2 * (int64_t)cu_count();  // two workgroups a CU
   a.slots = a.pairs < slots ? (int)slots : 0;
   a.grid = a.slots ? slots : a.pairs;
   if (a.slots) a.bytes = (size_t)a.grid * a.rows * (D + 2) * 4 + (size_t)a.pairs * 32 + 16;
@@ -638,6 +888,7 @@ extern "C" int sl8_attn_paged_block8(const void* q, int dtype, int rotate, float
   p.out = out;
   p.Hq = (int)Hq; p.Hkv = (int)Hkv; p.G = (int)(Hq / Hkv);
   p.q_mul = q_scale_mul;
+  p.rotate = rotate != 0;
   p.window = window_left < 0 ? -1 : (int)(window_left < (1 << 30) ? window_left : (1 << 30));
   p.slots = plan.slots;
   if (num_blocks == 0) p.s.maxb = 0;  // nothing to read: no key is there
@@ -650,18 +901,23 @@ extern "C" int sl8_attn_paged_block8(const void* q, int dtype, int rotate, float
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const unsigned grid = (unsigned)(plan.grid > 0 ? plan.grid : 1);
   using std::integral_constant;
-  auto go = [&](auto dt, auto d, auto rt) {
-    constexpr int DT = decltype(dt)::value, DD = decltype(d)::value, RT = decltype(rt)::value;
-    if (rotate) attn_block8_stream_kernel<DT, DD, RT, true><<<grid, A8_THREADS, 0, st>>>(p);
-    else attn_block8_stream_kernel<DT, DD, RT, false><<<grid, A8_THREADS, 0, st>>>(p);
-    if (plan.slots)
-      attn_block8_join_kernel<DT, DD, 16 * RT><<<dim3((unsigned)plan.pairs, 16 * RT), 64, 0, st>>>(p);
+  auto go = [&](auto dt, auto d, auto rt, auto nw) {
+    constexpr int DT = decltype(dt)::value, DD = decltype(d)::value, RT = decltype(rt)::value, NW = decltype(nw)::value;
+    constexpr int ROWS = 16 * RT * (NW ? NW : 1);
+    if constexpr (NW) attn_block8_tile_kernel<DT, DD, RT, NW><<<grid, 64 * NW, 0, st>>>(p);
+    else attn_block8_stream_kernel<DT, DD, RT><<<grid, A8_THREADS, 0, st>>>(p);
+    if (plan.slots) attn_block8_join_kernel<DT, DD, ROWS><<<dim3((unsigned)plan.pairs, ROWS), 64, 0, st>>>(p);
   };
   auto by_rows = [&](auto dt, auto d) {
+    const integral_constant<int, 0> stream;
+    const integral_constant<int, 1> one;
+    const integral_constant<int, 2> two;
+    const integral_constant<int, 4> waves;
+    if (plan.nw) return plan.rt == 1 ? go(dt, d, one, waves) : go(dt, d, two, waves);
     if constexpr (decltype(d)::value < 256) {
-      if (plan.rows == 32) return go(dt, d, integral_constant<int, 2>{});
+      if (plan.rt == 2) return go(dt, d, two, stream);
     }
-    go(dt, d, integral_constant<int, 1>{});
+    go(dt, d, one, stream);
   };
   auto by_d = [&](auto dt) {
     if (D == 64) by_rows(dt, integral_constant<int, 64>{});
