@@ -425,8 +425,10 @@ int sl8_kv_append_block8(const void* k_new, const void* v_new, const void* q, in
  * with one scale times q_scale_mul (softmax_scale * log2 e) -> out [T,Hq,D] of q's type. Row i of a
  * sequence's n sees keys <= context_lens - n + i, and with window_left >= 0 keys > that -
  * window_left; zeros where it sees none and in rows behind the last sequence. All 16-byte aligned.
- * workspace: sl8_attn_paged_block8_workspace() bytes (current device), uninitialised. */
-size_t sl8_attn_paged_block8_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D);
+ * workspace: sl8_attn_paged_block8_workspace() bytes (current device; max_context_len =
+ * max_blocks_per_seq * block_size), uninitialised. */
+size_t sl8_attn_paged_block8_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                       int64_t max_context_len);
 int sl8_attn_paged_block8(const void* q, int dtype, int rotate, float q_scale_mul,
                           const int8_t* k_cache, const float* k_scale, const int8_t* v_cache,
                           const float* v_scale, const int32_t* cu_lens, const int32_t* context_lens,

@@ -961,7 +961,7 @@ def attn_paged_block8(q, q_mul, rotate, k_cache, k_scale, v_cache, v_scale, bloc
     out = q.new_empty((T, Hq, D))
     if T and Hq:
         with on_device(q):
-            ws_bytes = _lib.load().sl8_attn_paged_block8_workspace(T, B, Hq, Hkv, D)
+            ws_bytes = _lib.load().sl8_attn_paged_block8_workspace(T, B, Hq, Hkv, D, maxb * bs)
             ws = q.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
             call("sl8_attn_paged_block8", q.data_ptr(), dtype_code(q.dtype), int(bool(rotate)),
                  float(q_mul), k_cache.data_ptr(), k_scale.data_ptr(), v_cache.data_ptr(),

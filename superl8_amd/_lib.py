@@ -79,7 +79,7 @@ SIGNATURES = {
                  + [_I64] * 6 + [_P]),
     "sl8_kv_append_block8": (_I, [_P, _P, _P, _I, _P, _P, _P, _P, _I, _P, _I64, _P, _I, _I, _I]
                              + [_P] * 8 + [_I64] * 9 + [_P]),
-    "sl8_attn_paged_block8_workspace": (_SZ, [_I64] * 5),
+    "sl8_attn_paged_block8_workspace": (_SZ, [_I64] * 6),
     "sl8_attn_paged_block8": (_I, [_P, _I, _I, _F] + [_P] * 8 + [_I64] * 9 + [_P, _SZ, _P]),
     "sl8_gemm_decode_q4k": (_I, [_P, _P, _P, _P, _I, _I64, _I64, _I64, _P]),
     "sl8_gemm_decode_q4k_xblock": (_I, [_P, _P, _P, _P, _I, _I64, _I64, _I64, _P]),

@@ -14,6 +14,7 @@
 //
 // Rows of a sequence and KV head are (token, query head of the group), G = Hq / Hkv to a token; a
 // unit is ROWS of them that share every byte of K and V.
+#include <atomic>
 #include <climits>
 
 #include "attn_common.hpp"
@@ -26,6 +27,7 @@ namespace {
 constexpr int A8_THREADS = 256, A8_WAVES = 4;
 constexpr int A8_TILE = 64;       // keys: what splits and units' first keys are multiples of
 constexpr int A8_MIN_TILES = 4;   // least keys of a split: a tile for each wave
+constexpr int A8_WHOLE_KEYS = 1024; // contexts up to here are not split
 constexpr float A8_NONE = -1e30f; // reference of nothing
 constexpr float A8_LAG = 12.f;    // log2 of the largest weight (fp16 holds 2^15)
 
@@ -44,7 +46,8 @@ struct AttnArgs {
   float q_mul;
   int window;  // below 0: none
   bool rotate;
-  int slots;   // workgroups to split the keys over, 0: no splits
+  int slots;      // workgroups to split the keys over, 0: no splits
+  int max_pairs;  // that the workspace has places for
   // splits only: partial sums [grid][ROWS][D], (m, l) [grid][ROWS], what to join of each pair
   float* part;
   float2* ml;
@@ -63,33 +66,59 @@ struct AttnArgs {
 // the units that read a head's keys meet in its L2.
 // ---------------------------------------------------------------------------
 struct SeqWork {
+  int row0, n, len;  // first row, rows, context
   int units, tiles;
 };
 
 struct Item {
-  int b, unit, kvh, split, splits, units, pair;
+  int b, row0, n, len;
+  int unit, kvh, split, splits, units, pair;
+  int64_t end;  // rows of all sequences
   bool live;
 };
 
 template <int ROWS>
 __device__ __forceinline__ SeqWork seq_work(const AttnArgs& p, int b) {
-  SeqWork w{0, 1};
+  SeqWork w{0, 0, 0, 0, 1};
   if (b < p.s.B) {
-    const int n = max(0, (int)(p.s.row(b + 1) - p.s.row(b)));
-    const int cap = p.s.maxb * p.s.bs;
-    int span = min(max(p.s.lens[b], 0), cap);
+    w.row0 = (int)p.s.row(b);
+    w.n = max(0, (int)p.s.row(b + 1) - w.row0);
+    w.len = p.s.lens[b];
+    int span = min(max(w.len, 0), p.s.maxb * p.s.bs);
     if (p.window >= 0) span = (int)min((int64_t)span, (int64_t)p.window + ROWS / p.G + A8_TILE);
-    w.units = (n * p.G + ROWS - 1) / ROWS;
+    w.units = (w.n * p.G + ROWS - 1) / ROWS;
     w.tiles = max(1, (span + A8_TILE - 1) / A8_TILE);
   }
   return w;
+}
+
+// Splits of a sequence: near tiles / L, rounded up (a unit's keys are cut in that many equal parts,
+// so a rounding of the quotient leaves nothing out).
+__device__ __forceinline__ int splits_of(int tiles, float over_l) {
+  return max(1, (int)ceilf((float)tiles * over_l));
+}
+
+// Inclusive sum over the wave: DPP row shifts, then the rows' last lanes.
+__device__ __forceinline__ int wave_scan(int x) {
+  auto add = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
+    x += __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
+  };
+  using std::integral_constant;
+  const integral_constant<int, 0xF> all;
+  add(integral_constant<int, 0x111>{}, all);  // row_shr:1
+  add(integral_constant<int, 0x112>{}, all);
+  add(integral_constant<int, 0x114>{}, all);
+  add(integral_constant<int, 0x118>{}, all);
+  add(integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{});  // row_bcast:15
+  add(integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{});  // row_bcast:31
+  return x;
 }
 
 template <int ROWS>
 __device__ __forceinline__ Item find_item(const AttnArgs& p, int lane, int id) {
   const SeqWork mine = seq_work<ROWS>(p, lane);
   auto work = [&](int b0) { return b0 == 0 ? mine : seq_work<ROWS>(p, b0 + lane); };
-  int L = INT_MAX / 2;
+  float over_l = 0.f;
   if (p.slots) {
     int most = 1, pairs = 0;
     float all = 0.f;
@@ -99,80 +128,91 @@ __device__ __forceinline__ Item find_item(const AttnArgs& p, int lane, int id) {
       pairs += w.units;
       all += (float)w.units * (float)w.tiles;
     }
-    most = (int)lane_group_reduce<64>((uint32_t)most, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
-    pairs = lane_group_sum<64>(pairs) * p.Hkv;
+    most = __builtin_amdgcn_readfirstlane(
+        (int)lane_group_reduce<64>((uint32_t)most, [](uint32_t a, uint32_t b) { return a > b ? a : b; }));
+    pairs = __builtin_amdgcn_readfirstlane(lane_group_sum<64>(pairs)) * p.Hkv;
     all = wave_sum(all) * (float)p.Hkv;
-    // the least L with items(L) <= slots
-    int lo = max(A8_MIN_TILES, (int)(all / (float)p.slots * 0.999f)), hi = most;
-    if (pairs < p.slots) hi = min(hi, (int)(all / (float)(p.slots - pairs)) + 2);
+    // the least L with items(L) <= slots, four candidates at once
+    int lo = __builtin_amdgcn_readfirstlane(max(A8_MIN_TILES, (int)(all / (float)p.slots * 0.999f))), hi = most;
+    if (pairs < p.slots) hi = min(hi, __builtin_amdgcn_readfirstlane((int)(all / (float)(p.slots - pairs))) + 2);
     while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      int n = 0;
+      const int step = (hi - lo + 4) / 5 > 1 ? (hi - lo + 4) / 5 : 1;
+      int n[4] = {0, 0, 0, 0};
+      float r[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) r[k] = 1.f / (float)(lo + k * step);
       for (int b0 = 0; b0 < p.s.B; b0 += 64) {
         const SeqWork w = work(b0);
-        n += w.units * ((w.tiles + mid - 1) / mid);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) n[k] += w.units * splits_of(w.tiles, r[k]);
       }
-      n = __builtin_amdgcn_readfirstlane(lane_group_sum<64>(n)) * p.Hkv;
-      if (n <= p.slots) hi = mid;
-      else lo = mid + 1;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) n[k] = __builtin_amdgcn_readfirstlane(lane_group_sum<64>(n[k])) * p.Hkv;
+      int fit = 4;
+#pragma unroll
+      for (int k = 3; k >= 0; --k)
+        if (n[k] <= p.slots) fit = k;
+      if (fit < 4) hi = min(hi, lo + fit * step);
+      if (fit) lo = min(hi, lo + (fit < 4 ? fit - 1 : 3) * step + 1);
     }
-    L = max(lo, 1);
+    over_l = 1.f / (float)max(lo, 1);
   }
   Item it{};
   int items = 0, pairs = 0;
   for (int b0 = 0; b0 < p.s.B; b0 += 64) {
     const SeqWork w = work(b0);
-    const int s = (w.tiles + L - 1) / L;
+    const int s = splits_of(w.tiles, over_l);
     const int np = w.units * p.Hkv, ni = np * s;
-    int ii = ni, pp = np;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int x = __shfl_up(ii, o, 64), y = __shfl_up(pp, o, 64);
-      if (lane >= o) ii += x, pp += y;
-    }
+    const int ii = wave_scan(ni), pp = wave_scan(np);
     const uint64_t past = __builtin_amdgcn_ballot_w64(items + ii > id);
     if (past && !it.live) {
       const int at = __builtin_ctzll(past);
+      auto of = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
       it.live = true;
       it.b = b0 + at;
-      it.splits = __builtin_amdgcn_readlane(s, at);
-      it.units = __builtin_amdgcn_readlane(w.units, at);
-      const int r = id - (items + __builtin_amdgcn_readlane(ii - ni, at));
+      it.row0 = of(w.row0);
+      it.n = of(w.n);
+      it.len = of(w.len);
+      it.splits = of(s);
+      it.units = of(w.units);
+      const int r = id - (items + of(ii - ni));
       it.kvh = r % p.Hkv;
       it.unit = it.units - 1 - r / p.Hkv % it.units;  // (those that see the most keys first)
       it.split = r / p.Hkv / it.units;
-      it.pair = pairs + __builtin_amdgcn_readlane(pp - np, at) + it.unit * p.Hkv + it.kvh;
-      if (id) break;  // (the first workgroup counts all pairs)
+      it.pair = pairs + of(pp - np) + it.unit * p.Hkv + it.kvh;
+      if (id && p.s.B > 64) break;  // (the first workgroup counts all pairs)
     }
     items += __builtin_amdgcn_readlane(ii, 63);
     pairs += __builtin_amdgcn_readlane(pp, 63);
   }
-  if (p.slots && id == 0 && threadIdx.x == 0) *p.count = pairs;
+  // (more pairs than places: the offsets fall somewhere, against the contract)
+  if (p.slots && id == 0 && threadIdx.x == 0) *p.count = pairs <= p.max_pairs ? pairs : 0;
+  it.end = p.s.T;
+  if (p.s.cu) it.end = p.s.B >= 1 && p.s.B <= 64 ? __builtin_amdgcn_readlane(mine.row0 + mine.n, p.s.B - 1) : p.s.row(p.s.B);
   return it;
 }
 
 // The rows and keys of an item.
 struct Span {
-  int64_t row0;   // first row (token) of the sequence
-  int r0, cnt;    // the unit's first of its rows, and how many
-  int pos0;       // position of the sequence's first new token
-  int hi, cap;    // keys that there are, and that the table holds
-  int k0, k1;     // keys of the item: from a multiple of a tile
+  int64_t row0;  // first row (token) of the sequence
+  int r0, cnt;   // the unit's first of its rows, and how many
+  int pos0;      // position of the sequence's first new token
+  int k0, k1;    // keys of the item: from a multiple of a tile
 };
 
 template <int ROWS>
 __device__ __forceinline__ Span item_span(const AttnArgs& p, const Item& it) {
   Span w;
-  w.row0 = p.s.row(it.b);
-  const int n = (int)(p.s.row(it.b + 1) - w.row0);
-  const int64_t len = p.s.lens[it.b];
+  w.row0 = it.row0;
+  const int n = it.n;
+  const int64_t len = it.len;
   w.r0 = it.unit * ROWS;
   w.cnt = min(ROWS, n * p.G - w.r0);
   // (contexts below the new tokens: positions below 0, which see nothing)
   const int64_t pos0 = max(len - n, (int64_t)-(1 << 28));
   w.pos0 = (int)min(pos0, (int64_t)INT_MAX - (1 << 29));
-  w.hi = (int)max((int64_t)0, min(len, (int64_t)p.s.maxb * p.s.bs));
-  const int last = min(w.hi, w.pos0 + (w.r0 + w.cnt - 1) / p.G + 1);
+  const int keys = (int)max((int64_t)0, min(len, (int64_t)p.s.maxb * p.s.bs));
+  const int last = min(keys, w.pos0 + (w.r0 + w.cnt - 1) / p.G + 1);
   int first = 0;
   if (p.window >= 0) {
     first = (int)max((int64_t)0, (int64_t)w.pos0 + w.r0 / p.G - p.window + 1);
@@ -187,16 +227,17 @@ __device__ __forceinline__ Span item_span(const AttnArgs& p, const Item& it) {
 
 // What the joining kernel needs of a pair (unit, KV head); from its first item.
 __device__ __forceinline__ void note_pair(const AttnArgs& p, const Span& w, const Item& it) {
+  if (it.pair >= p.max_pairs) return;
   p.pairs[2 * it.pair] = make_int4(blockIdx.x, it.splits, it.units * p.Hkv, it.kvh);
   p.pairs[2 * it.pair + 1] = make_int4((int)w.row0, w.r0, w.cnt, 0);
 }
 
-// Rows behind the last sequence are zeros.
-__device__ __forceinline__ void zero_tail(const AttnArgs& p, int D) {
-  if (!p.s.cu) return;
+// Rows behind the last sequence (from `end`) are zeros.
+__device__ __forceinline__ void zero_tail(const AttnArgs& p, int64_t end, int D) {
+  if (end >= p.s.T) return;
   const int64_t chunks = (int64_t)p.Hq * D / 8;
   uint4* o = static_cast<uint4*>(p.out);
-  for (int64_t t = p.s.row(p.s.B) + blockIdx.x; t < p.s.T; t += gridDim.x)
+  for (int64_t t = end + blockIdx.x; t < p.s.T; t += gridDim.x)
     for (int64_t i = threadIdx.x; i < chunks; i += blockDim.x) o[t * chunks + i] = make_uint4(0, 0, 0, 0);
 }
 
@@ -212,7 +253,7 @@ template <int DT, int D, int ROWS, int THREADS, typename F>
 __device__ __forceinline__ void quant_rows(const AttnArgs& p, const Span& w, int kvh, F place, float* qs_s) {
   constexpr int LPR = row_lanes(D), RPB = THREADS / LPR;
   const int lane = threadIdx.x % LPR;
-#pragma unroll
+#pragma unroll 1
   for (int r1 = 0; r1 < ROWS; r1 += RPB) {
     const int r = r1 + threadIdx.x / LPR;
     if (ROWS % RPB && r >= ROWS) break;
@@ -407,22 +448,10 @@ __global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, g4 = lane >> 4;
 
-  zero_tail(p, D);
   const Item it = find_item<ROWS>(p, lane, blockIdx.x);
+  zero_tail(p, it.end, D);
   if (!it.live) return;
   const Span w = item_span<ROWS>(p, it);
-  quant_rows<DT, D, ROWS, A8_THREADS>(p, w, it.kvh, [&](int r) { return q_s + r * D; }, qs_s);
-  __syncthreads();
-
-  v4i qb[RT][KS];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-      qb[rt][s] = *reinterpret_cast<const v4i*>(q_s + (16 * rt + col) * D + 64 * s + 16 * g4);
-  RowState<RT, D> st;
-  st.init(p, w, 0, col, qs_s);
-
   // places: K's lane in a group, the copies' lanes (16-byte chunk of the row that goes to the
   // lane's place) for even and odd groups, the transposed reads' rows
   const int k_off = col * D + 16 * g4;
@@ -467,6 +496,18 @@ __global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const
     }
   };
   if (ntiles) load(cur, 0, v0_s);
+
+  quant_rows<DT, D, ROWS, A8_THREADS>(p, w, it.kvh, [&](int r) { return q_s + r * D; }, qs_s);
+  __syncthreads();
+
+  v4i qb[RT][KS];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+      qb[rt][s] = *reinterpret_cast<const v4i*>(q_s + (16 * rt + col) * D + 64 * s + 16 * g4);
+  RowState<RT, D> st;
+  st.init(p, w, 0, col, qs_s);
 
   auto tile = [&](int j, const int8_t* ring, int8_t* next) __attribute__((always_inline)) {
     const int i0 = j % TPM * NG;  // the tile's groups are in lanes i0 .. i0 + NG - 1 of cur
@@ -624,8 +665,8 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_block8_tile_kernel(const Attn
   typedef short v4s __attribute__((ext_vector_type(4)));
   typedef short v8s __attribute__((ext_vector_type(8)));
 
-  zero_tail(p, D);
   const Item it = find_item<ROWS>(p, lane, blockIdx.x);
+  zero_tail(p, it.end, D);
   if (!it.live) return;
   const Span w = item_span<ROWS>(p, it);
 
@@ -776,35 +817,49 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_block8_tile_kernel(const Attn
 
 // ---------------------------------------------------------------------------
 // The splits of a pair (unit, KV head) joined: a wave per row, D / 64 channels a lane; sums in
-// the order of the splits.
+// the order of the splits. Bound by the chain of loads: the first partial sums are read beside the
+// maxima that weigh them.
 // ---------------------------------------------------------------------------
+constexpr int JOIN_ROWS = 4, JOIN_AHEAD = 8;
 template <int DT, int D, int ROWS>
-__global__ void __launch_bounds__(64) attn_block8_join_kernel(const AttnArgs p) {
+__global__ void __launch_bounds__(64 * JOIN_ROWS) attn_block8_join_kernel(const AttnArgs p) {
   constexpr int C = D / 64;
-  const int lane = threadIdx.x, r = blockIdx.y;
-  if ((int)blockIdx.x >= *p.count) return;
+  typedef float vc __attribute__((ext_vector_type(C)));
+  const int lane = threadIdx.x & 63, r = blockIdx.y * JOIN_ROWS + (threadIdx.x >> 6);
   const int4 a = p.pairs[2 * blockIdx.x], u = p.pairs[2 * blockIdx.x + 1];
-  if (a.y == 1 || r >= u.z) return;
+  if ((int)blockIdx.x >= *p.count || a.y == 1 || r >= u.z) return;
   const int64_t row0 = (int64_t)a.x * ROWS + r, step = (int64_t)a.z * ROWS;
+  auto part = [&](int s) {
+    if constexpr (C == 1) return vc{p.part[(row0 + s * step) * D + lane]};
+    else return *reinterpret_cast<const vc*>(p.part + (row0 + s * step) * D + C * lane);
+  };
+  vc x[JOIN_AHEAD];
+#pragma unroll
+  for (int s = 0; s < JOIN_AHEAD; ++s) x[s] = part(min(s, a.y - 1));
   float mm = A8_NONE;
   for (int s = lane; s < a.y; s += 64) mm = fmaxf(mm, p.ml[row0 + s * step].x);
   mm = wave_max(mm);
-  float den = 0.f, o[C] = {};
+  float den = 0.f;
+  vc o = {};
   for (int s0 = 0; s0 < a.y; s0 += 64) {
     float f = 0.f, l = 0.f;
     if (s0 + lane < a.y) {
-      const float2 x = p.ml[row0 + (s0 + lane) * step];
-      f = __builtin_amdgcn_exp2f(x.x - mm);
-      l = x.y * f;
+      const float2 y = p.ml[row0 + (s0 + lane) * step];
+      f = __builtin_amdgcn_exp2f(y.x - mm);
+      l = y.y * f;
     }
     den += wave_sum(l);
     const int n = min(64, a.y - s0);
-#pragma unroll 8
-    for (int s = 0; s < n; ++s) {
-      const float* x = p.part + (row0 + (s0 + s) * step) * D + C * lane;
-      const float fs = lane_value(f, s);
+    for (int s = 0; s < n; s += JOIN_AHEAD) {
+      vc y[JOIN_AHEAD];
 #pragma unroll
-      for (int c = 0; c < C; ++c) o[c] = fmaf(x[c], fs, o[c]);
+      for (int k = 0; k < JOIN_AHEAD; ++k)
+        if (s0 + s + JOIN_AHEAD < a.y) y[k] = part(min(s0 + s + JOIN_AHEAD + k, a.y - 1));
+#pragma unroll
+      for (int k = 0; k < JOIN_AHEAD; ++k)
+        if (s + k < n) o += x[k] * lane_value(f, s + k);
+#pragma unroll
+      for (int k = 0; k < JOIN_AHEAD; ++k) x[k] = y[k];
     }
   }
   const float inv = den > 0.f ? 1.f / den : 0.f;
@@ -814,31 +869,77 @@ __global__ void __launch_bounds__(64) attn_block8_join_kernel(const AttnArgs p) 
   for (int c = 0; c < C; ++c) st_out<DT>(p.out, to + c, o[c] * inv);
 }
 
-// How a call runs: the kernel and its rows of a unit, a bound on the pairs, whether keys are split
-// over workgroups, and the bytes that that takes.
+// The kernels by head dim and rows: NW 0 streams.
+template <int D_, int RT_, int NW_> struct Shape {
+  static constexpr int D = D_, RT = RT_, NW = NW_, ROWS = 16 * RT_ * (NW_ ? NW_ : 1);
+  static constexpr int THREADS = NW_ ? 64 * NW_ : A8_THREADS;
+  template <int DT> static auto kernel() {
+    if constexpr (NW_) return attn_block8_tile_kernel<DT, D, RT, NW>;
+    else return attn_block8_stream_kernel<DT, D, RT>;
+  }
+  // workgroups resident on one CU (asked once)
+  static int wgs_per_cu() {
+    static std::atomic<int> n{0};
+    int v = n.load(std::memory_order_relaxed);
+    if (v == 0) {
+      if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&v, reinterpret_cast<const void*>(kernel<0>()), THREADS, 0) !=
+              hipSuccess || v < 1) {
+        (void)hipGetLastError();
+        return 2;  // no device: any figure (nothing is launched)
+      }
+      n.store(v, std::memory_order_relaxed);
+    }
+    return v;
+  }
+};
+
+// f(Shape) for `rows` rows of a sequence and KV head on average: what holds them in the fewest units
+// without many empty rows, up to 128.
+template <typename F>
+auto with_shape(int64_t D, int64_t rows, F&& f) {
+  auto by_rows = [&](auto d) {
+    constexpr int DD = decltype(d)::value;
+    if (rows <= 16) return f(Shape<DD, 1, 0>{});
+    if constexpr (DD < 256) {
+      if (rows <= 32) return f(Shape<DD, 2, 0>{});
+    }
+    if (rows <= 64) return f(Shape<DD, 1, 4>{});
+    return f(Shape<DD, 2, 4>{});
+  };
+  if (D == 64) return by_rows(std::integral_constant<int, 64>{});
+  if (D == 128) return by_rows(std::integral_constant<int, 128>{});
+  return by_rows(std::integral_constant<int, 256>{});
+}
+
+// How a call runs: a bound on the pairs (unit, KV head), whether keys are split over workgroups, and
+// the bytes that that takes.
 struct AttnPlan {
-  int rt, nw;  // nw 0: streaming
-  int rows;
+  int64_t rows;  // of a sequence and KV head on average
   int64_t pairs;
   int slots;
   int64_t grid;
   size_t bytes;
 };
 
-AttnPlan attn_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D) {
+AttnPlan attn_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t keys) {
   AttnPlan a{};
-  a.rt = 1;
   if (T == 0 || B == 0 || Hq == 0) return a;
-  const int64_t rows = (T * (Hq / Hkv) + B - 1) / B;  // of a sequence and KV head on average
-  if (rows <= 16) a.rt = 1;
-  else if (rows <= 32 && D < 256) a.rt = 2;
-  else a.nw = 4, a.rt = rows <= 64 ? 1 : 2;
-  a.rows = 16 * a.rt * (a.nw ? a.nw : 1);
-  a.pairs = Hkv * (T * (Hq / Hkv) / a.rows + B);
-  const int64_t slots = 2 * (int64_t)cu_count();  // two workgroups a CU
-  a.slots = a.pairs < slots ? (int)slots : 0;
-  a.grid = a.slots ? slots : a.pairs;
-  if (a.slots) a.bytes = (size_t)a.grid * a.rows * (D + 2) * 4 + (size_t)a.pairs * 32 + 16;
+  const int64_t G = Hq / Hkv;
+  a.rows = (T * G + B - 1) / B;
+  with_shape(D, a.rows, [&](auto sh) {
+    constexpr int ROWS = decltype(sh)::ROWS;
+    a.pairs = Hkv * (T * G / ROWS + B);
+    // Splits pay where workgroups would idle, or wait for the longest sequence of a batch: with few
+    // rows, whose joining is cheap, up to as many pairs as slots; with many, up to half of them
+    // (720 pairs of 128 rows on 768 slots, D = 64: 48 us whole, 70 split).
+    const int64_t slots = (int64_t)cu_count() * decltype(sh)::wgs_per_cu();
+    // Short contexts stay whole: joining costs a launch (one token on 777 keys, 32/8 heads: 13.7 us
+    // whole, 17.0 split).
+    const bool split = keys > A8_WHOLE_KEYS && (decltype(sh)::NW ? 2 * a.pairs : a.pairs) <= slots;
+    a.slots = split ? (int)slots : 0;
+    a.grid = a.slots ? slots : a.pairs;
+    if (a.slots) a.bytes = (size_t)a.grid * ROWS * (D + 2) * 4 + (size_t)a.pairs * 32 + 16;
+  });
   return a;
 }
 
@@ -847,9 +948,10 @@ AttnPlan attn_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D) {
 
 using namespace sl8;
 
-extern "C" size_t sl8_attn_paged_block8_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D) {
+extern "C" size_t sl8_attn_paged_block8_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                                    int64_t max_context_len) {
   if (T <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || T >= (1LL << 28) || B >= (1 << 24) || Hq >= (1 << 16)) return 0;
-  return attn_plan(T, B, Hq, Hkv, D).bytes;
+  return attn_plan(T, B, Hq, Hkv, D, max_context_len).bytes;
 }
 
 extern "C" int sl8_attn_paged_block8(const void* q, int dtype, int rotate, float q_scale_mul,
@@ -880,7 +982,7 @@ extern "C" int sl8_attn_paged_block8(const void* q, int dtype, int rotate, float
                 "fni8 %s: null pointer", tag);
   SL8_CHECK_ARG(aligned(q, 16) && aligned(out, 16) && aligned(k_cache, 16) && aligned(v_cache, 16),
                 "fni8 %s: q/k_cache/v_cache must be 16-byte aligned", tag);
-  const AttnPlan plan = attn_plan(T, B, Hq, Hkv, D);
+  const AttnPlan plan = attn_plan(T, B, Hq, Hkv, D, max_blocks_per_seq * block_size);
   SL8_CHECK_ARG(plan.bytes == 0 || (workspace && workspace_bytes >= plan.bytes && aligned(workspace, 16)),
                 "fni8 %s: workspace needs %zu bytes", tag, plan.bytes);
   p.q = static_cast<const uint16_t*>(q);
@@ -891,41 +993,28 @@ extern "C" int sl8_attn_paged_block8(const void* q, int dtype, int rotate, float
   p.rotate = rotate != 0;
   p.window = window_left < 0 ? -1 : (int)(window_left < (1 << 30) ? window_left : (1 << 30));
   p.slots = plan.slots;
+  p.max_pairs = (int)plan.pairs;
   if (num_blocks == 0) p.s.maxb = 0;  // nothing to read: no key is there
-  if (plan.slots) {
-    p.part = static_cast<float*>(workspace);
-    p.pairs = reinterpret_cast<int4*>(p.part + (size_t)plan.grid * plan.rows * D);
-    p.count = reinterpret_cast<int*>(p.pairs + 2 * plan.pairs);
-    p.ml = reinterpret_cast<float2*>(p.count + 4);
-  }
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const unsigned grid = (unsigned)(plan.grid > 0 ? plan.grid : 1);
-  using std::integral_constant;
-  auto go = [&](auto dt, auto d, auto rt, auto nw) {
-    constexpr int DT = decltype(dt)::value, DD = decltype(d)::value, RT = decltype(rt)::value, NW = decltype(nw)::value;
-    constexpr int ROWS = 16 * RT * (NW ? NW : 1);
-    if constexpr (NW) attn_block8_tile_kernel<DT, DD, RT, NW><<<grid, 64 * NW, 0, st>>>(p);
-    else attn_block8_stream_kernel<DT, DD, RT><<<grid, A8_THREADS, 0, st>>>(p);
-    if (plan.slots) attn_block8_join_kernel<DT, DD, ROWS><<<dim3((unsigned)plan.pairs, ROWS), 64, 0, st>>>(p);
-  };
-  auto by_rows = [&](auto dt, auto d) {
-    const integral_constant<int, 0> stream;
-    const integral_constant<int, 1> one;
-    const integral_constant<int, 2> two;
-    const integral_constant<int, 4> waves;
-    if (plan.nw) return plan.rt == 1 ? go(dt, d, one, waves) : go(dt, d, two, waves);
-    if constexpr (decltype(d)::value < 256) {
-      if (plan.rt == 2) return go(dt, d, two, stream);
+  with_shape(D, plan.rows, [&](auto sh) {
+    using S = decltype(sh);
+    if (plan.slots) {
+      p.pairs = static_cast<int4*>(workspace);
+      p.count = reinterpret_cast<int*>(p.pairs + 2 * plan.pairs);
+      p.part = reinterpret_cast<float*>(p.count + 4);
+      p.ml = reinterpret_cast<float2*>(p.part + (size_t)plan.grid * S::ROWS * D);
     }
-    go(dt, d, one, stream);
-  };
-  auto by_d = [&](auto dt) {
-    if (D == 64) by_rows(dt, integral_constant<int, 64>{});
-    else if (D == 128) by_rows(dt, integral_constant<int, 128>{});
-    else by_rows(dt, integral_constant<int, 256>{});
-  };
-  if (dtype == SL8_DTYPE_F16) by_d(integral_constant<int, SL8_DTYPE_F16>{});
-  else by_d(integral_constant<int, SL8_DTYPE_BF16>{});
+    auto go = [&](auto dt) {
+      constexpr int DT = decltype(dt)::value;
+      S::template kernel<DT>()<<<grid, S::THREADS, 0, st>>>(p);
+      if (plan.slots)
+        attn_block8_join_kernel<DT, S::D, S::ROWS>
+            <<<dim3((unsigned)plan.pairs, S::ROWS / JOIN_ROWS), 64 * JOIN_ROWS, 0, st>>>(p);
+    };
+    if (dtype == SL8_DTYPE_F16) go(std::integral_constant<int, SL8_DTYPE_F16>{});
+    else go(std::integral_constant<int, SL8_DTYPE_BF16>{});
+  });
   SL8_CHECK_LAUNCH(tag);
   return SL8_OK;
 }

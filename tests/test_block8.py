@@ -26,7 +26,7 @@ def append(**c):
 
 def attn(**c):
     a = dict(q=16, dtype=0, rot=0, mul=1.0, k=16, ks=16, v=16, vs=16, cu=None, lens=16, bt=16, out=16, T=2,
-             B=2, Hq=2, Hkv=1, D=64, nb=4, bs=16, maxb=2, window=-1,
+             B=2, Hq=2, Hkv=1, D=64, nb=400, bs=16, maxb=200, window=-1,
              ws=16, ws_bytes=1 << 40)
     return _lib.load().sl8_attn_paged_block8(*(a | c).values(), None)
 
