@@ -28,7 +28,8 @@ struct AppendArgs {
   float *k_scale, *v_scale;
   int Hkv;
   bool rope;
-  int64_t page_wgs;  // workgroups before those of Q
+  bool has_q;
+  uint32_t share;  // with Q: the part of the workgroups that have blocks (32 fraction bits)
 };
 
 // Elements 8 lane .. 8 lane + 7 of a row held by LPR lanes, turned.
@@ -65,14 +66,17 @@ __device__ __forceinline__ void rope_row(const RopeArgs& a, int64_t token, float
 template <int DT, int D, int NP, bool ROT>
 __global__ void __launch_bounds__(APP_THREADS)
 append_block8_kernel(const AppendArgs p, const RopeArgs a, const RopeRows q) {
-  if ((int64_t)blockIdx.x >= p.page_wgs) return rope_block<DT, 8>(a, q, blockIdx.x - p.page_wgs);
+  // workgroups of blocks and of Q by turns: the former wait for chains of loads while the latter stream
+  const uint32_t wg = __umulhi(blockIdx.x, p.share), next = __umulhi(blockIdx.x + 1, p.share);
+  if (p.has_q && wg == next) return rope_block<DT, 8>(a, q, blockIdx.x - wg);
+  const uint32_t page = p.has_q ? wg : blockIdx.x;
   constexpr int LPR = D / 8, RPB = APP_THREADS / LPR;
   __shared__ float amax_s[APP_THREADS / 64];
   const Block8Seqs& s = p.s;
   const int lane = threadIdx.x % LPR, r0 = threadIdx.x / LPR;
-  const bool is_v = blockIdx.x & 1;
-  const int h = (blockIdx.x >> 1) % p.Hkv;
-  const int64_t unit = (blockIdx.x >> 1) / p.Hkv;
+  const bool is_v = page & 1;
+  const int h = (page >> 1) % p.Hkv;
+  const int64_t unit = (page >> 1) / p.Hkv;
 
   // sequence b has units row(b) / bs + 2 b and up, at least as many as blocks that n rows can touch
   auto first = [&](int b) { return s.cu ? s.row(b) / s.bs + 2LL * b : b; };
@@ -96,22 +100,27 @@ append_block8_kernel(const AppendArgs p, const RopeArgs a, const RopeRows q) {
   const int64_t st = is_v ? p.vst[0] : p.kst[0], sh = is_v ? p.vst[1] : p.kst[1];
   const float old = off ? *scale : 0.f;
 
+  // all rows' loads go out before the first is used; rows past the last repeat it
+  uint4 raw[NP];
+#pragma unroll
+  for (int i = 0; i < NP; ++i)
+    if (NP <= 4 || i * RPB < cnt)
+      raw[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) +
+                                               (tok + min(i * RPB + r0, cnt - 1)) * st + h * sh + 8 * lane);
   float f[NP][8];
   float amax = 0.f;
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
     if (i * RPB >= cnt) break;
-    const int r = i * RPB + r0;
-    const int64_t row = tok + (r < cnt ? r : 0);
-    ld_elems<DT, 8>(x, row * st + h * sh + 8 * lane, f[i]);
+    VecIO<DT>::unpack(raw[i], f[i]);
     if (!is_v) {
-      if (p.rope) rope_row<LPR>(a, row, f[i], lane);
+      if (p.rope) rope_row<LPR>(a, tok + min(i * RPB + r0, cnt - 1), f[i], lane);
       if constexpr (ROT) hadamard_row<D, DT != SL8_DTYPE_F16>(f[i], lane);
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(f[i][e]));
   }
-  amax = lane_group_max<64>(amax);  // (rows past the last repeat the first)
+  amax = lane_group_max<64>(amax);
   if ((threadIdx.x & 63) == 0) amax_s[threadIdx.x / 64] = amax;
   __syncthreads();
 #pragma unroll
@@ -195,7 +204,7 @@ extern "C" int sl8_kv_append_block8(const void* k_new, const void* v_new, const 
   p.k_cache = k_cache; p.v_cache = v_cache; p.k_scale = k_scale; p.v_scale = v_scale;
   p.Hkv = (int)Hkv;
   const int64_t units = cu_lens ? T / block_size + 2 * B : B;
-  p.page_wgs = num_blocks ? units * Hkv * 2 : 0;
+  const int64_t page_wgs = num_blocks ? units * Hkv * 2 : 0;
   int64_t q_wgs = 0;
   if (Hq) {
     qr = RopeRows{q, nullptr, q_out, nullptr, {0, q_strides[1], q_strides[0]}, {}, {0, D, Hq * D}, {}, T, T,
@@ -203,9 +212,12 @@ extern "C" int sl8_kv_append_block8(const void* k_new, const void* v_new, const 
     rope_shape(qr, APP_THREADS / (int)(D / 16));
     q_wgs = (T + qr.tokens - 1) / qr.tokens;
   }
-  const int64_t grid = p.page_wgs + q_wgs;
+  const int64_t grid = page_wgs + q_wgs;
   if (grid == 0) return SL8_OK;
   SL8_CHECK_ARG(grid < (1LL << 31), "fni8 %s: shape too large", tag);
+  // ceil(2^32 page_wgs / grid): workgroup i has (i share) >> 32 of blocks before it, all of them page_wgs
+  p.has_q = q_wgs > 0;
+  p.share = p.has_q ? (uint32_t)((((uint64_t)page_wgs << 32) + grid - 1) / grid) : 0;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   using std::integral_constant;
   auto go = [&](auto dt, auto d, auto np) {

@@ -191,8 +191,8 @@ __device__ __forceinline__ void rope_block(const RopeArgs& a, const RopeRows& t,
 inline int rope_pairs(int64_t D, int64_t R, int dtype, const void* const* ptrs, int np,
                       const int64_t* strides, int ns) {
   const int64_t size = dtype == SL8_DTYPE_F32 ? 4 : 2;
-  for (int n = 8; n >= 4; n /= 2) {
-    const int64_t bytes = n * size < 16 ? n * size : 16;
+  for (int n = 16 / (int)size; n >= 4; n /= 2) {  // (16-byte accesses next to each other, or 8)
+    const int64_t bytes = n * size;
     bool ok = D % (2 * n) == 0 && R % (2 * n) == 0;
     for (int i = 0; i < np; ++i) ok = ok && aligned(ptrs[i], (uintptr_t)bytes);
     for (int i = 0; i < ns; ++i) ok = ok && strides[i] * size % bytes == 0;
