@@ -386,9 +386,10 @@ int sl8_kv_write_paged_rotated(const void* k_new, const void* v_new, const int32
  *   (pos_b 0: shared by the batch); outside the table: its nearest end. sections int32[axes] (host):
  *   how many consecutive pairs each axis turns (axes = 1: ignored). D even, at most 512; R even.
  * ---------------------------------------------------------------------- */
-int sl8_rope(const void* q, const void* k, int dtype, const int64_t* q_strides,
-             const int64_t* k_strides, const void* positions, int positions_i64, int64_t pos_axis,
-             int64_t pos_b, const float* table, int64_t table_rows, const int32_t* sections, int axes,
+int sl8_rope(const void* q, const void* k, int dtype, int64_t q_stride_b, int64_t q_stride_h,
+             int64_t q_stride_s, int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_s,
+             const void* positions, int positions_i64, int64_t pos_axis, int64_t pos_b,
+             const float* table, int64_t table_rows, const int32_t* sections, int axes,
              int interleaved, int inverse, void* q_out, void* k_out, int64_t B, int64_t Hq,
              int64_t Hkv, int64_t S, int64_t D, int64_t R, void* stream);
 
@@ -411,7 +412,8 @@ int sl8_rope(const void* q, const void* k, int dtype, const int64_t* q_strides,
  *   sequence of a call. Values must be finite.
  * ---------------------------------------------------------------------- */
 int sl8_kv_append_block8(const void* k_new, const void* v_new, const void* q, int dtype,
-                         const int64_t* k_strides, const int64_t* v_strides, const int64_t* q_strides,
+                         int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h,
+                         int64_t q_stride_t, int64_t q_stride_h,
                          const void* positions, int positions_i64, const float* table,
                          int64_t table_rows, const int32_t* sections, int axes, int interleaved,
                          int rotate, const int32_t* cu_lens, const int32_t* context_lens,

@@ -55,6 +55,14 @@ def _on_gpu(*ts: torch.Tensor) -> None:
             _fail("all inputs must be on the same device")
 
 
+def _one_gpu(*ts: torch.Tensor) -> None:
+    """_on_gpu in one look at each tensor."""
+    dev = ts[0].get_device()
+    for t in ts:
+        if t.get_device() != dev or dev < 0:
+            _on_gpu(*ts)
+
+
 def _contig(*ts: torch.Tensor) -> None:
     for t in ts:
         if not t.is_contiguous():
@@ -807,16 +815,11 @@ def _rope_checks(tag, positions, table, sections, want, D):
     return axes, cs, positions.contiguous(), table
 
 
-def _strides(t, *dims):
-    """Strides of t's dimensions as the entry points take them (a dimension of one has none)."""
-    return (ctypes.c_int64 * len(dims))(*(t.stride(d) if t.shape[d] != 1 else 0 for d in dims))
-
-
 def rope(q, k, positions, table, sections=None, interleaved=False, inverse=False):
     """Rotary positions of q [B,Hq,S,D] and k [B,Hkv,S,D] (or None), fp16/bf16/fp32, any strides:
     (q', k') contiguous. positions int32/int64 [S] or [B,S], with sections [A,S] or [A,B,S];
     table fp32 [P,R]: cos of R/2 pairs, then sin."""
-    _on_gpu(q, positions, table)
+    _one_gpu(q, positions, table)
     _check(q.dtype in (torch.float16, torch.bfloat16, torch.float32),
            "rope: q/k must be float16/bfloat16/float32")
     _check(q.dim() == 4, "rope: expect q[B,Hq,S,D]")
@@ -824,7 +827,7 @@ def rope(q, k, positions, table, sections=None, interleaved=False, inverse=False
     if D < 2 or D % 2 or D > 512:
         _fail(f"rope: head dim must be even, 2..512, got {D}")
     if k is not None:
-        _on_gpu(q, k)
+        _one_gpu(q, k)
         _check(k.dtype == q.dtype, "rope: q and k must have one dtype")
         _check(k.dim() == 4 and k.shape[0] == B and k.shape[2] == S and k.shape[3] == D,
                "rope: expect k[B,Hkv,S,D] like q")
@@ -832,14 +835,18 @@ def rope(q, k, positions, table, sections=None, interleaved=False, inverse=False
     per_batch = positions.dim() - (sections is not None) == 2
     q = q if q.stride(-1) == 1 else q.contiguous()
     q_out = q.new_empty((B, Hq, S, D))
-    Hkv, k_out, k_ptr, ks = 0, None, None, None
+    # (the stride of a dimension of one says nothing)
+    qb, qh, qt, _ = q.stride()
+    qb, qh, qt = qb if B > 1 else 0, qh if Hq > 1 else 0, qt if S > 1 else 0
+    Hkv, k_out, k_ptr, kb, kh, kt = 0, None, None, 0, 0, 0
     if k is not None:
         k = k if k.stride(-1) == 1 else k.contiguous()
-        Hkv, k_out = k.shape[1], k.new_empty(k.shape)
-        k_ptr, ks = k.data_ptr(), _strides(k, 0, 1, 2)
+        Hkv, k_out, k_ptr = k.shape[1], k.new_empty(k.shape), k.data_ptr()
+        kb, kh, kt, _ = k.stride()
+        kb, kh, kt = kb if B > 1 else 0, kh if Hkv > 1 else 0, kt if S > 1 else 0
     if B and S and Hq + Hkv:
         with on_device(q):
-            call("sl8_rope", q.data_ptr(), k_ptr, dtype_code(q.dtype), _strides(q, 0, 1, 2), ks,
+            call("sl8_rope", q.data_ptr(), k_ptr, dtype_code(q.dtype), qb, qh, qt, kb, kh, kt,
                  positions.data_ptr(), int(positions.dtype == torch.int64), positions.numel() // axes,
                  S if per_batch else 0, table.data_ptr(), table.shape[0], cs, axes,
                  int(bool(interleaved)), int(bool(inverse)), q_out.data_ptr(), _lib.ptr(k_out), B, Hq,
@@ -860,7 +867,7 @@ def _block8_checks(tag, k_cache, k_scale, v_cache, v_scale, block_table, context
     if v_cache.shape != k_cache.shape:
         _fail(f"{tag}: v_cache shape must match k_cache")
     nblk, _, bs, _ = k_cache.shape
-    if tuple(k_scale.shape) != (nblk, Hkv) or tuple(v_scale.shape) != (nblk, Hkv):
+    if k_scale.shape != (nblk, Hkv) or v_scale.shape != (nblk, Hkv):
         _fail(f"{tag}: k_scale/v_scale must be [num_blocks,H_kv]")
     _contig(k_cache, k_scale, v_cache, v_scale, block_table, context_lens)
     if block_table.dtype != torch.int32 or context_lens.dtype != torch.int32:
@@ -875,7 +882,7 @@ def _block8_checks(tag, k_cache, k_scale, v_cache, v_scale, block_table, context
             _fail(f"{tag}: without cu_lens there is one row per sequence, got {T} for {B}")
     else:
         _contig(cu_lens)
-        if cu_lens.dtype != torch.int32 or tuple(cu_lens.shape) != (B + 1,):
+        if cu_lens.dtype != torch.int32 or cu_lens.shape != (B + 1,):
             _fail(f"{tag}: cu_lens must be int32 [B + 1]")
     if D not in _HEAD_DIMS_BLOCK8:
         _fail(f"{tag}: head dim must be {_dims_msg(_HEAD_DIMS_BLOCK8)}, got {D}")
@@ -885,11 +892,14 @@ def _block8_checks(tag, k_cache, k_scale, v_cache, v_scale, block_table, context
 
 
 def _rows16(t):
-    """t [T, H, D], copied where its rows are not 16-byte aligned."""
-    if t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(
-            t.shape[d] == 1 or t.stride(d) % 8 == 0 for d in (0, 1)):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+    """t [T, H, D], copied where its rows are not 16-byte aligned, with its strides of T and H."""
+    st, sh, sd = t.stride()
+    T, H, _ = t.shape
+    st, sh = st if T > 1 else 0, sh if H > 1 else 0
+    if sd == 1 and st % 8 == 0 and sh % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t, st, sh
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride(0), t.stride(1)
 
 
 def kv_append_block8(k_new, v_new, k_cache, k_scale, v_cache, v_scale, block_table, context_lens,
@@ -899,8 +909,8 @@ def kv_append_block8(k_new, v_new, k_cache, k_scale, v_cache, v_scale, block_tab
     in place; K turned by position (positions not None) and then, with rotate, multiplied by the
     Hadamard matrix. Returns the turned q [T,Hq,D], None without one."""
     tag = "kv_append_block8"
-    _on_gpu(k_new, v_new, k_cache, k_scale, v_cache, v_scale, block_table, context_lens,
-            *(t for t in (cu_lens, q, positions, table) if t is not None))
+    given = [t for t in (cu_lens, q, positions, table) if t is not None]
+    _one_gpu(k_new, v_new, k_cache, k_scale, v_cache, v_scale, block_table, context_lens, *given)
     dt = k_new.dtype
     if dt not in (torch.float16, torch.bfloat16) or v_new.dtype != dt:
         _fail(f"{tag}: k_new/v_new must both be float16 or bfloat16")
@@ -919,19 +929,21 @@ def kv_append_block8(k_new, v_new, k_cache, k_scale, v_cache, v_scale, block_tab
         rows, R = table.shape
         if R % 16:
             _fail(f"{tag}: rotary dim must be a multiple of 16, got {R}")
-    q_out = qs = None
+    q_out, qt, qh = None, 0, 0
     if q is not None:
         if positions is None:
             _fail(f"{tag}: q needs positions")
         if q.dtype != dt or q.dim() != 3 or q.shape[0] != T or q.shape[2] != D:
             _fail(f"{tag}: q must be [T,H_q,D] of k_new's dtype")
-        q, Hq = _rows16(q), q.shape[1]
-        q_out, qs = q.new_empty((T, Hq, D)), _strides(q, 0, 1)
+        Hq = q.shape[1]
+        q, qt, qh = _rows16(q)
+        q_out = q.new_empty((T, Hq, D))
     if T:
-        k_new, v_new = _rows16(k_new), _rows16(v_new)
+        k_new, kt, kh = _rows16(k_new)
+        v_new, vt, vh = _rows16(v_new)
         with on_device(k_new):
             call("sl8_kv_append_block8", k_new.data_ptr(), v_new.data_ptr(), _lib.ptr(q),
-                 dtype_code(dt), _strides(k_new, 0, 1), _strides(v_new, 0, 1), qs,
+                 dtype_code(dt), kt, kh, vt, vh, qt, qh,
                  _lib.ptr(positions), int(positions is not None and positions.dtype == torch.int64),
                  _lib.ptr(table), rows, cs, axes, int(bool(interleaved)), int(bool(rotate)),
                  _lib.ptr(cu_lens), context_lens.data_ptr(), block_table.data_ptr(),
@@ -945,8 +957,8 @@ def attn_paged_block8(q, q_mul, rotate, k_cache, k_scale, v_cache, v_scale, bloc
     """Attention of the new tokens q [T,Hq,D] (fp16/bf16) over a block-scaled paged int8 cache that
     holds them already -> [T,Hq,D] of q's dtype; q_mul is softmax_scale * log2(e)."""
     tag = "attn_paged_block8"
-    _on_gpu(q, k_cache, k_scale, v_cache, v_scale, block_table, context_lens,
-            *(() if cu_lens is None else (cu_lens,)))
+    _one_gpu(q, k_cache, k_scale, v_cache, v_scale, block_table, context_lens,
+             q if cu_lens is None else cu_lens)
     if q.dtype not in (torch.float16, torch.bfloat16):
         _fail(f"{tag}: q must be float16 or bfloat16")
     if q.dim() != 3 or k_cache.dim() != 4:

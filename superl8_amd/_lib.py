@@ -75,9 +75,9 @@ SIGNATURES = {
     "sl8_kv_write_paged": (_I, [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P]),
     "sl8_kv_write_paged_rotated": (_I, [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64,
                                         _P]),
-    "sl8_rope": (_I, [_P, _P, _I, _P, _P, _P, _I, _I64, _I64, _P, _I64, _P, _I, _I, _I, _P, _P]
+    "sl8_rope": (_I, [_P, _P, _I] + [_I64] * 6 + [_P, _I, _I64, _I64, _P, _I64, _P, _I, _I, _I, _P, _P]
                  + [_I64] * 6 + [_P]),
-    "sl8_kv_append_block8": (_I, [_P, _P, _P, _I, _P, _P, _P, _P, _I, _P, _I64, _P, _I, _I, _I]
+    "sl8_kv_append_block8": (_I, [_P, _P, _P, _I] + [_I64] * 6 + [_P, _I, _P, _I64, _P, _I, _I, _I]
                              + [_P] * 8 + [_I64] * 9 + [_P]),
     "sl8_attn_paged_block8_workspace": (_SZ, [_I64] * 6),
     "sl8_attn_paged_block8": (_I, [_P, _I, _I, _F] + [_P] * 8 + [_I64] * 9 + [_P, _SZ, _P]),

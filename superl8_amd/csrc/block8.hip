@@ -155,9 +155,9 @@ append_block8_kernel(const AppendArgs p, const RopeArgs a, const RopeRows q) {
 using namespace sl8;
 
 extern "C" int sl8_kv_append_block8(const void* k_new, const void* v_new, const void* q, int dtype,
-                                    const int64_t* k_strides, const int64_t* v_strides,
-                                    const int64_t* q_strides, const void* positions,
-                                    int positions_i64, const float* table, int64_t table_rows,
+                                    int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t,
+                                    int64_t v_stride_h, int64_t q_stride_t, int64_t q_stride_h,
+                                    const void* positions, int positions_i64, const float* table, int64_t table_rows,
                                     const int32_t* sections, int axes, int interleaved, int rotate,
                                     const int32_t* cu_lens, const int32_t* context_lens,
                                     const int32_t* block_table, int8_t* k_cache, float* k_scale,
@@ -187,19 +187,17 @@ extern "C" int sl8_kv_append_block8(const void* k_new, const void* v_new, const 
                                  sections, axes, interleaved, 0)) return rc;
     SL8_CHECK_ARG(R % 16 == 0, "fni8 %s: rotary dim must be a multiple of 16, got %lld", tag, (long long)R);
   }
-  SL8_CHECK_ARG(k_new && v_new && k_strides && v_strides && context_lens &&
+  SL8_CHECK_ARG(k_new && v_new && context_lens &&
                     (max_blocks_per_seq == 0 || block_table) &&
                     (num_blocks == 0 || (k_cache && k_scale && v_cache && v_scale)) &&
-                    (Hq == 0 || (q && q_out && q_strides)),
+                    (Hq == 0 || (q && q_out)),
                 "fni8 %s: null pointer", tag);
-  bool ok = aligned(k_new, 16) && aligned(v_new, 16) && aligned(q, 16) && aligned(q_out, 16) &&
-            aligned(k_cache, 8) && aligned(v_cache, 8);
-  for (int i = 0; i < 2; ++i) {
-    p.kst[i] = k_strides[i];
-    p.vst[i] = v_strides[i];
-    ok = ok && p.kst[i] % 8 == 0 && p.vst[i] % 8 == 0 && (Hq == 0 || q_strides[i] % 8 == 0);
-  }
+  const bool ok = aligned(k_new, 16) && aligned(v_new, 16) && aligned(q, 16) && aligned(q_out, 16) &&
+                  aligned(k_cache, 8) && aligned(v_cache, 8) &&
+                  (k_stride_t | k_stride_h | v_stride_t | v_stride_h | (Hq ? q_stride_t | q_stride_h : 0)) % 8 == 0;
   SL8_CHECK_ARG(ok, "fni8 %s: rows must be 16-byte aligned", tag);
+  p.kst[0] = k_stride_t; p.kst[1] = k_stride_h;
+  p.vst[0] = v_stride_t; p.vst[1] = v_stride_h;
   p.k = k_new; p.v = v_new;
   p.k_cache = k_cache; p.v_cache = v_cache; p.k_scale = k_scale; p.v_scale = v_scale;
   p.Hkv = (int)Hkv;
@@ -207,7 +205,7 @@ extern "C" int sl8_kv_append_block8(const void* k_new, const void* v_new, const 
   const int64_t page_wgs = num_blocks ? units * Hkv * 2 : 0;
   int64_t q_wgs = 0;
   if (Hq) {
-    qr = RopeRows{q, nullptr, q_out, nullptr, {0, q_strides[1], q_strides[0]}, {}, {0, D, Hq * D}, {}, T, T,
+    qr = RopeRows{q, nullptr, q_out, nullptr, {0, q_stride_h, q_stride_t}, {}, {0, D, Hq * D}, {}, T, T,
                   (int)Hq, 0, (int)D, 1, 1};
     rope_shape(qr, APP_THREADS / (int)(D / 16));
     q_wgs = (T + qr.tokens - 1) / qr.tokens;

@@ -17,12 +17,12 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const RopeArgs a, co
 
 using namespace sl8;
 
-extern "C" int sl8_rope(const void* q, const void* k, int dtype, const int64_t* q_strides,
-                        const int64_t* k_strides, const void* positions, int positions_i64,
-                        int64_t pos_axis, int64_t pos_b, const float* table, int64_t table_rows,
-                        const int32_t* sections, int axes, int interleaved, int inverse, void* q_out,
-                        void* k_out, int64_t B, int64_t Hq, int64_t Hkv, int64_t S, int64_t D,
-                        int64_t R, void* stream) {
+extern "C" int sl8_rope(const void* q, const void* k, int dtype, int64_t q_stride_b, int64_t q_stride_h,
+                        int64_t q_stride_s, int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_s,
+                        const void* positions, int positions_i64, int64_t pos_axis, int64_t pos_b,
+                        const float* table, int64_t table_rows, const int32_t* sections, int axes,
+                        int interleaved, int inverse, void* q_out, void* k_out, int64_t B, int64_t Hq,
+                        int64_t Hkv, int64_t S, int64_t D, int64_t R, void* stream) {
   clear_error();
   SL8_CHECK_ARG(dtype == SL8_DTYPE_F16 || dtype == SL8_DTYPE_BF16 || dtype == SL8_DTYPE_F32,
                 "fni8 rope: q/k must be float16/bfloat16/float32");
@@ -35,19 +35,19 @@ extern "C" int sl8_rope(const void* q, const void* k, int dtype, const int64_t* 
   RopeArgs a;
   if (const int rc = rope_args("rope", a, positions, positions_i64, pos_axis, pos_b, table, table_rows,
                                R, D, sections, axes, interleaved, inverse)) return rc;
-  SL8_CHECK_ARG((Hq == 0 || (q && q_out && q_strides)) && (Hkv == 0 || (k && k_out && k_strides)),
+  SL8_CHECK_ARG((Hq == 0 || (q && q_out)) && (Hkv == 0 || (k && k_out)),
                 "fni8 rope: null pointer");
-  RopeRows t{q, k, q_out, k_out, {}, {}, {Hq * S * D, S * D, D}, {Hkv * S * D, S * D, D}, B * S, S,
-             (int)Hq, (int)Hkv, (int)D, 1, 1};
+  RopeRows t{q, k, q_out, k_out, {q_stride_b, q_stride_h, q_stride_s}, {k_stride_b, k_stride_h, k_stride_s},
+             {Hq * S * D, S * D, D}, {Hkv * S * D, S * D, D}, B * S, S, (int)Hq, (int)Hkv, (int)D, 1, 1};
   const void* ptrs[4];
   int64_t strides[6];
   int np = 0, ns = 0;
-  for (int i = 0; i < 3; ++i) {
-    if (Hq) strides[ns++] = t.qs[i] = q_strides[i];
-    if (Hkv) strides[ns++] = t.ks[i] = k_strides[i];
-  }
   if (Hq) ptrs[np++] = q, ptrs[np++] = q_out;
   if (Hkv) ptrs[np++] = k, ptrs[np++] = k_out;
+  for (int i = 0; i < 3; ++i) {
+    if (Hq) strides[ns++] = t.qs[i];
+    if (Hkv) strides[ns++] = t.ks[i];
+  }
   const int n = rope_pairs(D, R, dtype, ptrs, np, strides, ns);
   rope_shape(t, ROPE_THREADS / (int)(D / (2 * n)));
   const unsigned grid = (unsigned)((t.T + t.tokens - 1) / t.tokens);

@@ -14,6 +14,7 @@ import math
 import torch
 
 from . import _C
+from .quant.core import LOG2E
 from .quant.rotation import hadamard_dim
 
 # Decode-shape M cap for the k-quant linear (reference ops.py:1289).
@@ -381,8 +382,6 @@ def attn_paged_block8(q: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.Ten
     q = q.contiguous()
     if q.data_ptr() % 16:
         q = q.clone()
-    from .quant import LOG2E
-
     return _C.attn_paged_block8(q, softmax_scale * LOG2E, rotate, k_cache, k_scale, v_cache, v_scale,
                                 block_table.contiguous(), context_lens.contiguous(),
                                 None if cu_lens is None else cu_lens.contiguous(), window_left)

@@ -8,17 +8,15 @@ import torch
 import superl8_amd as sl8
 from superl8_amd import _lib
 
-I3 = (ctypes.c_int64 * 3)(0, 0, 0)
-
 
 def rope(**c):
-    a = dict(q=16, k=16, dtype=0, qs=I3, ks=I3, pos=16, pos64=0, pos_axis=4, pos_b=0, table=16, rows=8,
+    a = dict(q=16, k=16, dtype=0, qb=0, qh=0, q_s=0, kb=0, kh=0, k_s=0, pos=16, pos64=0, pos_axis=4, pos_b=0, table=16, rows=8,
              sections=None, axes=1, inter=0, inv=0, qo=16, ko=16, B=1, Hq=1, Hkv=1, S=4, D=64, R=64)
     return _lib.load().sl8_rope(*(a | c).values(), None)
 
 
 def append(**c):
-    a = dict(k=16, v=16, q=None, dtype=0, ks=I3, vs=I3, qs=None, pos=None, pos64=0, table=None, rows=0,
+    a = dict(k=16, v=16, q=None, dtype=0, kt=0, kh=0, vt=0, vh=0, qt=0, qh=0, pos=None, pos64=0, table=None, rows=0,
              sections=None, axes=1, inter=0, rot=0, cu=None, lens=16, bt=16, kc=16, ksc=16, vc=16, vsc=16,
              qo=None, T=2, B=2, Hq=0, Hkv=1, D=64, R=0, nb=4, bs=16, maxb=2)
     return _lib.load().sl8_kv_append_block8(*(a | c).values(), None)
@@ -40,10 +38,11 @@ def attn(**c):
     (rope, dict(table=20), b"aligned"), (rope, dict(S=1 << 31), b"too large"), (rope, dict(B=-1), b"shape"),
     (append, dict(dtype=2), b"float16"), (append, dict(D=96), b"head dim"), (append, dict(bs=24), b"block_size"),
     (append, dict(bs=144), b"block_size"), (append, dict(bs=0), b"block_size"), (append, dict(T=3), b"one row"),
-    (append, dict(q=16, qo=16, qs=I3, Hq=1), b"positions"), (append, dict(pos=16, table=16, rows=4, R=40), b"16"),
+    (append, dict(q=16, qo=16, Hq=1), b"positions"), (append, dict(pos=16, table=16, rows=4, R=40), b"16"),
     (append, dict(lens=None), b"null"), (append, dict(bt=None), b"null"), (append, dict(ksc=None), b"null"),
     (append, dict(k=24), b"aligned"), (append, dict(kc=20), b"aligned"), (append, dict(T=1 << 28, B=1), b"large"),
-    (append, dict(ks=(ctypes.c_int64 * 2)(4, 64)), b"aligned"),
+    (append, dict(kt=4), b"aligned"), (append, dict(vh=12), b"aligned"),
+    (append, dict(q=16, qo=16, Hq=1, pos=16, table=16, rows=4, R=32, qt=4), b"aligned"),
     (attn, dict(dtype=2), b"float16"), (attn, dict(D=32), b"head dim"), (attn, dict(bs=8), b"block_size"),
     (attn, dict(Hq=3, Hkv=2), b"divisible"), (attn, dict(T=3), b"one row"), (attn, dict(q=None), b"null"),
     (attn, dict(lens=None), b"null"), (attn, dict(vs=None), b"null"), (attn, dict(q=24), b"aligned"),
