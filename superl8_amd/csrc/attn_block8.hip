@@ -767,7 +767,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_block8_tile_kernel(const Attn
     st.weights(sc, gks, glv, giv, key0, key0 + KT, g4, wb);
 
     int swz = vt_swz;
-    asm volatile("" : "+v"(swz));  // (the places are the tile's own: kept over the loop they spill)
+    if (D > 128) asm volatile("" : "+v"(swz));  // (the tile's own: 16 places kept over the loop spill)
 #pragma unroll
     for (int kk = 0; kk < NG / 2; ++kk)
 #pragma unroll
@@ -780,6 +780,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_block8_tile_kernel(const Attn
         for (int rt = 0; rt < RT; ++rt)
           st.o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wb[rt][kk], st.o[rt][d], 0, 0, 0);
       }
+    __builtin_amdgcn_iglp_opt(0);  // reads and products interleaved: 2 % of a long chunk
     store_v(vnext);
     wait_dma();
     __syncthreads();
