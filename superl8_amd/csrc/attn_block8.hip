@@ -196,9 +196,17 @@ __device__ __forceinline__ Item find_item(const AttnArgs& p, int lane, int id) {
 struct Span {
   int64_t row0;  // first row (token) of the sequence
   int r0, cnt;   // the unit's first of its rows, and how many
+  int tok, head; // r0 / G, r0 % G
+  float over_g;  // 1 / G
   int pos0;      // position of the sequence's first new token
   int k0, k1;    // keys of the item: from a multiple of a tile
 };
+
+// Token (of the sequence's new ones) of a unit's row: (r0 + r) / G. A quotient of less than 2^17 by
+// less than 2^16, kept half a row from the next whole number, survives the product's rounding.
+__device__ __forceinline__ int token_of(const Span& w, int r) {
+  return w.tok + (int)(((float)(w.head + r) + 0.5f) * w.over_g);
+}
 
 template <int ROWS>
 __device__ __forceinline__ Span item_span(const AttnArgs& p, const Item& it) {
@@ -208,14 +216,17 @@ __device__ __forceinline__ Span item_span(const AttnArgs& p, const Item& it) {
   const int64_t len = it.len;
   w.r0 = it.unit * ROWS;
   w.cnt = min(ROWS, n * p.G - w.r0);
+  w.tok = w.r0 / p.G;
+  w.head = w.r0 - w.tok * p.G;
+  w.over_g = 1.f / (float)p.G;
   // (contexts below the new tokens: positions below 0, which see nothing)
   const int64_t pos0 = max(len - n, (int64_t)-(1 << 28));
   w.pos0 = (int)min(pos0, (int64_t)INT_MAX - (1 << 29));
   const int keys = (int)max((int64_t)0, min(len, (int64_t)p.s.maxb * p.s.bs));
-  const int last = min(keys, w.pos0 + (w.r0 + w.cnt - 1) / p.G + 1);
+  const int last = min(keys, w.pos0 + token_of(w, w.cnt - 1) + 1);
   int first = 0;
   if (p.window >= 0) {
-    first = (int)max((int64_t)0, (int64_t)w.pos0 + w.r0 / p.G - p.window + 1);
+    first = (int)max((int64_t)0, (int64_t)w.pos0 + w.tok - p.window + 1);
     first &= ~(A8_TILE - 1);
   }
   const int tiles = max(0, last - first + A8_TILE - 1) / A8_TILE;
@@ -243,8 +254,8 @@ __device__ __forceinline__ void zero_tail(const AttnArgs& p, int64_t end, int D)
 
 // Row r of a unit: its offset in q and out.
 __device__ __forceinline__ int64_t row_at(const AttnArgs& p, const Span& w, int kvh, int r, int D) {
-  const int i = w.r0 + r;
-  return ((w.row0 + i / p.G) * p.Hq + kvh * p.G + i % p.G) * D;
+  const int t = token_of(w, r);
+  return ((w.row0 + t) * p.Hq + kvh * p.G + w.head + r - (t - w.tok) * p.G) * D;
 }
 
 // The unit's rows as int8 codes in LDS (row r at place(r)) with their scales (times q_mul); rows past
@@ -329,7 +340,7 @@ struct RowState {
     for (int rt = 0; rt < RT; ++rt) {
       const int r = r0 + 16 * rt + col;
       qs[rt] = qs_s[r];
-      const int pos = w.pos0 + (w.r0 + min(r, w.cnt - 1)) / p.G;  // (rows past the last: as the last)
+      const int pos = w.pos0 + token_of(w, min(r, w.cnt - 1));  // (rows past the last: as the last)
       lim[rt] = min(pos + 1, w.k1);
       low[rt] = p.window >= 0 ? (int)max((int64_t)pos - p.window + 1, (int64_t)0) : 0;
       m[rt] = A8_NONE;
@@ -337,8 +348,8 @@ struct RowState {
 #pragma unroll
       for (int t = 0; t < D / 16; ++t) o[rt][t] = v4f{0.f, 0.f, 0.f, 0.f};
     }
-    in1 = min(w.pos0 + w.r0 / p.G + 1, w.k1);
-    in0 = p.window >= 0 ? w.pos0 + (w.r0 + w.cnt - 1) / p.G - p.window + 1 : 0;
+    in1 = min(w.pos0 + w.tok + 1, w.k1);
+    in0 = p.window >= 0 ? w.pos0 + token_of(w, w.cnt - 1) - p.window + 1 : 0;
   }
 
   // Weights of NG groups of 16 keys from their scores (lane (g4, col): keys 16 g + 4 g4 + i from
