@@ -408,8 +408,8 @@ int sl8_rope(const void* q, const void* k, int dtype, int64_t q_stride_b, int64_
  *   multiple of 16); rotate != 0: K's rows then pass through the normalised Hadamard matrix. In fp32,
  *   a block and head with new rows gets scale' = max(scale of the rows it keeps, amax|new| *
  *   fp32(1/127), 2^-60), its new rows codes rint(x / scale'), kept codes c become rint(c * (scale /
- *   scale')). Rows past a sequence's last token are left as they were. A block is written by one
- *   sequence of a call. Values must be finite.
+ *   scale')). Rows past a sequence's last token are left as they were. A call writes a block once:
+ *   no sequences share one that they write. Values must be finite.
  * ---------------------------------------------------------------------- */
 int sl8_kv_append_block8(const void* k_new, const void* v_new, const void* q, int dtype,
                          int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h,

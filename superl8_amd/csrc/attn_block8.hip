@@ -116,6 +116,19 @@ __device__ __forceinline__ int wave_scan(int x) {
 
 template <int ROWS>
 __device__ __forceinline__ Item find_item(const AttnArgs& p, int lane, int id) {
+  if (!p.slots && !p.s.cu) {  // one row a sequence, whole: nothing to look for
+    Item it{};
+    it.units = (p.G + ROWS - 1) / ROWS;
+    const int r = id / p.Hkv;
+    it.kvh = id - r * p.Hkv;
+    it.b = it.row0 = r / it.units;
+    it.unit = r - it.b * it.units;
+    it.live = it.b < p.s.B;
+    it.n = it.splits = 1;
+    it.len = it.live ? p.s.lens[it.b] : 0;
+    it.end = p.s.T;
+    return it;
+  }
   const SeqWork mine = seq_work<ROWS>(p, lane);
   auto work = [&](int b0) { return b0 == 0 ? mine : seq_work<ROWS>(p, b0 + lane); };
   float over_l = 0.f;
@@ -297,7 +310,8 @@ __device__ __forceinline__ Group key_group(const AttnArgs& p, int b, int kvh, in
     const int id = p.s.block(b, j);
     if (id >= 0) {
       const int64_t bh = (int64_t)id * p.Hkv + kvh;
-      const float vs = p.vs[bh];
+      float vs = p.vs[bh];
+      vs = vs < 0x1p-60f ? 0x1p-60f : vs;  // (a block of zeros by any other writer)
       g = Group{(bh * p.s.bs + off) * D, p.ks[bh], __builtin_amdgcn_logf(vs), 1.f / vs};
     }
   }

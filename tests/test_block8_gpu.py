@@ -333,6 +333,18 @@ def test_many_sequences():
     attn_and_check(c, coded_queries(sum(new), 8, 64, F16, False), new, total)
 
 
+@pytest.mark.parametrize("B,new", [(100, 1), (70, 3), (130, 20)])
+@pytest.mark.parametrize("cu", [True, False])
+def test_many_sequences_one_long(B, new, cu):
+    """More sequences than a wave holds, and keys split over workgroups for the long ones."""
+    if not cu and new > 1:
+        return
+    total = [new + (i * 31) % 90 for i in range(B)]
+    total[B // 2], total[B - 1] = 3333, 1500
+    c = Cache(total, 1, 128, 16)
+    attn_and_check(c, coded_queries(B * new, 4, 128, F16, False), [new] * B, total, cu=cu)
+
+
 @pytest.mark.parametrize("new", [1, 4, 300])
 def test_long_contexts(new):
     total = [40000, 9, 20001] if new < 100 else [20001]
@@ -364,6 +376,20 @@ def test_scales_of_blocks_far_apart(new):
     c.vs[:] = 2.0 ** -60  # nothing but least scales: weights as usual, an output of nearly nothing
     assert float(sl8.attn_paged_block8(q, *c.args(), i32(total), cu_lens=offsets([new] * 2),
                                        rotate=False).abs().max()) <= 127 * 2.0 ** -60 * (1 + 2.0 ** -7)
+
+
+@pytest.mark.parametrize("new", [1, 3, 90])
+def test_scales_of_zero(new):
+    """Blocks of zeros whose scales say 0: V adds nothing and its keys keep their weights."""
+    total = [150, 200]
+    c = Cache(total, 1, 64, 16)
+    for scale in (c.ks, c.vs):
+        scale[::4] = 0
+    q = coded_queries(2 * new, 4, 64, F16, False)
+    attn_and_check(c, q, [new] * 2, total)
+    c.ks[:], c.vs[:] = 0, 0
+    # no weight times 127 codes of 2^-60
+    assert not sl8.attn_paged_block8(q, *c.args(), i32(total), cu_lens=offsets([new] * 2), rotate=False).any()
 
 
 @pytest.mark.parametrize("new", [1, 3, 90])
