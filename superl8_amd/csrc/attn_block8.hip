@@ -7,8 +7,8 @@
 //   s_j = qs * scale * log2(e) * ks[block(j)] * <q, k_j> (exact integers inside),
 //   out = sum_j 2^s_j vs[block(j)] v_j / sum_j 2^s_j;
 // a row that sees nothing gives zeros. The scale of V goes into the exponent: with
-//   t_j = s_j + log2 vs, m = max t_j, w_j = 2^(t_j - m):  out = sum w_j v_j / sum w_j / vs,
-// so that the weights that meet the codes v_j in 16 bits are at most 1 whatever the scales, the
+//   t_j = s_j + log2 vs, m near max t_j, w_j = 2^(t_j - m):  out = sum w_j v_j / sum w_j / vs,
+// so that the weights that meet the codes v_j in 16 bits fit them whatever the scales, the
 // largest contribution has full precision, and a block's scale costs one fma that the product s_j
 // needs anyway. (Least scale 2^-60: the sum of w / vs stays within 32 bits.)
 //
@@ -29,7 +29,8 @@ constexpr int A8_TILE = 64;       // keys: what splits and units' first keys are
 constexpr int A8_MIN_TILES = 4;   // least keys of a split: a tile for each wave
 constexpr int A8_WHOLE_KEYS = 1024; // contexts up to here are not split
 constexpr float A8_NONE = -1e30f; // reference of nothing
-constexpr float A8_LAG = 12.f;    // log2 of the largest weight (fp16 holds 2^15)
+constexpr float A8_LAG = 15.f;    // log2 of the largest weight (fp16 holds it)
+constexpr float A8_HEAD = 8.f;    // log2 of a maximum's weight when it becomes the reference
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -367,10 +368,13 @@ struct RowState {
   }
 
   // Weights of NG groups of 16 keys from their scores (lane (g4, col): keys 16 g + 4 g4 + i from
-  // key0): B operands of keys 32 kk + {4 g4 + i, 16 + 4 g4 + i}. The reference m lags behind the
-  // maximum by up to A8_LAG, so that most tiles need no exchange across lanes and no scaling: 16-bit
-  // weights reach 2^A8_LAG, and are as exact there as near 1. The sum takes them in 32 bits: in a
-  // block of small values a large weight may have no 16-bit form beside V's largest.
+  // key0): B operands of keys 32 kk + {4 g4 + i, 16 + 4 g4 + i}. The reference m stands 2^A8_HEAD
+  // to 2^A8_LAG below the maximum, so that most tiles need no exchange across lanes and no scaling,
+  // and the 16-bit weights, as exact there as near 1, still hold 2^-32 of the largest: 2^20 keys below
+  // that are 2^-13 of the output at most (with the maximum as reference, a tail of 2^17 keys of
+  // weight 2^-26 was lost; the two steps of the reference cost 1 %, 3 % in short prompts). The sum
+  // takes the weights in 32 bits: in a block of small values a large one may have no 16-bit form beside
+  // V's largest.
   template <int NG>
   __device__ __forceinline__ void weights(const v4i (&sc)[RT][NG], const float (&ks)[NG], const float (&lv)[NG],
                                           const float (&iv)[NG], int key0, int keys_end, int g4,
@@ -413,8 +417,8 @@ struct RowState {
       for (int rt = 0; rt < RT; ++rt) {
         const bool none = m[rt] == A8_NONE;
         const float mt = max_xor32(max_xor16(top[rt]));
-        const float by = none ? (mt == -INFINITY ? 0.f : mt) : fmaxf(mt, 0.f);
-        m[rt] = none ? (mt == -INFINITY ? A8_NONE : mt) : m[rt] + by;
+        const float by = none ? (mt == -INFINITY ? 0.f : mt - A8_HEAD) : fmaxf(mt - A8_HEAD, 0.f);
+        m[rt] = none ? (mt == -INFINITY ? A8_NONE : mt - A8_HEAD) : m[rt] + by;
         const float r = none ? 1.f : __builtin_amdgcn_exp2f(-by);
         l[rt] *= r;
 #pragma unroll

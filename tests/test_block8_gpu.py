@@ -450,6 +450,24 @@ def test_attention_skips_what_is_not_there(new):
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("new", [1, 40, 1024])
+def test_long_tail_of_small_weights(new):
+    """One key of weight 1 whose value is zero, 2^17 of weight 2^-26.2, which make the output. They stand
+    2^8 above where the 16-bit weights put the largest at least, 2^-18.2: half a step there is 2^-25,
+    2^-6.8 of the weight, and all of them are rounded alike."""
+    N, step = 1 << 17, 26.2
+    c = Cache([N], 1, 64, 128)
+    c.k[:], c.v[:], c.ks[:], c.vs[:] = 0, 127, 1 / 127, 1
+    first = int(c.table[0, 0])
+    c.k[first, 0, 0, 0], c.v[first, 0, 0] = 127, 0
+    q = torch.zeros(new, 64, 64, device=DEV, dtype=F16)
+    q[..., 0] = 1
+    got = sl8.attn_paged_block8(q, *c.args(), i32([N]), cu_lens=offsets([new]), scale=step / LOG2E, rotate=False)
+    tail = (torch.arange(N - new, N, device=DEV, dtype=torch.float64) * 2.0 ** -step)[:, None, None]
+    want = 127 * tail / (1 + tail)
+    assert float(((got.double() - want) / want).abs().max()) <= 2.0 ** -6
+
+
 def test_empty_calls():
     c = Cache([20], 2, 64, 16)
     q = torch.zeros(0, 4, 64, device=DEV, dtype=F16)
