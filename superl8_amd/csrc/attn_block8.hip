@@ -214,6 +214,7 @@ struct Span {
   float over_g;  // 1 / G
   int pos0;      // position of the sequence's first new token
   int k0, k1;    // keys of the item: from a multiple of a tile
+  int low;       // the first key that any row sees
 };
 
 // Token (of the sequence's new ones) of a unit's row: (r0 + r) / G. A quotient of less than 2^17 by
@@ -238,11 +239,8 @@ __device__ __forceinline__ Span item_span(const AttnArgs& p, const Item& it) {
   w.pos0 = (int)min(pos0, (int64_t)INT_MAX - (1 << 29));
   const int keys = (int)max((int64_t)0, min(len, (int64_t)p.s.maxb * p.s.bs));
   const int last = min(keys, w.pos0 + token_of(w, w.cnt - 1) + 1);
-  int first = 0;
-  if (p.window >= 0) {
-    first = (int)max((int64_t)0, (int64_t)w.pos0 + w.tok - p.window + 1);
-    first &= ~(A8_TILE - 1);
-  }
+  w.low = p.window >= 0 ? (int)max((int64_t)0, (int64_t)w.pos0 + w.tok - p.window + 1) : 0;
+  const int first = w.low & ~(A8_TILE - 1);
   const int tiles = max(0, last - first + A8_TILE - 1) / A8_TILE;
   const int per = (tiles + it.splits - 1) / it.splits * A8_TILE;
   w.k0 = first + it.split * per;
@@ -298,15 +296,15 @@ __device__ __forceinline__ void quant_rows(const AttnArgs& p, const Span& w, int
 }
 
 // 16 consecutive keys lie in one block: their first row's offset in the caches and the block's
-// scales, none (log2 vs = -inf: weight 0) where there is no block or no key.
+// scales, none (log2 vs = -inf: weight 0) where there is no block or no key in [low, end).
 struct Group {
   int64_t at;  // bytes
   float ks, lv, iv;
 };
 template <int D>
-__device__ __forceinline__ Group key_group(const AttnArgs& p, int b, int kvh, int key, int end) {
+__device__ __forceinline__ Group key_group(const AttnArgs& p, int b, int kvh, int key, int low, int end) {
   Group g{0, 0.f, -INFINITY, 0.f};
-  if (key < end) {
+  if (key < end && key + 15 >= low) {
     const int j = key / p.s.bs, off = key - j * p.s.bs;
     const int id = p.s.block(b, j);
     if (id >= 0) {
@@ -499,7 +497,7 @@ __global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const
   const int ntiles = first < w.k1 ? (w.k1 - first + step - 1) / step : 0;
   // lane i: group i % NG of the wave's tile i / NG (of each TPM)
   auto groups = [&](int tile) {
-    return key_group<D>(p, it.b, it.kvh, first + (tile + lane / NG) * step + 16 * (lane % NG), w.k1);
+    return key_group<D>(p, it.b, it.kvh, first + (tile + lane / NG) * step + 16 * (lane % NG), w.low, w.k1);
   };
   Group cur = groups(0), nxt = cur;
   v4i ka[NG][KS];
@@ -710,7 +708,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_block8_tile_kernel(const Attn
   }
   const int ntiles = w.k0 < w.k1 ? (w.k1 - w.k0 + KT - 1) / KT : 0;
   auto groups = [&](int tile) {
-    return key_group<D>(p, it.b, it.kvh, w.k0 + (tile + lane / NG) * KT + 16 * (lane % NG), w.k1);
+    return key_group<D>(p, it.b, it.kvh, w.k0 + (tile + lane / NG) * KT + 16 * (lane % NG), w.low, w.k1);
   };
   Group cur = groups(0), nxt = cur;
   auto base = [&](int i) {

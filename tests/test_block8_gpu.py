@@ -450,6 +450,22 @@ def test_attention_skips_what_is_not_there(new):
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("new", [1, 3, 90])
+def test_blocks_that_left_the_window(new):
+    """Blocks in front of every row's window may be anyone's: their codes and scales are not used."""
+    total, bs, window = [300, 170], 16, 20
+    c = Cache(total, 2, 64, bs)
+    q = coded_queries(2 * new, 4, 64, F16, False)
+    run = lambda: sl8.attn_paged_block8(q, *c.args(), i32(total), cu_lens=offsets([new] * 2), rotate=False,
+                                        window_left=window)
+    want = run()
+    for bad in (math.nan, math.inf):
+        for b, n in enumerate(total):
+            gone = c.table[b, :(n - new - window + 1) // bs].long()
+            c.k[gone], c.v[gone], c.ks[gone], c.vs[gone] = 127, -127, bad, bad
+        assert bool(want.isfinite().all()) and torch.equal(run(), want)
+
+
 @pytest.mark.parametrize("new", [1, 40, 1024])
 def test_long_tail_of_small_weights(new):
     """One key of weight 1 whose value is zero, 2^17 of weight 2^-26.2, which make the output. They stand
