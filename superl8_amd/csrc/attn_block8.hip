@@ -1011,6 +1011,7 @@ extern "C" int sl8_attn_paged_block8(const void* q, int dtype, int rotate, float
   SL8_CHECK_ARG(aligned(q, 16) && aligned(out, 16) && aligned(k_cache, 16) && aligned(v_cache, 16),
                 "fni8 %s: q/k_cache/v_cache must be 16-byte aligned", tag);
   const AttnPlan plan = attn_plan(T, B, Hq, Hkv, D, max_blocks_per_seq * block_size);
+  SL8_CHECK_ARG(plan.grid < (1LL << 32) / A8_THREADS, "fni8 %s: shape too large", tag);
   SL8_CHECK_ARG(plan.bytes == 0 || (workspace && workspace_bytes >= plan.bytes && aligned(workspace, 16)),
                 "fni8 %s: workspace needs %zu bytes", tag, plan.bytes);
   p.q = static_cast<const uint16_t*>(q);

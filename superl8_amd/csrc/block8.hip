@@ -212,7 +212,7 @@ extern "C" int sl8_kv_append_block8(const void* k_new, const void* v_new, const 
   }
   const int64_t grid = page_wgs + q_wgs;
   if (grid == 0) return SL8_OK;
-  SL8_CHECK_ARG(grid < (1LL << 31), "fni8 %s: shape too large", tag);
+  SL8_CHECK_ARG(grid < (1LL << 32) / APP_THREADS, "fni8 %s: shape too large", tag);
   // ceil(2^32 page_wgs / grid): workgroup i has (i share) >> 32 of blocks before it, all of them page_wgs
   p.has_q = q_wgs > 0;
   p.share = p.has_q ? (uint32_t)((((uint64_t)page_wgs << 32) + grid - 1) / grid) : 0;

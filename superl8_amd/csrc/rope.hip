@@ -50,13 +50,14 @@ extern "C" int sl8_rope(const void* q, const void* k, int dtype, int64_t q_strid
   }
   const int n = rope_pairs(D, R, dtype, ptrs, np, strides, ns);
   rope_shape(t, ROPE_THREADS / (int)(D / (2 * n)));
-  const unsigned grid = (unsigned)((t.T + t.tokens - 1) / t.tokens);
+  const int64_t grid = (t.T + t.tokens - 1) / t.tokens;
+  SL8_CHECK_ARG(grid < (1LL << 32) / ROPE_THREADS, "fni8 rope: shape too large");
   const hipStream_t st = static_cast<hipStream_t>(stream);
   auto by_n = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    if (n == 8) rope_kernel<DT, 8><<<grid, ROPE_THREADS, 0, st>>>(a, t);
-    else if (n == 4) rope_kernel<DT, 4><<<grid, ROPE_THREADS, 0, st>>>(a, t);
-    else rope_kernel<DT, 1><<<grid, ROPE_THREADS, 0, st>>>(a, t);
+    if (n == 8) rope_kernel<DT, 8><<<(unsigned)grid, ROPE_THREADS, 0, st>>>(a, t);
+    else if (n == 4) rope_kernel<DT, 4><<<(unsigned)grid, ROPE_THREADS, 0, st>>>(a, t);
+    else rope_kernel<DT, 1><<<(unsigned)grid, ROPE_THREADS, 0, st>>>(a, t);
   };
   if (dtype == SL8_DTYPE_F16) by_n(std::integral_constant<int, SL8_DTYPE_F16>{});
   else if (dtype == SL8_DTYPE_BF16) by_n(std::integral_constant<int, SL8_DTYPE_BF16>{});

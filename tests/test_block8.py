@@ -47,6 +47,9 @@ def attn(**c):
     (attn, dict(Hq=3, Hkv=2), b"divisible"), (attn, dict(T=3), b"one row"), (attn, dict(q=None), b"null"),
     (attn, dict(lens=None), b"null"), (attn, dict(vs=None), b"null"), (attn, dict(q=24), b"aligned"),
     (attn, dict(k=8), b"aligned"), (attn, dict(maxb=1 << 31), b"large"), (attn, dict(maxb=1 << 26), b"large"),
+    (rope, dict(S=(1 << 31) - 1), b"too large"), (append, dict(T=(1 << 28) - 1, B=1, cu=16), b"too large"),
+    (append, dict(T=1 << 23, B=1 << 23), b"too large"),
+    (attn, dict(T=(1 << 24) - 1, B=(1 << 24) - 1, Hq=1), b"too large"),
     (attn, dict(ws=None), b"workspace"), (attn, dict(ws_bytes=100), b"workspace"), (attn, dict(ws=24), b"workspace"),
 ])
 def test_refused(call, change, word):
