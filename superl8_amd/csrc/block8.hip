@@ -75,38 +75,34 @@ append_block8_kernel(const AppendArgs p, const RopeArgs a, const RopeRows q) {
   const Block8Seqs& s = p.s;
   const int lane = threadIdx.x % LPR, r0 = threadIdx.x / LPR;
   const bool is_v = page & 1;
-  const int h = (page >> 1) % p.Hkv;
-  const int64_t unit = (page >> 1) / p.Hkv;
+  const int h = (page >> 1) % p.Hkv, unit = (page >> 1) / p.Hkv;
 
-  // sequence b has units row(b) / bs + 2 b and up, at least as many as blocks that n rows can touch
-  auto first = [&](int b) { return s.cu ? s.row(b) / s.bs + 2LL * b : b; };
-  const int b = s.cu ? seq_of(s.B, threadIdx.x & 63, unit, first) : (int)unit;
-  if (b < 0) return;
-  const int64_t t0 = s.row(b);
-  const int64_t n = s.row(b + 1) - t0, len = s.lens[b], start = len - n;
-  if (n <= 0 || start < 0) return;
-  const int64_t pg = start / s.bs + (unit - first(b));
-  const int64_t lo = max(start, pg * s.bs), hi = min(len, (pg + 1) * s.bs);
+  const Seq q0 = seq_of(s, threadIdx.x & 63, unit);
+  if (q0.n <= 0 || q0.len < q0.n) return;
+  const int start = q0.len - q0.n;
+  const int pg = start / s.bs + q0.nth;
+  if (pg >= s.maxb) return;
+  const int lo = max(start, pg * s.bs), hi = min(q0.len, (pg + 1) * s.bs);
   if (lo >= hi) return;
-  const int id = pg < s.maxb ? s.block(b, (int)pg) : -1;
-  if (id < 0) return;
-  const int off = (int)(lo - pg * s.bs), cnt = (int)(hi - lo);
-  const int64_t tok = t0 + (lo - start);
-
-  const int64_t bh = (int64_t)id * p.Hkv + h;
-  int8_t* cache = (is_v ? p.v_cache : p.k_cache) + bh * s.bs * D;
-  float* scale = (is_v ? p.v_scale : p.k_scale) + bh;
+  const int id = s.block(q0.b, pg);
+  const int off = lo - pg * s.bs, cnt = hi - lo;
+  const int64_t tok = q0.row0 + (lo - start);
   const void* x = is_v ? p.v : p.k;
   const int64_t st = is_v ? p.vst[0] : p.kst[0], sh = is_v ? p.vst[1] : p.kst[1];
-  const float old = off ? *scale : 0.f;
 
-  // all rows' loads go out before the first is used; rows past the last repeat it
+  // all rows' loads go out before the first is used and beside the block's; rows past the last repeat it
   uint4 raw[NP];
 #pragma unroll
   for (int i = 0; i < NP; ++i)
     if (NP <= 4 || i * RPB < cnt)
       raw[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) +
                                                (tok + min(i * RPB + r0, cnt - 1)) * st + h * sh + 8 * lane);
+  if (id < 0) return;
+  const int64_t bh = (int64_t)id * p.Hkv + h;
+  int8_t* cache = (is_v ? p.v_cache : p.k_cache) + bh * s.bs * D;
+  float* scale = (is_v ? p.v_scale : p.k_scale) + bh;
+  const float old = off ? *scale : 0.f;
+
   float f[NP][8];
   float amax = 0.f;
 #pragma unroll

@@ -32,17 +32,27 @@ struct Block8Seqs {
   }
 };
 
-// The last b with first(b) <= i, by a wave (first does not fall, first(0) = 0): 64 sequences a step.
-template <typename F>
-__device__ __forceinline__ int seq_of(int B, int lane, int64_t i, F first) {
-  int n = 0;
-  for (int b0 = 0; b0 < B; b0 += 64) {
-    const int b = b0 + lane;
-    const uint64_t le = __builtin_amdgcn_ballot_w64(b < B && first(b) <= i);
-    n += __popcll(le);
+// The sequence of a unit, by a wave: without cu unit b is sequence b, else sequence b has the units
+// from row(b) / bs + 2 b, at least as many as blocks that n rows can touch. 64 sequences a step, with
+// all that is asked of them: one chain of loads.
+struct Seq {
+  int b, row0, n, len;  // n = 0: none
+  int nth;              // of its units
+};
+__device__ __forceinline__ Seq seq_of(const Block8Seqs& s, int lane, int unit) {
+  if (!s.cu) return {unit, unit, unit < s.B, unit < s.B ? s.lens[unit] : 0, 0};
+  Seq q{};
+  for (int b0 = 0; b0 < s.B; b0 += 64) {
+    const int b = min(b0 + lane, s.B - 1);
+    const int row0 = (int)s.row(b), row1 = (int)s.row(b + 1), len = s.lens[b], first = row0 / s.bs + 2 * b;
+    const uint64_t le = __builtin_amdgcn_ballot_w64(b0 + lane < s.B && first <= unit);
+    if (le == 0) break;
+    const int at = 63 - __builtin_clzll(le);
+    auto of = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
+    q = {b0 + at, of(row0), of(row1) - of(row0), of(len), unit - of(first)};
     if (le != ~0ull) break;
   }
-  return n - 1;
+  return q;
 }
 
 inline int block8_check(const char* tag, const Block8Seqs& s, int64_t Hkv, int64_t D) {
