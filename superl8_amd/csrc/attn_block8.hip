@@ -275,23 +275,33 @@ __device__ __forceinline__ int64_t row_at(const AttnArgs& p, const Span& w, int 
 template <int DT, int D, int ROWS, int THREADS, typename F>
 __device__ __forceinline__ void quant_rows(const AttnArgs& p, const Span& w, int kvh, F place, float* qs_s) {
   constexpr int LPR = row_lanes(D), RPB = THREADS / LPR;
+  constexpr int N = ROWS / RPB > 4 ? 4 : ROWS / RPB > 1 ? ROWS / RPB : 1;  // rows a thread reads at once
+  static_assert(ROWS < RPB || ROWS % (N * RPB) == 0, "whole passes");
   const int lane = threadIdx.x % LPR;
 #pragma unroll 1
-  for (int r1 = 0; r1 < ROWS; r1 += RPB) {
-    const int r = r1 + threadIdx.x / LPR;
-    if (ROWS % RPB && r >= ROWS) break;
-    const bool live = r < w.cnt;
-    float f[8];
-    VecIO<DT>::unpack(reinterpret_cast<const uint4*>(p.q + row_at(p, w, kvh, live ? r : 0, D))[lane], f);
-    if (p.rotate) hadamard_row<D, DT != SL8_DTYPE_F16>(f, lane);
-    float amax = 0.f;
+  for (int r1 = threadIdx.x / LPR; r1 < ROWS; r1 += N * RPB) {
+    uint4 raw[N];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(f[e]));
-    amax = lane_group_max<LPR>(amax);
-    const float s = amax * (1.0f / 127.0f), safe = s == 0.f ? 1.f : s;
-    const uint2 c = row_codes8<DT>(f, safe);
-    reinterpret_cast<uint2*>(place(r))[lane] = live ? c : make_uint2(0, 0);
-    if (lane == 0) qs_s[r] = live ? safe * p.q_mul : 0.f;
+    for (int i = 0; i < N; ++i) {
+      const int r = r1 + i * RPB;
+      raw[i] = reinterpret_cast<const uint4*>(p.q + row_at(p, w, kvh, r < w.cnt ? r : 0, D))[lane];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = r1 + i * RPB;
+      const bool live = r < w.cnt;
+      float f[8];
+      VecIO<DT>::unpack(raw[i], f);
+      if (p.rotate) hadamard_row<D, DT != SL8_DTYPE_F16>(f, lane);
+      float amax = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(f[e]));
+      amax = lane_group_max<LPR>(amax);
+      const float s = amax * (1.0f / 127.0f), safe = s == 0.f ? 1.f : s;
+      const uint2 c = row_codes8<DT>(f, safe);
+      reinterpret_cast<uint2*>(place(r))[lane] = live ? c : make_uint2(0, 0);
+      if (lane == 0) qs_s[r] = live ? safe * p.q_mul : 0.f;
+    }
   }
 }
 
@@ -760,7 +770,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_block8_tile_kernel(const Attn
   const int vt_swz = 16 * v16_swizzle<D>(vkey);
   static_assert(D != 64 || tile_keys<D>() == 64, "");
 
-  auto tile = [&](int j, const int8_t* kt, const uint16_t* vt, int8_t* knext, uint16_t* vnext)
+  auto tile = [&](auto rows, int j, const int8_t* kt, const uint16_t* vt, int8_t* knext, uint16_t* vnext)
       __attribute__((always_inline)) {
     const int i0 = j % TPM * NG;
     const int key0 = w.k0 + j * KT;
@@ -775,48 +785,60 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_block8_tile_kernel(const Attn
     if (i0 + NG == 64) cur = nxt;
     load((i0 + NG) & 63, knext);  // (past the last tile: the pool's first rows)
 
-    v4i sc[RT][NG];
+    if (rows) {
+      v4i sc[RT][NG];
 #pragma unroll
-    for (int g1 = 0; g1 < NG; ++g1) {
-      v4i ka[KS];
+      for (int g1 = 0; g1 < NG; ++g1) {
+        v4i ka[KS];
 #pragma unroll
-      for (int s = 0; s < KS; ++s)
-        ka[s] = *reinterpret_cast<const v4i*>(kt + (16 * g1 + col) * D + 16 * ((4 * s + g4) ^ k_swz));
+        for (int s = 0; s < KS; ++s)
+          ka[s] = *reinterpret_cast<const v4i*>(kt + (16 * g1 + col) * D + 16 * ((4 * s + g4) ^ k_swz));
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        v4i acc = {0, 0, 0, 0};
+        for (int rt = 0; rt < RT; ++rt) {
+          v4i acc = {0, 0, 0, 0};
 #pragma unroll
-        for (int s = 0; s < KS; ++s) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(ka[s], qb[rt][s], acc, 0, 0, 0);
-        sc[rt][g1] = acc;
+          for (int s = 0; s < KS; ++s) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(ka[s], qb[rt][s], acc, 0, 0, 0);
+          sc[rt][g1] = acc;
+        }
       }
-    }
-    v8h wb[RT][NG / 2];
-    st.weights(sc, gks, glv, giv, key0, key0 + KT, g4, wb);
+      v8h wb[RT][NG / 2];
+      st.weights(sc, gks, glv, giv, key0, key0 + KT, g4, wb);
 
-    int swz = vt_swz;
-    if (D > 128) asm volatile("" : "+v"(swz));  // (the tile's own: 16 places kept over the loop spill)
+      int swz = vt_swz;
+      if (D > 128) asm volatile("" : "+v"(swz));  // (the tile's own: 16 places kept over the loop spill)
 #pragma unroll
-    for (int kk = 0; kk < NG / 2; ++kk)
+      for (int kk = 0; kk < NG / 2; ++kk)
 #pragma unroll
-      for (int d = 0; d < DTL; ++d) {
-        const uint16_t* a0 = vt + vt_off + 32 * kk * D + ((16 * d) ^ swz);
-        const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(a0));
-        const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(a0 + 16 * D));
-        const v8h a = __builtin_bit_cast(v8h, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        for (int d = 0; d < DTL; ++d) {
+          const uint16_t* a0 = vt + vt_off + 32 * kk * D + ((16 * d) ^ swz);
+          const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(a0));
+          const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(a0 + 16 * D));
+          const v8h a = __builtin_bit_cast(v8h, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-          st.o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wb[rt][kk], st.o[rt][d], 0, 0, 0);
-      }
-    __builtin_amdgcn_iglp_opt(0);  // reads and products interleaved: 2 % of a long chunk
+          for (int rt = 0; rt < RT; ++rt)
+            st.o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wb[rt][kk], st.o[rt][d], 0, 0, 0);
+        }
+      __builtin_amdgcn_iglp_opt(0);  // reads and products interleaved: 2 % of a long chunk
+    }
     store_v(vnext);
     wait_dma();
     __syncthreads();
   };
-  for (int j = 0; j < ntiles;) {
-    tile(j++, k0_s, v0_s, k1_s, v1_s);
-    if (j >= ntiles) break;
-    tile(j++, k1_s, v1_s, k0_s, v0_s);
-  }
+  auto tiles = [&](auto rows) __attribute__((always_inline)) {
+    for (int j = 0; j < ntiles;) {
+      tile(rows, j++, k0_s, v0_s, k1_s, v1_s);
+      if (j >= ntiles) break;
+      tile(rows, j++, k1_s, v1_s, k0_s, v0_s);
+    }
+  };
+  // A wave whose rows lie behind the unit's last has copies to make and no products. 64 rows: a branch
+  // in the tile, which also keeps the schedule from taking more registers (138 instead of 162 at
+  // D = 128; 40 rows a unit, 191 MB: 58 us, 60 with two loops, 62 without either); 128 rows: two
+  // loops, as the branch costs a full unit 2.5 %.
+  const bool live = 16 * RT * wave < w.cnt;
+  if constexpr (RT == 1) tiles(live);
+  else if (live) tiles(std::true_type{});
+  else tiles(std::false_type{});
 
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
@@ -848,7 +870,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_block8_tile_kernel(const Attn
 // the order of the splits. Bound by the chain of loads: the first partial sums are read beside the
 // maxima that weigh them.
 // ---------------------------------------------------------------------------
-constexpr int JOIN_ROWS = 4, JOIN_AHEAD = 8;
+constexpr int JOIN_ROWS = 4, JOIN_4 = 8;
 template <int DT, int D, int ROWS>
 __global__ void __launch_bounds__(64 * JOIN_ROWS) attn_block8_join_kernel(const AttnArgs p) {
   constexpr int C = D / 64;
@@ -861,9 +883,9 @@ __global__ void __launch_bounds__(64 * JOIN_ROWS) attn_block8_join_kernel(const 
     if constexpr (C == 1) return vc{p.part[(row0 + s * step) * D + lane]};
     else return *reinterpret_cast<const vc*>(p.part + (row0 + s * step) * D + C * lane);
   };
-  vc x[JOIN_AHEAD];
+  vc x[JOIN_4];
 #pragma unroll
-  for (int s = 0; s < JOIN_AHEAD; ++s) x[s] = part(min(s, a.y - 1));
+  for (int s = 0; s < JOIN_4; ++s) x[s] = part(min(s, a.y - 1));
   float mm = A8_NONE;
   for (int s = lane; s < a.y; s += 64) mm = fmaxf(mm, p.ml[row0 + s * step].x);
   mm = wave_max(mm);
@@ -878,16 +900,16 @@ __global__ void __launch_bounds__(64 * JOIN_ROWS) attn_block8_join_kernel(const 
     }
     den += wave_sum(l);
     const int n = min(64, a.y - s0);
-    for (int s = 0; s < n; s += JOIN_AHEAD) {
-      vc y[JOIN_AHEAD];
+    for (int s = 0; s < n; s += JOIN_4) {
+      vc y[JOIN_4];
 #pragma unroll
-      for (int k = 0; k < JOIN_AHEAD; ++k)
-        if (s0 + s + JOIN_AHEAD < a.y) y[k] = part(min(s0 + s + JOIN_AHEAD + k, a.y - 1));
+      for (int k = 0; k < JOIN_4; ++k)
+        if (s0 + s + JOIN_4 < a.y) y[k] = part(min(s0 + s + JOIN_4 + k, a.y - 1));
 #pragma unroll
-      for (int k = 0; k < JOIN_AHEAD; ++k)
+      for (int k = 0; k < JOIN_4; ++k)
         if (s + k < n) o += x[k] * lane_value(f, s + k);
 #pragma unroll
-      for (int k = 0; k < JOIN_AHEAD; ++k) x[k] = y[k];
+      for (int k = 0; k < JOIN_4; ++k) x[k] = y[k];
     }
   }
   const float inv = den > 0.f ? 1.f / den : 0.f;
