@@ -464,6 +464,11 @@ struct RowState {
 //     (ds_read_b64_tr_b8: 8 keys of a channel), in the order of keys that the weights have, and
 //     turned into fp16: O^T += V^T W on v_mfma_f32_16x16x32_f16. 16-byte chunks of a row are
 //     placed by an xor of its key, so that the 16 rows of half a wave lie in different banks.
+// 16 sequences of 32768 tokens, 32 / 8 heads, D = 128, bf16 (1.07 GB): 183 us and 5 for the join, 5.8
+// TB/s, the rate of pure reading. 32 of 270 to 8192 tokens (186 MB): 35 and 5, of which about 10 are
+// the same for any size: the work list, the first loads and the waves' join. One of 777: 11.7, all
+// of that kind (the first kernel, a wave for each row and head with the codes multiplied one by one,
+// took 20 ms, 5 ms and 258 us).
 // ---------------------------------------------------------------------------
 template <int D> constexpr int stream_keys() { return D == 256 ? 32 : 64; }
 template <int D> __device__ __forceinline__ int v_swizzle(int key) {
@@ -674,6 +679,17 @@ __global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const
 // once on its way (10 instructions for 8 codes, which each wave for itself would spend again). The
 // products, the layouts and the softmax are the streaming kernel's; V is read transposed with
 // ds_read_b64_tr_b16. One barrier a tile; other workgroups of the CU run across it.
+//
+// 2048 tokens behind 14336, 32 / 8 heads, D = 128, fp16 (515 GFLOP): 450 us, 1.15 PFLOP/s; its
+// products at the rates of large int8 and fp16 ones would take 359. VALU is busy in 60 % of the
+// cycles (8 instructions a score, 5 of them conversion, fma, maximum, exp2, sum; 1.2 for V's codes)
+// and the matrix pipe in 36 %, and they overlap little. Measured and not taken: 8 waves a workgroup
+// (the same), 32 keys a tile (479), 3 waves a SIMD (spills: 605), products of one tile beside the
+// softmax of another in one wave (541), s_setprio around either (490, 500), accumulators that start at
+// 1.5 * 2^23 instead of the conversion (442, but logits shift by up to 0.75 of a step of the score).
+// 5 tokens of 16 sequences of 1.8 to 16.4 thousand, 64 / 8 heads (40 of 64 rows, 191 MB): 49 us and 6
+// for the join. Prompts of 650 to 1301 tokens with a window of 1024, D = 64, 16 / 4 heads: 46 us, a third of
+// it before the first tile.
 // ---------------------------------------------------------------------------
 template <int D> constexpr int tile_keys() { return D == 256 ? 32 : 64; }
 template <int D> __device__ __forceinline__ int k_swizzle(int key) {  // 16-byte chunks, 16 keys apart
@@ -768,7 +784,6 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_block8_tile_kernel(const Attn
   const int vkey = 4 * g4 + (col >> 2);
   const int vt_off = vkey * D + 4 * (col & 3);                           // (fp16 elements)
   const int vt_swz = 16 * v16_swizzle<D>(vkey);
-  static_assert(D != 64 || tile_keys<D>() == 64, "");
 
   auto tile = [&](auto rows, int j, const int8_t* kt, const uint16_t* vt, int8_t* knext, uint16_t* vnext)
       __attribute__((always_inline)) {
@@ -944,7 +959,10 @@ template <int D_, int RT_, int NW_> struct Shape {
 };
 
 // f(Shape) for `rows` rows of a sequence and KV head on average: what holds them in the fewest units
-// without many empty rows, up to 128.
+// without many empty rows, up to 128. Up to 32 rows the waves stream keys of their own: 20 rows, 16
+// sequences of 8192 keys, D = 128: 34.9 us, 38.3 in tiles of 64 rows; 64 of 2000 keys: 34.0 and 50.2. 40
+// rows (the drafts above) take 57 in tiles, 88 streamed as two units. At D = 256 32 rows' sums do
+// not fit a wave's registers.
 template <typename F>
 auto with_shape(int64_t D, int64_t rows, F&& f) {
   auto by_rows = [&](auto d) {

@@ -120,9 +120,10 @@ __device__ __forceinline__ void st_elems(void* base, int64_t i, const float* f) 
   }
 }
 
-// Rows of Q and K [B, H, S, D] in any strides (elements; the last dimension dense), in and out. A thread holds 2 N elements of a row: N pairs, or 2 N that pass; CH = D / (2 N) threads a
-// row. It keeps its pairs' angles for the heads that it visits: the angles are 2 R / D times an
-// fp16 row's bytes. A workgroup has `tokens` tokens by `slots` head slots.
+// Rows of Q and K [B, H, S, D] in any strides (elements; the last dimension dense), in and out. A
+// thread holds 2 N elements of a row: N pairs, or 2 N that pass; D / (2 N) threads a row. It keeps
+// its pairs' angles for the heads that it visits: the angles are 2 R / D times an fp16 row's
+// bytes. A workgroup has `tokens` tokens by `slots` head slots.
 struct RopeRows {
   const void *q, *k;
   void *q_out, *k_out;
