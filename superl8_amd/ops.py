@@ -334,7 +334,8 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, table
     sin; see rope_table); (p, p + R/2) is a pair, or (2p, 2p+1) with `interleaved`. positions
     int32/int64 [S] or [B,S]; with `sections` (up to 4 counts of consecutive pairs, in order)
     [A,S] or [A,B,S], an axis for each. Positions outside the table count as its nearest end.
-    `inverse` turns back: the gradient of q and k from that of q' and k'."""
+    `inverse` turns back: the gradient of q and k from that of q' and k' (like every operator
+    here it records nothing for autograd; a Function's backward calls it)."""
     return _C.rope(q, k, positions, table, sections, interleaved, inverse)
 
 
@@ -377,7 +378,8 @@ def attn_paged_block8(q: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.Ten
     q [T,Hq,D] fp16/bf16 -> [T,Hq,D] of its dtype: sequence b's rows are cu_lens[b]..cu_lens[b+1]-1
     (None: row b), the last of its context_lens[b] tokens, which the cache holds already. Each sees
     the keys up to itself and, with window_left >= 0, only the last window_left of them; a row
-    that sees none and rows behind the last sequence are zeros."""
+    that sees none and rows behind the last sequence are zeros. Sequences of one call are cut alike,
+    by their mean number of rows: long prompts and single tokens run faster in calls of their own."""
     softmax_scale = (1.0 / (q.shape[-1] ** 0.5)) if scale is None else scale
     q = q.contiguous()
     if q.data_ptr() % 16:
