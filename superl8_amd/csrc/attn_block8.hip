@@ -681,9 +681,9 @@ __global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const
 // ds_read_b64_tr_b16. One barrier a tile; other workgroups of the CU run across it.
 //
 // 2048 tokens behind 14336, 32 / 8 heads, D = 128, fp16 (515 GFLOP): 450 us, 1.15 PFLOP/s; its
-// products at the rates of large int8 and fp16 ones would take 359. VALU is busy in 60 % of the
+// products at the rates of large int8 and fp16 ones would take 359. VALU is busy in 65 % of the
 // cycles (8 instructions a score, 5 of them conversion, fma, maximum, exp2, sum; 1.2 for V's codes)
-// and the matrix pipe in 36 %, and they overlap little. Measured and not taken: 8 waves a workgroup
+// and the matrix pipe in 35 %: they hardly overlap, so every cycle is taken. Measured and not taken: 8 waves a workgroup
 // (the same), 32 keys a tile (479), 3 waves a SIMD (spills: 605), products of one tile beside the
 // softmax of another in one wave (541), s_setprio around either (490, 500), accumulators that start at
 // 1.5 * 2^23 instead of the conversion (442, but logits shift by up to 0.75 of a step of the score).
