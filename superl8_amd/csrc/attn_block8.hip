@@ -61,7 +61,9 @@ struct AttnArgs {
 // known to the host, and a launch to make it costs more than these few hundred cycles (a wave
 // counts 64 sequences at once).
 //
-// Items of a sequence: units x Hkv x splits. A split has at most L tiles, L the least for which
+// Items of a sequence: units x Hkv x splits; unsplit calls have room for a unit more a sequence, so
+// that where one's begin follows from the offsets alone (1024 of one token on 500 to 3000 keys: 644 us, 681
+// with all lengths counted). A split has at most L tiles, L the least for which
 // the items fit the slots that are resident at once, so that a batch of mixed lengths gives every
 // slot about the same number of keys. KV heads are next to each other: item % 8 is the XCD, and
 // the units that read a head's keys meet in its L2.
@@ -130,47 +132,60 @@ __device__ __forceinline__ Item find_item(const AttnArgs& p, int lane, int id) {
     it.end = p.s.T;
     return it;
   }
+  if (!p.slots) {  // whole: units from row0 G / ROWS + b, at least as many as there are
+    Item it{};
+    it.end = p.s.row(p.s.B);
+    const int r = id / p.Hkv;
+    const Seq q = seq_of(p.s, lane, r, [&](int row0, int b) { return row0 * p.G / ROWS + b; });
+    it.kvh = id - r * p.Hkv;
+    it.b = q.b;
+    it.row0 = q.row0;
+    it.n = q.n;
+    it.len = q.len;
+    it.splits = 1;
+    it.units = (max(q.n, 0) * p.G + ROWS - 1) / ROWS;
+    it.unit = it.units - 1 - q.nth;  // (those that see the most keys first)
+    it.live = it.unit >= 0;
+    return it;
+  }
   const SeqWork mine = seq_work<ROWS>(p, lane);
   auto work = [&](int b0) { return b0 == 0 ? mine : seq_work<ROWS>(p, b0 + lane); };
-  float over_l = 0.f;
-  if (p.slots) {
-    int most = 1, pairs = 0;
-    float all = 0.f;
+  int most = 1, whole = 0;
+  float all = 0.f;
+  for (int b0 = 0; b0 < p.s.B; b0 += 64) {
+    const SeqWork w = work(b0);
+    most = max(most, w.units ? w.tiles : 1);
+    whole += w.units;
+    all += (float)w.units * (float)w.tiles;
+  }
+  most = __builtin_amdgcn_readfirstlane(
+      (int)lane_group_reduce<64>((uint32_t)most, [](uint32_t a, uint32_t b) { return a > b ? a : b; }));
+  whole = __builtin_amdgcn_readfirstlane(lane_group_sum<64>(whole)) * p.Hkv;  // items that none is split
+  all = wave_sum(all) * (float)p.Hkv;
+  // the least L with items(L) <= slots, four candidates at once
+  int lo = __builtin_amdgcn_readfirstlane(max(A8_MIN_TILES, (int)(all / (float)p.slots * 0.999f))), hi = most;
+  if (whole < p.slots) hi = min(hi, __builtin_amdgcn_readfirstlane((int)(all / (float)(p.slots - whole))) + 2);
+  while (lo < hi) {
+    const int step = (hi - lo + 4) / 5 > 1 ? (hi - lo + 4) / 5 : 1;
+    int n[4] = {0, 0, 0, 0};
+    float r[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) r[k] = 1.f / (float)(lo + k * step);
     for (int b0 = 0; b0 < p.s.B; b0 += 64) {
       const SeqWork w = work(b0);
-      most = max(most, w.units ? w.tiles : 1);
-      pairs += w.units;
-      all += (float)w.units * (float)w.tiles;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) n[k] += w.units * splits_of(w.tiles, r[k]);
     }
-    most = __builtin_amdgcn_readfirstlane(
-        (int)lane_group_reduce<64>((uint32_t)most, [](uint32_t a, uint32_t b) { return a > b ? a : b; }));
-    pairs = __builtin_amdgcn_readfirstlane(lane_group_sum<64>(pairs)) * p.Hkv;
-    all = wave_sum(all) * (float)p.Hkv;
-    // the least L with items(L) <= slots, four candidates at once
-    int lo = __builtin_amdgcn_readfirstlane(max(A8_MIN_TILES, (int)(all / (float)p.slots * 0.999f))), hi = most;
-    if (pairs < p.slots) hi = min(hi, __builtin_amdgcn_readfirstlane((int)(all / (float)(p.slots - pairs))) + 2);
-    while (lo < hi) {
-      const int step = (hi - lo + 4) / 5 > 1 ? (hi - lo + 4) / 5 : 1;
-      int n[4] = {0, 0, 0, 0};
-      float r[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) r[k] = 1.f / (float)(lo + k * step);
-      for (int b0 = 0; b0 < p.s.B; b0 += 64) {
-        const SeqWork w = work(b0);
+    for (int k = 0; k < 4; ++k) n[k] = __builtin_amdgcn_readfirstlane(lane_group_sum<64>(n[k])) * p.Hkv;
+    int fit = 4;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) n[k] += w.units * splits_of(w.tiles, r[k]);
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) n[k] = __builtin_amdgcn_readfirstlane(lane_group_sum<64>(n[k])) * p.Hkv;
-      int fit = 4;
-#pragma unroll
-      for (int k = 3; k >= 0; --k)
-        if (n[k] <= p.slots) fit = k;
-      if (fit < 4) hi = min(hi, lo + fit * step);
-      if (fit) lo = min(hi, lo + (fit < 4 ? fit - 1 : 3) * step + 1);
-    }
-    over_l = 1.f / (float)max(lo, 1);
+    for (int k = 3; k >= 0; --k)
+      if (n[k] <= p.slots) fit = k;
+    if (fit < 4) hi = min(hi, lo + fit * step);
+    if (fit) lo = min(hi, lo + (fit < 4 ? fit - 1 : 3) * step + 1);
   }
+  const float over_l = 1.f / (float)max(lo, 1);
   Item it{};
   int items = 0, pairs = 0;
   for (int b0 = 0; b0 < p.s.B; b0 += 64) {
@@ -200,7 +215,7 @@ __device__ __forceinline__ Item find_item(const AttnArgs& p, int lane, int id) {
     pairs += __builtin_amdgcn_readlane(pp, 63);
   }
   // (more pairs than places: the offsets fall somewhere, against the contract)
-  if (p.slots && id == 0 && threadIdx.x == 0) *p.count = pairs <= p.max_pairs ? pairs : 0;
+  if (id == 0 && threadIdx.x == 0) *p.count = pairs <= p.max_pairs ? pairs : 0;
   it.end = p.s.T;
   if (p.s.cu) it.end = p.s.B >= 1 && p.s.B <= 64 ? __builtin_amdgcn_readlane(mine.row0 + mine.n, p.s.B - 1) : p.s.row(p.s.B);
   return it;

@@ -83,7 +83,9 @@ append_block8_kernel(const AppendArgs p, const RopeArgs a, const RopeRows q) {
   const bool is_v = page & 1;
   const int h = (page >> 1) % p.Hkv, unit = (page >> 1) / p.Hkv;
 
-  const Seq q0 = seq_of(s, threadIdx.x & 63, unit);
+  // (rows / bs + 2: at least as many units as blocks that n rows can touch)
+  const Seq q0 = s.cu ? seq_of(s, threadIdx.x & 63, unit, [&](int row0, int b) { return row0 / s.bs + 2 * b; })
+                      : Seq{unit, unit, unit < s.B ? 1 : 0, unit < s.B ? s.lens[unit] : 0, 0};
   if (q0.n <= 0 || q0.len < q0.n) return;
   const int start = q0.len - q0.n;
   const int pg = start / s.bs + q0.nth;

@@ -32,27 +32,30 @@ struct Block8Seqs {
   }
 };
 
-// The sequence of a unit, by a wave: without cu unit b is sequence b, else sequence b has the units
-// from row(b) / bs + 2 b, at least as many as blocks that n rows can touch. 64 sequences a step, with
-// all that is asked of them: one chain of loads.
+// The sequence of a unit of work, by a wave: sequence b has the units from first(row(b), b), which rises
+// with b. A 64th of the sequences at a step, then one of 64, with all that is asked of it.
 struct Seq {
   int b, row0, n, len;  // n = 0: none
   int nth;              // of its units
 };
-__device__ __forceinline__ Seq seq_of(const Block8Seqs& s, int lane, int unit) {
-  if (!s.cu) return {unit, unit, unit < s.B, unit < s.B ? s.lens[unit] : 0, 0};
-  Seq q{};
-  for (int b0 = 0; b0 < s.B; b0 += 64) {
-    const int b = min(b0 + lane, s.B - 1);
-    const int row0 = (int)s.row(b), row1 = (int)s.row(b + 1), len = s.lens[b], first = row0 / s.bs + 2 * b;
-    const uint64_t le = __builtin_amdgcn_ballot_w64(b0 + lane < s.B && first <= unit);
-    if (le == 0) break;
-    const int at = 63 - __builtin_clzll(le);
-    auto of = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
-    q = {b0 + at, of(row0), of(row1) - of(row0), of(len), unit - of(first)};
-    if (le != ~0ull) break;
+template <typename F>
+__device__ __forceinline__ Seq seq_of(const Block8Seqs& s, int lane, int unit, F first) {
+  if (s.B == 0) return {};
+  int lo = 0, span = s.B;
+  while (span > 64) {
+    const int step = (span + 63) / 64, b = min(lo + lane * step, s.B - 1);
+    const uint64_t le = __builtin_amdgcn_ballot_w64(lane * step < span && first((int)s.row(b), b) <= unit);
+    const int at = le ? 63 - __builtin_clzll(le) : 0;
+    lo += at * step;
+    span = min(step, span - at * step);
   }
-  return q;
+  const int b = min(lo + lane, s.B - 1);
+  const int row0 = (int)s.row(b), row1 = (int)s.row(b + 1), len = s.lens[b], f = first(row0, b);
+  const uint64_t le = __builtin_amdgcn_ballot_w64(lane < span && f <= unit);
+  if (le == 0) return {};
+  const int at = 63 - __builtin_clzll(le);
+  auto of = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
+  return {lo + at, of(row0), of(row1) - of(row0), of(len), unit - of(f)};
 }
 
 inline int block8_check(const char* tag, const Block8Seqs& s, int64_t Hkv, int64_t D) {

@@ -261,7 +261,7 @@ def plain_attn(c, q, new, total, rotate, scale, window):
     G = q.shape[1] // Hkv
     t = 0
     for b, (m, n) in enumerate(zip(new, total)):
-        for h in range(Hkv):
+        for h in range(Hkv if m else 0):
             k, v, vs = c.rows(b, h, n)
             for j in range(h * G, h * G + G):
                 w = x[t:t + m, j] @ k.T * scale
@@ -343,6 +343,30 @@ def test_many_sequences_one_long(B, new, cu):
     total[B // 2], total[B - 1] = 3333, 1500
     c = Cache(total, 1, 128, 16)
     attn_and_check(c, coded_queries(B * new, 4, 128, F16, False), [new] * B, total, cu=cu)
+
+
+@pytest.mark.parametrize("B", [63, 65, 700, 5000])
+def test_many_sequences_some_without_rows(B):
+    """Sequences of 0 to 3 new tokens found by their offsets, the first and the last ones empty."""
+    new = [0, 0] + [(i * 7) % 4 for i in range(B - 4)] + [0, 0]
+    total = [n + (i * 5) % 21 for i, n in enumerate(new)]
+    c = Cache(total, 1, 64, 16)
+    q, k, v = news(sum(new), 1, 1, 64, F16)
+    append_and_check(c, new, total, k, v)
+    for Hq in (2, 80)[:1 if B > 100 else 2]:  # a unit or several of a token
+        attn_and_check(c, coded_queries(sum(new), Hq, 64, F16, False), new, total)
+
+
+@pytest.mark.parametrize("new", [1, 2, 7])
+@pytest.mark.parametrize("Hq,D", [(17, 128), (33, 64), (65, 128), (130, 64), (200, 256), (300, 128)])
+@pytest.mark.parametrize("cu", [True, False])
+def test_wide_groups(new, Hq, D, cu):
+    """All query heads on one KV head: groups that end inside a unit or span several."""
+    if not cu and new > 1:
+        return
+    total = [30 + new, 1500, new]
+    c = Cache(total, 1, D, 32)
+    attn_and_check(c, coded_queries(3 * new, Hq, D, F16, False), [new] * 3, total, cu=cu)
 
 
 @pytest.mark.parametrize("new", [1, 4, 300])
