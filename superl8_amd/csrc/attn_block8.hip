@@ -14,6 +14,7 @@
 //
 // Rows of a sequence and KV head are (token, query head of the group), G = Hq / Hkv to a token; a
 // unit is ROWS of them that share every byte of K and V.
+#include <algorithm>
 #include <atomic>
 #include <climits>
 
@@ -1012,13 +1013,16 @@ AttnPlan attn_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int
   with_shape(D, a.rows, [&](auto sh) {
     constexpr int ROWS = decltype(sh)::ROWS;
     a.pairs = Hkv * (T * G / ROWS + B);
-    // Splits pay where workgroups would idle, or wait for the longest sequence of a batch: with few
-    // rows, whose joining is cheap, up to as many pairs as slots; with many, up to half of them
-    // (720 pairs of 128 rows on 768 slots, D = 64: 48 us whole, 70 split).
+    // Splits pay where workgroups would idle, or wait for the longest sequence of a batch, and all
+    // pairs fit the slots. With many rows, whose joining costs, only where half the slots may lie idle:
+    // full units or sequences for no more than that (8 x 120 tokens on 5000 keys, 32/8 heads: 106 us, 149
+    // whole; 512 tokens beside 31 of one on 2 to 6 thousand keys: 79, 115 whole; but 720 pairs of 128
+    // rows on 768 slots, D = 64: 48 us whole, 70 split).
     const int64_t slots = (int64_t)cu_count() * decltype(sh)::wgs_per_cu();
     // Short contexts stay whole: joining costs a launch (one token on 777 keys, 32/8 heads: 13.7 us
     // whole, 17.0 split).
-    const bool split = keys > A8_WHOLE_KEYS && (decltype(sh)::NW ? 2 * a.pairs : a.pairs) <= slots;
+    const int64_t least = Hkv * std::max(B, T * G / ROWS);
+    const bool split = keys > A8_WHOLE_KEYS && a.pairs <= slots && (decltype(sh)::NW == 0 || 2 * least <= slots);
     a.slots = split ? (int)slots : 0;
     a.grid = a.slots ? slots : a.pairs;
     if (a.slots) a.bytes = (size_t)a.grid * ROWS * (D + 2) * 4 + (size_t)a.pairs * 32 + 16;
