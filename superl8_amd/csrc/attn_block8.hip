@@ -28,7 +28,6 @@ namespace {
 constexpr int A8_THREADS = 256, A8_WAVES = 4;
 constexpr int A8_TILE = 64;       // keys: what splits and units' first keys are multiples of
 constexpr int A8_MIN_TILES = 4;   // least keys of a split: a tile for each wave
-constexpr int A8_WHOLE_KEYS = 1024; // contexts up to here are not split
 constexpr float A8_NONE = -1e30f; // reference of nothing
 constexpr float A8_LAG = 15.f;    // log2 of the largest weight (fp16 holds it)
 constexpr float A8_HEAD = 8.f;    // log2 of a maximum's weight when it becomes the reference
@@ -49,6 +48,7 @@ struct AttnArgs {
   int window;  // below 0: none
   bool rotate;
   int slots;      // workgroups to split the keys over, 0: no splits
+  int whole;      // contexts of up to so many tiles are not split
   int max_pairs;  // that the workspace has places for
   // splits only: partial sums [grid][ROWS][D], (m, l) [grid][ROWS], what to join of each pair
   float* part;
@@ -98,8 +98,8 @@ __device__ __forceinline__ SeqWork seq_work(const AttnArgs& p, int b) {
 
 // Splits of a sequence: near tiles / L, rounded up (a unit's keys are cut in that many equal parts,
 // so a rounding of the quotient leaves nothing out).
-__device__ __forceinline__ int splits_of(int tiles, float over_l) {
-  return max(1, (int)ceilf((float)tiles * over_l));
+__device__ __forceinline__ int splits_of(const AttnArgs& p, int tiles, float over_l) {
+  return tiles <= p.whole ? 1 : max(1, (int)ceilf((float)tiles * over_l));
 }
 
 // Inclusive sum over the wave: DPP row shifts, then the rows' last lanes.
@@ -175,7 +175,7 @@ __device__ __forceinline__ Item find_item(const AttnArgs& p, int lane, int id) {
     for (int b0 = 0; b0 < p.s.B; b0 += 64) {
       const SeqWork w = work(b0);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) n[k] += w.units * splits_of(w.tiles, r[k]);
+      for (int k = 0; k < 4; ++k) n[k] += w.units * splits_of(p, w.tiles, r[k]);
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) n[k] = __builtin_amdgcn_readfirstlane(lane_group_sum<64>(n[k])) * p.Hkv;
@@ -191,7 +191,7 @@ __device__ __forceinline__ Item find_item(const AttnArgs& p, int lane, int id) {
   int items = 0, pairs = 0;
   for (int b0 = 0; b0 < p.s.B; b0 += 64) {
     const SeqWork w = work(b0);
-    const int s = splits_of(w.tiles, over_l);
+    const int s = splits_of(p, w.tiles, over_l);
     const int np = w.units * p.Hkv, ni = np * s;
     const int ii = wave_scan(ni), pp = wave_scan(np);
     const uint64_t past = __builtin_amdgcn_ballot_w64(items + ii > id);
@@ -1000,7 +1000,7 @@ auto with_shape(int64_t D, int64_t rows, F&& f) {
 struct AttnPlan {
   int64_t rows;  // of a sequence and KV head on average
   int64_t pairs;
-  int slots;
+  int slots, whole;
   int64_t grid;
   size_t bytes;
 };
@@ -1019,10 +1019,14 @@ AttnPlan attn_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int
     // whole; 512 tokens beside 31 of one on 2 to 6 thousand keys: 79, 115 whole; but 720 pairs of 128
     // rows on 768 slots, D = 64: 48 us whole, 70 split).
     const int64_t slots = (int64_t)cu_count() * decltype(sh)::wgs_per_cu();
-    // Short contexts stay whole: joining costs a launch (one token on 777 keys, 32/8 heads: 13.7 us
-    // whole, 17.0 split).
     const int64_t least = Hkv * std::max(B, T * G / ROWS);
-    const bool split = keys > A8_WHOLE_KEYS && a.pairs <= slots && (decltype(sh)::NW == 0 || 2 * least <= slots);
+    // Short contexts stay whole: joining costs a launch (one token on 777 keys, 32/8 heads: 13.7 us
+    // whole, 17.0 split), and with many rows 2 D sums of 32 bits for each of them, against a time that
+    // goes by D: 300 tokens on 1000 keys (72 of 512 slots) 31 us whole, 33 split, on 2000 48 and 38;
+    // 4 x 250 (248 slots) on 1200 keys 47 and 53, on 2000 69 and 62; D = 64, 4 x 300 on 2000 37 and 41,
+    // on 3000 50 and 47; D = 256, 2 x 180 on 751 52 and 40.
+    a.whole = decltype(sh)::NW ? (int)(128 * (12 * slots + 32 * std::min(least, slots)) / (D * slots)) : 16;
+    const bool split = keys > a.whole * A8_TILE && a.pairs <= slots && (decltype(sh)::NW == 0 || 2 * least <= slots);
     a.slots = split ? (int)slots : 0;
     a.grid = a.slots ? slots : a.pairs;
     if (a.slots) a.bytes = (size_t)a.grid * ROWS * (D + 2) * 4 + (size_t)a.pairs * 32 + 16;
@@ -1081,6 +1085,7 @@ extern "C" int sl8_attn_paged_block8(const void* q, int dtype, int rotate, float
   p.rotate = rotate != 0;
   p.window = window_left < 0 ? -1 : (int)(window_left < (1 << 30) ? window_left : (1 << 30));
   p.slots = plan.slots;
+  p.whole = plan.whole;
   p.max_pairs = (int)plan.pairs;
   if (num_blocks == 0) p.s.maxb = 0;  // nothing to read: no key is there
   const hipStream_t st = static_cast<hipStream_t>(stream);
