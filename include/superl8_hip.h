@@ -428,7 +428,7 @@ int sl8_kv_append_block8(const void* k_new, const void* v_new, const void* q, in
  * sequence's n sees keys <= context_lens - n + i, and with window_left >= 0 keys > that -
  * window_left; zeros where it sees none and in rows behind the last sequence. All 16-byte aligned.
  * workspace: sl8_attn_paged_block8_workspace() bytes (current device; max_context_len =
- * max_blocks_per_seq * block_size), uninitialised. */
+ * max_blocks_per_seq * block_size; 0 for sizes that the call refuses), uninitialised. */
 size_t sl8_attn_paged_block8_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
                                        int64_t max_context_len);
 int sl8_attn_paged_block8(const void* q, int dtype, int rotate, float q_scale_mul,

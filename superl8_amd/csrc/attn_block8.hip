@@ -1042,7 +1042,9 @@ using namespace sl8;
 
 extern "C" size_t sl8_attn_paged_block8_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
                                                     int64_t max_context_len) {
+  // (sizes that the call refuses: nothing to compute, and no quotient by a head dim of 0)
   if (T <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || T >= (1LL << 28) || B >= (1 << 24) || Hq >= (1 << 16)) return 0;
+  if ((D != 64 && D != 128 && D != 256) || Hq % Hkv) return 0;
   return attn_plan(T, B, Hq, Hkv, D, max_context_len).bytes;
 }
 

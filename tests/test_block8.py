@@ -1,12 +1,17 @@
 """The C entries of rope and the block-scaled paged cache refuse what they cannot run before any device
 work: no GPU needed."""
 import ctypes
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
 
 import superl8_amd as sl8
 from superl8_amd import _lib
+
+ROOT = Path(__file__).resolve().parent.parent
 
 
 def rope(**c):
@@ -61,6 +66,17 @@ def test_refused(call, change, word):
                                          (attn, dict(T=0, B=0)), (attn, dict(Hq=0))])
 def test_nothing_to_do(call, change):
     assert call(**change) == 0
+
+
+@pytest.mark.parametrize("T,B,Hq,Hkv,D", [(100, 1, 8, 2, 0), (100, 1, 8, 2, 96), (100, 1, 8, 2, -64), (100, 1, 8, 3, 64),
+                                          (100, 1, 2, 4, 64), (0, 1, 8, 2, 64), (100, 0, 8, 2, 64), (100, 1, 0, 2, 64),
+                                          (100, 1, 8, 0, 64), (-1, 1, 8, 2, 64), (1 << 28, 1, 8, 2, 64)])
+def test_workspace_of_refused_sizes(T, B, Hq, Hkv, D):
+    """A C caller asks before the call that refuses: nothing to reserve, and the process goes on."""
+    code = f"from superl8_amd import _lib; assert _lib.load().sl8_attn_paged_block8_workspace({T}, {B}, {Hq}, " \
+           f"{Hkv}, {D}, 1 << 20) == 0"
+    assert subprocess.run([sys.executable, "-c", code], cwd=ROOT).returncode == 0
+    assert _lib.load().sl8_attn_paged_block8_workspace(100, 1, 8, 2, 64, 1 << 20) > 0
 
 
 def test_cpu_tensors_are_refused():
