@@ -397,7 +397,7 @@ int sl8_rope(const void* q, const void* k, int dtype, int64_t q_stride_b, int64_
  * Block-scaled paged int8 KV cache: codes int8 [num_blocks, Hkv, block_size, D] with one fp32
  * scale per block and head [num_blocks, Hkv], for K and for V; D 64 / 128 / 256, block_size a
  * multiple of 16 up to 128. New tokens are rows of one list [T, H, D]: sequence b's are rows
- * cu_lens[b] .. cu_lens[b+1] - 1 (cu_lens int32 [B+1] on the device, not falling, from 0; NULL:
+ * cu_lens[b] .. cu_lens[b+1] - 1 (cu_lens int32 [B+1] on the device, not falling; NULL:
  * row b, T = B) and the last of its context_lens[b] tokens; block_table int32
  * [B, max_blocks_per_seq] as in the paged cache above. Block ids outside the pool are skipped.
  * No counterpart in the reference, whose paged cache has a scale per token.
@@ -426,7 +426,8 @@ int sl8_kv_append_block8(const void* k_new, const void* v_new, const void* q, in
  * (rotate != 0: times the normalised Hadamard matrix first, as the keys), each row quantised to int8
  * with one scale times q_scale_mul (softmax_scale * log2 e) -> out [T,Hq,D] of q's type. Row i of a
  * sequence's n sees keys <= context_lens - n + i, and with window_left >= 0 keys > that -
- * window_left; zeros where it sees none and in rows behind the last sequence. All 16-byte aligned.
+ * window_left; zeros where it sees none and in rows of no sequence (in front of the first, behind the
+ * last). All 16-byte aligned.
  * workspace: sl8_attn_paged_block8_workspace() bytes (current device; max_context_len =
  * max_blocks_per_seq * block_size; 0 for sizes that the call refuses), uninitialised. */
 size_t sl8_attn_paged_block8_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,

@@ -77,7 +77,7 @@ struct SeqWork {
 struct Item {
   int b, row0, n, len;
   int unit, kvh, split, splits, units, pair;
-  int64_t end;  // rows of all sequences
+  int64_t begin, end;  // rows of all sequences
   bool live;
 };
 
@@ -135,6 +135,7 @@ __device__ __forceinline__ Item find_item(const AttnArgs& p, int lane, int id) {
   }
   if (!p.slots) {  // whole: units from row0 G / ROWS + b, at least as many as there are
     Item it{};
+    it.begin = p.s.row(0);
     it.end = p.s.row(p.s.B);
     const int r = id / p.Hkv;
     const Seq q = seq_of(p.s, lane, r, [&](int row0, int b) { return row0 * p.G / ROWS + b; });
@@ -217,6 +218,7 @@ __device__ __forceinline__ Item find_item(const AttnArgs& p, int lane, int id) {
   }
   // (more pairs than places: the offsets fall somewhere, against the contract)
   if (id == 0 && threadIdx.x == 0) *p.count = pairs <= p.max_pairs ? pairs : 0;
+  it.begin = __builtin_amdgcn_readlane(mine.row0, 0);
   it.end = p.s.T;
   if (p.s.cu) it.end = p.s.B >= 1 && p.s.B <= 64 ? __builtin_amdgcn_readlane(mine.row0 + mine.n, p.s.B - 1) : p.s.row(p.s.B);
   return it;
@@ -271,13 +273,16 @@ __device__ __forceinline__ void note_pair(const AttnArgs& p, const Span& w, cons
   p.pairs[2 * it.pair + 1] = make_int4((int)w.row0, w.r0, w.cnt, 0);
 }
 
-// Rows behind the last sequence (from `end`) are zeros.
-__device__ __forceinline__ void zero_tail(const AttnArgs& p, int64_t end, int D) {
-  if (end >= p.s.T) return;
+// Rows in front of the first sequence and behind the last are zeros.
+__device__ __forceinline__ void zero_rest(const AttnArgs& p, const Item& it, int D) {
+  const int64_t n = it.begin + p.s.T - it.end;
+  if (n == 0) return;
   const int64_t chunks = (int64_t)p.Hq * D / 8;
   uint4* o = static_cast<uint4*>(p.out);
-  for (int64_t t = end + blockIdx.x; t < p.s.T; t += gridDim.x)
-    for (int64_t i = threadIdx.x; i < chunks; i += blockDim.x) o[t * chunks + i] = make_uint4(0, 0, 0, 0);
+  for (int64_t i = blockIdx.x; i < n; i += gridDim.x) {
+    const int64_t t = i < it.begin ? i : it.end + i - it.begin;
+    for (int64_t c = threadIdx.x; c < chunks; c += blockDim.x) o[t * chunks + c] = make_uint4(0, 0, 0, 0);
+  }
 }
 
 // Row r of a unit: its offset in q and out.
@@ -507,7 +512,7 @@ __global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const
   const int col = lane & 15, g4 = lane >> 4;
 
   const Item it = find_item<ROWS>(p, lane, blockIdx.x);
-  zero_tail(p, it.end, D);
+  zero_rest(p, it, D);
   if (!it.live) return;
   const Span w = item_span<ROWS>(p, it);
   // places: K's lane in a group, the copies' lanes (16-byte chunk of the row that goes to the
@@ -736,7 +741,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_block8_tile_kernel(const Attn
   typedef short v8s __attribute__((ext_vector_type(8)));
 
   const Item it = find_item<ROWS>(p, lane, blockIdx.x);
-  zero_tail(p, it.end, D);
+  zero_rest(p, it, D);
   if (!it.live) return;
   const Span w = item_span<ROWS>(p, it);
 

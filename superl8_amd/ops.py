@@ -378,7 +378,7 @@ def attn_paged_block8(q: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.Ten
     q [T,Hq,D] fp16/bf16 -> [T,Hq,D] of its dtype: sequence b's rows are cu_lens[b]..cu_lens[b+1]-1
     (None: row b), the last of its context_lens[b] tokens, which the cache holds already. Each sees
     the keys up to itself and, with window_left >= 0, only the last window_left of them; a row
-    that sees none and rows behind the last sequence are zeros."""
+    that sees none and rows of no sequence (a padded batch, offsets of a part of one) are zeros."""
     softmax_scale = (1.0 / (q.shape[-1] ** 0.5)) if scale is None else scale
     q = q.contiguous()
     if q.data_ptr() % 16:

@@ -438,6 +438,32 @@ def test_unread_places(new):
     assert torch.equal(got, want) and not got[3 * new:].any() and bool(got[:3 * new].isfinite().all())
 
 
+@pytest.mark.parametrize("B,new,n", [(2, 1, 90), (3, 3, 150), (2, 90, 201), (100, 1, 40), (3, 1, 3000), (70, 5, 2500),
+                                     (2, 100, 5000)])
+def test_rows_of_no_sequence(B, new, n):
+    """Offsets that start behind row 0 and end in front of the last, as a part of a batch has them: the rows of no
+    sequence append nothing and are zeros in whole and in split calls, whatever the memory held."""
+    total = [n - 3 * (i % 9) for i in range(B)]
+    front, back, rows = 6, 5, B * new
+    c = Cache(total, 1, 64, 16)
+    q, k, v = news(front + rows + back, 4, 1, 64, F16)
+    part = slice(front, front + rows)
+    cu, lens = offsets([new] * B), i32(total)
+    d = c.copy()
+    sl8.quantize_kv_append_block8(k, v, *c.args(), lens, cu_lens=cu + front, rotate=False)
+    sl8.quantize_kv_append_block8(k[part], v[part], *d.args(), lens, cu_lens=cu, rotate=False)
+    assert torch.equal(c.k, d.k) and torch.equal(c.v, d.v) and torch.equal(c.ks, d.ks) and torch.equal(c.vs, d.vs)
+    q = q.contiguous()
+    want = sl8.attn_paged_block8(q[part], *c.args(), lens, cu_lens=cu, rotate=False)
+    torch.full_like(q, math.nan)  # (its memory is the output's next)
+    got = sl8.attn_paged_block8(q, *c.args(), lens, cu_lens=cu + front, rotate=False)
+    assert not got[:front].any() and not got[front + rows:].any()
+    # (the mean rows of a sequence may choose another kernel: both within 2^-10 of sum p |v| and half a step)
+    assert float((got[part].double() - want.double()).abs().max()) <= 2.0 ** -9 * 127 * 1.5 * 3.5 / 127
+    none = sl8.attn_paged_block8(q, *c.args()[:4], c.table[:0], i32([]), cu_lens=i32([front]))
+    assert not none.any()
+
+
 @pytest.mark.parametrize("new", [1, 3, 90])
 def test_attention_skips_what_is_not_there(new):
     """A block id outside the pool hides its keys; contexts beyond the table end with it; negative ones
