@@ -398,12 +398,13 @@ struct RowState {
 
   // Weights of NG groups of 16 keys from their scores (lane (g4, col): keys 16 g + 4 g4 + i from
   // key0): B operands of keys 32 kk + {4 g4 + i, 16 + 4 g4 + i}. The reference m stands 2^A8_HEAD
-  // to 2^A8_LAG below the maximum, so that most tiles need no exchange across lanes and no scaling,
-  // and the 16-bit weights, as exact there as near 1, still hold 2^-32 of the largest: 2^20 keys below
-  // that are 2^-13 of the output at most (with the maximum as reference, a tail of 2^17 keys of
-  // weight 2^-26 was lost; the two steps of the reference cost 1 %, 3 % in short prompts). The sum
-  // takes the weights in 32 bits: in a block of small values a large one may have no 16-bit form beside
-  // V's largest.
+  // to 2^A8_LAG below the maximum, so that most tiles need no exchange across lanes and no scaling.
+  // The largest 16-bit weight is 2^A8_HEAD at least, half a step of the subnormal ones 2^-25: beside its
+  // relative 2^-11 a weight is off by 2^-33 of the largest, and one below that is lost. N keys shift
+  // the output by N * 2^-33 * 127 vs of the largest contribution at most, whatever that one's own
+  // value is (with the maximum as reference, a tail of 2^17 keys of weight 2^-26 behind a value of zero
+  // was lost; the two steps of the reference cost 1 %, 3 % in short prompts). The sum takes the weights
+  // in 32 bits: in a block of small values a large one may have no 16-bit form beside V's largest.
   template <int NG>
   __device__ __forceinline__ void weights(const v4i (&sc)[RT][NG], const float (&ks)[NG], const float (&lv)[NG],
                                           const float (&iv)[NG], int key0, int keys_end, int g4,

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import superl8_amd as sl8
-from superl8_amd import _C
+from superl8_amd import _C, _lib
 from tests.test_rope_gpu import check as check_rope
 from tests.test_rope_gpu import turned
 
@@ -294,6 +294,34 @@ def attn_and_check(c, q, new, total, rotate=False, scale=None, window=-1, cu=Tru
     return got
 
 
+def attn_and_check_small_weights(c, q, new, total, window=-1, scale=None):
+    """attn_and_check with what the 16-bit weights keep: the largest contribution's weight is 2^8 at least, half a
+    step of the subnormal ones 2^-25, so a weight is off by 2^-33 of that contribution's beside its 2^-11."""
+    got = attn_and_check(c, q, new, total, window=window, scale=scale)
+    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    want, size, top = plain_attn(c, q, new, total, False, scale, window)
+    N, eps = max(total), torch.finfo(q.dtype).eps / 2
+    lim = size * (2.0 ** -11 + 2.0 ** -15 + N * 2.0 ** -24) + N * 127 * 2.0 ** -33 * top + \
+        eps * (1 + 2.0 ** -8) * want.abs() + 2.0 ** -25
+    err = (got.double() - want).abs()
+    assert bool((err <= lim).all()), (float((err - lim).max()), float(err.max()))
+
+
+def split_tiles(T, B, Hq, Hkv, D, keys):
+    """Tiles of 64 keys above which a sequence's keys are split over workgroups, from the size of the
+    workspace (which holds ROWS rows for every workgroup that is resident at once); no workspace, no split."""
+    ws = _lib.load().sl8_attn_paged_block8_workspace(T, B, Hq, Hkv, D, keys)
+    assert ws > 0
+    G = Hq // Hkv
+    rows = -(-T * G // B)
+    ROWS = 16 if rows <= 16 else 32 if rows <= 32 and D < 256 else 64 if rows <= 64 else 128
+    pairs = Hkv * (T * G // ROWS + B)
+    slots = (ws - 32 * pairs - 16) // (ROWS * (D + 2) * 4)
+    if ROWS <= 32:
+        return 16
+    return 128 * (12 * slots + 32 * min(Hkv * max(B, T * G // ROWS), slots)) // (D * slots)
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("bs", [16, 48, 128])
 @pytest.mark.parametrize("Hq,Hkv", [(4, 4), (8, 2), (8, 1), (6, 2)])
@@ -514,6 +542,34 @@ def test_blocks_that_left_the_window(new):
             gone = c.table[b, :(n - new - window + 1) // bs].long()
             c.k[gone], c.v[gone], c.ks[gone], c.vs[gone] = 127, -127, bad, bad
         assert bool(want.isfinite().all()) and torch.equal(run(), want)
+
+
+@pytest.mark.parametrize("D,window", [(64, 3001), (128, 1500), (128, 3001), (256, 1500), (256, 3001)])
+@pytest.mark.parametrize("B,new", [(3, 1), (3, 5), (3, 12), (2, 20), (2, 150), (70, 1), (70, 5)])
+@pytest.mark.parametrize("Hq,Hkv", [(4, 1), (2, 2)])
+def test_window_over_split_keys(D, window, B, new, Hq, Hkv):
+    """Windows that begin and end inside the keys of a split, with splits that some rows of a unit do not see."""
+    total = [9000, 5003, 2600][:B] + [new + (i * 31) % 90 for i in range(B - 3)]
+    T, bs = B * new, 16
+    assert window // 64 > split_tiles(T, B, Hq, Hkv, D, -(-9000 // bs) * bs)
+    c = Cache(total, Hkv, D, bs)
+    attn_and_check_small_weights(c, coded_queries(T, Hq, D, F16, False), [new] * B, total, window)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 5, 30, 200])
+@pytest.mark.parametrize("step", [10.0, 20.0, 24.5])
+def test_small_weights(D, new, step):
+    """The key of the largest weight has a value of zero; 40000 of 2^-step to 2^-(1.16 step) of it make the output."""
+    N = 40000
+    c = Cache([N], 1, D, 64)
+    c.k[:], c.v[:], c.ks[:], c.vs[:] = 0, c.v.abs().clamp(min=1), 1 / 127, 1
+    c.k[..., 0].random_(-20, 1)
+    first = int(c.table[0, 0])
+    c.k[first, 0, 0, 0], c.v[first, 0, 0] = 127, 0
+    q = torch.zeros(new, 4, D, device=DEV, dtype=F16)
+    q[..., 0] = 1
+    attn_and_check_small_weights(c, q, [new], [N], scale=step / LOG2E)
 
 
 @pytest.mark.parametrize("new", [1, 40, 1024])
