@@ -325,6 +325,31 @@ def rope_table(max_positions: int, rotary_dim: int, *, base: float = 10000.0, se
     return torch.cat([angle.cos(), angle.sin()], 1).float()
 
 
+class _Rope(torch.autograd.Function):
+    """`rope` where a gradient is wanted: that of q and k is the turn back of that of q' and k'."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, table, sections, interleaved, inverse):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(positions, table)
+        ctx.how = dict(sections=sections, interleaved=interleaved, inverse=not inverse)
+        return _C.rope(q, k, positions, table, sections, interleaved, inverse)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        if torch.cuda.is_current_stream_capturing():
+            # (a leaf's node of an eager graph that lives waits on its own stream, which is none of
+            # the capture: that ends the process)
+            raise RuntimeError("fni8 rope: its backward cannot be captured; capture "
+                               "rope(dq, dk, ..., inverse=True) under no_grad instead")
+        dq, dk = (d if need else None for d, need in zip((dq, dk), ctx.needs_input_grad))
+        if dq is not None:
+            dq, dk = rope(dq, dk, *ctx.saved_tensors, **ctx.how)
+        elif dk is not None:
+            dk, _ = rope(dk, None, *ctx.saved_tensors, **ctx.how)
+        return dq, dk, None, None, None, None, None
+
+
 def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, table: torch.Tensor, *,
          sections=None, interleaved: bool = False, inverse: bool = False):
     """Rotary positions of q [B,Hq,S,D] and k [B,Hkv,S,D] (or None) in one launch, fp16/bf16/fp32:
@@ -334,8 +359,12 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, table
     sin; see rope_table); (p, p + R/2) is a pair, or (2p, 2p+1) with `interleaved`. positions
     int32/int64 [S] or [B,S]; with `sections` (up to 4 counts of consecutive pairs, in order)
     [A,S] or [A,B,S], an axis for each. Positions outside the table count as its nearest end.
-    `inverse` turns back: the gradient of q and k from that of q' and k' (like every operator
-    here it records nothing for autograd; a Function's backward calls it)."""
+    `inverse` turns back, which is the gradient of q and k from that of q' and k': autograd records
+    it for q and k that require one (not for the table), except that the backward cannot be captured
+    into a graph: there call rope(dq, dk, ..., inverse=True)."""
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _Rope.apply(q, k, positions, table, None if sections is None else tuple(sections),
+                           interleaved, inverse)
     return _C.rope(q, k, positions, table, sections, interleaved, inverse)
 
 

@@ -138,6 +138,71 @@ def test_inverse_is_the_gradient(interleaved):
     assert abs(float(num - (got.double() * d.double()).sum())) <= q.numel() * 2.0 ** -20
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("sections,interleaved,inverse", [(None, False, False), ((9, 23), True, False),
+                                                          ((16, 8, 8), False, True)])
+def test_autograd(dtype, sections, interleaved, inverse):
+    """What requires a gradient gets the turn back of the outputs' gradients, whichever of them there are."""
+    q, k, pos, table = inputs(2, 4, 2, 9, 80, 64, len(sections or (0,)), dtype)
+    pos = pos if sections else pos[0]
+    how = dict(sections=sections, interleaved=interleaved)
+    gq, gk = torch.randn_like(q), torch.randn_like(k)
+    wq, wk = sl8.rope(gq, gk, pos, table, **how, inverse=not inverse)
+    run = lambda q, k: sl8.rope(q, k, pos, table, **how, inverse=inverse)
+    plain = run(q, k)
+    assert not any(t.requires_grad for t in plain)
+    lq, lk = q.clone().requires_grad_(), k.clone().requires_grad_()
+    yq, yk = run(lq, lk)
+    assert torch.equal(yq, plain[0]) and torch.equal(yk, plain[1])
+    torch.autograd.backward((yq, yk), (gq, gk))
+    assert torch.equal(lq.grad, wq) and torch.equal(lk.grad, wk)
+    x = q.double().requires_grad_()
+    p = pos if sections else pos[None]
+    turned(x, p, table, sections, interleaved, inverse)[0].backward(gq.double())
+    check(lq.grad, x.grad, turned(gq, p, table, sections, interleaved, not inverse)[1])
+    # one of the outputs, one of the inputs, no k, nothing
+    assert torch.equal(torch.autograd.grad(run(lq, lk)[1], lk, gk)[0], wk)
+    assert torch.equal(torch.autograd.grad(run(lq, lk)[0], lq, gq)[0], wq)
+    assert torch.autograd.grad(run(lq, lk)[0], lk, gq, allow_unused=True)[0] is None
+    assert torch.equal(torch.autograd.grad(run(q, lk), lk, (gq, gk))[0], wk)
+    assert torch.equal(torch.autograd.grad(run(lq, k), lq, (gq, gk))[0], wq)
+    assert torch.equal(torch.autograd.grad(run(lq, None)[0], lq, gq)[0], wq)
+    with torch.no_grad():
+        assert not run(lq, lk)[0].requires_grad
+    # views of one leaf, a broadcast gradient
+    both = torch.cat([q, k], 1).requires_grad_()
+    one = torch.ones((), device="cuda", dtype=dtype)
+    d, = torch.autograd.grad(run(both[:, :4], both[:, 4:]), both, (one.expand(q.shape), one.expand(k.shape)))
+    dq, dk = sl8.rope(torch.ones_like(q), torch.ones_like(k), pos, table, **how, inverse=not inverse)
+    assert torch.equal(d, torch.cat([dq, dk], 1))
+    # the gradient's own gradient: the turn again
+    v = gq.clone().requires_grad_()
+    d, = torch.autograd.grad(run(lq, None)[0], lq, v, create_graph=True)
+    assert torch.equal(torch.autograd.grad(d, v, q)[0], plain[0])
+
+
+def test_captured_gradient():
+    """A captured backward is refused beside a living eager graph of the same leaves, and the explicit call is not."""
+    q, _, pos, table = inputs(2, 4, 2, 9, 64, 64, 1, F32)
+    leaf, g = q.clone().requires_grad_(), torch.randn_like(q)
+    alive = sl8.rope(leaf, None, pos[0], table)[0]  # noqa: F841
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(graph):
+            torch.autograd.grad(sl8.rope(leaf, None, pos[0], table)[0], leaf, g)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):  # (what needs no backward is captured as ever)
+        y, _ = sl8.rope(leaf, None, pos[0], table)
+        with torch.no_grad():
+            d, _ = sl8.rope(g, None, pos[0], table, inverse=True)
+    want, = torch.autograd.grad(alive, leaf, g)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, alive) and torch.equal(d, want)
+
+
 def test_rope_table_far_positions():
     """Angles of far positions from 64 bits, rounded once."""
     t = sl8.rope_table(200001, 64, base=500000.0)
