@@ -405,10 +405,11 @@ struct RowState {
   // value is (with the maximum as reference, a tail of 2^17 keys of weight 2^-26 behind a value of zero
   // was lost; the two steps of the reference cost 1 %, 3 % in short prompts). The sum takes the weights
   // in 32 bits: in a block of small values a large one may have no 16-bit form beside V's largest.
-  template <int NG>
+  // PARTS 2: what the rounding to 16 bits left over, in 16 bits too, as operands of their own.
+  template <int NG, int PARTS>
   __device__ __forceinline__ void weights(const v4i (&sc)[RT][NG], const float (&ks)[NG], const float (&lv)[NG],
                                           const float (&iv)[NG], int key0, int keys_end, int g4,
-                                          v8h (&wb)[RT][NG / 2]) {
+                                          v8h (&wb)[RT][NG / 2][PARTS]) {
     float x[RT][NG][4];
     bool move = false;
 #pragma unroll
@@ -469,7 +470,11 @@ struct RowState {
         l[rt] = fmaf((w[0] + w[1]) + (w[2] + w[3]), iv[g], l[rt]);
         const h2 r[2] = {__builtin_convertvector((v2f{w[0], w[1]}), h2), __builtin_convertvector((v2f{w[2], w[3]}), h2)};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) wb[rt][g / 2][4 * (g & 1) + i] = r[i / 2][i & 1];
+        for (int i = 0; i < 4; ++i) {
+          const _Float16 hi = r[i / 2][i & 1];
+          wb[rt][g / 2][0][4 * (g & 1) + i] = hi;
+          if constexpr (PARTS == 2) wb[rt][g / 2][1][4 * (g & 1) + i] = (_Float16)(w[i] - (float)hi);
+        }
       }
   }
 };
@@ -485,7 +490,13 @@ struct RowState {
 //   * V comes by direct copies into a ring of two tiles in LDS and is read transposed
 //     (ds_read_b64_tr_b8: 8 keys of a channel), in the order of keys that the weights have, and
 //     turned into fp16: O^T += V^T W on v_mfma_f32_16x16x32_f16. 16-byte chunks of a row are
-//     placed by an xor of its key, so that the 16 rows of half a wave lie in different banks.
+//     placed by an xor of its key, so that the 16 rows of half a wave lie in different banks;
+//   * fp16, up to 16 rows: a weight is two fp16 parts, as one alone adds a quarter to what the output's
+//     rounding leaves (2.7e-4 for 2.06e-4 relative: 32 sequences of 512 to 8192 keys, 32 / 8 heads). It
+//     costs 0.4 of 44.9 us there, 1 of 24.7 at D = 64, 1.7 of 31 for 128 sequences on 1000 keys. One part
+//     where it would cost more: 32 rows, whose registers spill already (5 tokens of 16 such
+//     sequences 37.6 for 33.4 us), and tiles of many rows, which VALU and MFMA bound; bf16's own
+//     rounding hides it (1.70e-3 for 1.68e-3).
 // 16 sequences of 32768 tokens, 32 / 8 heads, D = 128, bf16 (1.07 GB): 183 us and 5 for the join, 5.8
 // TB/s, the rate of pure reading. 32 of 270 to 8192 tokens (186 MB): 35 and 5, of which about 10 are
 // the same for any size: the work list, the first loads and the waves' join. One of 777: 11.7, all
@@ -503,6 +514,7 @@ template <int DT, int D, int RT>
 __global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const AttnArgs p) {
   constexpr int ROWS = 16 * RT, KT = stream_keys<D>(), NG = KT / 16, KS = D / 64, DTL = D / 16;
   constexpr int TPM = 64 / NG;  // tiles whose groups the lanes hold
+  constexpr int PARTS = DT == SL8_DTYPE_F16 && RT == 1 ? 2 : 1;  // of a weight
   // Two arrays, not one of two stages: the compiler sees that the reads of one tile are not of the
   // copies in flight, and waits for none of those. The waves' sums are joined in them (o_place).
   __shared__ __attribute__((aligned(16))) int8_t v0_s[A8_WAVES * KT * D], v1_s[A8_WAVES * KT * D];
@@ -599,7 +611,7 @@ __global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const
     __builtin_amdgcn_sched_barrier(0);  // (K's registers are taken again, not others beside them)
     load(cur, (i0 + NG) & 63, next);
 
-    v8h wb[RT][NG / 2];
+    v8h wb[RT][NG / 2][PARTS];
     st.weights(sc, gks, glv, giv, key0, key0 + KT, g4, wb);
 
     // V(j): copied before the NG * KS loads and NG * CPG copies of the next tile
@@ -629,7 +641,9 @@ __global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const
         const int kk = (n0 + i) / DTL, d = (n0 + i) % DTL;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
-          st.o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wb[rt][kk], st.o[rt][d], 0, 0, 0);
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part)
+            st.o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wb[rt][kk][part], st.o[rt][d], 0, 0, 0);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -839,7 +853,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_block8_tile_kernel(const Attn
           sc[rt][g1] = acc;
         }
       }
-      v8h wb[RT][NG / 2];
+      v8h wb[RT][NG / 2][1];
       st.weights(sc, gks, glv, giv, key0, key0 + KT, g4, wb);
 
       int swz = vt_swz;
@@ -854,7 +868,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_block8_tile_kernel(const Attn
           const v8h a = __builtin_bit_cast(v8h, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt)
-            st.o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wb[rt][kk], st.o[rt][d], 0, 0, 0);
+            st.o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, wb[rt][kk][0], st.o[rt][d], 0, 0, 0);
         }
       __builtin_amdgcn_iglp_opt(0);  // reads and products interleaved: 2 % of a long chunk
     }

@@ -333,6 +333,22 @@ def test_decode(D, bs, Hq, Hkv):
 
 
 @pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("Hq,new", [(2, 1), (8, 1), (6, 2), (8, 4), (2, 16), (32, 1)])
+def test_fp16_weights_in_two_parts(D, Hq, new):
+    """Up to 16 rows of a sequence and KV head in fp16: no 2^-11 of sum p |v|, which one 16-bit weight alone
+    would add. The parts leave 2^-22 of a weight and 2^-33 of the largest."""
+    total = [new, new + 1, 17, 40, 130, 777, 3000]
+    c = Cache(total, 2, D, 16)
+    q = coded_queries(new * 7, Hq, D, F16, False)
+    got = sl8.attn_paged_block8(q, *c.args(), i32(total), cu_lens=offsets([new] * 7), rotate=False)
+    want, size, top = plain_attn(c, q, [new] * 7, total, False, D ** -0.5, -1)
+    N = max(total)
+    lim = size * (2.0 ** -22 + 2.0 ** -15 + N * 2.0 ** -24) + N * 127 * 2.0 ** -33 * top + \
+        2.0 ** -11 * (1 + 2.0 ** -8) * want.abs() + 2.0 ** -25
+    assert bool(((got.double() - want).abs() <= lim).all())
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("new", [2, 5, 8, 16])
 @pytest.mark.parametrize("G", [1, 3, 8])
 def test_drafts(D, new, G):
