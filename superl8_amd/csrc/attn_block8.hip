@@ -498,10 +498,11 @@ struct RowState {
 //     sequences 37.6 for 33.4 us), and tiles of many rows, which VALU and MFMA bound; bf16's own
 //     rounding hides it (1.70e-3 for 1.68e-3).
 // 16 sequences of 32768 tokens, 32 / 8 heads, D = 128, bf16 (1.07 GB): 183 us and 5 for the join, 5.8
-// TB/s, the rate of pure reading. 32 of 270 to 8192 tokens (186 MB): 35 and 5, of which about 10 are
-// the same for any size: the work list, the first loads and the waves' join. One of 777: 11.7, all
-// of that kind (the first kernel, a wave for each row and head with the codes multiplied one by one,
-// took 20 ms, 5 ms and 258 us).
+// TB/s, the rate of pure reading. 32 of 513 to 8192 tokens (186 MB): 36 and 5; the call takes 44.8 us,
+// and 18.6 where each wave stops after its first tile: launches, the work list, the first loads and the
+// joins. One of 777: 12.4, all of that kind: the first keys wait for the block's id and scale, and Q,
+// whose loads are issued behind theirs, for the keys (the first kernel, a wave for each row and head
+// with the codes multiplied one by one, took 20 ms, 5 ms and 258 us).
 // ---------------------------------------------------------------------------
 template <int D> constexpr int stream_keys() { return D == 256 ? 32 : 64; }
 template <int D> __device__ __forceinline__ int v_swizzle(int key) {
@@ -723,9 +724,9 @@ __global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const
 // (the same), 32 keys a tile (479), 3 waves a SIMD (spills: 605), products of one tile beside the
 // softmax of another in one wave (541), s_setprio around either (490, 500), accumulators that start at
 // 1.5 * 2^23 instead of the conversion (442, but logits shift by up to 0.75 of a step of the score).
-// 5 tokens of 16 sequences of 1.8 to 16.4 thousand, 64 / 8 heads (40 of 64 rows, 191 MB): 49 us and 6
-// for the join. Prompts of 650 to 1301 tokens with a window of 1024, D = 64, 16 / 4 heads: 45 us, a third of
-// it before the first tile. K and V two tiles ahead through registers instead: 61 us for the 59.5 of the
+// 5 tokens of 16 sequences of 1.0 to 16.4 thousand, 64 / 8 heads (40 of 64 rows, 191 MB): 48 us and 6
+// for the join. Prompts of 651 to 1301 tokens with a window of 1024, D = 64, 16 / 4 heads: a call of 45 us,
+// 22 where each workgroup stops after its first tile (launch, search, Q, that tile, output). K and V two tiles ahead through registers instead: 61 us for the 59.5 of the
 // drafts on that box, 46.7 for 45.8.
 // ---------------------------------------------------------------------------
 template <int D> constexpr int tile_keys() { return D == 256 ? 32 : 64; }
@@ -996,10 +997,13 @@ template <int D_, int RT_, int NW_> struct Shape {
 };
 
 // f(Shape) for `rows` rows of a sequence and KV head on average: what holds them in the fewest units
-// without many empty rows, up to 128. Up to 32 rows the waves stream keys of their own: 20 rows, 16
-// sequences of 8192 keys, D = 128: 34.9 us, 38.3 in tiles of 64 rows; 64 of 2000 keys: 34.0 and 50.2. 40
-// rows (the drafts above) take 57 in tiles, 88 streamed as two units. At D = 256 32 rows' sums do
-// not fit a wave's registers.
+// without many empty rows, up to 128. Up to 32 rows the waves stream keys of their own. 5 tokens (20 rows)
+// of 16 sequences, 32 / 8 heads, D = 128: 33.4 us, 41.6 in tiles of 64 rows, where their lengths go from 517 to
+// 8192; 76 and 67 where all have 8192. 64 sequences of 130 to 2000: 38 and 49, all of 2000: 89 and 66. D = 64:
+// 21.8 and 36.9, 31.9 and 38.1; 23 and 33, 36 and 42. (The lengths are on the device: mixed ones decide.) 40
+// rows (the drafts above) take 57 in tiles, 88 streamed as two units. 32 streamed rows at D = 128 need more
+// than the 256 registers of two waves a SIMD: 27 spill (96 to 112 bytes a lane) and come back in the loop
+// over keys; 16 rows at D = 256 spill 2, and 32 rows there, whose sums take 128, are not built.
 template <typename F>
 auto with_shape(int64_t D, int64_t rows, F&& f) {
   auto by_rows = [&](auto d) {
@@ -1041,8 +1045,8 @@ AttnPlan attn_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int
     // rows on 768 slots, D = 64: 48 us whole, 70 split).
     const int64_t slots = (int64_t)cu_count() * decltype(sh)::wgs_per_cu();
     const int64_t least = Hkv * std::max(B, T * G / ROWS);
-    // Short contexts stay whole: joining costs a launch (one token on 777 keys, 32/8 heads: 13.7 us
-    // whole, 17.0 split), and with many rows 2 D sums of 32 bits for each of them, against a time that
+    // Short contexts stay whole: joining costs a launch (one token on 777 keys, 32/8 heads: 11.9 us
+    // whole; 14.7 in a table for 32768, whose call has the work list and the launch), and with many rows 2 D sums of 32 bits for each of them, against a time that
     // goes by D: 300 tokens on 1000 keys (72 of 512 slots) 31 us whole, 33 split, on 2000 48 and 38;
     // 4 x 250 (248 slots) on 1200 keys 47 and 53, on 2000 69 and 62; D = 64, 4 x 300 on 2000 37 and 41,
     // on 3000 50 and 47; D = 256, 2 x 180 on 751 52 and 40.

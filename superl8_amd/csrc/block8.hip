@@ -11,9 +11,9 @@
 // One workgroup per (block, head, K or V): it owns the block's scale, so nothing is shared or
 // atomic. It holds its rows in registers between the maximum and the codes, 8 elements a thread,
 // D / 8 threads a row. 7312 tokens of four prompts, 32 / 8 heads, D = 128, bf16, three position
-// axes, Q with them (165 MB): 45 us, 3.6 TB/s. The bytes alone would take 32; what bounds it is the
-// chain of each workgroup (offsets and lengths, rows beside block id and angles, maximum, barrier,
-// codes) at four waves a SIMD (104 registers), with VALU busy in 64 % of the cycles, most of it the
+// axes, Q with them (165 MB): 43 to 45 us, 3.7 TB/s. The bytes alone would take 32; what bounds it is the
+// chain of each workgroup (offsets and lengths, rows beside the block id, then for each pass over them the
+// positions and after those the angles, maximum, barrier, codes) at four waves a SIMD (104 registers), with VALU busy in 64 % of the cycles, most of it the
 // Hadamard rotation (25 instructions an element of K, 7 of V).
 // Held to 96 or 80 registers it spills (101, 113 us with the 42 of reading the values back, against
 // 93); workgroups of 512 or 1024 threads wait longer at the barrier (kernel 53, 61 against 47 then). A decode

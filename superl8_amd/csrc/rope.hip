@@ -5,7 +5,7 @@
 // pairs' angles over the heads, so that the table and the positions are read once a token. 6121
 // tokens of 32 + 8 heads, D = 128, bf16, three axes (129 MB): 25.2 us, 5.1 TB/s, the rate of a
 // copy; 4 x 4096 tokens of 16 + 16 heads, D = 80, fp32 (341 MB): 73.6 us, 4.6 TB/s (88 with 8-byte
-// accesses). 64 tokens (1.3 MB): 5.8 us, the chain position, angles, store. Two heads of a thread in
+// accesses). 64 tokens (1.3 MB): 5.8 us, the chain position, angles, rows (loaded behind the angles), store. Two heads of a thread in
 // flight at once are slower (26.7 us for the 25.2 above: more registers, fewer waves).
 #include "rope.hpp"
 
