@@ -726,8 +726,8 @@ __global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const
 // 1.5 * 2^23 instead of the conversion (442, but logits shift by up to 0.75 of a step of the score).
 // 5 tokens of 16 sequences of 1.0 to 16.4 thousand, 64 / 8 heads (40 of 64 rows, 191 MB): 48 us and 6
 // for the join. Prompts of 651 to 1301 tokens with a window of 1024, D = 64, 16 / 4 heads: a call of 45 us,
-// 22 where each workgroup stops after its first tile (launch, search, Q, that tile, output). K and V two tiles ahead through registers instead: 61 us for the 59.5 of the
-// drafts on that box, 46.7 for 45.8.
+// 22 where each workgroup stops after its first tile (launch, search, Q, that tile, output). K
+// and V two tiles ahead through registers instead: 61 us for the 59.5 of the drafts on that box, 46.7 for 45.8.
 // ---------------------------------------------------------------------------
 template <int D> constexpr int tile_keys() { return D == 256 ? 32 : 64; }
 template <int D> __device__ __forceinline__ int k_swizzle(int key) {  // 16-byte chunks, 16 keys apart
@@ -1046,8 +1046,8 @@ AttnPlan attn_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int
     const int64_t slots = (int64_t)cu_count() * decltype(sh)::wgs_per_cu();
     const int64_t least = Hkv * std::max(B, T * G / ROWS);
     // Short contexts stay whole: joining costs a launch (one token on 777 keys, 32/8 heads: 11.9 us
-    // whole; 14.7 in a table for 32768, whose call has the work list and the launch), and with many rows 2 D sums of 32 bits for each of them, against a time that
-    // goes by D: 300 tokens on 1000 keys (72 of 512 slots) 31 us whole, 33 split, on 2000 48 and 38;
+    // whole; 14.7 in a table for 32768, whose call has the work list and the launch), and with many
+    // rows 2 D sums of 32 bits for each of them, against a time that goes by D: 300 tokens on 1000 keys (72 of 512 slots) 31 us whole, 33 split, on 2000 48 and 38;
     // 4 x 250 (248 slots) on 1200 keys 47 and 53, on 2000 69 and 62; D = 64, 4 x 300 on 2000 37 and 41,
     // on 3000 50 and 47; D = 256, 2 x 180 on 751 52 and 40.
     a.whole = decltype(sh)::NW ? (int)(128 * (12 * slots + 32 * std::min(least, slots)) / (D * slots)) : 16;

@@ -13,8 +13,8 @@
 // D / 8 threads a row. 7312 tokens of four prompts, 32 / 8 heads, D = 128, bf16, three position
 // axes, Q with them (165 MB): 43 to 45 us, 3.7 TB/s. The bytes alone would take 32; what bounds it is the
 // chain of each workgroup (offsets and lengths, rows beside the block id, then for each pass over them the
-// positions and after those the angles, maximum, barrier, codes) at four waves a SIMD (104 registers), with VALU busy in 64 % of the cycles, most of it the
-// Hadamard rotation (25 instructions an element of K, 7 of V).
+// positions and after those the angles, maximum, barrier, codes) at four waves a SIMD (104 registers),
+// with VALU busy in 64 % of the cycles, most of it the Hadamard rotation (25 instructions an element of K, 7 of V).
 // Held to 96 or 80 registers it spills (101, 113 us with the 42 of reading the values back, against
 // 93); workgroups of 512 or 1024 threads wait longer at the barrier (kernel 53, 61 against 47 then). A decode
 // step of 32 sequences (0.7 MB): 5.7 us, that chain once.

@@ -51,8 +51,9 @@ __device__ __forceinline__ void ld_f32(const float* p, float* f) {
 
 // cos and sin of pairs p0 .. p0 + N - 1 (N = 4, 8: p0, R / 2 and the table aligned to 4 floats)
 // of a token; sin negated for the inverse. Where a thread's pairs belong to several axes, each
-// takes a position and two angles of its own: 4 x 4096 tokens, 16 + 16 heads, D = 80, fp16, two axes of 20 pairs 49 us, one axis 40;
-// 6121 tokens, bf16, axes of (15, 25, 24) pairs 25.9, of (16, 24, 24), which no thread's 8 straddle, 22.7.
+// takes a position and two angles of its own: 4 x 4096 tokens, 16 + 16 heads, D = 80, fp16, two axes of
+// 20 pairs 49 us, one axis 40; 6121 tokens, bf16, axes of (15, 25, 24) pairs 25.9, of (16, 24, 24), which
+// no thread's 8 straddle, 22.7.
 template <int N>
 __device__ __forceinline__ void rope_angles(const RopeArgs& a, int64_t token, int p0, float* c, float* s) {
   const int half = a.R / 2;
