@@ -1045,11 +1045,11 @@ AttnPlan attn_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int
     // rows on 768 slots, D = 64: 48 us whole, 70 split).
     const int64_t slots = (int64_t)cu_count() * decltype(sh)::wgs_per_cu();
     const int64_t least = Hkv * std::max(B, T * G / ROWS);
-    // Short contexts stay whole: joining costs a launch (one token on 777 keys, 32/8 heads: 11.9 us
-    // whole; 14.7 in a table for 32768, whose call has the work list and the launch), and with many
-    // rows 2 D sums of 32 bits for each of them, against a time that goes by D: 300 tokens on 1000 keys (72 of 512
-    // slots) 31 us whole, 33 split, on 2000 48 and 38; 4 x 250 (248 slots) on 1200 keys 47 and 53, on 2000 69 and 62; D = 64, 4 x 300 on 2000 37 and 41,
-    // on 3000 50 and 47; D = 256, 2 x 180 on 751 52 and 40.
+    // Short contexts stay whole: joining costs a launch (one token on 777 keys, 32/8 heads: 11.9 us whole;
+    // 14.7 in a table for 32768, whose call has the work list and the launch), and with many rows 2 D sums
+    // of 32 bits for each of them, against a time that goes by D: 300 tokens on 1000 keys (72 of 512
+    // slots) 31 us whole, 33 split, on 2000 48 and 38; 4 x 250 (248 slots) on 1200 keys 47 and 53, on 2000
+    // 69 and 62; D = 64, 4 x 300 on 2000 37 and 41, on 3000 50 and 47; D = 256, 2 x 180 on 751 52 and 40.
     a.whole = decltype(sh)::NW ? (int)(128 * (12 * slots + 32 * std::min(least, slots)) / (D * slots)) : 16;
     const bool split = keys > a.whole * A8_TILE && a.pairs <= slots && (decltype(sh)::NW == 0 || 2 * least <= slots);
     a.slots = split ? (int)slots : 0;
