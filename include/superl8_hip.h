@@ -440,6 +440,67 @@ int sl8_attn_paged_block8(const void* q, int dtype, int rotate, float q_scale_mu
                           int64_t max_blocks_per_seq, int64_t window_left, void* workspace,
                           size_t workspace_bytes, void* stream);
 
+/* The same with a tree of drafted tokens, and with the sums' logarithms. tree_mask (NULL: as above)
+ * int64 [T][mask_words] (1 .. 4 words, 8-byte aligned): row i of a sequence sees the tokens in front of
+ * the new ones, and new token t < 64 * mask_words where bit t % 64 of word t / 64 of its mask is set. A window
+ * keeps the last window_left of those: the marked ones, all of them, and of the tokens in front the last
+ * max(0, window_left - marked). lse (NULL: not wanted) fp32 [T,Hq]: ln of the row's sum of e^score,
+ * -inf for a row that sees nothing or of no sequence. Workspace as above. */
+int sl8_attn_paged_block8_tree(const void* q, int dtype, int rotate, float q_scale_mul,
+                               const int8_t* k_cache, const float* k_scale, const int8_t* v_cache,
+                               const float* v_scale, const int32_t* cu_lens,
+                               const int32_t* context_lens, const int32_t* block_table,
+                               const int64_t* tree_mask, int64_t mask_words, void* out, float* lse,
+                               int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                               int64_t num_blocks, int64_t block_size, int64_t max_blocks_per_seq,
+                               int64_t window_left, void* workspace, size_t workspace_bytes,
+                               void* stream);
+
+/* Each cached key's softmax weights of a step's new rows, gathered: weights fp32 [B][Hkv][>=
+ * max_blocks_per_seq * block_size] (strides of sequence and head in elements; no two may overlap), in place:
+ *   w[b,h,j] = (j < context_lens[b] - n ? decay * w : 0) + sum over the n new rows i that see j and the
+ *              group's heads of e^(score_ij - lse_i),   j < context_lens[b]; others are left alone.
+ * q (rows as codes; rotate, window_left, cu_lens as in sl8_attn_paged_block8, causal rows) 16-byte aligned;
+ * lse fp32 [T,Hq] of the same rows, as sl8_attn_paged_block8_tree gives it (-inf: the row adds nothing).
+ * Keys in blocks outside the pool get nothing added. workspace: sl8_attn_weights_block8_workspace() bytes,
+ * uninitialised, 16-byte aligned. */
+size_t sl8_attn_weights_block8_workspace(int64_t T, int64_t Hq, int64_t D);
+int sl8_attn_weights_block8(const void* q, int dtype, int rotate, float q_scale_mul, const float* lse,
+                            const int8_t* k_cache, const float* k_scale, const int32_t* cu_lens,
+                            const int32_t* context_lens, const int32_t* block_table, float* weights,
+                            int64_t weights_stride_b, int64_t weights_stride_h, float decay, int64_t T,
+                            int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t num_blocks,
+                            int64_t block_size, int64_t max_blocks_per_seq, int64_t window_left,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
+/* Eviction: of each sequence and KV head min(context_lens, budget) tokens stay, the first `sinks`, the last
+ * `recent` (sinks + recent <= budget) and between them those of the largest weights (as above; no NaN), ties
+ * to the lowest index. They move, in their order, into the blocks of new_table int32 [B][new_max_blocks]
+ * (blocks that no row of block_table in the call holds), the j-th into slot j: a block and head takes
+ * scale' = max(scales of the blocks that its rows come from, 2^-60), codes rint(c * (scale / scale')). Rows
+ * behind the last one stay as they are, blocks of block_table too. new_lens int32 [B] = min(context_lens,
+ * budget); kept int32 [B][Hkv][budget]: the tokens' old indexes, -1 behind the last; weights of the kept are
+ * packed to the front, those behind stay. Tokens in blocks outside the pool are zeros where they arrive. */
+int sl8_kv_evict_block8(int8_t* k_cache, float* k_scale, int8_t* v_cache, float* v_scale,
+                        const int32_t* context_lens, const int32_t* block_table, float* weights,
+                        int64_t weights_stride_b, int64_t weights_stride_h, const int32_t* new_table,
+                        int32_t* new_lens, int32_t* kept, int64_t B, int64_t Hkv, int64_t D,
+                        int64_t num_blocks, int64_t block_size, int64_t max_blocks_per_seq,
+                        int64_t new_max_blocks, int64_t budget, int64_t sinks, int64_t recent,
+                        void* stream);
+
+/* ------------------------------------------------------------------------
+ * Linear layer of int8 weights with a scale per output channel: x [M,K] f16 / bf16 / f32, each row
+ * quantised to int8 as sl8_quantize_i8_rowwise; w int8 [N,K]; w_scale fp32 [N]; bias [N] (f16 / bf16 /
+ * f32; NULL: none) -> out [M,N] = x_scale[m] * w_scale[n] * sum_k x_i8 w + bias[n], the sums exact, rounded
+ * once. K a multiple of 4, 16 to 131068; w 16-byte aligned (4 where K % 16 != 0). workspace:
+ * sl8_linear_w8a8_workspace() bytes, uninitialised, 16-byte aligned.
+ * ---------------------------------------------------------------------- */
+size_t sl8_linear_w8a8_workspace(int64_t M, int64_t N, int64_t K);
+int sl8_linear_w8a8(const void* x, int x_dtype, const int8_t* w, const float* w_scale,
+                    const void* bias, int bias_dtype, void* out, int out_dtype, int64_t M, int64_t N,
+                    int64_t K, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------------
  * Q4_K GEMM/GEMV over native GGUF super-blocks (144 B per 256 weights:
  * fp16 d, fp16 dmin, 12 B packed 6-bit sub-scales/mins, 128 B nibbles).

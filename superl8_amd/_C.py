@@ -783,6 +783,7 @@ def kv_write_paged(k_new, v_new, slot_mapping, k_cache, k_scale, v_cache, v_scal
 # ---------------------------------------------------------------------------
 _HEAD_DIMS_BLOCK8 = (64, 128, 256)
 _BLOCK8_MAX = 128
+_TREE_MAX_WORDS = 4
 
 
 def _rope_checks(tag, positions, table, sections, want, D):
@@ -953,12 +954,14 @@ def kv_append_block8(k_new, v_new, k_cache, k_scale, v_cache, v_scale, block_tab
 
 
 def attn_paged_block8(q, q_mul, rotate, k_cache, k_scale, v_cache, v_scale, block_table,
-                      context_lens, cu_lens=None, window_left=-1):
+                      context_lens, cu_lens=None, window_left=-1, tree_mask=None, return_lse=False):
     """Attention of the new tokens q [T,Hq,D] (fp16/bf16) over a block-scaled paged int8 cache that
-    holds them already -> [T,Hq,D] of q's dtype; q_mul is softmax_scale * log2(e)."""
+    holds them already -> [T,Hq,D] of q's dtype; q_mul is softmax_scale * log2(e). tree_mask int64
+    [T] or [T,1..4]: the new tokens of its sequence that a row sees. return_lse: (out, ln of the
+    rows' sums, fp32 [T,Hq])."""
     tag = "attn_paged_block8"
-    _one_gpu(q, k_cache, k_scale, v_cache, v_scale, block_table, context_lens,
-             q if cu_lens is None else cu_lens)
+    given = [t for t in (cu_lens, tree_mask) if t is not None]
+    _one_gpu(q, k_cache, k_scale, v_cache, v_scale, block_table, context_lens, *given)
     if q.dtype not in (torch.float16, torch.bfloat16):
         _fail(f"{tag}: q must be float16 or bfloat16")
     if q.dim() != 3 or k_cache.dim() != 4:
@@ -970,16 +973,159 @@ def attn_paged_block8(q, q_mul, rotate, k_cache, k_scale, v_cache, v_scale, bloc
         _fail(f"{tag}: H_q must be divisible by H_kv (GQA)")
     B, nblk, bs, maxb = _block8_checks(tag, k_cache, k_scale, v_cache, v_scale, block_table,
                                        context_lens, cu_lens, T, Hkv, D)
+    words = 0
+    if tree_mask is not None:
+        if tree_mask.dtype != torch.int64 or tree_mask.dim() not in (1, 2) or tree_mask.shape[0] != T:
+            _fail(f"{tag}: tree_mask must be int64 [T] or [T, words]")
+        words = tree_mask.shape[1] if tree_mask.dim() == 2 else 1
+        if not 1 <= words <= _TREE_MAX_WORDS:
+            _fail(f"{tag}: tree_mask must have 1..{_TREE_MAX_WORDS} words a row, got {words}")
+        tree_mask = tree_mask.contiguous()
     out = q.new_empty((T, Hq, D))
+    lse = q.new_empty((T, Hq), dtype=torch.float32) if return_lse else None
     if T and Hq:
         with on_device(q):
             ws_bytes = _lib.load().sl8_attn_paged_block8_workspace(T, B, Hq, Hkv, D, maxb * bs)
             ws = q.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
-            call("sl8_attn_paged_block8", q.data_ptr(), dtype_code(q.dtype), int(bool(rotate)),
-                 float(q_mul), k_cache.data_ptr(), k_scale.data_ptr(), v_cache.data_ptr(),
-                 v_scale.data_ptr(), _lib.ptr(cu_lens), context_lens.data_ptr(),
-                 block_table.data_ptr(), out.data_ptr(), T, B, Hq, Hkv, D, nblk, bs, maxb,
-                 int(window_left), _lib.ptr(ws), ws_bytes, stream_of(q))
+            if words or return_lse:
+                call("sl8_attn_paged_block8_tree", q.data_ptr(), dtype_code(q.dtype), int(bool(rotate)),
+                     float(q_mul), k_cache.data_ptr(), k_scale.data_ptr(), v_cache.data_ptr(),
+                     v_scale.data_ptr(), _lib.ptr(cu_lens), context_lens.data_ptr(),
+                     block_table.data_ptr(), _lib.ptr(tree_mask), words, out.data_ptr(), _lib.ptr(lse),
+                     T, B, Hq, Hkv, D, nblk, bs, maxb, int(window_left), _lib.ptr(ws), ws_bytes,
+                     stream_of(q))
+            else:
+                call("sl8_attn_paged_block8", q.data_ptr(), dtype_code(q.dtype), int(bool(rotate)),
+                     float(q_mul), k_cache.data_ptr(), k_scale.data_ptr(), v_cache.data_ptr(),
+                     v_scale.data_ptr(), _lib.ptr(cu_lens), context_lens.data_ptr(),
+                     block_table.data_ptr(), out.data_ptr(), T, B, Hq, Hkv, D, nblk, bs, maxb,
+                     int(window_left), _lib.ptr(ws), ws_bytes, stream_of(q))
+    return (out, lse) if return_lse else out
+
+
+def _weight_strides(tag, weights, B, Hkv, most):
+    """The checks on weights [B,H_kv,>= most]; its strides of sequence and head."""
+    if weights.dtype != torch.float32 or weights.dim() != 3 or tuple(weights.shape[:2]) != (B, Hkv):
+        _fail(f"{tag}: weights must be float32 [B,H_kv,tokens]")
+    n = weights.shape[2]
+    if n < most:
+        _fail(f"{tag}: weights must hold a table's {most} tokens, got {n}")
+    sb, sh, st = weights.stride()
+    sb, sh, st = sb if B > 1 else n * Hkv, sh if Hkv > 1 else n, st if n > 1 else 1
+    # rows of their own (a broadcast or overlapping view would be written by two workgroups)
+    lo, hi, few, many = (sh, sb, Hkv, B) if sh <= sb else (sb, sh, B, Hkv)
+    if st != 1 or lo < n or (many > 1 and hi < lo * (few - 1) + n):
+        _fail(f"{tag}: weights must have dense rows that do not overlap")
+    return sb, sh
+
+
+def attn_weights_block8(q, q_mul, rotate, lse, k_cache, k_scale, block_table, context_lens, weights,
+                        cu_lens=None, window_left=-1, decay=1.0):
+    """The softmax weights of the new rows q [T,Hq,D] (fp16/bf16; lse fp32 [T,Hq] of
+    attn_paged_block8) added up by cached key and KV head, in place: weights fp32 [B,Hkv,tokens] =
+    decay * weights (the new tokens' own: 0) + sum over rows and the group's heads."""
+    tag = "attn_weights_block8"
+    _one_gpu(q, lse, k_cache, k_scale, block_table, context_lens, weights, q if cu_lens is None else cu_lens)
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        _fail(f"{tag}: q must be float16 or bfloat16")
+    if q.dim() != 3 or k_cache.dim() != 4:
+        _fail(f"{tag}: q must be [T,H_q,D], k_cache [num_blocks,H_kv,block_size,D]")
+    T, Hq, D = q.shape
+    Hkv = k_cache.shape[1]
+    if Hkv < 1 or Hq < 1 or Hq % Hkv:
+        _fail(f"{tag}: H_q must be divisible by H_kv (GQA)")
+    if lse.dtype != torch.float32 or tuple(lse.shape) != (T, Hq):
+        _fail(f"{tag}: lse must be float32 [T,H_q]")
+    _contig(q, lse)
+    B, nblk, bs, maxb = _block8_checks(tag, k_cache, k_scale, k_cache, k_scale, block_table,
+                                       context_lens, cu_lens, T, Hkv, D)
+    sb, sh = _weight_strides(tag, weights, B, Hkv, maxb * bs)
+    if not math.isfinite(decay):
+        _fail(f"{tag}: decay must be finite, got {decay}")
+    if B and maxb:
+        with on_device(q):
+            ws_bytes = _lib.load().sl8_attn_weights_block8_workspace(T, Hq, D)
+            ws = q.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
+            call("sl8_attn_weights_block8", q.data_ptr(), dtype_code(q.dtype), int(bool(rotate)),
+                 float(q_mul), lse.data_ptr(), k_cache.data_ptr(), k_scale.data_ptr(), _lib.ptr(cu_lens),
+                 context_lens.data_ptr(), block_table.data_ptr(), weights.data_ptr(), sb, sh, float(decay),
+                 T, B, Hq, Hkv, D, nblk, bs, maxb, int(window_left), _lib.ptr(ws), ws_bytes, stream_of(q))
+
+
+def kv_evict_block8(k_cache, k_scale, v_cache, v_scale, block_table, context_lens, weights, new_table,
+                    budget, sinks=0, recent=0):
+    """Keeps min(context, budget) tokens of each sequence and KV head: the first sinks, the last
+    recent, and between them those of the largest weights (fp32 [B,Hkv,tokens]); they move into the
+    blocks of new_table, their weights to the front. Returns (lengths int32 [B], kept indexes int32
+    [B,Hkv,budget], -1 behind the last)."""
+    tag = "kv_evict_block8"
+    _one_gpu(k_cache, k_scale, v_cache, v_scale, block_table, context_lens, weights, new_table)
+    if k_cache.dim() != 4 or k_cache.shape[1] < 1:
+        _fail(f"{tag}: k_cache must be [num_blocks,H_kv,block_size,D]")
+    Hkv, D = k_cache.shape[1], k_cache.shape[3]
+    B, nblk, bs, maxb = _block8_checks(tag, k_cache, k_scale, v_cache, v_scale, block_table,
+                                       context_lens, None, context_lens.numel(), Hkv, D)
+    sb, sh = _weight_strides(tag, weights, B, Hkv, maxb * bs)
+    budget, sinks, recent = int(budget), int(sinks), int(recent)
+    if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
+        _fail(f"{tag}: budget must be at least 1 and hold sinks and recent, got {budget}, {sinks}, {recent}")
+    if new_table.dtype != torch.int32 or new_table.dim() != 2 or new_table.shape[0] != B:
+        _fail(f"{tag}: new_table must be int32 [B, blocks]")
+    _contig(new_table)
+    if new_table.shape[1] * bs < min(budget, maxb * bs):
+        _fail(f"{tag}: new_table must hold the {min(budget, maxb * bs)} tokens that stay, got "
+              f"{new_table.shape[1]} blocks of {bs}")
+    lens = context_lens.new_empty((B,))
+    kept = context_lens.new_empty((B, Hkv, budget))
+    if B:
+        with on_device(k_cache):
+            call("sl8_kv_evict_block8", k_cache.data_ptr(), k_scale.data_ptr(), v_cache.data_ptr(),
+                 v_scale.data_ptr(), context_lens.data_ptr(), block_table.data_ptr(), weights.data_ptr(),
+                 sb, sh, new_table.data_ptr(), lens.data_ptr(), kept.data_ptr(), B, Hkv, D, nblk, bs, maxb,
+                 new_table.shape[1], budget, sinks, recent, stream_of(k_cache))
+    return lens, kept
+
+
+# ---------------------------------------------------------------------------
+# int8 weights with a scale per output channel
+# ---------------------------------------------------------------------------
+_W8_MAX_K = 1 << 17
+
+
+def linear_w8a8(x, w, w_scale, bias=None, out_dtype=torch.float16):
+    """x [M,K] (fp16/bf16/fp32; quantised per row as quantize_i8_rowwise), w int8 [N,K], w_scale
+    fp32 [N], bias [N] or None -> [M,N] = x_scale * w_scale * (x_i8 @ w^T) + bias, rounded once."""
+    tag = "linear_w8a8"
+    _one_gpu(x, w, w_scale, x if bias is None else bias)
+    floats = (torch.float16, torch.bfloat16, torch.float32)
+    if x.dtype not in floats:
+        _fail(f"{tag}: x must be float16/bfloat16/float32")
+    if out_dtype not in floats:
+        _fail(f"{tag}: out_dtype must be float16/bfloat16/float32, got {out_dtype}")
+    if w.dtype != torch.int8 or w_scale.dtype != torch.float32:
+        _fail(f"{tag}: w must be int8 and w_scale float32")
+    if x.dim() != 2 or w.dim() != 2 or w.shape[1] != x.shape[1]:
+        _fail(f"{tag}: expect x[M,K] and w[N,K], got {list(x.shape)} and {list(w.shape)}")
+    M, K = x.shape
+    N = w.shape[0]
+    if K < 16 or K % 4 or K >= _W8_MAX_K:
+        _fail(f"{tag}: K must be a multiple of 4, 16 to {_W8_MAX_K - 4}, got {K}")
+    if w_scale.numel() != N:
+        _fail(f"{tag}: w_scale must be [N], got {list(w_scale.shape)} for N={N}")
+    if bias is not None and (bias.dtype not in floats or tuple(bias.shape) != (N,)):
+        _fail(f"{tag}: bias must be float16/bfloat16/float32 [N]")
+    _contig(x, w, w_scale)
+    out = x.new_empty((M, N), dtype=out_dtype)
+    if M and N:
+        if w.data_ptr() % (4 if K % 16 else 16):
+            w = w.clone()
+        bias = None if bias is None else bias.contiguous()
+        with on_device(x):
+            ws_bytes = _lib.load().sl8_linear_w8a8_workspace(M, N, K)
+            ws = x.new_empty((ws_bytes,), dtype=torch.uint8)
+            call("sl8_linear_w8a8", x.data_ptr(), dtype_code(x.dtype), w.data_ptr(), w_scale.data_ptr(),
+                 _lib.ptr(bias), 0 if bias is None else dtype_code(bias.dtype), out.data_ptr(),
+                 dtype_code(out_dtype), M, N, K, ws.data_ptr(), ws_bytes, stream_of(x))
     return out
 
 

@@ -12,6 +12,11 @@
 // largest contribution has full precision, and a block's scale costs one fma that the product s_j
 // needs anyway. (Least scale 2^-60: the sum of w / vs stays within 32 bits.)
 //
+// With a tree of drafted tokens (a mask of 64-bit words a row) row i sees the keys in front of the new
+// ones, j < len - n, and new key len - n + t where bit t of its mask is set. A window keeps the last
+// window of what it sees so: the marked keys, and of those in front the last max(0, window - marked).
+// The sums' logarithms, ln sum_j e^{s_j}, can be had too: what the weights of a key are taken against.
+//
 // Rows of a sequence and KV head are (token, query head of the group), G = Hq / Hkv to a token; a
 // unit is ROWS of them that share every byte of K and V.
 #include <algorithm>
@@ -47,6 +52,9 @@ struct AttnArgs {
   float q_mul;
   int window;  // below 0: none
   bool rotate;
+  const uint2* tree;  // [T][words] of 64 bits, with TREE
+  int words;
+  float* lse;  // [T][Hq] or null
   int slots;      // workgroups to split the keys over, 0: no splits
   int whole;      // contexts of up to so many tiles are not split
   int max_pairs;  // that the workspace has places for
@@ -81,7 +89,7 @@ struct Item {
   bool live;
 };
 
-template <int ROWS>
+template <int ROWS, bool TREE>
 __device__ __forceinline__ SeqWork seq_work(const AttnArgs& p, int b) {
   SeqWork w{0, 0, 0, 0, 1};
   if (b < p.s.B) {
@@ -89,7 +97,7 @@ __device__ __forceinline__ SeqWork seq_work(const AttnArgs& p, int b) {
     w.n = max(0, (int)p.s.row(b + 1) - w.row0);
     w.len = p.s.lens[b];
     int span = min(max(w.len, 0), p.s.maxb * p.s.bs);
-    if (p.window >= 0) span = (int)min((int64_t)span, (int64_t)p.window + ROWS / p.G + A8_TILE);
+    if (p.window >= 0) span = (int)min((int64_t)span, (int64_t)p.window + (TREE ? w.n : ROWS / p.G) + A8_TILE);
     w.units = (w.n * p.G + ROWS - 1) / ROWS;
     w.tiles = max(1, (span + A8_TILE - 1) / A8_TILE);
   }
@@ -118,7 +126,7 @@ __device__ __forceinline__ int wave_scan(int x) {
   return x;
 }
 
-template <int ROWS>
+template <int ROWS, bool TREE>
 __device__ __forceinline__ Item find_item(const AttnArgs& p, int lane, int id) {
   if (!p.slots && !p.s.cu) {  // one row a sequence, whole: nothing to look for
     Item it{};
@@ -150,8 +158,8 @@ __device__ __forceinline__ Item find_item(const AttnArgs& p, int lane, int id) {
     it.live = it.unit >= 0;
     return it;
   }
-  const SeqWork mine = seq_work<ROWS>(p, lane);
-  auto work = [&](int b0) { return b0 == 0 ? mine : seq_work<ROWS>(p, b0 + lane); };
+  const SeqWork mine = seq_work<ROWS, TREE>(p, lane);
+  auto work = [&](int b0) { return b0 == 0 ? mine : seq_work<ROWS, TREE>(p, b0 + lane); };
   int most = 1, whole = 0;
   float all = 0.f;
   for (int b0 = 0; b0 < p.s.B; b0 += 64) {
@@ -241,7 +249,7 @@ __device__ __forceinline__ int token_of(const Span& w, int r) {
   return w.tok + (int)(((float)(w.head + r) + 0.5f) * w.over_g);
 }
 
-template <int ROWS>
+template <int ROWS, bool TREE>
 __device__ __forceinline__ Span item_span(const AttnArgs& p, const Item& it) {
   Span w;
   w.row0 = it.row0;
@@ -256,8 +264,9 @@ __device__ __forceinline__ Span item_span(const AttnArgs& p, const Item& it) {
   const int64_t pos0 = max(len - n, (int64_t)-(1 << 28));
   w.pos0 = (int)min(pos0, (int64_t)INT_MAX - (1 << 29));
   const int keys = (int)max((int64_t)0, min(len, (int64_t)p.s.maxb * p.s.bs));
-  const int last = min(keys, w.pos0 + token_of(w, w.cnt - 1) + 1);
-  w.low = p.window >= 0 ? (int)max((int64_t)0, (int64_t)w.pos0 + w.tok - p.window + 1) : 0;
+  // (a tree's rows may see any of the new keys, and up to the window's length in front of them)
+  const int last = min(keys, w.pos0 + (TREE ? n : token_of(w, w.cnt - 1) + 1));
+  w.low = p.window >= 0 ? (int)max((int64_t)0, (int64_t)w.pos0 - p.window + (TREE ? 0 : w.tok + 1)) : 0;
   const int first = w.low & ~(A8_TILE - 1);
   const int tiles = max(0, last - first + A8_TILE - 1) / A8_TILE;
   const int per = (tiles + it.splits - 1) / it.splits * A8_TILE;
@@ -273,7 +282,7 @@ __device__ __forceinline__ void note_pair(const AttnArgs& p, const Span& w, cons
   p.pairs[2 * it.pair + 1] = make_int4((int)w.row0, w.r0, w.cnt, 0);
 }
 
-// Rows in front of the first sequence and behind the last are zeros.
+// Rows in front of the first sequence and behind the last are zeros (the logarithm of their sums -inf).
 __device__ __forceinline__ void zero_rest(const AttnArgs& p, const Item& it, int D) {
   const int64_t n = it.begin + p.s.T - it.end;
   if (n == 0) return;
@@ -282,6 +291,8 @@ __device__ __forceinline__ void zero_rest(const AttnArgs& p, const Item& it, int
   for (int64_t i = blockIdx.x; i < n; i += gridDim.x) {
     const int64_t t = i < it.begin ? i : it.end + i - it.begin;
     for (int64_t c = threadIdx.x; c < chunks; c += blockDim.x) o[t * chunks + c] = make_uint4(0, 0, 0, 0);
+    if (p.lse)
+      for (int64_t h = threadIdx.x; h < p.Hq; h += blockDim.x) p.lse[t * p.Hq + h] = -INFINITY;
   }
 }
 
@@ -324,6 +335,23 @@ __device__ __forceinline__ void quant_rows(const AttnArgs& p, const Span& w, int
       if (lane == 0) qs_s[r] = live ? safe * p.q_mul : 0.f;
     }
   }
+}
+
+// The masks of a unit's rows in LDS, with zeros past the last word (rows past the last: as the last).
+constexpr int TREE_MAX = 4, TREE_WORDS = 2 * TREE_MAX;  // words of 64 bits and of 32
+template <int ROWS, int THREADS>
+__device__ __forceinline__ void load_tree(const AttnArgs& p, const Span& w, uint32_t* tree_s) {
+  for (int i = threadIdx.x; i < ROWS * TREE_MAX; i += THREADS) {
+    const int r = i / TREE_MAX, x = i % TREE_MAX;
+    uint2 v = make_uint2(0, 0);
+    if (x < p.words) v = p.tree[(w.row0 + token_of(w, min(r, w.cnt - 1))) * p.words + x];
+    *reinterpret_cast<uint2*>(tree_s + 2 * i) = v;
+  }
+}
+
+// The logarithm of a row's sum l of weights under reference m (log2).
+__device__ __forceinline__ float row_lse(float m, float l) {
+  return l > 0.f ? 0.6931471805599453f * (m + __builtin_amdgcn_logf(l)) : -INFINITY;
 }
 
 // 16 consecutive keys lie in one block: their first row's offset in the caches and the block's
@@ -371,29 +399,56 @@ __device__ __forceinline__ float max_xor16(float x) {
 }
 
 // Softmax state of 16 RT rows in the layout of S^T: row 16 rt + col in the lanes of column col.
-template <int RT, int D>
+template <int RT, int D, bool TREE>
 struct RowState {
   float qs[RT];
   int lim[RT], low[RT];  // the row sees keys [low, lim)
   int in0, in1;          // keys that every row of the unit sees: [in0, in1)
   float m[RT], l[RT];    // reference (log2) and sum of weights / vs
   v4f o[RT][D / 16];
+  const uint32_t* bits;  // TREE: the mask of row col in LDS; of row 16 rt + col TREE_WORDS * 16 rt further
+  int pos0;
 
-  __device__ __forceinline__ void init(const AttnArgs& p, const Span& w, int r0, int col, const float* qs_s) {
+  __device__ __forceinline__ void init(const AttnArgs& p, const Span& w, int r0, int col, const float* qs_s,
+                                       const uint32_t* tree_s) {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const int r = r0 + 16 * rt + col;
       qs[rt] = qs_s[r];
       const int pos = w.pos0 + token_of(w, min(r, w.cnt - 1));  // (rows past the last: as the last)
-      lim[rt] = min(pos + 1, w.k1);
-      low[rt] = p.window >= 0 ? (int)max((int64_t)pos - p.window + 1, (int64_t)0) : 0;
+      lim[rt] = TREE ? w.k1 : min(pos + 1, w.k1);
+      low[rt] = 0;
+      if (p.window >= 0) {
+        int64_t from = (int64_t)pos - p.window + 1;
+        if constexpr (TREE) {
+          int marked = 0;
+          for (int x = 0; x < 2 * p.words; ++x) marked += __builtin_popcount(tree_s[(r0 + 16 * rt + col) * TREE_WORDS + x]);
+          from = (int64_t)w.pos0 - max(p.window - marked, 0);
+        }
+        low[rt] = (int)max(from, (int64_t)0);
+      }
       m[rt] = A8_NONE;
       l[rt] = 0.f;
 #pragma unroll
       for (int t = 0; t < D / 16; ++t) o[rt][t] = v4f{0.f, 0.f, 0.f, 0.f};
     }
-    in1 = min(w.pos0 + w.tok + 1, w.k1);
-    in0 = p.window >= 0 ? w.pos0 + token_of(w, w.cnt - 1) - p.window + 1 : 0;
+    in1 = min(w.pos0 + (TREE ? 0 : w.tok + 1), w.k1);
+    in0 = p.window >= 0 ? w.pos0 - (TREE ? 0 : p.window - 1 - token_of(w, w.cnt - 1)) : 0;
+    if constexpr (TREE) {
+      bits = tree_s + (r0 + col) * TREE_WORDS;
+      pos0 = w.pos0;
+    }
+  }
+
+  // Whether the row of lane col in row tile rt sees a key.
+  __device__ __forceinline__ bool sees(int rt, int key) const {
+    if constexpr (TREE) {
+      if (key >= pos0) {  // (bits past the mask's last word were cleared)
+        const int t = key - pos0;
+        return key < lim[rt] && t < 32 * TREE_WORDS && (bits[16 * rt * TREE_WORDS + (t >> 5)] >> (t & 31) & 1);
+      }
+    }
+    return key < lim[rt] && key >= low[rt];
   }
 
   // Weights of NG groups of 16 keys from their scores (lane (g4, col): keys 16 g + 4 g4 + i from
@@ -430,7 +485,7 @@ struct RowState {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int key = key0 + 16 * g + 4 * g4 + i;
-            if (key >= lim[rt] || key < low[rt]) x[rt][g][i] = -INFINITY;
+            if (!sees(rt, key)) x[rt][g][i] = -INFINITY;
           }
     }
     float top[RT];
@@ -511,7 +566,7 @@ template <int D> __device__ __forceinline__ int v_swizzle(int key) {
   else return (key & 7) | ((key >> 4) & 1) << 3;
 }
 
-template <int DT, int D, int RT>
+template <int DT, int D, int RT, bool TREE>
 __global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const AttnArgs p) {
   constexpr int ROWS = 16 * RT, KT = stream_keys<D>(), NG = KT / 16, KS = D / 64, DTL = D / 16;
   constexpr int TPM = 64 / NG;  // tiles whose groups the lanes hold
@@ -521,14 +576,15 @@ __global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const
   __shared__ __attribute__((aligned(16))) int8_t v0_s[A8_WAVES * KT * D], v1_s[A8_WAVES * KT * D];
   __shared__ __attribute__((aligned(16))) int8_t q_s[ROWS * D];
   __shared__ float qs_s[ROWS], m_s[A8_WAVES][ROWS], l_s[A8_WAVES][ROWS];
+  __shared__ __attribute__((aligned(8))) uint32_t tree_s[TREE ? ROWS * TREE_WORDS : 2];
   static_assert(ROWS * D * 4 * A8_WAVES <= 2 * A8_WAVES * KT * D, "the sums fit the ring");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, g4 = lane >> 4;
 
-  const Item it = find_item<ROWS>(p, lane, blockIdx.x);
+  const Item it = find_item<ROWS, TREE>(p, lane, blockIdx.x);
   zero_rest(p, it, D);
   if (!it.live) return;
-  const Span w = item_span<ROWS>(p, it);
+  const Span w = item_span<ROWS, TREE>(p, it);
   // places: K's lane in a group, the copies' lanes (16-byte chunk of the row that goes to the
   // lane's place) for even and odd groups, the transposed reads' rows
   const int k_off = col * D + 16 * g4;
@@ -575,6 +631,7 @@ __global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const
   if (ntiles) load(cur, 0, v0_s);
 
   quant_rows<DT, D, ROWS, A8_THREADS>(p, w, it.kvh, [&](int r) { return q_s + r * D; }, qs_s);
+  if constexpr (TREE) load_tree<ROWS, A8_THREADS>(p, w, tree_s);
   __syncthreads();
 
   v4i qb[RT][KS];
@@ -583,8 +640,8 @@ __global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const
 #pragma unroll
     for (int s = 0; s < KS; ++s)
       qb[rt][s] = *reinterpret_cast<const v4i*>(q_s + (16 * rt + col) * D + 64 * s + 16 * g4);
-  RowState<RT, D> st;
-  st.init(p, w, 0, col, qs_s);
+  RowState<RT, D, TREE> st;
+  st.init(p, w, 0, col, qs_s, tree_s);
 
   auto tile = [&](int j, const int8_t* ring, int8_t* next) __attribute__((always_inline)) {
     const int i0 = j % TPM * NG;  // the tile's groups are in lanes i0 .. i0 + NG - 1 of cur
@@ -701,6 +758,7 @@ __global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const
       const int64_t to = row_at(p, w, it.kvh, r, D) + d;
 #pragma unroll
       for (int e = 0; e < 4; ++e) st_out<DT>(p.out, to + e, a[e]);
+      if (p.lse && d == 0) p.lse[to / D] = row_lse(mm, den);
     } else {
       const int64_t row = (int64_t)blockIdx.x * ROWS + r;
       *reinterpret_cast<v4f*>(p.part + row * D + d) = a;
@@ -740,7 +798,7 @@ template <int D> __device__ __forceinline__ int v16_swizzle(int key) {  // 32-by
   else return key & 7;
 }
 
-template <int DT, int D, int RT, int NW>
+template <int DT, int D, int RT, int NW, bool TREE>
 __global__ void __launch_bounds__(64 * NW, 2) attn_block8_tile_kernel(const AttnArgs p) {
   constexpr int THREADS = 64 * NW, ROWS = 16 * RT * NW, KT = tile_keys<D>(), NG = KT / 16;
   constexpr int KS = D / 64, DTL = D / 16, CPR = D / 16;
@@ -750,16 +808,17 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_block8_tile_kernel(const Attn
   __shared__ __attribute__((aligned(16))) int8_t k0_s[KT * D], k1_s[KT * D];
   __shared__ __attribute__((aligned(16))) uint16_t v0_s[KT * D], v1_s[KT * D];
   __shared__ float qs_s[ROWS];
+  __shared__ __attribute__((aligned(8))) uint32_t tree_s[TREE ? ROWS * TREE_WORDS : 2];
   static_assert(ROWS <= 4 * KT, "the rows' codes fit where V will be");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, g4 = lane >> 4;
   typedef short v4s __attribute__((ext_vector_type(4)));
   typedef short v8s __attribute__((ext_vector_type(8)));
 
-  const Item it = find_item<ROWS>(p, lane, blockIdx.x);
+  const Item it = find_item<ROWS, TREE>(p, lane, blockIdx.x);
   zero_rest(p, it, D);
   if (!it.live) return;
-  const Span w = item_span<ROWS>(p, it);
+  const Span w = item_span<ROWS, TREE>(p, it);
 
   // a thread's copies: 16-byte chunk `ch` of key `key` of the tile (64 threads: one group of 16 keys)
   int k_src[COPIES], v_src[COPIES], v_dst[COPIES];
@@ -804,6 +863,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_block8_tile_kernel(const Attn
     return r < FIT ? reinterpret_cast<int8_t*>(v0_s) + r * D : reinterpret_cast<int8_t*>(v1_s) + (r - FIT) * D;
   };
   quant_rows<DT, D, ROWS, THREADS>(p, w, it.kvh, q_place, qs_s);
+  if constexpr (TREE) load_tree<ROWS, THREADS>(p, w, tree_s);
   __syncthreads();
   v4i qb[RT][KS];
 #pragma unroll
@@ -811,8 +871,8 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_block8_tile_kernel(const Attn
 #pragma unroll
     for (int s = 0; s < KS; ++s)
       qb[rt][s] = *reinterpret_cast<const v4i*>(q_place(16 * (RT * wave + rt) + col) + 64 * s + 16 * g4);
-  RowState<RT, D> st;
-  st.init(p, w, 16 * RT * wave, col, qs_s);
+  RowState<RT, D, TREE> st;
+  st.init(p, w, 16 * RT * wave, col, qs_s, tree_s);
   __syncthreads();
   if (ntiles) store_v(v0_s);
   wait_dma();
@@ -902,7 +962,9 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_block8_tile_kernel(const Attn
     if (r >= w.cnt) continue;
     if (it.splits == 1) {
       const float inv = l > 0.f ? 1.f / l : 0.f;
-      uint16_t* to = static_cast<uint16_t*>(p.out) + row_at(p, w, it.kvh, r, D) + 4 * g4;
+      const int64_t at = row_at(p, w, it.kvh, r, D);
+      if (p.lse && g4 == 0) p.lse[at / D] = row_lse(st.m[rt], l);
+      uint16_t* to = static_cast<uint16_t*>(p.out) + at + 4 * g4;
 #pragma unroll
       for (int d = 0; d < DTL; ++d) {
         const v4f a = st.o[rt][d] * inv;
@@ -970,22 +1032,23 @@ __global__ void __launch_bounds__(64 * JOIN_ROWS) attn_block8_join_kernel(const 
   const int64_t to = (((int64_t)u.x + i / p.G) * p.Hq + a.w * p.G + i % p.G) * D + C * lane;
 #pragma unroll
   for (int c = 0; c < C; ++c) st_out<DT>(p.out, to + c, o[c] * inv);
+  if (p.lse && lane == 0) p.lse[to / D] = row_lse(mm, den);
 }
 
 // The kernels by head dim and rows: NW 0 streams.
 template <int D_, int RT_, int NW_> struct Shape {
   static constexpr int D = D_, RT = RT_, NW = NW_, ROWS = 16 * RT_ * (NW_ ? NW_ : 1);
   static constexpr int THREADS = NW_ ? 64 * NW_ : A8_THREADS;
-  template <int DT> static auto kernel() {
-    if constexpr (NW_) return attn_block8_tile_kernel<DT, D, RT, NW>;
-    else return attn_block8_stream_kernel<DT, D, RT>;
+  template <int DT, bool TREE> static auto kernel() {
+    if constexpr (NW_) return attn_block8_tile_kernel<DT, D, RT, NW, TREE>;
+    else return attn_block8_stream_kernel<DT, D, RT, TREE>;
   }
   // workgroups resident on one CU (asked once)
   static int wgs_per_cu() {
     static std::atomic<int> n{0};
     int v = n.load(std::memory_order_relaxed);
     if (v == 0) {
-      if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&v, reinterpret_cast<const void*>(kernel<0>()), THREADS, 0) !=
+      if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&v, reinterpret_cast<const void*>(kernel<0, false>()), THREADS, 0) !=
               hipSuccess || v < 1) {
         (void)hipGetLastError();
         return 2;  // no device: any figure (nothing is launched)
@@ -1072,17 +1135,16 @@ extern "C" size_t sl8_attn_paged_block8_workspace(int64_t T, int64_t B, int64_t 
   return attn_plan(T, B, Hq, Hkv, D, max_context_len).bytes;
 }
 
-extern "C" int sl8_attn_paged_block8(const void* q, int dtype, int rotate, float q_scale_mul,
-                                     const int8_t* k_cache, const float* k_scale,
-                                     const int8_t* v_cache, const float* v_scale,
-                                     const int32_t* cu_lens, const int32_t* context_lens,
-                                     const int32_t* block_table, void* out, int64_t T, int64_t B,
-                                     int64_t Hq, int64_t Hkv, int64_t D, int64_t num_blocks,
-                                     int64_t block_size, int64_t max_blocks_per_seq,
-                                     int64_t window_left, void* workspace, size_t workspace_bytes,
-                                     void* stream) {
+namespace {
+
+// The two entries; tag: what errors call them. Either of tree_mask (with words) and lse may be null.
+int attn_paged(const char* tag, const void* q, int dtype, int rotate, float q_scale_mul, const int8_t* k_cache,
+               const float* k_scale, const int8_t* v_cache, const float* v_scale, const int32_t* cu_lens,
+               const int32_t* context_lens, const int32_t* block_table, const void* tree_mask, int64_t words,
+               void* out, float* lse, int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t num_blocks,
+               int64_t block_size, int64_t max_blocks_per_seq, int64_t window_left, void* workspace,
+               size_t workspace_bytes, void* stream) {
   clear_error();
-  const char* tag = "attn_paged_block8";
   SL8_CHECK_ARG(dtype == SL8_DTYPE_F16 || dtype == SL8_DTYPE_BF16, "fni8 %s: q must be float16 or bfloat16", tag);
   SL8_CHECK_ARG(T >= 0 && T < (1LL << 28) && B >= 0 && B < (1 << 24) && Hq >= 0 && Hq < (1 << 16) &&
                     num_blocks >= 0 && num_blocks < (1LL << 31) && max_blocks_per_seq >= 0 &&
@@ -1093,6 +1155,8 @@ extern "C" int sl8_attn_paged_block8(const void* q, int dtype, int rotate, float
                    (int)block_size};
   if (const int rc = block8_check(tag, p.s, Hkv, D)) return rc;
   SL8_CHECK_ARG(Hq % Hkv == 0, "fni8 %s: H_q must be divisible by H_kv (GQA)", tag);
+  SL8_CHECK_ARG(!tree_mask || (words >= 1 && words <= TREE_MAX), "fni8 %s: tree_mask must have 1..%d words a row, got %lld",
+                tag, TREE_MAX, (long long)words);
   SL8_CHECK_ARG(T * Hq < (1LL << 30) && T * (Hq / Hkv) + B < (1LL << 30) / Hkv, "fni8 %s: shape too large", tag);
   if (T == 0 || Hq == 0) return SL8_OK;
   SL8_CHECK_ARG(q && out && (B == 0 || (context_lens && (max_blocks_per_seq == 0 || block_table))) &&
@@ -1100,6 +1164,7 @@ extern "C" int sl8_attn_paged_block8(const void* q, int dtype, int rotate, float
                 "fni8 %s: null pointer", tag);
   SL8_CHECK_ARG(aligned(q, 16) && aligned(out, 16) && aligned(k_cache, 16) && aligned(v_cache, 16),
                 "fni8 %s: q/k_cache/v_cache must be 16-byte aligned", tag);
+  SL8_CHECK_ARG(aligned(tree_mask, 8) && aligned(lse, 4), "fni8 %s: tree_mask/lse must be aligned", tag);
   const AttnPlan plan = attn_plan(T, B, Hq, Hkv, D, max_blocks_per_seq * block_size);
   SL8_CHECK_ARG(plan.grid < (1LL << 32) / A8_THREADS, "fni8 %s: shape too large", tag);
   SL8_CHECK_ARG(plan.bytes == 0 || (workspace && workspace_bytes >= plan.bytes && aligned(workspace, 16)),
@@ -1110,6 +1175,9 @@ extern "C" int sl8_attn_paged_block8(const void* q, int dtype, int rotate, float
   p.Hq = (int)Hq; p.Hkv = (int)Hkv; p.G = (int)(Hq / Hkv);
   p.q_mul = q_scale_mul;
   p.rotate = rotate != 0;
+  p.tree = static_cast<const uint2*>(tree_mask);
+  p.words = tree_mask ? (int)words : 0;
+  p.lse = lse;
   p.window = window_left < 0 ? -1 : (int)(window_left < (1 << 30) ? window_left : (1 << 30));
   p.slots = plan.slots;
   p.whole = plan.whole;
@@ -1127,7 +1195,8 @@ extern "C" int sl8_attn_paged_block8(const void* q, int dtype, int rotate, float
     }
     auto go = [&](auto dt) {
       constexpr int DT = decltype(dt)::value;
-      S::template kernel<DT>()<<<grid, S::THREADS, 0, st>>>(p);
+      if (tree_mask) S::template kernel<DT, true>()<<<grid, S::THREADS, 0, st>>>(p);
+      else S::template kernel<DT, false>()<<<grid, S::THREADS, 0, st>>>(p);
       if (plan.slots)
         attn_block8_join_kernel<DT, S::D, S::ROWS>
             <<<dim3((unsigned)plan.pairs, S::ROWS / JOIN_ROWS), 64 * JOIN_ROWS, 0, st>>>(p);
@@ -1137,4 +1206,35 @@ extern "C" int sl8_attn_paged_block8(const void* q, int dtype, int rotate, float
   });
   SL8_CHECK_LAUNCH(tag);
   return SL8_OK;
+}
+
+}  // namespace
+
+extern "C" int sl8_attn_paged_block8(const void* q, int dtype, int rotate, float q_scale_mul,
+                                     const int8_t* k_cache, const float* k_scale,
+                                     const int8_t* v_cache, const float* v_scale,
+                                     const int32_t* cu_lens, const int32_t* context_lens,
+                                     const int32_t* block_table, void* out, int64_t T, int64_t B,
+                                     int64_t Hq, int64_t Hkv, int64_t D, int64_t num_blocks,
+                                     int64_t block_size, int64_t max_blocks_per_seq,
+                                     int64_t window_left, void* workspace, size_t workspace_bytes,
+                                     void* stream) {
+  return attn_paged("attn_paged_block8", q, dtype, rotate, q_scale_mul, k_cache, k_scale, v_cache, v_scale, cu_lens,
+                    context_lens, block_table, nullptr, 0, out, nullptr, T, B, Hq, Hkv, D, num_blocks, block_size,
+                    max_blocks_per_seq, window_left, workspace, workspace_bytes, stream);
+}
+
+extern "C" int sl8_attn_paged_block8_tree(const void* q, int dtype, int rotate, float q_scale_mul,
+                                          const int8_t* k_cache, const float* k_scale,
+                                          const int8_t* v_cache, const float* v_scale,
+                                          const int32_t* cu_lens, const int32_t* context_lens,
+                                          const int32_t* block_table, const int64_t* tree_mask,
+                                          int64_t mask_words, void* out, float* lse, int64_t T, int64_t B,
+                                          int64_t Hq, int64_t Hkv, int64_t D, int64_t num_blocks,
+                                          int64_t block_size, int64_t max_blocks_per_seq,
+                                          int64_t window_left, void* workspace, size_t workspace_bytes,
+                                          void* stream) {
+  return attn_paged("attn_paged_block8", q, dtype, rotate, q_scale_mul, k_cache, k_scale, v_cache, v_scale, cu_lens,
+                    context_lens, block_table, tree_mask, mask_words, out, lse, T, B, Hq, Hkv, D, num_blocks,
+                    block_size, max_blocks_per_seq, window_left, workspace, workspace_bytes, stream);
 }

@@ -399,7 +399,8 @@ def attn_paged_block8(q: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.Ten
                       v_cache: torch.Tensor, v_scale: torch.Tensor, block_table: torch.Tensor,
                       context_lens: torch.Tensor, *, cu_lens: torch.Tensor | None = None,
                       scale: float | None = None, rotate: bool = True,
-                      window_left: int = -1) -> torch.Tensor:
+                      window_left: int = -1, tree_mask: torch.Tensor | None = None,
+                      return_lse: bool = False):
     """Attention over a paged int8 cache with one scale per block and head, written by
     quantize_kv_append_block8 (the same `rotate`): one to thousands of new tokens per sequence,
     mixed in one call, nothing read on the host.
@@ -407,14 +408,90 @@ def attn_paged_block8(q: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.Ten
     q [T,Hq,D] fp16/bf16 -> [T,Hq,D] of its dtype: sequence b's rows are cu_lens[b]..cu_lens[b+1]-1
     (None: row b), the last of its context_lens[b] tokens, which the cache holds already. Each sees
     the keys up to itself and, with window_left >= 0, only the last window_left of them; a row
-    that sees none and rows of no sequence (a padded batch, offsets of a part of one) are zeros."""
+    that sees none and rows of no sequence (a padded batch, offsets of a part of one) are zeros.
+
+    tree_mask int64 [T] or [T,1..4] (see tree_mask): drafted tokens in a tree. A row sees its
+    sequence's tokens in front of the new ones, and of those the j-th where bit j of its mask is set
+    (bits stand for the first 64 to 256; itself too only if marked); a window counts the marked ones
+    first and takes what is left of it in front. return_lse: (out, lse fp32 [T,Hq]), the logarithm
+    of each row's sum of e^score, -inf where it sees nothing."""
     softmax_scale = (1.0 / (q.shape[-1] ** 0.5)) if scale is None else scale
     q = q.contiguous()
     if q.data_ptr() % 16:
         q = q.clone()
     return _C.attn_paged_block8(q, softmax_scale * LOG2E, rotate, k_cache, k_scale, v_cache, v_scale,
                                 block_table.contiguous(), context_lens.contiguous(),
-                                None if cu_lens is None else cu_lens.contiguous(), window_left)
+                                None if cu_lens is None else cu_lens.contiguous(), window_left,
+                                tree_mask, return_lse)
+
+
+def tree_mask(parents: torch.Tensor, cu_lens: torch.Tensor | None = None, *, words: int = 1) -> torch.Tensor:
+    """The masks of drafted tokens from their parents, for attn_paged_block8: int64 [T, words] with the
+    bits of a token and of all above it. parents int32/int64 [T]: the parent's place among its
+    sequence's new tokens (in front of or behind it), -1 for those that follow the context; cu_lens as
+    there (None: one sequence of all rows). Tokens past a sequence's 64 * words-th have no bits."""
+    if parents.dim() != 1 or parents.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"tree_mask needs parents int32 or int64 [T], got {parents.dtype} {list(parents.shape)}")
+    if not 1 <= words <= _C._TREE_MAX_WORDS:
+        raise ValueError(f"words must be 1..{_C._TREE_MAX_WORDS}, got {words}")
+    T = parents.shape[0]
+    t = torch.arange(T, device=parents.device)
+    first, end = torch.zeros_like(t), torch.full_like(t, T)
+    if cu_lens is not None:
+        cu = cu_lens.long().contiguous()
+        b = (torch.searchsorted(cu, t, right=True) - 1).clamp(0, max(cu.shape[0] - 2, 0))
+        first, end = cu[b], cu[(b + 1).clamp(max=cu.shape[0] - 1)]
+    place = t - first
+    bit = torch.where((place >= 0) & (place < 64 * words), torch.ones_like(t) << (place % 64), 0)
+    mask = torch.where(place[:, None] // 64 == torch.arange(words, device=t.device), bit[:, None], 0)
+    up = torch.where(parents >= 0, first + parents.long(), T)
+    up = torch.where((up >= first) & (up < end), up, T)
+    none = mask.new_zeros(1, words)
+    for _ in range((64 * words - 1).bit_length()):  # the masks of twice as many levels, each time
+        mask = mask | torch.cat([mask, none])[up]
+        up = torch.cat([up, up.new_full((1,), T)])[up]
+    return mask
+
+
+def attn_weights_block8(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.Tensor,
+                        block_table: torch.Tensor, context_lens: torch.Tensor, weights: torch.Tensor, *,
+                        cu_lens: torch.Tensor | None = None, scale: float | None = None,
+                        rotate: bool = True, window_left: int = -1, decay: float = 1.0) -> None:
+    """Add up by cached key what softmax weights a step's rows gave it, in place: what kv_evict_block8
+    decides by. weights fp32 [B,Hkv,tokens] (a table's max_blocks * block_size at least; dense rows) of
+    sequence b, KV head h and token j becomes decay * weights plus the sum over its new rows, and over
+    the heads of the group, of e^(score - lse); a new token's own starts from 0, so reused rows need no
+    clearing, and entries behind the context are left alone.
+
+    q [T,Hq,D], k_cache, k_scale, block_table, context_lens, cu_lens, scale, rotate and window_left as in
+    attn_paged_block8, whose lse [T,Hq] (return_lse) this takes; rows are causal (drafted trees: the
+    accepted rows with their lse, once they are appended). Rows of lse -inf add nothing."""
+    softmax_scale = (1.0 / (q.shape[-1] ** 0.5)) if scale is None else scale
+    q = q.contiguous()
+    if q.data_ptr() % 16:
+        q = q.clone()
+    _C.attn_weights_block8(q, softmax_scale * LOG2E, rotate, lse.contiguous(), k_cache, k_scale,
+                           block_table.contiguous(), context_lens.contiguous(), weights,
+                           None if cu_lens is None else cu_lens.contiguous(), window_left, decay)
+
+
+def kv_evict_block8(k_cache: torch.Tensor, k_scale: torch.Tensor, v_cache: torch.Tensor,
+                    v_scale: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor,
+                    weights: torch.Tensor, new_table: torch.Tensor, *, budget: int, sinks: int = 0,
+                    recent: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
+    """Cut sequences of a block-scaled paged cache down to `budget` tokens a KV head: the first
+    `sinks`, the last `recent` and, between them, those of the largest weights (attn_weights_block8;
+    ties to the lowest index, no NaN); heads keep different ones. Shorter sequences keep all.
+
+    The kept tokens move in order into the blocks of new_table int32 [B,blocks], which no row of
+    block_table in the call may hold: from then on that is the sequence's table (the old blocks are
+    only read: shared prefixes stay whole). A block takes the largest scale of those its rows come
+    from; rows of others are rounded again, rows of the same are copied. weights [B,Hkv,tokens] of the
+    kept tokens move to the front, in place. Returns (lengths int32 [B], kept int32 [B,Hkv,budget]: the
+    tokens' old places, -1 behind the last). Nothing is read on the host."""
+    return _C.kv_evict_block8(k_cache, k_scale, v_cache, v_scale, block_table.contiguous(),
+                              context_lens.contiguous(), weights, new_table.contiguous(), budget, sinks,
+                              recent)
 
 
 def quantize_kv_cache_3bit(k: torch.Tensor, v: torch.Tensor, *, rotate: bool = True,
@@ -487,6 +564,18 @@ def linear_q6k(x: torch.Tensor, w_bytes: torch.Tensor, *, bias: torch.Tensor | N
                           getattr(_C, "gemm_decode_q6k", None))
 
 
+def linear_w8a8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *,
+                bias: torch.Tensor | None = None,
+                out_dtype: torch.dtype = torch.float16) -> torch.Tensor:
+    """Linear layer of int8 weights: x [..., K] fp16/bf16/fp32, each row quantised as by
+    quantize_i8_rowwise; w int8 [N,K] with w_scale fp32 [N] (a scale per output channel: the
+    per_row_i8 QTensor) -> [..., N] of out_dtype. K a multiple of 4, at least 16. The integer sums are
+    exact; scales and bias are applied in fp32 and the result is rounded once."""
+    *lead, K = x.shape
+    y = _C.linear_w8a8(x.reshape(-1, K).contiguous(), w.contiguous(), w_scale.contiguous(), bias, out_dtype)
+    return y.reshape(*lead, y.shape[-1])
+
+
 _FUSED_KQUANT_OPS = {"q4_k": linear_q4k, "q5_k": linear_q5k, "q6_k": linear_q6k}
 
 
@@ -494,12 +583,17 @@ def linear(x: torch.Tensor, qt, *, bias: torch.Tensor | None = None,
            out_dtype: torch.dtype = torch.float16) -> torch.Tensor:
     """Scheme-dispatched linear over a ``superl8_amd.format.QTensor`` (reference
     ops.py:2088-2150, the ``gguf_kquant`` arm): native Q4_K / Q5_K / Q6_K bytes run
-    on the fused kernels; any other scheme or type tag raises ValueError."""
+    on the fused kernels, ``per_row_i8`` weights that are not rotated on linear_w8a8; any other
+    scheme or type tag raises ValueError."""
     if qt.scheme == "gguf_kquant":
         op = _FUSED_KQUANT_OPS.get(qt.codebook)
         if op is not None:
             return op(x, qt.data, bias=bias, out_dtype=out_dtype)
         raise ValueError(f"superl8.linear: gguf_kquant type {qt.codebook!r} has no fused kernel")
+    if qt.scheme == "per_row_i8":
+        if qt.rotated:
+            raise ValueError("superl8.linear: rotated per_row_i8 weights have no product here")
+        return linear_w8a8(x, qt.data, qt.scale, bias=bias, out_dtype=out_dtype)
     raise ValueError(f"superl8.linear: unsupported weight scheme {qt.scheme!r}")
 
 
