@@ -4,6 +4,7 @@
 //   y[m,n] = xs[m] * ws[n] * sum_k c[m,k] w[n,k] + bias[n], rounded once.
 // The sums are exact integers (K < 2^17).
 #include <algorithm>
+#include <cmath>
 
 #include "attn_common.hpp"
 #include "rowquant.hpp"
@@ -12,12 +13,14 @@ namespace sl8 {
 namespace {
 
 constexpr int W8_MAX_K = 1 << 17;
-constexpr int W8_BK = 64;      // bytes of K a stage of the tile kernel, and what a row's codes are padded to
-constexpr int W8_STREAM = 64;  // most rows of x that stream the weights
+constexpr int W8_BK = 128;     // what a row's codes are padded to
+constexpr int W8_STREAM_ROWS = 16, W8_STREAM_K = 5120;  // the most that the streaming kernel takes
 
-// A row's codes in scratch, [M][Kp]: chunk c holds elements 16 c .. 16 c + 15. Where K is no multiple of
-// 16 the last one holds the row's last 16 elements, those of the chunk in front as zeros, so that 16 bytes of
-// a weight row that meet it end where the row ends; zeros up to Kp.
+// The rows' codes in scratch, [Kp / 128][M16][128]: the rows that meet at a step of K are next to each other,
+// in whole lines (rows K bytes apart can have all their lines in a few channels of the L2). Chunk c of a row
+// holds elements 16 c .. 16 c + 15. Where K is no multiple of 16 the last one holds the row's last 16 elements,
+// those of the chunk in front as zeros, so that 16 bytes of a weight row that meet it end where the row ends;
+// zeros up to Kp. Rows from M to M16 are not written: what they meet is not kept.
 struct W8Args {
   const void* x;
   const int8_t* w;
@@ -28,6 +31,7 @@ struct W8Args {
   float* xs;
   v4i* part;  // sums of the tiles that are split over K
   int M, N, K, Kp;
+  int M16;  // M in whole 16s
   int bias_dt;  // -1: none
   int nt_m, nt_n, whole, splits;  // tiles; those before `whole` are not split
 };
@@ -89,7 +93,7 @@ __global__ void __launch_bounds__(256) w8_quant_kernel(const W8Args p) {
   if (threadIdx.x == 0) p.xs[row] = safe;
   auto put = [&](int c, const float* x) {
     const uint2 lo = row_codes8<DT>(x, safe), hi = row_codes8<DT>(x + 8, safe);
-    if (c < chunks) *reinterpret_cast<uint4*>(p.codes + row * p.Kp + 16 * c) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+    if (c < chunks) *reinterpret_cast<uint4*>(p.codes + ((int64_t)(c >> 3) * p.M16 + row) * 128 + 16 * (c & 7)) = make_uint4(lo.x, lo.y, hi.x, hi.y);
   };
   if constexpr (NV > 0) {
 #pragma unroll
@@ -102,6 +106,15 @@ __global__ void __launch_bounds__(256) w8_quant_kernel(const W8Args p) {
   }
 }
 
+// A barrier behind which the workgroup's copies have arrived but for the last N of each thread, and the reads
+// in front of it are done. (A fence would wait for all copies.)
+template <int N> __device__ __forceinline__ void w8_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14);  // vmcnt(N) lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 typedef v4i v4i_u __attribute__((aligned(4)));  // rows of K % 16 != 0 are 4-byte aligned
 
 __device__ __forceinline__ float w8_bias(const W8Args& p, int n) {
@@ -111,86 +124,112 @@ __device__ __forceinline__ float w8_bias(const W8Args& p, int n) {
   return p.bias_dt == SL8_DTYPE_F16 ? h2f(b) : bf2f(b);
 }
 
-// ---------------------------------------------------------------------------
-// Few rows: each wave streams 16 NR weight rows' part of K straight into A operands of
-// v_mfma_i32_16x16x64_i8 (lane (g4, col): 16 bytes of row col), x's codes are the B operands; the 8 waves of a
-// workgroup have an eighth of K each and add their sums in LDS. Bound by the weights' bytes.
-// ---------------------------------------------------------------------------
-constexpr int WS_WAVES = 8;
-
-template <int ODT, int RT, int NR>
-__global__ void __launch_bounds__(64 * WS_WAVES) w8_stream_kernel(const W8Args p) {
-  constexpr int U = NR * RT <= 2 ? 4 : 2;  // steps whose loads go out together
-  __shared__ v4i sum_s[WS_WAVES][NR * RT][64];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col = lane & 15, g4 = lane >> 4;
-  const int n0 = blockIdx.x * 16 * NR;
-  const int8_t *w[NR], *x[RT];
+template <int ODT>
+__device__ __forceinline__ void w8_st4(void* out, int64_t i, const float* y) {
+  if constexpr (ODT == SL8_DTYPE_F32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(out) + i) = make_float4(y[0], y[1], y[2], y[3]);
+  } else {
+    uint32_t z[4];
 #pragma unroll
-  for (int r = 0; r < NR; ++r) w[r] = p.w + (int64_t)min(n0 + 16 * r + col, p.N - 1) * p.K;
-#pragma unroll
-  for (int r = 0; r < RT; ++r) x[r] = p.codes + (int64_t)min(16 * r + col, p.M - 1) * p.Kp;
-  v4i acc[NR][RT] = {};
-  const int steps = p.Kp / 64, s0 = wave * steps / WS_WAVES, s1 = (wave + 1) * steps / WS_WAVES;
-  for (int s = s0; s < s1; s += U) {
-    v4i a[U][NR], b[U][RT];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int k = 64 * min(s + u, s1 - 1) + 16 * g4;
-#pragma unroll
-      for (int r = 0; r < NR; ++r) a[u][r] = *reinterpret_cast<const v4i_u*>(w[r] + min(k, p.K - 16));
-#pragma unroll
-      for (int r = 0; r < RT; ++r) b[u][r] = *reinterpret_cast<const v4i*>(x[r] + k);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (s + u >= s1) break;
-#pragma unroll
-      for (int r = 0; r < NR; ++r)
-#pragma unroll
-        for (int t = 0; t < RT; ++t)
-          acc[r][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[u][r], b[u][t], acc[r][t], 0, 0, 0);
-    }
+    for (int e = 0; e < 4; ++e) z[e] = ODT == SL8_DTYPE_F16 ? f2h_bits(y[e]) : f2bf_bits(y[e]);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + i) = make_uint2(z[0] | z[1] << 16, z[2] | z[3] << 16);
   }
+}
+
+// ---------------------------------------------------------------------------
+// Up to 16 rows: 16 channels at a time, each wave with its part of K: weights straight from memory into A operands
+// of v_mfma_i32_16x16x64_i8 (lane (g4, col): 16 bytes of row col), the codes as B operands. The waves' sums
+// meet in LDS. Bound by the weights' bytes. The codes of a wave's part stay in registers while the workgroup goes
+// through its groups of channels, a group's weights on their way while the one before is multiplied; the two
+// halves of a line are read next to each other (U units of 128 bytes a wave).
+// ---------------------------------------------------------------------------
+constexpr int W8_WAVES = 8;
+
+// The sums y of channels n .. n + 3 of a row to its outputs.
+template <int ODT>
+__device__ __forceinline__ void w8_out4(const W8Args& p, v4i y, int m, int n) {
+  const float xs = p.xs[m];
+  float z[4];
 #pragma unroll
-  for (int r = 0; r < NR; ++r)
-#pragma unroll
-    for (int t = 0; t < RT; ++t) sum_s[wave][r * RT + t][lane] = acc[r][t];
-  __syncthreads();
-  for (int i = threadIdx.x; i < NR * RT * 64; i += 64 * WS_WAVES) {
-    const int blk = i >> 6, l = i & 63, m = 16 * (blk % RT) + (l & 15), n = n0 + 16 * (blk / RT) + 4 * (l >> 4);
-    v4i y = {0, 0, 0, 0};
-#pragma unroll
-    for (int x2 = 0; x2 < WS_WAVES; ++x2) y += sum_s[x2][blk][l];
-    if (m >= p.M) continue;
-    const float xs = p.xs[m];
+  for (int e = 0; e < 4; ++e) z[e] = (float)y[e] * xs * p.ws[min(n + e, p.N - 1)] + w8_bias(p, min(n + e, p.N - 1));
+  const int64_t to = (int64_t)m * p.N + n;
+  if (p.N % 4 == 0) {
+    w8_st4<ODT>(p.out, to, z);
+  } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (n + e < p.N) st_out<ODT>(p.out, (int64_t)m * p.N + n + e, (float)y[e] * xs * p.ws[n + e] + w8_bias(p, n + e));
+      if (n + e < p.N) st_out<ODT>(p.out, to + e, z[e]);
+  }
+}
+
+template <int ODT, int U>
+__global__ void __launch_bounds__(64 * W8_WAVES) w8_stream_kernel(const W8Args p) {
+  __shared__ v4i sum_s[2][W8_WAVES][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, g4 = lane >> 4;
+  const int groups = (p.N + 15) / 16, units = p.Kp / 128;
+  const int u0 = wave * units / W8_WAVES, u1 = (wave + 1) * units / W8_WAVES;
+  auto load = [&](int64_t g, v4i (&a)[U][2]) __attribute__((always_inline)) {
+    const int8_t* w = p.w + (int64_t)min(16 * (int)min(g, (int64_t)groups - 1) + col, p.N - 1) * p.K;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        a[u][i] = *reinterpret_cast<const v4i_u*>(w + min(128 * min(u0 + u, units - 1) + 64 * i + 16 * g4, p.K - 16));
+  };
+  v4i a0[U][2], a1[U][2], b[U][2];
+  load(blockIdx.x, a0);
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      // (rows past the last as the last; units past the wave's own are zeros)
+      const int8_t* x = p.codes + ((int64_t)min(u0 + u, units - 1) * p.M16 + min(col, p.M - 1)) * 128;
+      const v4i c = *reinterpret_cast<const v4i*>(x + 64 * i + 16 * g4);
+      b[u][i] = u0 + u < u1 ? c : v4i{0, 0, 0, 0};
+    }
+  int turn = 0;
+  auto group = [&](int64_t g, const v4i (&a)[U][2], v4i (&next)[U][2]) __attribute__((always_inline)) {
+    load(g + gridDim.x, next);
+    __builtin_amdgcn_sched_barrier(0);
+    v4i acc = {};
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[u][i], b[u][i], acc, 0, 0, 0);
+    sum_s[turn & 1][wave][lane] = acc;
+    w8_barrier<63>();  // (a turn's sums are read in front of the next barrier and written again behind it)
+    if (wave == turn % W8_WAVES) {  // by turns
+      const int m = lane >> 2, n = 16 * (int)g + 4 * (lane & 3);
+      v4i y = {0, 0, 0, 0};
+#pragma unroll
+      for (int x = 0; x < W8_WAVES; ++x) y += sum_s[turn & 1][x][16 * (lane & 3) + m];
+      if (m < p.M && n < p.N) w8_out4<ODT>(p, y, m, n);
+    }
+    ++turn;
+  };
+#pragma unroll 1
+  for (int64_t g = blockIdx.x; g < groups; g += 2 * gridDim.x) {
+    group(g, a0, a1);
+    if (g + gridDim.x < groups) group(g + gridDim.x, a1, a0);
   }
 }
 
 // ---------------------------------------------------------------------------
 // Many rows: BN x BM output tiles (channels x rows), MW waves along the rows and NW along the channels, each
-// with 32 NB x 32 MB of them on v_mfma_i32_32x32x32_i8. Stages of 64 bytes of K go through a ring of four in
-// LDS by direct copies, three stages ahead; 16-byte chunks of a row are placed by an xor of the row, so that
+// with 32 NB x 32 MB of them on v_mfma_i32_32x32x32_i8. Stages of 128 bytes of K (whole lines) go through two places
+// in LDS by direct copies, a stage ahead; 16-byte chunks of a row are placed by an xor of the row, so that
 // 16 rows of a read lie in different banks.
 // ---------------------------------------------------------------------------
-template <int BM_, int BN_, int MW_, int NW_> struct W8Tile {
-  static constexpr int BM = BM_, BN = BN_, MW = MW_, NW = NW_, THREADS = 64 * MW_ * NW_;
+template <int BM_, int BN_, int MW_, int NW_, int RING_> struct W8Tile {
+  static constexpr int RING = RING_;  // stages in LDS
+  static constexpr int BM = BM_, BN = BN_, MW = MW_, NW = NW_, BK = W8_BK, THREADS = 64 * MW_ * NW_;
   static constexpr int MB = BM / MW / 32, NB = BN / NW / 32;  // blocks of a wave
-  static constexpr int COPIES = (BM + BN) * 4 / THREADS;      // of 16 bytes a thread and stage
-  static_assert((BM + BN) * 4 % THREADS == 0 && BN * 4 % THREADS == 0, "whole copies");
+  static constexpr int CPR = BK / 16;                           // 16-byte chunks of a row and stage
+  static constexpr int COPIES = (BM + BN) * CPR / THREADS;      // of 16 bytes a thread and stage
+  static_assert((BM + BN) * CPR % THREADS == 0 && BN * CPR % THREADS == 0, "whole copies");
+  __device__ __forceinline__ static int swizzle(int row) { return (row >> 1) & 7; }
 };
-
-// A barrier behind which the workgroup's copies have arrived but for the last N of each thread, and the reads
-// in front of it are done. (A fence would wait for all copies.)
-template <int N> __device__ __forceinline__ void w8_barrier() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14);  // vmcnt(N) lgkmcnt(0)
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
 
 // Tile t: each XCD (workgroup id modulo 8) has a run of them, 8 rows of tiles at a time.
 __device__ __forceinline__ void w8_tile_at(const W8Args& p, int id, int& rt, int& ct) {
@@ -275,10 +314,11 @@ __device__ __forceinline__ void w8_store(const W8Args& p, const v16i (&acc)[S::N
 // DMA: 16-byte aligned weight rows, copied straight to LDS; else through registers.
 template <int ODT, typename S, bool DMA>
 __global__ void __launch_bounds__(S::THREADS, 2) w8_tile_kernel(const W8Args p) {
-  constexpr int ROWB = W8_BK, STAGE = (S::BM + S::BN) * ROWB, WCOP = S::BN * 4 / S::THREADS;
+  constexpr int ROWB = S::BK, STAGE = (S::BM + S::BN) * ROWB, WCOP = S::BN * S::CPR / S::THREADS;
   constexpr int OS = ODT == SL8_DTYPE_F32 ? 4 : 2;
   // one LDS object per stage: a copy into one never aliases reads of another
-  __shared__ __attribute__((aligned(16))) int8_t s0[STAGE], s1[STAGE], s2[STAGE], s3[STAGE];
+  __shared__ __attribute__((aligned(16))) int8_t s0[STAGE], s1[STAGE], s2[S::RING > 2 ? STAGE : 16],
+      s3[S::RING > 3 ? STAGE : 16];
   static_assert(S::MW * S::NW * 32 * S::NB * 32 * OS <= 2 * STAGE, "the outputs fit two stages");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, h = lane >> 5;
@@ -292,30 +332,32 @@ __global__ void __launch_bounds__(S::THREADS, 2) w8_tile_kernel(const W8Args p) 
   int rt, ct;
   w8_tile_at(p, id, rt, ct);
   const int m0 = rt * S::BM, n0 = ct * S::BN;
-  const int nk = p.Kp / W8_BK, k0 = split * nk / parts, k1 = (split + 1) * nk / parts;
+  const int nk = p.Kp / S::BK, k0 = split * nk / parts, k1 = (split + 1) * nk / parts;
   const int mw = wave % S::MW, nw = wave / S::MW;
 
   // chunk P of a stage: row P / 4 (weights, then x), place P % 4 of it
   const brsrc_t rw = make_rsrc(p.w + (int64_t)n0 * p.K, (uint32_t)(min(S::BN, p.N - n0) * p.K));
-  const brsrc_t rx = make_rsrc(p.codes + (int64_t)m0 * p.Kp, (uint32_t)(min(S::BM, p.M - m0) * p.Kp));
-  int off[S::COPIES], ch[S::COPIES];
+    int off[S::COPIES], ch[S::COPIES];
 #pragma unroll
   for (int i = 0; i < S::COPIES; ++i) {
-    const int P = i * S::THREADS + tid, row = P / 4;
-    ch[i] = 16 * ((P & 3) ^ ((row >> 2) & 3));
+    const int P = i * S::THREADS + tid, row = P / S::CPR;
+    ch[i] = 16 * ((P % S::CPR) ^ S::swizzle(row));
     if (i < WCOP) off[i] = min(row, p.N - n0 - 1) * p.K;
-    else off[i] = min(row - S::BN, p.M - m0 - 1) * p.Kp;
+    else off[i] = min(row - S::BN, p.M16 - m0 - 1) * 128;
   }
   v4i held[DMA ? 1 : S::COPIES];
   auto load = [&](int kt, int8_t* to) __attribute__((always_inline)) {
-    const int k = min(kt, k1 - 1) * W8_BK;
+    kt = min(kt, k1 - 1);
+    const int k = kt * S::BK;
+    const int8_t* x = p.codes + ((int64_t)kt * p.M16 + m0) * 128;
+    const brsrc_t rx = make_rsrc(x, (uint32_t)(S::BM * 128));
 #pragma unroll
     for (int i = 0; i < S::COPIES; ++i) {
       const bool is_w = i < WCOP;
-      const int at = is_w ? off[i] + min(k + ch[i], p.K - 16) : off[i] + k + ch[i];
+      const int at = is_w ? off[i] + min(k + ch[i], p.K - 16) : off[i] + ch[i];
       if constexpr (DMA) buf16_to_lds(is_w ? rw : rx, to + (i * S::THREADS + wave * 64) * 16, at, 0);
       else if (is_w) held[i] = *reinterpret_cast<const v4i_u*>(p.w + (int64_t)n0 * p.K + at);
-      else held[i] = *reinterpret_cast<const v4i*>(p.codes + (int64_t)m0 * p.Kp + at);
+      else held[i] = *reinterpret_cast<const v4i*>(x + at);
     }
   };
   auto keep = [&](int8_t* to) __attribute__((always_inline)) {
@@ -330,11 +372,11 @@ __global__ void __launch_bounds__(S::THREADS, 2) w8_tile_kernel(const W8Args p) 
   for (int nb = 0; nb < S::NB; ++nb)
 #pragma unroll
     for (int mb = 0; mb < S::MB; ++mb) acc[nb][mb] = v16i{};
-  const int swz = (l32 >> 2) & 3;
+  const int swz = S::swizzle(l32);
   const int wrow = (nw * S::NB * 32 + l32) * ROWB, xrow = (S::BN + mw * S::MB * 32 + l32) * ROWB;
   auto compute = [&](const int8_t* st) __attribute__((always_inline)) {
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
+    for (int ks = 0; ks < S::BK / 32; ++ks) {
       const int c = 16 * ((2 * ks + h) ^ swz);
       v4i a[S::NB], b[S::MB];
 #pragma unroll
@@ -348,41 +390,54 @@ __global__ void __launch_bounds__(S::THREADS, 2) w8_tile_kernel(const W8Args p) 
           acc[nb][mb] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[nb], b[mb], acc[nb][mb], 0, 0, 0);
     }
   };
-  // stage kt is there when all but the copies of the two behind it have arrived; the ring's place of the stage
-  // before it is free behind the barrier
+  // the other stage's place is free behind the barrier
   auto step = [&](int kt, const int8_t* st, int8_t* to) __attribute__((always_inline)) {
-    w8_barrier<DMA ? 2 * S::COPIES : 63>();
-    load(kt + 3, to);
+    w8_barrier<DMA ? (S::RING - 2) * S::COPIES : 63>();
+    load(kt + S::RING - 1, to);
+    __builtin_amdgcn_sched_barrier(0);
     compute(st);
     keep(to);
   };
+  int kt = k0;
   load(k0, s0);
   keep(s0);
-  load(k0 + 1, s1);
-  keep(s1);
-  load(k0 + 2, s2);
-  keep(s2);
-  int kt = k0;
-#pragma unroll 1
-  for (; kt + 4 <= k1; kt += 4) {
-    step(kt, s0, s3);
-    step(kt + 1, s1, s0);
-    step(kt + 2, s2, s1);
-    step(kt + 3, s3, s2);
+  if constexpr (S::RING > 2) {
+    load(k0 + 1, s1);
+    keep(s1);
   }
-  if (kt < k1) step(kt, s0, s3);
-  if (kt + 1 < k1) step(kt + 1, s1, s0);
-  if (kt + 2 < k1) step(kt + 2, s2, s1);
+  if constexpr (S::RING > 3) {
+    load(k0 + 2, s2);
+    keep(s2);
+  }
+#pragma unroll 1
+  for (; kt + S::RING <= k1; kt += S::RING) {
+    if constexpr (S::RING == 2) {
+      step(kt, s0, s1);
+      step(kt + 1, s1, s0);
+    } else if constexpr (S::RING == 3) {
+      step(kt, s0, s2);
+      step(kt + 1, s1, s0);
+      step(kt + 2, s2, s1);
+    } else {
+      step(kt, s0, s3);
+      step(kt + 1, s1, s0);
+      step(kt + 2, s2, s1);
+      step(kt + 3, s3, s2);
+    }
+  }
+  if (kt < k1) step(kt, s0, S::RING == 2 ? s1 : S::RING == 3 ? s2 : s3);
+  if (S::RING > 2 && kt + 1 < k1) step(kt + 1, s1, s0);
+  if (S::RING > 3 && kt + 2 < k1) step(kt + 2, s2, s1);
   w8_barrier<0>();  // (copies past the last stage land where the outputs go)
   if (parts > 1) {
-    v4i* to = p.part + ((int64_t)(blockIdx.x - p.whole) * S::THREADS + tid) * (S::NB * S::MB * 4);
+    v4i* to = p.part + (int64_t)(blockIdx.x - p.whole) * S::THREADS * (S::NB * S::MB * 4) + tid;
 #pragma unroll
     for (int nb = 0; nb < S::NB; ++nb)
 #pragma unroll
       for (int mb = 0; mb < S::MB; ++mb)
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          to[(nb * S::MB + mb) * 4 + q] = v4i{acc[nb][mb][4 * q], acc[nb][mb][4 * q + 1], acc[nb][mb][4 * q + 2],
+          to[((nb * S::MB + mb) * 4 + q) * S::THREADS] = v4i{acc[nb][mb][4 * q], acc[nb][mb][4 * q + 1], acc[nb][mb][4 * q + 2],
                                               acc[nb][mb][4 * q + 3]};
     return;
   }
@@ -391,68 +446,72 @@ __global__ void __launch_bounds__(S::THREADS, 2) w8_tile_kernel(const W8Args p) 
   w8_store<ODT, S>(p, acc, m0 + mw * S::MB * 32, n0 + nw * S::NB * 32, lane, lds);
 }
 
-// The parts of a tile that was split over K, added up.
+// The parts of the tiles that were split over K, added up: a workgroup for a block of a wave's, a thread for
+// four channels of a row, a row's next to each other.
 template <int ODT, typename S>
-__global__ void __launch_bounds__(S::THREADS) w8_join_kernel(const W8Args p) {
-  constexpr int OS = ODT == SL8_DTYPE_F32 ? 4 : 2, OUTB = 32 * S::NB * 32 * OS;
-  __shared__ __attribute__((aligned(16))) int8_t lds[S::MW * S::NW * OUTB];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+__global__ void __launch_bounds__(256) w8_join_kernel(const W8Args p) {
+  constexpr int BLOCKS = S::MW * S::NW * S::NB * S::MB, TILE = BLOCKS * 256;  // of 32 x 32; v4i of a tile
+  const int tile = blockIdx.x / BLOCKS, blk = blockIdx.x % BLOCKS;
+  const int wave = blk % (S::MW * S::NW), mb = blk / (S::MW * S::NW) % S::MB, nb = blk / (S::MW * S::NW * S::MB);
+  const int l32 = threadIdx.x >> 3, q = threadIdx.x >> 1 & 3, h = threadIdx.x & 1;
   int rt, ct;
-  w8_tile_at(p, p.whole + blockIdx.x, rt, ct);
-  v16i acc[S::NB][S::MB];
-#pragma unroll
-  for (int nb = 0; nb < S::NB; ++nb)
-#pragma unroll
-    for (int mb = 0; mb < S::MB; ++mb) acc[nb][mb] = v16i{};
-  for (int s = 0; s < p.splits; ++s) {
-    const v4i* from = p.part + ((int64_t)(blockIdx.x * p.splits + s) * S::THREADS + tid) * (S::NB * S::MB * 4);
-#pragma unroll
-    for (int nb = 0; nb < S::NB; ++nb)
-#pragma unroll
-      for (int mb = 0; mb < S::MB; ++mb)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const v4i y = from[(nb * S::MB + mb) * 4 + q];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[nb][mb][4 * q + e] += y[e];
-        }
-  }
-  w8_store<ODT, S>(p, acc, rt * S::BM + wave % S::MW * S::MB * 32, ct * S::BN + wave / S::MW * S::NB * 32, lane,
-                   lds + wave * OUTB);
+  w8_tile_at(p, p.whole + tile, rt, ct);
+  const int m = rt * S::BM + (wave % S::MW * S::MB + mb) * 32 + l32;
+  const int n = ct * S::BN + (wave / S::MW * S::NB + nb) * 32 + 8 * q + 4 * h;
+  if (m >= p.M || n >= p.N) return;
+  const v4i* from = p.part + (int64_t)tile * p.splits * TILE + ((nb * S::MB + mb) * 4 + q) * S::THREADS + wave * 64 +
+                    32 * h + l32;
+  v4i y = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) y += from[(int64_t)s * TILE];
+  w8_out4<ODT>(p, y, m, n);
 }
 
-using Tile256 = W8Tile<256, 256, 2, 4>;
-using Tile128 = W8Tile<128, 128, 2, 2>;
+using Tile256 = W8Tile<256, 256, 2, 4, 2>;
+using Tile128 = W8Tile<128, 128, 2, 2, 2>;
+using Tile64 = W8Tile<64, 128, 1, 4, 3>;
+using Tile32 = W8Tile<32, 128, 1, 4, 4>;
 
 // How a call runs.
 struct W8Plan {
-  int rows;  // streamed: rows of x in steps of 16; 0: tiles
-  bool big;
+  int tile;  // rows of an output tile; 0: streamed
   int nt_m, nt_n, whole, splits;
   size_t code_bytes, bytes;
 };
 
+// What takes the least time: streaming, or a tile and the parts in which the last round's tiles are cut along K.
+// Tiles: rounds of the workgroups that are resident at once, each of as many stages as K has, a stage taking
+// one_us where a CU has one workgroup, up to full_us where it has per_cu; a join costs its launch and its
+// partial sums. Neither is faster than the weights' bytes.
 W8Plan w8_plan(int64_t M, int64_t N, int64_t K) {
+  struct Shape { int bm, bn, per_cu; double one_us, full_us; };
+  static const Shape shapes[] = {{256, 256, 1, 1.7, 1.7}, {128, 128, 2, 0.9, 1.2}, {64, 128, 2, 0.6, 0.95}, {32, 128, 2, 0.45, 0.8}};
   W8Plan a{};
-  a.code_bytes = ((size_t)M * (w8_padded(K) + sizeof(float)) + 15) / 16 * 16;
+  a.code_bytes = ((size_t)((M + 15) / 16 * 16) * w8_padded(K) + (size_t)M * sizeof(float) + 15) / 16 * 16;
   a.bytes = a.code_bytes;
   a.splits = 1;
-  if (M <= W8_STREAM) {
-    a.rows = (int)((M + 15) / 16);
-    return a;
-  }
-  const int64_t cus = cu_count();
-  auto tiles = [&](int64_t b) { return ((M + b - 1) / b) * ((N + b - 1) / b); };
-  a.big = tiles(256) >= cus;
-  const int64_t b = a.big ? 256 : 128, n = tiles(b), slots = a.big ? cus : 2 * cus;
-  a.nt_m = (int)((M + b - 1) / b);
-  a.nt_n = (int)((N + b - 1) / b);
-  const int64_t rest = n % slots;
-  a.whole = (int)n;
-  if (rest && rest * 2 <= slots && K >= 1024) {
-    a.splits = (int)std::min<int64_t>(std::min<int64_t>(slots / rest, K / 512), 8);
-    a.whole = (int)(n - rest);
-    a.bytes += (size_t)rest * a.splits * b * b * 4;
+  const double stages = (double)w8_padded(K) / W8_BK, cus = cu_count();
+  double best = 1e30;
+  if (M <= W8_STREAM_ROWS && K <= W8_STREAM_K) best = 3. + (double)N * K / 4e6;
+  for (const Shape& s : shapes) {
+    if (s.bm < 128 && M > s.bm) continue;
+    const int64_t nt_m = (M + s.bm - 1) / s.bm, nt_n = (N + s.bn - 1) / s.bn, n = nt_m * nt_n;
+    const int64_t slots = (int64_t)cus * s.per_cu, rest = n % slots, most = n - rest;
+    for (int S = 1; S <= 8; ++S) {
+      if (S > 1 && (rest == 0 || stages < 4 * S || rest * S > slots)) break;
+      const double more = std::ceil((double)rest * S / cus) - 1.;
+      const double part = rest ? std::ceil(stages / S) * (s.one_us + (s.full_us - s.one_us) * more / std::max(1, s.per_cu - 1)) : 0.;
+      double us = std::max((double)(most / slots) * stages * s.full_us + part, (double)N * K / 4.8e6) + 3.;
+      if (S > 1) us += 3. + (double)rest * S * s.bm * s.bn * 4 / 4e6;
+      if (us >= best) continue;
+      best = us;
+      a.tile = s.bm;
+      a.nt_m = (int)nt_m;
+      a.nt_n = (int)nt_n;
+      a.splits = S;
+      a.whole = (int)(S > 1 ? most : n);
+      a.bytes = a.code_bytes + (S > 1 ? (size_t)rest * S * s.bm * s.bn * 4 : 0);
+    }
   }
   return a;
 }
@@ -489,9 +548,9 @@ extern "C" int sl8_linear_w8a8(const void* x, int x_dtype, const int8_t* w, cons
   W8Args p{};
   p.x = x; p.w = w; p.ws = w_scale; p.bias = bias; p.out = out;
   p.bias_dt = bias ? bias_dtype : -1;
-  p.M = (int)M; p.N = (int)N; p.K = (int)K; p.Kp = (int)w8_padded(K);
+  p.M = (int)M; p.N = (int)N; p.K = (int)K; p.Kp = (int)w8_padded(K); p.M16 = (int)((M + 15) / 16 * 16);
   p.codes = static_cast<int8_t*>(workspace);
-  p.xs = reinterpret_cast<float*>(p.codes + M * p.Kp);
+  p.xs = reinterpret_cast<float*>(p.codes + (int64_t)p.M16 * p.Kp);
   p.part = reinterpret_cast<v4i*>(p.codes + plan.code_bytes);
   p.nt_m = plan.nt_m; p.nt_n = plan.nt_n; p.whole = plan.whole; p.splits = plan.splits;
   const int64_t split = (int64_t)plan.nt_m * plan.nt_n - plan.whole, grid = plan.whole + split * plan.splits;
@@ -510,22 +569,23 @@ extern "C" int sl8_linear_w8a8(const void* x, int x_dtype, const int8_t* w, cons
   else quant(integral_constant<int, SL8_DTYPE_F32>{});
   auto go = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    if (plan.rows) {
-      constexpr int NR = 2;
-      const unsigned wgs = (unsigned)((N + 16 * NR - 1) / (16 * NR));
-      if (plan.rows == 1) w8_stream_kernel<DT, 1, NR><<<wgs, 64 * WS_WAVES, 0, st>>>(p);
-      else if (plan.rows == 2) w8_stream_kernel<DT, 2, NR><<<wgs, 64 * WS_WAVES, 0, st>>>(p);
-      else w8_stream_kernel<DT, 4, NR><<<wgs, 64 * WS_WAVES, 0, st>>>(p);
+    if (plan.tile == 0) {
+      const unsigned wgs = (unsigned)std::min<int64_t>((N + 15) / 16, 2 * cu_count());
+      if (K <= 2048) w8_stream_kernel<DT, 2><<<wgs, 64 * W8_WAVES, 0, st>>>(p);
+      else if (K <= 4096) w8_stream_kernel<DT, 4><<<wgs, 64 * W8_WAVES, 0, st>>>(p);
+      else w8_stream_kernel<DT, 5><<<wgs, 64 * W8_WAVES, 0, st>>>(p);
       return;
     }
     auto tile = [&](auto shape) {
       using S = decltype(shape);
       if (K % 16 == 0) w8_tile_kernel<DT, S, true><<<(unsigned)grid, S::THREADS, 0, st>>>(p);
       else w8_tile_kernel<DT, S, false><<<(unsigned)grid, S::THREADS, 0, st>>>(p);
-      if (split) w8_join_kernel<DT, S><<<(unsigned)split, S::THREADS, 0, st>>>(p);
+      if (split) w8_join_kernel<DT, S><<<(unsigned)(split * (S::BM * S::BN / 1024)), 256, 0, st>>>(p);
     };
-    if (plan.big) tile(Tile256{});
-    else tile(Tile128{});
+    if (plan.tile == 256) tile(Tile256{});
+    else if (plan.tile == 128) tile(Tile128{});
+    else if (plan.tile == 64) tile(Tile64{});
+    else tile(Tile32{});
   };
   if (out_dtype == SL8_DTYPE_F16) go(integral_constant<int, SL8_DTYPE_F16>{});
   else if (out_dtype == SL8_DTYPE_BF16) go(integral_constant<int, SL8_DTYPE_BF16>{});
