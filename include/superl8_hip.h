@@ -445,7 +445,10 @@ int sl8_attn_paged_block8(const void* q, int dtype, int rotate, float q_scale_mu
  * the new ones, and new token t < 64 * mask_words where bit t % 64 of word t / 64 of its mask is set. A window
  * keeps the last window_left of those: the marked ones, all of them, and of the tokens in front the last
  * max(0, window_left - marked). lse (NULL: not wanted) fp32 [T,Hq]: ln of the row's sum of e^score,
- * -inf for a row that sees nothing or of no sequence. Workspace as above. */
+ * -inf for a row that sees nothing or of no sequence. Workspace, with a mask:
+ * sl8_attn_paged_block8_tree_workspace() bytes, else as above. */
+size_t sl8_attn_paged_block8_tree_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                            int64_t max_context_len);
 int sl8_attn_paged_block8_tree(const void* q, int dtype, int rotate, float q_scale_mul,
                                const int8_t* k_cache, const float* k_scale, const int8_t* v_cache,
                                const float* v_scale, const int32_t* cu_lens,

@@ -985,7 +985,9 @@ def attn_paged_block8(q, q_mul, rotate, k_cache, k_scale, v_cache, v_scale, bloc
     lse = q.new_empty((T, Hq), dtype=torch.float32) if return_lse else None
     if T and Hq:
         with on_device(q):
-            ws_bytes = _lib.load().sl8_attn_paged_block8_workspace(T, B, Hq, Hkv, D, maxb * bs)
+            lib = _lib.load()
+            ws_bytes = (lib.sl8_attn_paged_block8_tree_workspace if words else
+                        lib.sl8_attn_paged_block8_workspace)(T, B, Hq, Hkv, D, maxb * bs)
             ws = q.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
             if words or return_lse:
                 call("sl8_attn_paged_block8_tree", q.data_ptr(), dtype_code(q.dtype), int(bool(rotate)),

@@ -52,7 +52,7 @@ struct AttnArgs {
   float q_mul;
   int window;  // below 0: none
   bool rotate;
-  const uint2* tree;  // [T][words] of 64 bits, with TREE
+  const uint64_t* tree;  // [T][words], with TREE
   int words;
   float* lse;  // [T][Hq] or null
   int slots;      // workgroups to split the keys over, 0: no splits
@@ -303,8 +303,9 @@ __device__ __forceinline__ int64_t row_at(const AttnArgs& p, const Span& w, int 
 }
 
 // The unit's rows as int8 codes in LDS (row r at place(r)) with their scales (times q_mul); rows past
-// the last are zeros.
-template <int DT, int D, int ROWS, int THREADS, typename F>
+// the last are zeros. WIDE: as row_codes_wide has them (a tree's lse goes to callers in 32 bits, and a code
+// that another one stands for moves it by up to 10^-3: 1e-6 of 16 trees' 24000, 4e-8 with these).
+template <int DT, int D, int ROWS, int THREADS, bool WIDE, typename F>
 __device__ __forceinline__ void quant_rows(const AttnArgs& p, const Span& w, int kvh, F place, float* qs_s) {
   constexpr int LPR = row_lanes(D), RPB = THREADS / LPR;
   constexpr int N = ROWS / RPB > 4 ? 4 : ROWS / RPB > 1 ? ROWS / RPB : 1;  // rows a thread reads at once
@@ -324,6 +325,13 @@ __device__ __forceinline__ void quant_rows(const AttnArgs& p, const Span& w, int
       const bool live = r < w.cnt;
       float f[8];
       VecIO<DT>::unpack(raw[i], f);
+      if constexpr (WIDE) {
+        float safe;
+        const uint2 c = row_codes_wide<D>(f, lane, p.rotate, safe);
+        reinterpret_cast<uint2*>(place(r))[lane] = live ? c : make_uint2(0, 0);
+        if (lane == 0) qs_s[r] = live ? safe * p.q_mul : 0.f;
+        continue;
+      }
       if (p.rotate) hadamard_row<D, DT != SL8_DTYPE_F16>(f, lane);
       float amax = 0.f;
 #pragma unroll
@@ -337,16 +345,20 @@ __device__ __forceinline__ void quant_rows(const AttnArgs& p, const Span& w, int
   }
 }
 
-// The masks of a unit's rows in LDS, with zeros past the last word (rows past the last: as the last).
-constexpr int TREE_MAX = 4, TREE_WORDS = 2 * TREE_MAX;  // words of 64 bits and of 32
+// The masks of a unit's rows in LDS (rows past the last: as the last), zeros behind the last word.
+constexpr int TREE_MAX = 4, TREE_ROW = TREE_MAX + 1;  // words of 64 bits
 template <int ROWS, int THREADS>
-__device__ __forceinline__ void load_tree(const AttnArgs& p, const Span& w, uint32_t* tree_s) {
-  for (int i = threadIdx.x; i < ROWS * TREE_MAX; i += THREADS) {
-    const int r = i / TREE_MAX, x = i % TREE_MAX;
-    uint2 v = make_uint2(0, 0);
-    if (x < p.words) v = p.tree[(w.row0 + token_of(w, min(r, w.cnt - 1))) * p.words + x];
-    *reinterpret_cast<uint2*>(tree_s + 2 * i) = v;
+__device__ __forceinline__ void load_tree(const AttnArgs& p, const Span& w, uint64_t* tree_s) {
+  for (int i = threadIdx.x; i < ROWS * TREE_ROW; i += THREADS) {
+    const int r = i / TREE_ROW, x = i % TREE_ROW;
+    tree_s[i] = x < p.words ? p.tree[(w.row0 + token_of(w, min(r, w.cnt - 1))) * p.words + x] : 0;
   }
+}
+// Bits [a, b) of 64.
+__device__ __forceinline__ uint64_t bit_range(int a, int b) {
+  a = max(a, 0);
+  b = min(b, 64);
+  return a < b ? ~0ull >> (64 - (b - a)) << a : 0;
 }
 
 // The logarithm of a row's sum l of weights under reference m (log2).
@@ -406,11 +418,11 @@ struct RowState {
   int in0, in1;          // keys that every row of the unit sees: [in0, in1)
   float m[RT], l[RT];    // reference (log2) and sum of weights / vs
   v4f o[RT][D / 16];
-  const uint32_t* bits;  // TREE: the mask of row col in LDS; of row 16 rt + col TREE_WORDS * 16 rt further
+  const uint64_t* bits;  // TREE: the mask of row col in LDS; of row 16 rt + col TREE_ROW * 16 rt further
   int pos0;
 
   __device__ __forceinline__ void init(const AttnArgs& p, const Span& w, int r0, int col, const float* qs_s,
-                                       const uint32_t* tree_s) {
+                                       const uint64_t* tree_s) {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const int r = r0 + 16 * rt + col;
@@ -422,7 +434,7 @@ struct RowState {
         int64_t from = (int64_t)pos - p.window + 1;
         if constexpr (TREE) {
           int marked = 0;
-          for (int x = 0; x < 2 * p.words; ++x) marked += __builtin_popcount(tree_s[(r0 + 16 * rt + col) * TREE_WORDS + x]);
+          for (int x = 0; x < p.words; ++x) marked += __builtin_popcountll(tree_s[(r0 + 16 * rt + col) * TREE_ROW + x]);
           from = (int64_t)w.pos0 - max(p.window - marked, 0);
         }
         low[rt] = (int)max(from, (int64_t)0);
@@ -433,22 +445,27 @@ struct RowState {
       for (int t = 0; t < D / 16; ++t) o[rt][t] = v4f{0.f, 0.f, 0.f, 0.f};
     }
     in1 = min(w.pos0 + (TREE ? 0 : w.tok + 1), w.k1);
-    in0 = p.window >= 0 ? w.pos0 - (TREE ? 0 : p.window - 1 - token_of(w, w.cnt - 1)) : 0;
+    in0 = 0;
+    if (p.window >= 0) in0 = TREE ? w.pos0 - max(p.window - 64 * p.words, 0) : w.pos0 + token_of(w, w.cnt - 1) - p.window + 1;
     if constexpr (TREE) {
-      bits = tree_s + (r0 + col) * TREE_WORDS;
+      bits = tree_s + (r0 + col) * TREE_ROW;
       pos0 = w.pos0;
     }
   }
 
-  // Whether the row of lane col in row tile rt sees a key.
-  __device__ __forceinline__ bool sees(int rt, int key) const {
-    if constexpr (TREE) {
-      if (key >= pos0) {  // (bits past the mask's last word were cleared)
-        const int t = key - pos0;
-        return key < lim[rt] && t < 32 * TREE_WORDS && (bits[16 * rt * TREE_WORDS + (t >> 5)] >> (t & 31) & 1);
-      }
+  // TREE: which of 64 keys the row of lane col in row tile rt sees.
+  __device__ __forceinline__ uint64_t seen(int rt, int key0) const {
+    const uint64_t* m = bits + 16 * rt * TREE_ROW;
+    const int at = key0 - pos0;  // place of the first among the new keys
+    uint64_t v = 0;
+    if (at >= 0 && at < 64 * TREE_MAX) {
+      v = m[at >> 6] >> (at & 63);
+      if (at & 63) v |= m[(at >> 6) + 1] << (64 - (at & 63));
+    } else if (at < 0) {
+      v = bit_range(low[rt] - key0, -at);
+      if (at > -64) v |= m[0] << -at;
     }
-    return key < lim[rt] && key >= low[rt];
+    return v & bit_range(0, lim[rt] - key0);
   }
 
   // Weights of NG groups of 16 keys from their scores (lane (g4, col): keys 16 g + 4 g4 + i from
@@ -479,14 +496,17 @@ struct RowState {
     }
     if (!(key0 >= in0 && keys_end <= in1)) {
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
+      for (int rt = 0; rt < RT; ++rt) {
+        uint64_t see = 0;
+        if constexpr (TREE) see = seen(rt, key0) >> (4 * g4);
 #pragma unroll
         for (int g = 0; g < NG; ++g)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int key = key0 + 16 * g + 4 * g4 + i;
-            if (!sees(rt, key)) x[rt][g][i] = -INFINITY;
+            if (TREE ? !(see >> (16 * g + i) & 1) : key >= lim[rt] || key < low[rt]) x[rt][g][i] = -INFINITY;
           }
+      }
     }
     float top[RT];
 #pragma unroll
@@ -576,7 +596,7 @@ __global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const
   __shared__ __attribute__((aligned(16))) int8_t v0_s[A8_WAVES * KT * D], v1_s[A8_WAVES * KT * D];
   __shared__ __attribute__((aligned(16))) int8_t q_s[ROWS * D];
   __shared__ float qs_s[ROWS], m_s[A8_WAVES][ROWS], l_s[A8_WAVES][ROWS];
-  __shared__ __attribute__((aligned(8))) uint32_t tree_s[TREE ? ROWS * TREE_WORDS : 2];
+  __shared__ uint64_t tree_s[TREE ? ROWS * TREE_ROW : 1];
   static_assert(ROWS * D * 4 * A8_WAVES <= 2 * A8_WAVES * KT * D, "the sums fit the ring");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, g4 = lane >> 4;
@@ -630,7 +650,7 @@ __global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const
   };
   if (ntiles) load(cur, 0, v0_s);
 
-  quant_rows<DT, D, ROWS, A8_THREADS>(p, w, it.kvh, [&](int r) { return q_s + r * D; }, qs_s);
+  quant_rows<DT, D, ROWS, A8_THREADS, TREE>(p, w, it.kvh, [&](int r) { return q_s + r * D; }, qs_s);
   if constexpr (TREE) load_tree<ROWS, A8_THREADS>(p, w, tree_s);
   __syncthreads();
 
@@ -808,7 +828,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_block8_tile_kernel(const Attn
   __shared__ __attribute__((aligned(16))) int8_t k0_s[KT * D], k1_s[KT * D];
   __shared__ __attribute__((aligned(16))) uint16_t v0_s[KT * D], v1_s[KT * D];
   __shared__ float qs_s[ROWS];
-  __shared__ __attribute__((aligned(8))) uint32_t tree_s[TREE ? ROWS * TREE_WORDS : 2];
+  __shared__ uint64_t tree_s[TREE ? ROWS * TREE_ROW : 1];
   static_assert(ROWS <= 4 * KT, "the rows' codes fit where V will be");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, g4 = lane >> 4;
@@ -862,7 +882,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_block8_tile_kernel(const Attn
   auto q_place = [&](int r) {
     return r < FIT ? reinterpret_cast<int8_t*>(v0_s) + r * D : reinterpret_cast<int8_t*>(v1_s) + (r - FIT) * D;
   };
-  quant_rows<DT, D, ROWS, THREADS>(p, w, it.kvh, q_place, qs_s);
+  quant_rows<DT, D, ROWS, THREADS, TREE>(p, w, it.kvh, q_place, qs_s);
   if constexpr (TREE) load_tree<ROWS, THREADS>(p, w, tree_s);
   __syncthreads();
   v4i qb[RT][KS];
@@ -1040,6 +1060,7 @@ template <int D_, int RT_, int NW_> struct Shape {
   static constexpr int D = D_, RT = RT_, NW = NW_, ROWS = 16 * RT_ * (NW_ ? NW_ : 1);
   static constexpr int THREADS = NW_ ? 64 * NW_ : A8_THREADS;
   template <int DT, bool TREE> static auto kernel() {
+    static_assert(!TREE || !NW_ || RT_ == 1, "trees go to tiles of 64 rows");
     if constexpr (NW_) return attn_block8_tile_kernel<DT, D, RT, NW, TREE>;
     else return attn_block8_stream_kernel<DT, D, RT, TREE>;
   }
@@ -1067,15 +1088,18 @@ template <int D_, int RT_, int NW_> struct Shape {
 // rows (the drafts above) take 57 in tiles, 88 streamed as two units. 32 streamed rows at D = 128 need more
 // than the 256 registers of two waves a SIMD: 27 spill (96 to 112 bytes a lane) and come back in the loop
 // over keys; 16 rows at D = 256 spill 2, and 32 rows there, whose sums take 128, are not built.
+// Trees go to tiles of 64 rows: their rows fill 128 badly, and the masks' registers are theirs. 16 trees of 31 to 60
+// tokens (124 to 240 rows) on 1024 to 8191 keys: 107 us, 116 in tiles of 128; D = 256, 4 of 66 to 129 (8 heads to a
+// KV head) on 513 to 4096: 55, 111.
 template <typename F>
-auto with_shape(int64_t D, int64_t rows, F&& f) {
+auto with_shape(int64_t D, int64_t rows, bool tree, F&& f) {
   auto by_rows = [&](auto d) {
     constexpr int DD = decltype(d)::value;
     if (rows <= 16) return f(Shape<DD, 1, 0>{});
     if constexpr (DD < 256) {
       if (rows <= 32) return f(Shape<DD, 2, 0>{});
     }
-    if (rows <= 64) return f(Shape<DD, 1, 4>{});
+    if (rows <= 64 || tree) return f(Shape<DD, 1, 4>{});
     return f(Shape<DD, 2, 4>{});
   };
   if (D == 64) return by_rows(std::integral_constant<int, 64>{});
@@ -1093,12 +1117,12 @@ struct AttnPlan {
   size_t bytes;
 };
 
-AttnPlan attn_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t keys) {
+AttnPlan attn_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t keys, bool tree) {
   AttnPlan a{};
   if (T == 0 || B == 0 || Hq == 0) return a;
   const int64_t G = Hq / Hkv;
   a.rows = (T * G + B - 1) / B;
-  with_shape(D, a.rows, [&](auto sh) {
+  with_shape(D, a.rows, tree, [&](auto sh) {
     constexpr int ROWS = decltype(sh)::ROWS;
     a.pairs = Hkv * (T * G / ROWS + B);
     // Splits pay where workgroups would idle, or wait for the longest sequence of a batch, and all
@@ -1127,12 +1151,25 @@ AttnPlan attn_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int
 
 using namespace sl8;
 
-extern "C" size_t sl8_attn_paged_block8_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
-                                                    int64_t max_context_len) {
+namespace {
+
+size_t paged_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_context_len, bool tree) {
   // (sizes that the call refuses: nothing to compute, and no quotient by a head dim of 0)
   if (T <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || T >= (1LL << 28) || B >= (1 << 24) || Hq >= (1 << 16)) return 0;
   if ((D != 64 && D != 128 && D != 256) || Hq % Hkv) return 0;
-  return attn_plan(T, B, Hq, Hkv, D, max_context_len).bytes;
+  return attn_plan(T, B, Hq, Hkv, D, max_context_len, tree).bytes;
+}
+
+}  // namespace
+
+extern "C" size_t sl8_attn_paged_block8_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                                    int64_t max_context_len) {
+  return paged_workspace(T, B, Hq, Hkv, D, max_context_len, false);
+}
+
+extern "C" size_t sl8_attn_paged_block8_tree_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                                       int64_t max_context_len) {
+  return paged_workspace(T, B, Hq, Hkv, D, max_context_len, true);
 }
 
 namespace {
@@ -1165,7 +1202,7 @@ int attn_paged(const char* tag, const void* q, int dtype, int rotate, float q_sc
   SL8_CHECK_ARG(aligned(q, 16) && aligned(out, 16) && aligned(k_cache, 16) && aligned(v_cache, 16),
                 "fni8 %s: q/k_cache/v_cache must be 16-byte aligned", tag);
   SL8_CHECK_ARG(aligned(tree_mask, 8) && aligned(lse, 4), "fni8 %s: tree_mask/lse must be aligned", tag);
-  const AttnPlan plan = attn_plan(T, B, Hq, Hkv, D, max_blocks_per_seq * block_size);
+  const AttnPlan plan = attn_plan(T, B, Hq, Hkv, D, max_blocks_per_seq * block_size, tree_mask != nullptr);
   SL8_CHECK_ARG(plan.grid < (1LL << 32) / A8_THREADS, "fni8 %s: shape too large", tag);
   SL8_CHECK_ARG(plan.bytes == 0 || (workspace && workspace_bytes >= plan.bytes && aligned(workspace, 16)),
                 "fni8 %s: workspace needs %zu bytes", tag, plan.bytes);
@@ -1175,7 +1212,7 @@ int attn_paged(const char* tag, const void* q, int dtype, int rotate, float q_sc
   p.Hq = (int)Hq; p.Hkv = (int)Hkv; p.G = (int)(Hq / Hkv);
   p.q_mul = q_scale_mul;
   p.rotate = rotate != 0;
-  p.tree = static_cast<const uint2*>(tree_mask);
+  p.tree = static_cast<const uint64_t*>(tree_mask);
   p.words = tree_mask ? (int)words : 0;
   p.lse = lse;
   p.window = window_left < 0 ? -1 : (int)(window_left < (1 << 30) ? window_left : (1 << 30));
@@ -1185,7 +1222,7 @@ int attn_paged(const char* tag, const void* q, int dtype, int rotate, float q_sc
   if (num_blocks == 0) p.s.maxb = 0;  // nothing to read: no key is there
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const unsigned grid = (unsigned)(plan.grid > 0 ? plan.grid : 1);
-  with_shape(D, plan.rows, [&](auto sh) {
+  with_shape(D, plan.rows, tree_mask != nullptr, [&](auto sh) {
     using S = decltype(sh);
     if (plan.slots) {
       p.pairs = static_cast<int4*>(workspace);
@@ -1195,8 +1232,10 @@ int attn_paged(const char* tag, const void* q, int dtype, int rotate, float q_sc
     }
     auto go = [&](auto dt) {
       constexpr int DT = decltype(dt)::value;
-      if (tree_mask) S::template kernel<DT, true>()<<<grid, S::THREADS, 0, st>>>(p);
-      else S::template kernel<DT, false>()<<<grid, S::THREADS, 0, st>>>(p);
+      if constexpr (!S::NW || S::RT == 1) {
+        if (tree_mask) S::template kernel<DT, true>()<<<grid, S::THREADS, 0, st>>>(p);
+      }
+      if (!tree_mask) S::template kernel<DT, false>()<<<grid, S::THREADS, 0, st>>>(p);
       if (plan.slots)
         attn_block8_join_kernel<DT, S::D, S::ROWS>
             <<<dim3((unsigned)plan.pairs, S::ROWS / JOIN_ROWS), 64 * JOIN_ROWS, 0, st>>>(p);

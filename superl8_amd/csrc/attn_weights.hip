@@ -33,8 +33,7 @@ struct WeightArgs {
   float2* rows;   // [Hkv][T * G]: scale * q_mul, lse * log2 e
 };
 
-// The rows as codes, KV head by KV head. The rotation is made in 64 bits: a quotient next to a half takes
-// the code that the definition gives it.
+// The rows as codes, KV head by KV head.
 template <int DT, int D>
 __global__ void __launch_bounds__(AW_THREADS) weights_rows_kernel(const WeightArgs p) {
   constexpr int LPR = row_lanes(D), RPB = AW_THREADS / LPR;
@@ -45,43 +44,11 @@ __global__ void __launch_bounds__(AW_THREADS) weights_rows_kernel(const WeightAr
   const int h = (int)(row - t * p.Hq), kvh = h / p.G;
   float f[8];
   VecIO<DT>::unpack(reinterpret_cast<const uint4*>(p.q + row * D)[lane], f);
-  double x[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = f[e];
-  if (p.rotate) {
-#pragma unroll
-    for (int s = 1; s < 8; s <<= 1)
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (!(e & s)) {
-          const double a = x[e], b = x[e | s];
-          x[e] = a + b;
-          x[e | s] = a - b;
-        }
-#pragma unroll
-    for (int s = 1; s < LPR; s <<= 1)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const double o = __shfl_xor(x[e], s, 64);
-        x[e] = lane & s ? o - x[e] : x[e] + o;
-      }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] *= 1.0 / __builtin_sqrt((double)D);
-  }
-  double top = 0.;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) top = fmax(top, fabs(x[e]));
-  const float amax = lane_group_max<LPR>((float)top);  // (rounding keeps the order)
-  const float s = amax * (1.0f / 127.0f), safe = s == 0.f ? 1.f : s;
-  uint32_t c[2] = {0, 0};
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float r = fminf(fmaxf(rintf((float)(x[e] / (double)safe)), -127.f), 127.f);
-    c[e / 4] |= (uint32_t)(uint8_t)(int8_t)r << (8 * (e % 4));
-  }
+  float safe;
+  const uint2 c = row_codes_wide<D>(f, lane, p.rotate, safe);
   if (i >= n) return;
   const int64_t to = ((int64_t)kvh * p.s.T + t) * p.G + h - kvh * p.G;
-  reinterpret_cast<uint2*>(p.codes + to * D)[lane] = make_uint2(c[0], c[1]);
+  reinterpret_cast<uint2*>(p.codes + to * D)[lane] = c;
   if (lane == 0) {
     const float l = p.lse[row];
     // (a row that sees nothing: no weights)

@@ -225,6 +225,50 @@ __device__ __forceinline__ void hadamard_row(float* f, int lane) {
   for (int e = 0; e < 8; ++e) f[e] *= rs;
 }
 
+// Eight codes of a 16-bit row of D values held as hadamard_row has it, rotated (with `rotate`) in 64 bits, with
+// the row's scale: a quotient next to a half takes the code that the exact value has but for the quotient's one
+// rounding, where sums in 32 bits give the neighbouring code now and then.
+template <int D>
+__device__ __forceinline__ uint2 row_codes_wide(const float* f, int lane, bool rotate, float& safe) {
+  constexpr int LPR = row_lanes(D);
+  double x[8], top = 0.;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = f[e];
+  if (rotate) {
+#pragma unroll
+    for (int s = 1; s < 8; s <<= 1)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (!(e & s)) {
+          const double a = x[e], b = x[e | s];
+          x[e] = a + b;
+          x[e | s] = a - b;
+        }
+#pragma unroll
+    for (int s = 1; s < LPR; s <<= 1)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const double o = __shfl_xor(x[e], s, 64);
+        x[e] = lane & s ? o - x[e] : x[e] + o;
+      }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= 1.0 / __builtin_sqrt((double)D);
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) top = fmax(top, fabs(x[e]));
+  const float amax = lane_group_max<LPR>((float)top);  // (rounding keeps the order)
+  const float s = amax * (1.0f / 127.0f);
+  safe = s == 0.f ? 1.f : s;
+  const double inv = 1.0 / (double)safe;  // (the product is within 2^-52 of the quotient, its rounding to fp32 the same but for 2^-27)
+  uint32_t c[2] = {0, 0};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float r = fminf(fmaxf(rintf((float)(x[e] * inv)), -127.f), 127.f);
+    c[e / 4] |= (uint32_t)(uint8_t)(int8_t)r << (8 * (e % 4));
+  }
+  return make_uint2(c[0], c[1]);
+}
+
 // The rotation of a row as its own pass would store it: rounded to its storage type.
 template <int DT, int D>
 __device__ __forceinline__ void rotate_row(float* f, int lane) {
