@@ -15,7 +15,23 @@
 namespace sl8 {
 namespace {
 
-constexpr int AW_THREADS = 256, AW_KEYS = 256;  // keys of a workgroup, 64 a wave
+constexpr int AW_THREADS = 256, AW_KEYS = 64;  // keys of an item
+
+// Inclusive sum over the wave: DPP row shifts, then the rows' last lanes.
+__device__ __forceinline__ int wave_scan(int x) {
+  auto add = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
+    x += __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
+  };
+  using std::integral_constant;
+  const integral_constant<int, 0xF> all;
+  add(integral_constant<int, 0x111>{}, all);  // row_shr:1
+  add(integral_constant<int, 0x112>{}, all);
+  add(integral_constant<int, 0x114>{}, all);
+  add(integral_constant<int, 0x118>{}, all);
+  add(integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{});  // row_bcast:15
+  add(integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{});  // row_bcast:31
+  return x;
+}
 
 struct WeightArgs {
   Block8Seqs s;
@@ -38,12 +54,11 @@ template <int DT, int D>
 __global__ void __launch_bounds__(AW_THREADS) weights_rows_kernel(const WeightArgs p) {
   constexpr int LPR = row_lanes(D), RPB = AW_THREADS / LPR;
   const int lane = threadIdx.x % LPR;
-  const int64_t n = p.s.T * p.Hq, i = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR;
-  const int64_t row = min(i, n - 1);  // (whole waves: rows past the last repeat it)
-  const int64_t t = row / p.Hq;
-  const int h = (int)(row - t * p.Hq), kvh = h / p.G;
+  const uint32_t n = (uint32_t)p.s.T * p.Hq, i = blockIdx.x * RPB + threadIdx.x / LPR;  // below 2^30
+  const uint32_t row = min(i, n - 1);  // (whole waves: rows past the last repeat it)
+  const uint32_t t = row / (uint32_t)p.Hq, h = row - t * p.Hq, kvh = h / (uint32_t)p.G;
   float f[8];
-  VecIO<DT>::unpack(reinterpret_cast<const uint4*>(p.q + row * D)[lane], f);
+  VecIO<DT>::unpack(reinterpret_cast<const uint4*>(p.q + (int64_t)row * D)[lane], f);
   float safe;
   const uint2 c = row_codes_wide<D>(f, lane, p.rotate, safe);
   if (i >= n) return;
@@ -56,114 +71,175 @@ __global__ void __launch_bounds__(AW_THREADS) weights_rows_kernel(const WeightAr
   }
 }
 
-template <int D>
-__global__ void __launch_bounds__(AW_THREADS) weights_kernel(const WeightArgs p) {
-  constexpr int KS = D / 64, KG = 4;
+// Loads of what is the same for a whole wave and not written here, beside the vector loads in flight (which are
+// waited for in their order).
+template <typename T>
+__device__ __forceinline__ T uniform(const T* p, int64_t i) {
+  return reinterpret_cast<const __attribute__((address_space(4))) T*>(reinterpret_cast<uint64_t>(p))[i];
+}
+
+// An item: 64 keys of a sequence and KV head, items being the tiles of all sequences in order, a KV head after the
+// other.
+struct KeyTile {
+  int b, kvh, key0, len;  // b < 0: none
+  int64_t at[AW_KEYS / 16];  // rows of the cache, by groups of 16 keys; those without a block read the first ones
+  float ks[AW_KEYS / 16], off[AW_KEYS / 16];  // and have off -inf
+  int64_t row0;
+  int n, pos0;
+};
+// lens: of sequence `lane` of the first 64
+__device__ __forceinline__ KeyTile key_tile(const WeightArgs& p, int lane, int lens, int id) {
+  KeyTile k;
+  k.b = -1;
+  const int unit = id / p.Hkv, cap = p.s.maxb * p.s.bs;
+  k.kvh = id - unit * p.Hkv;
+  int before = 0;
+  for (int b0 = 0; b0 < p.s.B; b0 += 64) {
+    if (b0) lens = b0 + lane < p.s.B ? p.s.lens[b0 + lane] : 0;
+    const int mine = (min(max(lens, 0), cap) + AW_KEYS - 1) / AW_KEYS, sum = before + wave_scan(mine);
+    const uint64_t past = __builtin_amdgcn_ballot_w64(sum > unit);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      k.b = b0 + at;
+      k.key0 = (unit - __builtin_amdgcn_readlane(sum - mine, at)) * AW_KEYS;
+      const int ctx = __builtin_amdgcn_readlane(lens, at);
+      k.len = min(ctx, cap);
+      // (no branches between the loads, which wait for each other only as they must)
+      const int64_t c0 = p.s.cu ? uniform(p.s.cu, k.b) : k.b, c1 = p.s.cu ? uniform(p.s.cu, k.b + 1) : k.b + 1;
+      int blk[AW_KEYS / 16], off[AW_KEYS / 16];
+#pragma unroll
+      for (int g = 0; g < AW_KEYS / 16; ++g) {
+        const int key = k.key0 + 16 * g, j = key / p.s.bs;
+        off[g] = key - j * p.s.bs;
+        blk[g] = uniform(p.s.table, (int64_t)k.b * p.s.maxb + min(j, p.s.maxb - 1));
+      }
+      const int64_t r0 = min(max(c0, (int64_t)0), p.s.T), r1 = min(max(c1, (int64_t)0), p.s.T);
+      k.row0 = r0;
+      k.n = (int)max(r1 - r0, (int64_t)0);
+      k.pos0 = (int)min(max((int64_t)ctx - k.n, (int64_t)-(1 << 28)), (int64_t)1 << 30);
+#pragma unroll
+      for (int g = 0; g < AW_KEYS / 16; ++g) {
+        const bool in = k.key0 + 16 * g < k.len && blk[g] >= 0 && blk[g] < p.s.num_blocks;
+        const int64_t bh = in ? (int64_t)blk[g] * p.Hkv + k.kvh : 0;
+        k.at[g] = in ? bh * p.s.bs + off[g] : 0;
+        k.ks[g] = uniform(p.ks, bh);
+        k.off[g] = in ? 0.f : -INFINITY;
+      }
+      break;
+    }
+    before = __builtin_amdgcn_readlane(sum, 63);
+  }
+  return k;
+}
+
+// 64 keys an item. WAVES 1: each wave for itself, its keys' loads being what counts; else the waves of a
+// workgroup share the rows and their sums meet in LDS. Keys are A operands in registers (v_mfma_i32_16x16x64_i8),
+// 16 rows at a time the B operands; lane (g4, col) then has keys 16 g + 4 g4 + i for row col.
+template <int D, int WAVES>
+__global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) weights_kernel(const WeightArgs p) {
+  constexpr int KS = D / 64, KG = AW_KEYS / 16;
+  __shared__ float sum_s[WAVES == 1 ? 1 : WAVES][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g4 = lane >> 4;
-  const int cap = p.s.maxb * p.s.bs;
-  for (int64_t id = blockIdx.x;; id += gridDim.x) {
-    // the sequence and tile of item id: tiles of all sequences in order, KV heads next to each other
-    const int64_t unit = id / p.Hkv;
-    const int kvh = (int)(id - unit * p.Hkv);
-    int b = -1, tile = 0;
-    int64_t before = 0;
-    for (int b0 = 0; b0 < p.s.B && b < 0; b0 += 64) {
-      const int len = b0 + lane < p.s.B ? min(max(p.s.lens[b0 + lane], 0), cap) : 0;
-      int64_t sum = (len + AW_KEYS - 1) / AW_KEYS;
-      const int mine = (int)sum;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int64_t x = __shfl_up(sum, o, 64);
-        if (lane >= o) sum += x;
-      }
-      const uint64_t past = __builtin_amdgcn_ballot_w64(before + sum > unit);
-      if (past) {
-        const int at = __builtin_ctzll(past);
-        b = b0 + at;
-        tile = (int)(unit - (before + __shfl(sum, at, 64) - __shfl(mine, at, 64)));
-      }
-      before += __shfl(sum, 63, 64);
-    }
-    b = __builtin_amdgcn_readfirstlane(b);
-    tile = __builtin_amdgcn_readfirstlane(tile);
-    if (b < 0) return;
-    const int len = min(max(p.s.lens[b], 0), cap);
-    const int64_t row0 = p.s.row(b);
-    const int n = max(0, (int)(p.s.row(b + 1) - row0));
-    const int64_t pos64 = max((int64_t)p.s.lens[b] - n, (int64_t)-(1 << 28));
-    const int pos0 = (int)min(pos64, (int64_t)1 << 30);
-    const int key0 = tile * AW_KEYS + wave * 64;
-    if (key0 >= len) continue;
-    // the wave's keys: group g, key col of it
+  const int first = WAVES == 1 ? blockIdx.x * 4 + wave : blockIdx.x, step = WAVES == 1 ? gridDim.x * 4 : gridDim.x;
+  const int lens = lane < p.s.B ? p.s.lens[lane] : 0;
+  int id = first;
+  for (KeyTile it = key_tile(p, lane, lens, id), next; it.b >= 0; it = next) {
+    const int key0 = it.key0, len = it.len, n = it.n, pos0 = it.pos0;
     v4i ka[KG][KS];
-    float ks[KG];
 #pragma unroll
     for (int g = 0; g < KG; ++g) {
-      const int key = key0 + 16 * g;
-      const int j = key / p.s.bs;
-      const int blk = key < len ? p.s.block(b, j) : -1;
-      ks[g] = 0.f;
+      const int8_t* from = p.k + (it.at[g] + col) * D + 16 * g4;
 #pragma unroll
-      for (int s = 0; s < KS; ++s) ka[g][s] = v4i{0, 0, 0, 0};
-      if (blk >= 0) {
-        const int64_t bh = (int64_t)blk * p.Hkv + kvh;
-        ks[g] = p.ks[bh];
-        const int8_t* at = p.k + (bh * p.s.bs + key - j * p.s.bs + col) * D + 16 * g4;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) ka[g][s] = *reinterpret_cast<const v4i*>(at + 64 * s);
-      } else {
-        ks[g] = -1.f;  // no keys
-      }
+      for (int s = 0; s < KS; ++s) ka[g][s] = *reinterpret_cast<const v4i*>(from + 64 * s);
     }
-    // the rows that see any of them: (token, head of the group) in order
+    const int key = key0 + 16 * (col >> 2) + 4 * g4 + (col & 3);  // the one that this lane writes
+    float* w = p.w + it.b * p.wb + it.kvh * p.wh;
+    const float was = w[min(key, len - 1)];
+    id += step;
+    next = key_tile(p, lane, lens, id);
+    // the rows that see any of the keys: (token, head of the group) in order
     const int64_t t0 = max(0, key0 - pos0);
-    const int64_t t1 = p.window < 0 ? n : min((int64_t)n, (int64_t)key0 + 63 + p.window - pos0);
+    const int64_t t1 = p.window < 0 ? n : min((int64_t)n, (int64_t)key0 + AW_KEYS - 1 + p.window - pos0);
     const int r0 = (int)min(t0, (int64_t)n) * p.G, r1 = (int)max(t1, (int64_t)0) * p.G;
-    const int8_t* codes = p.codes + ((int64_t)kvh * p.s.T + row0) * p.G * D;
-    const float2* rows = p.rows + ((int64_t)kvh * p.s.T + row0) * p.G;
+    const int8_t* codes = p.codes + ((int64_t)it.kvh * p.s.T + it.row0) * p.G * D;
+    const float2* rows = p.rows + ((int64_t)it.kvh * p.s.T + it.row0) * p.G;
     float acc[KG][4] = {};
-    for (int r = r0; r < r1; r += 16) {
+    const int rw = r0 + (WAVES == 1 ? 0 : 16 * wave);
+    v4i qb[KS], qn[KS];
+    float2 y, yn;
+    auto load = [&](int r, v4i (&q)[KS], float2& s) __attribute__((always_inline)) {
       const int row = min(r + col, r1 - 1);
-      v4i qb[KS];
 #pragma unroll
-      for (int s = 0; s < KS; ++s) qb[s] = *reinterpret_cast<const v4i*>(codes + (int64_t)row * D + 64 * s + 16 * g4);
-      const float2 y = rows[row];
-      const int pos = pos0 + row / p.G;
-      const int lim = r + col < r1 ? pos + 1 : 0;
-      const int low = p.window >= 0 ? pos - p.window + 1 : 0;
+      for (int i = 0; i < KS; ++i) q[i] = *reinterpret_cast<const v4i*>(codes + (int64_t)row * D + 64 * i + 16 * g4);
+      s = rows[row];
+    };
+    if (rw < r1) load(rw, qb, y);
+    for (int r = rw; r < r1; r += 16 * WAVES) {
+      load(r + 16 * WAVES, qn, yn);  // (past the last: as the last)
+      v4i sc[KG];
 #pragma unroll
       for (int g = 0; g < KG; ++g) {
-        v4i sc = {0, 0, 0, 0};
+        sc[g] = v4i{0, 0, 0, 0};
 #pragma unroll
-        for (int s = 0; s < KS; ++s) sc = __builtin_amdgcn_mfma_i32_16x16x64_i8(ka[g][s], qb[s], sc, 0, 0, 0);
-        const float a = y.x * ks[g];
+        for (int s = 0; s < KS; ++s) sc[g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(ka[g][s], qb[s], sc[g], 0, 0, 0);
+      }
+      float e[KG][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = key0 + 16 * g + 4 * g4 + i;
-          const float e = __builtin_amdgcn_exp2f(fmaf((float)sc[i], a, -y.y));
-          acc[g][i] += key < lim && key >= low && ks[g] >= 0.f ? e : 0.f;
-        }
+      for (int g = 0; g < KG; ++g) {
+        const float a = y.x * it.ks[g], c = it.off[g] - y.y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[g][i] = __builtin_amdgcn_exp2f(fmaf((float)sc[g][i], a, c));
+      }
+      // all rows see all keys, or each its own
+      const int p0 = pos0 + r / p.G, p1 = pos0 + (r + 15) / p.G;
+      if (!(r + 16 <= r1 && key0 + AW_KEYS - 1 <= p0 && (p.window < 0 || key0 > p1 - p.window))) {
+        const int pos = pos0 + (r + col) / p.G, lim = r + col < r1 ? pos + 1 : 0;
+        const int low = p.window >= 0 ? pos - p.window + 1 : 0;
+#pragma unroll
+        for (int g = 0; g < KG; ++g)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int k = key0 + 16 * g + 4 * g4 + i;
+            if (k >= lim || k < low) e[g][i] = 0.f;
+          }
+      }
+#pragma unroll
+      for (int g = 0; g < KG; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[g][i] += e[g][i];
+#pragma unroll
+      for (int s = 0; s < KS; ++s) qb[s] = qn[s];
+      y = yn;
+    }
+    // over the 16 rows of a lane group; lane (g4, col) keeps key 16 (col / 4) + 4 g4 + col % 4
+    float sum = 0.f;
+#pragma unroll
+    for (int g = 0; g < KG; ++g)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float v = acc[g][i];
+        auto add = [&](auto ctrl) __attribute__((always_inline)) {
+          v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, 0xF, 0xF, false));
+        };
+        using std::integral_constant;
+        add(integral_constant<int, 0xB1>{});   // quad_perm 1,0,3,2
+        add(integral_constant<int, 0x4E>{});   // quad_perm 2,3,0,1
+        add(integral_constant<int, 0x141>{});  // row_half_mirror
+        add(integral_constant<int, 0x140>{});  // row_mirror
+        if (col == 4 * g + i) sum = v;
+      }
+    if constexpr (WAVES > 1) {
+      sum_s[wave][lane] = sum;
+      __syncthreads();
+      sum = 0.f;
+      if (wave == 0) {
+#pragma unroll
+        for (int x = 0; x < WAVES; ++x) sum += sum_s[x][lane];
       }
     }
-#pragma unroll
-    for (int g = 0; g < KG; ++g)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) acc[g][i] += __shfl_xor(acc[g][i], o, 64);
-    // lane (g4, col) writes key 16 (col / 4) + 4 g4 + col % 4
-    float mine = 0.f;
-#pragma unroll
-    for (int g = 0; g < KG; ++g)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (col == 4 * g + i) mine = acc[g][i];
-    const int key = key0 + 16 * (col >> 2) + 4 * g4 + (col & 3);
-    if (key < len) {
-      float* w = p.w + b * p.wb + kvh * p.wh + key;
-      *w = (key < pos0 ? *w * p.decay : 0.f) + mine;
-    }
+    if (key < len && (WAVES == 1 || wave == 0)) w[key] = key < pos0 ? fmaf(was, p.decay, sum) : sum;
+    if constexpr (WAVES > 1) __syncthreads();  // (the next item's sums go to the same place)
   }
 }
 
@@ -200,7 +276,8 @@ extern "C" int sl8_attn_weights_block8(const void* q, int dtype, int rotate, flo
   SL8_CHECK_ARG(Hq > 0 && Hq % Hkv == 0, "fni8 %s: H_q must be divisible by H_kv (GQA)", tag);
   SL8_CHECK_ARG(T * Hq < (1LL << 30), "fni8 %s: shape too large", tag);
   if (B == 0 || max_blocks_per_seq == 0) return SL8_OK;
-  SL8_CHECK_ARG(context_lens && block_table && weights && (num_blocks == 0 || (k_cache && k_scale)) &&
+  SL8_CHECK_ARG(num_blocks > 0, "fni8 %s: the cache has no blocks", tag);
+  SL8_CHECK_ARG(context_lens && block_table && weights && k_cache && k_scale &&
                     (T == 0 || (q && lse)),
                 "fni8 %s: null pointer", tag);
   SL8_CHECK_ARG(aligned(q, 16) && aligned(k_cache, 16), "fni8 %s: q/k_cache must be 16-byte aligned", tag);
@@ -219,7 +296,8 @@ extern "C" int sl8_attn_weights_block8(const void* q, int dtype, int rotate, flo
   p.rows = reinterpret_cast<float2*>(p.codes + T * Hq * D);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t most = B * Hkv * ((max_blocks_per_seq * block_size + AW_KEYS - 1) / AW_KEYS);
-  const unsigned grid = (unsigned)std::min<int64_t>(most, (int64_t)cu_count() * 8);
+  SL8_CHECK_ARG(most < (1LL << 30), "fni8 %s: shape too large", tag);
+  const int64_t mean = T * p.G / B;  // of a sequence and KV head on average
   auto by_d = [&](auto d) {
     constexpr int DD = decltype(d)::value;
     constexpr int RPB = AW_THREADS / row_lanes(DD);
@@ -228,7 +306,14 @@ extern "C" int sl8_attn_weights_block8(const void* q, int dtype, int rotate, flo
       if (dtype == SL8_DTYPE_F16) weights_rows_kernel<SL8_DTYPE_F16, DD><<<pre, AW_THREADS, 0, st>>>(p);
       else weights_rows_kernel<SL8_DTYPE_BF16, DD><<<pre, AW_THREADS, 0, st>>>(p);
     }
-    weights_kernel<DD><<<grid, AW_THREADS, 0, st>>>(p);
+    auto go = [&](auto waves, int64_t items, int64_t per_cu) {
+      constexpr int WAVES = decltype(waves)::value;
+      weights_kernel<DD, WAVES><<<(unsigned)std::min((most + items - 1) / items, cu_count() * per_cu),
+                                  WAVES == 1 ? 256 : 64 * WAVES, 0, st>>>(p);
+    };
+    if (mean <= 32) go(std::integral_constant<int, 1>{}, 4, 8);
+    else if (mean <= 512) go(std::integral_constant<int, 4>{}, 1, 8);
+    else go(std::integral_constant<int, 16>{}, 1, 2);
   };
   if (D == 64) by_d(std::integral_constant<int, 64>{});
   else if (D == 128) by_d(std::integral_constant<int, 128>{});

@@ -244,13 +244,30 @@ __device__ __forceinline__ uint2 row_codes_wide(const float* f, int lane, bool r
           x[e] = a + b;
           x[e | s] = a - b;
         }
+    // (lane partners as in hadamard_row, both halves of a number)
+    auto both = [](double v, auto move) __attribute__((always_inline)) {
+      const uint64_t u = __builtin_bit_cast(uint64_t, v);
+      return __builtin_bit_cast(double, (uint64_t)move((uint32_t)(u >> 32)) << 32 | move((uint32_t)u));
+    };
+    auto dpp = [](uint32_t v, auto ctrl) __attribute__((always_inline)) {
+      return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, 0xF, 0xF, false);
+    };
+    auto stage = [&](int bit, auto move) __attribute__((always_inline)) {
+      const double sgn = (lane & bit) ? -1. : 1.;
 #pragma unroll
-    for (int s = 1; s < LPR; s <<= 1)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const double o = __shfl_xor(x[e], s, 64);
-        x[e] = lane & s ? o - x[e] : x[e] + o;
-      }
+      for (int e = 0; e < 8; ++e) x[e] = fma(x[e], sgn, both(x[e], move));
+    };
+    using std::integral_constant;
+    stage(1, [&](uint32_t v) { return dpp(v, integral_constant<int, 0xB1>{}); });
+    stage(2, [&](uint32_t v) { return dpp(v, integral_constant<int, 0x4E>{}); });
+    if constexpr (LPR >= 8)
+      stage(4, [&](uint32_t v) { return dpp(dpp(v, integral_constant<int, 0x141>{}), integral_constant<int, 0x1B>{}); });
+    if constexpr (LPR >= 16) stage(8, [&](uint32_t v) { return dpp(v, integral_constant<int, 0x128>{}); });
+    if constexpr (LPR >= 32)
+      stage(16, [&](uint32_t v) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return (uint32_t)((lane & 16) ? r[0] : r[1]);
+      });
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] *= 1.0 / __builtin_sqrt((double)D);
   }
