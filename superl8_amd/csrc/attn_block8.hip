@@ -110,22 +110,6 @@ __device__ __forceinline__ int splits_of(const AttnArgs& p, int tiles, float ove
   return tiles <= p.whole ? 1 : max(1, (int)ceilf((float)tiles * over_l));
 }
 
-// Inclusive sum over the wave: DPP row shifts, then the rows' last lanes.
-__device__ __forceinline__ int wave_scan(int x) {
-  auto add = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
-    x += __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
-  };
-  using std::integral_constant;
-  const integral_constant<int, 0xF> all;
-  add(integral_constant<int, 0x111>{}, all);  // row_shr:1
-  add(integral_constant<int, 0x112>{}, all);
-  add(integral_constant<int, 0x114>{}, all);
-  add(integral_constant<int, 0x118>{}, all);
-  add(integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{});  // row_bcast:15
-  add(integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{});  // row_bcast:31
-  return x;
-}
-
 template <int ROWS, bool TREE>
 __device__ __forceinline__ Item find_item(const AttnArgs& p, int lane, int id) {
   if (!p.slots && !p.s.cu) {  // one row a sequence, whole: nothing to look for

@@ -10,6 +10,7 @@
 #include <algorithm>
 
 #include "block8.hpp"
+#include "rowquant.hpp"
 
 namespace sl8 {
 namespace {
@@ -37,13 +38,35 @@ __device__ __forceinline__ uint32_t order_of(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// A workgroup for each sequence and KV head: the least weight that stays by its bytes, from the highest
-// (how many share the bytes found so far and have which next one), then the kept in order.
+__device__ __forceinline__ float weight_of(uint32_t u) { return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u); }
+
+// What the waves of a workgroup add up, in their order: (sum of the waves before, of all).
+__device__ __forceinline__ int2 over_waves(int mine, int wave, int* sums) {
+  if ((threadIdx.x & 63) == 63) sums[wave] = mine;
+  __syncthreads();
+  int2 r = make_int2(0, 0);
+#pragma unroll
+  for (int x = 0; x < EV_WAVES; ++x) {
+    if (x < wave) r.x += sums[x];
+    r.y += sums[x];
+  }
+  return r;
+}
+
+// A workgroup for each sequence and KV head. The least weight that stays is found by counting: 2048 bins over the
+// range that the weights take (by their bits as whole numbers: a bin's count rarely meets another's atomics there,
+// as the highest byte's would), then over the bin that holds it, three times at most. Which stay then follows in
+// order from the counts of each 64. VPT weights a thread are kept in registers; 0: longer contexts are read again
+// for each count.
+template <int VPT>
 __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictArgs p) {
-  __shared__ int hist[256];
-  __shared__ int wave_s[2][EV_WAVES][2];
+  constexpr int BINS = 2048, ROWS = VPT ? VPT : 1;
+  __shared__ int hist[BINS];
+  __shared__ int sums_a[EV_WAVES], sums_b[EV_WAVES];
+  __shared__ uint32_t ends_s[2][EV_WAVES];
   __shared__ int found_s[2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ int wave_s[ROWS][EV_WAVES], eq_s[ROWS][EV_WAVES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int b = blockIdx.x / p.Hkv, h = blockIdx.x - b * p.Hkv;
   const int len = p.len(b), m = min(len, p.budget);
   float* w = p.w + b * p.wb + h * p.wh;
@@ -54,67 +77,141 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictArg
     for (int i = tid; i < m; i += EV_THREADS) kept[i] = i;
     return;
   }
-  const int first = p.sinks, last = len - p.recent;  // between them the weights decide (sinks + recent <= budget < len)
+  // between the first and the last ones the weights decide (sinks + recent <= budget < len)
+  const int first = p.sinks, last = len - p.recent;
+  uint32_t u[ROWS];
+  if constexpr (VPT > 0) {
+    float x[ROWS];
+#pragma unroll
+    for (int c = 0; c < VPT; ++c) x[c] = w[min(c * EV_THREADS + tid, len - 1)];
+#pragma unroll
+    for (int c = 0; c < VPT; ++c) u[c] = order_of(x[c]);
+  }
+  auto each = [&](auto f) __attribute__((always_inline)) {  // f(weight) of those between
+    if constexpr (VPT > 0) {
+#pragma unroll
+      for (int c = 0; c < VPT; ++c) {
+        const int i = c * EV_THREADS + tid;
+        if (i >= first && i < last) f(u[c]);
+      }
+    } else {
+      for (int i = first + tid; i < last; i += EV_THREADS) f(order_of(w[i]));
+    }
+  };
   int want = m - p.sinks - p.recent;
   uint32_t least = 0xFFFFFFFFu;
   int equal = 0;  // how many of the least stay
   if (want > 0) {
-    uint32_t prefix = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
+    uint32_t lo = 0xFFFFFFFFu, hi = 0;
+    each([&](uint32_t x) {
+      lo = min(lo, x);
+      hi = max(hi, x);
+    });
+    lo = ~lane_group_reduce<64>(~lo, [](uint32_t a, uint32_t c) { return a > c ? a : c; });
+    hi = lane_group_reduce<64>(hi, [](uint32_t a, uint32_t c) { return a > c ? a : c; });
+    if (lane == 0) {
+      ends_s[0][wave] = lo;
+      ends_s[1][wave] = hi;
+    }
+    for (int i = tid; i < BINS; i += EV_THREADS) hist[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < EV_WAVES; ++x) {
+      lo = min(lo, ends_s[0][x]);
+      hi = max(hi, ends_s[1][x]);
+    }
+    uint32_t base = lo, span = hi - lo;  // the one looked for is in [base, base + span]
+    for (;;) {
+      const int bits = 32 - __clz((int)span);  // (of 0: 0)
+      const int shift = max(bits - 11, 0);
+      each([&](uint32_t x) {
+        const uint32_t d = x - base;
+        if (x >= base && d <= span) atomicAdd(&hist[d >> shift], 1);
+      });
       __syncthreads();
-      for (int i = first + tid; i < last; i += EV_THREADS) {
-        const uint32_t u = order_of(w[i]);
-        if (shift == 24 || u >> (shift + 8) == prefix) atomicAdd(&hist[u >> shift & 255], 1);
+      // bins from the highest, two a thread
+      const int b0 = BINS - 1 - 2 * tid;
+      const int h0 = hist[b0], h1 = hist[b0 - 1];
+      const int upto = wave_scan(h0 + h1);
+      const int2 before = over_waves(upto, wave, sums_a);
+      const int above = before.x + upto - h0 - h1;
+      if (above < want && want <= above + h0 + h1) {  // (one thread)
+        const bool second = want > above + h0;
+        found_s[0] = second ? b0 - 1 : b0;
+        found_s[1] = want - above - (second ? h0 : 0);
       }
+      hist[b0] = 0;
+      hist[b0 - 1] = 0;
       __syncthreads();
-      if (tid == 0) {
-        int x = 255, left = want;
-        while (x > 0 && hist[x] < left) left -= hist[x--];
-        found_s[0] = x;
-        found_s[1] = left;
-      }
-      __syncthreads();
-      prefix = prefix << 8 | (uint32_t)found_s[0];
+      base += (uint32_t)found_s[0] << shift;
       want = found_s[1];
+      if (shift == 0) break;
+      span = min(span, (1u << shift) - 1);
       __syncthreads();
     }
-    least = prefix;
+    least = base;
     equal = want;
   }
-  // in order: how many equal ones and how many kept ones stand in front
+  if constexpr (VPT > 0) {
+    // counts of each 64, then where their kept ones go
+    uint64_t eqs[ROWS], sures[ROWS];
+#pragma unroll
+    for (int c = 0; c < VPT; ++c) {
+      const int i = c * EV_THREADS + tid;
+      const bool between = i >= first && i < last;
+      eqs[c] = __ballot(between && equal > 0 && u[c] == least);
+      sures[c] = __ballot(i < len && (!between || u[c] > least));
+      if (lane == 0) {
+        eq_s[c][wave] = __popcll(eqs[c]);
+        wave_s[c][wave] = __popcll(sures[c]);
+      }
+    }
+    __syncthreads();
+    const int e = tid < VPT * EV_WAVES ? (&eq_s[0][0])[tid] : 0, s = tid < VPT * EV_WAVES ? (&wave_s[0][0])[tid] : 0;
+    const int es = wave_scan(e);
+    const int eq0 = over_waves(es, wave, sums_a).x + es - e;  // equal ones in front
+    const int k = s + min(eq0 + e, equal) - min(eq0, equal);
+    const int ks = wave_scan(k);
+    const int at0 = over_waves(ks, wave, sums_b).x + ks - k;
+    if (tid < VPT * EV_WAVES) {
+      (&eq_s[0][0])[tid] = eq0;
+      (&wave_s[0][0])[tid] = at0;
+    }
+    __syncthreads();
+    const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+    for (int c = 0; c < VPT; ++c) {
+      const int i = c * EV_THREADS + tid;
+      const int base_eq = eq_s[c][wave], rank = base_eq + __popcll(eqs[c] & below);
+      const bool sure = sures[c] >> lane & 1, eq = eqs[c] >> lane & 1;
+      if (sure || (eq && rank < equal)) {
+        const int at = wave_s[c][wave] + __popcll(sures[c] & below) + min(rank, equal) - min(base_eq, equal);
+        kept[at] = i;
+        w[at] = weight_of(u[c]);
+      }
+    }
+    return;
+  }
+  // in order, a weight a thread: how many equal ones and how many kept ones stand in front
   int equals = 0, keeps = 0;
-  for (int base = 0, turn = 0; base < len; base += EV_THREADS, turn ^= 1) {
-    const int i = base + tid;
+  for (int from = 0; from < len; from += EV_THREADS) {
+    const int i = from + tid;
     const float x = i < len ? w[i] : 0.f;
     const bool between = i >= first && i < last;
-    const uint32_t u = order_of(x);
-    const bool eq = between && want > 0 && u == least && i < len;
-    const bool sure = i < len && (!between || (u > least));
-    const uint64_t eqs = __ballot(eq), sures = __ballot(sure);
-    if (lane == 0) {
-      wave_s[turn][wave][0] = __popcll(eqs);
-      wave_s[turn][wave][1] = __popcll(sures);
-    }
-    __syncthreads();  // (all of this turn's weights are read)
-    const uint64_t below = (1ull << lane) - 1;
-    int e0 = equals, s0 = 0, e_all = 0, s_all = 0;
-    for (int x2 = 0; x2 < EV_WAVES; ++x2) {
-      const int e = wave_s[turn][x2][0], s = wave_s[turn][x2][1];
-      if (x2 < wave) { e0 += e; s0 += s; }
-      e_all += e;
-      s_all += s;
-    }
-    const int rank = e0 + __popcll(eqs & below);              // equal ones in front
-    const int taken = min(rank, equal) - min(equals, equal);  // of them, those of this turn that stay
-    const bool keep = sure || (eq && rank < equal);
-    if (keep) {
-      const int at = keeps + s0 + __popcll(sures & below) + taken;
+    const uint32_t v = order_of(x);
+    const bool eq = between && equal > 0 && v == least;
+    const bool sure = i < len && (!between || v > least);
+    const uint64_t eqs = __ballot(eq), sures = __ballot(sure), below = (1ull << lane) - 1;
+    const int2 e = over_waves(__popcll(eqs), wave, sums_a);  // (behind its barrier all of these weights are read)
+    const int2 s = over_waves(__popcll(sures), wave, sums_b);
+    const int rank = equals + e.x + __popcll(eqs & below);
+    if (sure || (eq && rank < equal)) {
+      const int at = keeps + s.x + __popcll(sures & below) + min(rank, equal) - min(equals, equal);
       kept[at] = i;
       w[at] = x;
     }
-    keeps += s_all + min(equals + e_all, equal) - min(equals, equal);
-    equals += e_all;
+    keeps += s.y + min(equals + e.y, equal) - min(equals, equal);
+    equals += e.y;
   }
 }
 
@@ -222,7 +319,14 @@ extern "C" int sl8_kv_evict_block8(int8_t* k_cache, float* k_scale, int8_t* v_ca
   p.lens = new_lens;
   p.Hkv = (int)Hkv; p.budget = (int)budget; p.sinks = (int)sinks; p.recent = (int)recent;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  evict_select_kernel<<<(unsigned)(B * Hkv), EV_THREADS, 0, st>>>(p);
+  auto select = [&](auto vpt) {
+    evict_select_kernel<decltype(vpt)::value><<<(unsigned)(B * Hkv), EV_THREADS, 0, st>>>(p);
+  };
+  const int64_t cap = max_blocks_per_seq * block_size;
+  if (cap <= 4 * EV_THREADS) select(std::integral_constant<int, 4>{});
+  else if (cap <= 16 * EV_THREADS) select(std::integral_constant<int, 16>{});
+  else if (cap <= 32 * EV_THREADS) select(std::integral_constant<int, 32>{});
+  else select(std::integral_constant<int, 0>{});
   const unsigned grid = (unsigned)(B * Hkv * blocks);
   if (grid && num_blocks) {
     if (D == 64) evict_move_kernel<64><<<grid, 256, 0, st>>>(p, (int)blocks);

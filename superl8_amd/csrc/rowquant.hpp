@@ -50,6 +50,22 @@ __device__ __forceinline__ int lane_group_sum(int v) {
   return (int)lane_group_reduce<LPR>((uint32_t)v, [](uint32_t a, uint32_t b) { return a + b; });
 }
 
+// Inclusive sum over the wave: DPP row shifts, then the rows' last lanes.
+__device__ __forceinline__ int wave_scan(int x) {
+  auto add = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
+    x += __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
+  };
+  using std::integral_constant;
+  const integral_constant<int, 0xF> all;
+  add(integral_constant<int, 0x111>{}, all);  // row_shr:1
+  add(integral_constant<int, 0x112>{}, all);
+  add(integral_constant<int, 0x114>{}, all);
+  add(integral_constant<int, 0x118>{}, all);
+  add(integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{});  // row_bcast:15
+  add(integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{});  // row_bcast:31
+  return x;
+}
+
 template <int DT> struct Elem;
 template <> struct Elem<SL8_DTYPE_F16> {
   using T = uint16_t;
