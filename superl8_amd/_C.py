@@ -1119,6 +1119,8 @@ def linear_w8a8(x, w, w_scale, bias=None, out_dtype=torch.float16):
     _contig(x, w, w_scale)
     out = x.new_empty((M, N), dtype=out_dtype)
     if M and N:
+        if x.data_ptr() % 16:
+            x = x.clone()
         if w.data_ptr() % (4 if K % 16 else 16):
             w = w.clone()
         bias = None if bias is None else bias.contiguous()
