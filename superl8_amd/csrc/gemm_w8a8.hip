@@ -494,7 +494,6 @@ W8Plan w8_plan(int64_t M, int64_t N, int64_t K) {
   double best = 1e30;
   if (M <= W8_STREAM_ROWS && K <= W8_STREAM_K) best = 3. + (double)N * K / 4e6;
   for (const Shape& s : shapes) {
-    if (s.bm < 128 && M > s.bm) continue;
     const int64_t nt_m = (M + s.bm - 1) / s.bm, nt_n = (N + s.bn - 1) / s.bn, n = nt_m * nt_n;
     const int64_t slots = (int64_t)cus * s.per_cu, rest = n % slots, most = n - rest;
     for (int S = 1; S <= 8; ++S) {
@@ -502,7 +501,7 @@ W8Plan w8_plan(int64_t M, int64_t N, int64_t K) {
       const double more = std::ceil((double)rest * S / cus) - 1.;
       const double part = rest ? std::ceil(stages / S) * (s.one_us + (s.full_us - s.one_us) * more / std::max(1, s.per_cu - 1)) : 0.;
       double us = std::max((double)(most / slots) * stages * s.full_us + part, (double)N * K / 4.8e6) + 3.;
-      if (S > 1) us += 3. + (double)rest * S * s.bm * s.bn * 4 / 4e6;
+      if (S > 1) us += 3.5 + (double)rest * S * s.bm * s.bn * 5 / 4e6;
       if (us >= best) continue;
       best = us;
       a.tile = s.bm;
