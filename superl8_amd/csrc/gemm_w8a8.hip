@@ -226,8 +226,7 @@ template <int BM_, int BN_, int MW_, int NW_, int RING_> struct W8Tile {
   static constexpr int BM = BM_, BN = BN_, MW = MW_, NW = NW_, BK = W8_BK, THREADS = 64 * MW_ * NW_;
   static constexpr int MB = BM / MW / 32, NB = BN / NW / 32;  // blocks of a wave
   static constexpr int CPR = BK / 16;                           // 16-byte chunks of a row and stage
-  static constexpr int COPIES = (BM + BN) * CPR / THREADS;      // of 16 bytes a thread and stage
-  static_assert((BM + BN) * CPR % THREADS == 0 && BN * CPR % THREADS == 0, "whole copies");
+  static_assert(BM * CPR % THREADS == 0 && BN * CPR % THREADS == 0, "whole copies");
   __device__ __forceinline__ static int swizzle(int row) { return (row >> 1) & 7; }
 };
 
@@ -311,10 +310,12 @@ __device__ __forceinline__ void w8_store(const W8Args& p, const v16i (&acc)[S::N
   }
 }
 
-// DMA: 16-byte aligned weight rows, copied straight to LDS; else through registers.
-template <int ODT, typename S, bool DMA>
+// WIDE: weight rows are 16-byte aligned and copied 16 bytes a thread; else 4 (which is what K % 4 == 0 allows).
+template <int ODT, typename S, bool WIDE>
 __global__ void __launch_bounds__(S::THREADS, 2) w8_tile_kernel(const W8Args p) {
-  constexpr int ROWB = S::BK, STAGE = (S::BM + S::BN) * ROWB, WCOP = S::BN * S::CPR / S::THREADS;
+  constexpr int ROWB = S::BK, STAGE = (S::BM + S::BN) * ROWB, PER = WIDE ? 1 : 4;
+  constexpr int WCOP = PER * S::BN * S::CPR / S::THREADS, XCOP = S::BM * S::CPR / S::THREADS;  // copies a thread
+  static_assert((S::RING - 2) * (WCOP + XCOP) < 64, "what the wait can count");
   constexpr int OS = ODT == SL8_DTYPE_F32 ? 4 : 2;
   // one LDS object per stage: a copy into one never aliases reads of another
   __shared__ __attribute__((aligned(16))) int8_t s0[STAGE], s1[STAGE], s2[S::RING > 2 ? STAGE : 16],
@@ -335,36 +336,35 @@ __global__ void __launch_bounds__(S::THREADS, 2) w8_tile_kernel(const W8Args p) 
   const int nk = p.Kp / S::BK, k0 = split * nk / parts, k1 = (split + 1) * nk / parts;
   const int mw = wave % S::MW, nw = wave / S::MW;
 
-  // chunk P of a stage: row P / 4 (weights, then x), place P % 4 of it
+  // copy i of a thread: 16 (weights, not WIDE: 4) bytes of row P / pieces, place P % pieces of it; weight rows past
+  // the last read as zeros, rows of codes as the last
+  constexpr int WPR = PER * S::CPR;
   const brsrc_t rw = make_rsrc(p.w + (int64_t)n0 * p.K, (uint32_t)(min(S::BN, p.N - n0) * p.K));
-    int off[S::COPIES], ch[S::COPIES];
+  int woff[WCOP], wch[WCOP], xoff[XCOP];
 #pragma unroll
-  for (int i = 0; i < S::COPIES; ++i) {
-    const int P = i * S::THREADS + tid, row = P / S::CPR;
-    ch[i] = 16 * ((P % S::CPR) ^ S::swizzle(row));
-    if (i < WCOP) off[i] = min(row, p.N - n0 - 1) * p.K;
-    else off[i] = min(row - S::BN, p.M16 - m0 - 1) * 128;
+  for (int i = 0; i < WCOP; ++i) {
+    const int P = i * S::THREADS + tid, row = P / WPR, piece = P % WPR;
+    wch[i] = 16 * ((piece / PER) ^ S::swizzle(row));
+    woff[i] = row * p.K + 4 * (piece % PER);
   }
-  v4i held[DMA ? 1 : S::COPIES];
+#pragma unroll
+  for (int i = 0; i < XCOP; ++i) {
+    const int P = i * S::THREADS + tid, row = P / S::CPR;  // (as many weight rows in front: a multiple of 16)
+    xoff[i] = min(row, p.M16 - m0 - 1) * 128 + 16 * ((P % S::CPR) ^ S::swizzle(row));
+  }
   auto load = [&](int kt, int8_t* to) __attribute__((always_inline)) {
     kt = min(kt, k1 - 1);
     const int k = kt * S::BK;
-    const int8_t* x = p.codes + ((int64_t)kt * p.M16 + m0) * 128;
-    const brsrc_t rx = make_rsrc(x, (uint32_t)(S::BM * 128));
+    const brsrc_t rx = make_rsrc(p.codes + ((int64_t)kt * p.M16 + m0) * 128, (uint32_t)(S::BM * 128));
 #pragma unroll
-    for (int i = 0; i < S::COPIES; ++i) {
-      const bool is_w = i < WCOP;
-      const int at = is_w ? off[i] + min(k + ch[i], p.K - 16) : off[i] + ch[i];
-      if constexpr (DMA) buf16_to_lds(is_w ? rw : rx, to + (i * S::THREADS + wave * 64) * 16, at, 0);
-      else if (is_w) held[i] = *reinterpret_cast<const v4i_u*>(p.w + (int64_t)n0 * p.K + at);
-      else held[i] = *reinterpret_cast<const v4i*>(x + at);
+    for (int i = 0; i < WCOP; ++i) {
+      const int at = woff[i] + min(k + wch[i], p.K - 16);
+      if constexpr (WIDE) buf16_to_lds(rw, to + (i * S::THREADS + wave * 64) * 16, at, 0);
+      else buf4_to_lds(rw, to + (i * S::THREADS + wave * 64) * 4, at, 0);
     }
-  };
-  auto keep = [&](int8_t* to) __attribute__((always_inline)) {
-    if constexpr (!DMA) {
 #pragma unroll
-      for (int i = 0; i < S::COPIES; ++i) *reinterpret_cast<v4i*>(to + (i * S::THREADS + tid) * 16) = held[i];
-    }
+    for (int i = 0; i < XCOP; ++i)
+      buf16_to_lds(rx, to + S::BN * S::BK + (i * S::THREADS + wave * 64) * 16, xoff[i], 0);
   };
 
   v16i acc[S::NB][S::MB];
@@ -392,22 +392,18 @@ __global__ void __launch_bounds__(S::THREADS, 2) w8_tile_kernel(const W8Args p) 
   };
   // the other stage's place is free behind the barrier
   auto step = [&](int kt, const int8_t* st, int8_t* to) __attribute__((always_inline)) {
-    w8_barrier<DMA ? (S::RING - 2) * S::COPIES : 63>();
+    w8_barrier<(S::RING - 2) * (WCOP + XCOP)>();
     load(kt + S::RING - 1, to);
     __builtin_amdgcn_sched_barrier(0);
     compute(st);
-    keep(to);
   };
   int kt = k0;
   load(k0, s0);
-  keep(s0);
   if constexpr (S::RING > 2) {
     load(k0 + 1, s1);
-    keep(s1);
   }
   if constexpr (S::RING > 3) {
     load(k0 + 2, s2);
-    keep(s2);
   }
 #pragma unroll 1
   for (; kt + S::RING <= k1; kt += S::RING) {
