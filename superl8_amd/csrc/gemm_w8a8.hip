@@ -62,6 +62,17 @@ __device__ __forceinline__ void w8_chunk(const W8Args& p, int64_t row, int c, fl
   }
 }
 
+// The same of a 16-bit row as it is; chunks past the row's last are zeros.
+__device__ __forceinline__ void w8_raw(const W8Args& p, int row, int c, uint2* r) {
+  const bool part = 16 * c + 16 > p.K;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int e = (part ? p.K - 16 : 16 * c) + 4 * j;
+    const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.x) + (int64_t)row * p.K + e);
+    r[j] = 16 * c < p.K && e >= 16 * c ? v : make_uint2(0, 0);
+  }
+}
+
 // A workgroup a row, 16 elements a thread and pass; NV passes stay in registers between the maximum and the
 // codes (0: rows too long for that are read twice).
 template <int DT, int NV>
@@ -147,8 +158,7 @@ constexpr int W8_WAVES = 8;
 
 // The sums y of channels n .. n + 3 of a row to its outputs.
 template <int ODT>
-__device__ __forceinline__ void w8_out4(const W8Args& p, v4i y, int m, int n) {
-  const float xs = p.xs[m];
+__device__ __forceinline__ void w8_out4(const W8Args& p, v4i y, float xs, int m, int n) {
   float z[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) z[e] = (float)y[e] * xs * p.ws[min(n + e, p.N - 1)] + w8_bias(p, min(n + e, p.N - 1));
@@ -162,9 +172,13 @@ __device__ __forceinline__ void w8_out4(const W8Args& p, v4i y, int m, int n) {
   }
 }
 
-template <int ODT, int U>
+// XDT 0, 1: x itself, a few fp16 / bf16 rows, is quantised in every workgroup (a launch less; each reads all of x).
+constexpr int W8_CODES = -1, W8_FUSED_ROWS = 4;
+template <int ODT, int U, int XDT>
 __global__ void __launch_bounds__(64 * W8_WAVES) w8_stream_kernel(const W8Args p) {
+  constexpr bool FUSED = XDT != W8_CODES;
   __shared__ v4i sum_s[2][W8_WAVES][64];
+  __shared__ float amax_s[FUSED ? W8_WAVES : 1][16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g4 = lane >> 4;
   const int groups = (p.N + 15) / 16, units = p.Kp / 128;
@@ -178,16 +192,62 @@ __global__ void __launch_bounds__(64 * W8_WAVES) w8_stream_kernel(const W8Args p
         a[u][i] = *reinterpret_cast<const v4i_u*>(w + min(128 * min(u0 + u, units - 1) + 64 * i + 16 * g4, p.K - 16));
   };
   v4i a0[U][2], a1[U][2], b[U][2];
-  load(blockIdx.x, a0);
+  float xs = 0.f;  // FUSED: the scale of row lane / 4, which this lane puts out
+  // (rows past the last as the last; units past the wave's own are zeros)
+  if constexpr (FUSED) {
+    uint2 raw[U][2][4];
 #pragma unroll
-  for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      // (rows past the last as the last; units past the wave's own are zeros)
-      const int8_t* x = p.codes + ((int64_t)min(u0 + u, units - 1) * p.M16 + min(col, p.M - 1)) * 128;
-      const v4i c = *reinterpret_cast<const v4i*>(x + 64 * i + 16 * g4);
-      b[u][i] = u0 + u < u1 ? c : v4i{0, 0, 0, 0};
+      for (int i = 0; i < 2; ++i) w8_raw(p, min(col, p.M - 1), u0 + u < u1 ? 8 * (u0 + u) + 4 * i + g4 : p.Kp / 16, raw[u][i]);
+    load(blockIdx.x, a0);
+    auto values = [&](const uint2 (&r)[4], float* f) __attribute__((always_inline)) {
+      VecIO<XDT>::unpack(make_uint4(r[0].x, r[0].y, r[1].x, r[1].y), f);
+      VecIO<XDT>::unpack(make_uint4(r[2].x, r[2].y, r[3].x, r[3].y), f + 8);
+    };
+    float amax = 0.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float f[16];
+        values(raw[u][i], f);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) amax = fmaxf(amax, fabsf(f[e]));
+      }
+    amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
+    amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
+    if (g4 == 0) amax_s[wave][col] = amax;
+    w8_barrier<63>();
+    float mine = 0.f;
+#pragma unroll
+    for (int x = 0; x < W8_WAVES; ++x) {
+      amax = fmaxf(amax, amax_s[x][col]);
+      mine = fmaxf(mine, amax_s[x][lane >> 2]);
     }
+    auto scale = [](float a) { return a * (1.0f / 127.0f) == 0.f ? 1.f : a * (1.0f / 127.0f); };
+    const float safe = scale(amax);
+    xs = scale(mine);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float f[16];
+        values(raw[u][i], f);
+        const uint2 lo = row_codes8<XDT>(f, safe), hi = row_codes8<XDT>(f + 8, safe);
+        b[u][i] = v4i{(int)lo.x, (int)lo.y, (int)hi.x, (int)hi.y};
+      }
+  } else {
+    load(blockIdx.x, a0);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int8_t* x = p.codes + ((int64_t)min(u0 + u, units - 1) * p.M16 + min(col, p.M - 1)) * 128;
+        const v4i c = *reinterpret_cast<const v4i*>(x + 64 * i + 16 * g4);
+        b[u][i] = u0 + u < u1 ? c : v4i{0, 0, 0, 0};
+      }
+  }
   int turn = 0;
   auto group = [&](int64_t g, const v4i (&a)[U][2], v4i (&next)[U][2]) __attribute__((always_inline)) {
     load(g + gridDim.x, next);
@@ -204,7 +264,7 @@ __global__ void __launch_bounds__(64 * W8_WAVES) w8_stream_kernel(const W8Args p
       v4i y = {0, 0, 0, 0};
 #pragma unroll
       for (int x = 0; x < W8_WAVES; ++x) y += sum_s[turn & 1][x][16 * (lane & 3) + m];
-      if (m < p.M && n < p.N) w8_out4<ODT>(p, y, m, n);
+      if (m < p.M && n < p.N) w8_out4<ODT>(p, y, FUSED ? xs : p.xs[m], m, n);
     }
     ++turn;
   };
@@ -460,7 +520,7 @@ __global__ void __launch_bounds__(256) w8_join_kernel(const W8Args p) {
   v4i y = {0, 0, 0, 0};
 #pragma unroll 4
   for (int s = 0; s < p.splits; ++s) y += from[(int64_t)s * TILE];
-  w8_out4<ODT>(p, y, m, n);
+  w8_out4<ODT>(p, y, p.xs[m], m, n);
 }
 
 using Tile256 = W8Tile<256, 256, 2, 4, 2>;
@@ -559,16 +619,25 @@ extern "C" int sl8_linear_w8a8(const void* x, int x_dtype, const int8_t* w, cons
     else if (p.Kp <= 16384) w8_quant_kernel<DT, 4><<<(unsigned)M, 256, 0, st>>>(p);
     else w8_quant_kernel<DT, 0><<<(unsigned)M, 256, 0, st>>>(p);
   };
-  if (x_dtype == SL8_DTYPE_F16) quant(integral_constant<int, SL8_DTYPE_F16>{});
+  // up to W8_FUSED_ROWS 16-bit rows that are streamed: no launch for their codes
+  const bool fused = plan.tile == 0 && M <= W8_FUSED_ROWS && x_dtype != SL8_DTYPE_F32;
+  if (fused) {
+  } else if (x_dtype == SL8_DTYPE_F16) quant(integral_constant<int, SL8_DTYPE_F16>{});
   else if (x_dtype == SL8_DTYPE_BF16) quant(integral_constant<int, SL8_DTYPE_BF16>{});
   else quant(integral_constant<int, SL8_DTYPE_F32>{});
   auto go = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     if (plan.tile == 0) {
       const unsigned wgs = (unsigned)std::min<int64_t>((N + 15) / 16, 2 * cu_count());
-      if (K <= 2048) w8_stream_kernel<DT, 2><<<wgs, 64 * W8_WAVES, 0, st>>>(p);
-      else if (K <= 4096) w8_stream_kernel<DT, 4><<<wgs, 64 * W8_WAVES, 0, st>>>(p);
-      else w8_stream_kernel<DT, 5><<<wgs, 64 * W8_WAVES, 0, st>>>(p);
+      auto stream = [&](auto xdt) {
+        constexpr int XDT = decltype(xdt)::value;
+        if (K <= 2048) w8_stream_kernel<DT, 2, XDT><<<wgs, 64 * W8_WAVES, 0, st>>>(p);
+        else if (K <= 4096) w8_stream_kernel<DT, 4, XDT><<<wgs, 64 * W8_WAVES, 0, st>>>(p);
+        else w8_stream_kernel<DT, 5, XDT><<<wgs, 64 * W8_WAVES, 0, st>>>(p);
+      };
+      if (!fused) stream(integral_constant<int, W8_CODES>{});
+      else if (x_dtype == SL8_DTYPE_F16) stream(integral_constant<int, SL8_DTYPE_F16>{});
+      else stream(integral_constant<int, SL8_DTYPE_BF16>{});
       return;
     }
     auto tile = [&](auto shape) {

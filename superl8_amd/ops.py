@@ -571,6 +571,8 @@ def linear_w8a8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *,
     quantize_i8_rowwise; w int8 [N,K] with w_scale fp32 [N] (a scale per output channel: the
     per_row_i8 QTensor) -> [..., N] of out_dtype. K a multiple of 4, at least 16. The integer sums are
     exact; scales and bias are applied in fp32 and the result is rounded once."""
+    if x.dim() == 2:
+        return _C.linear_w8a8(x.contiguous(), w.contiguous(), w_scale.contiguous(), bias, out_dtype)
     *lead, K = x.shape
     y = _C.linear_w8a8(x.reshape(-1, K).contiguous(), w.contiguous(), w_scale.contiguous(), bias, out_dtype)
     return y.reshape(*lead, y.shape[-1])
