@@ -266,7 +266,7 @@ __device__ __forceinline__ uint2 row_codes_wide(const float* f, int lane, bool r
       return __builtin_bit_cast(double, (uint64_t)move((uint32_t)(u >> 32)) << 32 | move((uint32_t)u));
     };
     auto dpp = [](uint32_t v, auto ctrl) __attribute__((always_inline)) {
-      return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, 0xF, 0xF, false);
+      return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, 0xF, 0xF, true);
     };
     auto stage = [&](int bit, auto move) __attribute__((always_inline)) {
       const double sgn = (lane & bit) ? -1. : 1.;
