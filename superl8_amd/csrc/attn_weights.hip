@@ -106,7 +106,8 @@ __device__ __forceinline__ KeyTile key_tile(const WeightArgs& p, int lane, int l
         const bool in = k.key0 + 16 * g < k.len && blk[g] >= 0 && blk[g] < p.s.num_blocks;
         const int64_t bh = in ? (int64_t)blk[g] * p.Hkv + k.kvh : 0;
         k.at[g] = in ? bh * p.s.bs + off[g] : 0;
-        k.ks[g] = uniform(p.ks, bh);
+        const float ks = uniform(p.ks, bh);
+        k.ks[g] = in ? ks : 0.f;  // (the first block's may be anything)
         k.off[g] = in ? 0.f : -INFINITY;
       }
       break;
@@ -130,6 +131,15 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) weights_kernel(
   int id = first;
   for (KeyTile it = key_tile(p, lane, lens, id), next; it.b >= 0; it = next) {
     const int key0 = it.key0, len = it.len, n = it.n, pos0 = it.pos0;
+    // the rows that see any of the keys: (token, head of the group) in order
+    const int64_t t0 = max(0, key0 - pos0);
+    const int64_t t1 = p.window < 0 ? n : min((int64_t)n, (int64_t)key0 + AW_KEYS - 1 + p.window - pos0);
+    const int r0 = (int)min(t0, (int64_t)n) * p.G, r1 = (int)max(t1, (int64_t)0) * p.G;
+    if (r0 >= r1 && p.decay == 1.f && min(key0 + AW_KEYS, len) <= pos0) {  // (behind every window) nothing changes
+      id += step;
+      next = key_tile(p, lane, lens, id);
+      continue;
+    }
     v4i ka[KG][KS];
 #pragma unroll
     for (int g = 0; g < KG; ++g) {
@@ -142,10 +152,6 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) weights_kernel(
     const float was = w[min(key, len - 1)];
     id += step;
     next = key_tile(p, lane, lens, id);
-    // the rows that see any of the keys: (token, head of the group) in order
-    const int64_t t0 = max(0, key0 - pos0);
-    const int64_t t1 = p.window < 0 ? n : min((int64_t)n, (int64_t)key0 + AW_KEYS - 1 + p.window - pos0);
-    const int r0 = (int)min(t0, (int64_t)n) * p.G, r1 = (int)max(t1, (int64_t)0) * p.G;
     const int8_t* codes = p.codes + ((int64_t)it.kvh * p.s.T + it.row0) * p.G * D;
     const float2* rows = p.rows + ((int64_t)it.kvh * p.s.T + it.row0) * p.G;
     float acc[KG][4] = {};

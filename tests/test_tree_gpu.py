@@ -258,6 +258,31 @@ def test_weights_of_long_contexts(new):
     weights_and_check(c, q, [new], [new + 3000], window=2000 if new == 33 else -1)
 
 
+@pytest.mark.parametrize("new", [1, 40, 700])
+def test_unread_places(new):
+    """Scales and codes that no key has do not matter: NaN in blocks of no sequence (the pool's first among them), old
+    codes behind a context's end, table entries past it."""
+    total = [new + 37, new + 5]
+    c = Cache(total, 2, 64, 16)
+    used = {x for b, n in enumerate(total) for x in c.table[b, :-(-n // 16)].tolist()}
+    if 0 in used:  # the pool's first block is nobody's
+        spare = next(i for i in range(c.k.shape[0]) if i not in used)
+        c.table[c.table == 0] = spare
+        for t in (c.k, c.ks, c.v, c.vs):
+            t[spare] = t[0]
+        used = (used - {0}) | {spare}
+    free = [i for i in range(c.k.shape[0]) if i not in used]
+    c.ks[free] = math.nan
+    c.table[1, -1] = 0
+    q = coded_queries(2 * new, 4, 64, F16, False)
+    w = weights_and_check(c, q, [new, new], total, window=20 if new == 40 else -1)
+    assert bool(torch.isfinite(w).all())
+    c.table[0, 0] = -1  # keys that are not there
+    lse = torch.zeros(2 * new, 4, device=DEV)
+    sl8.attn_weights_block8(q, lse, c.k, c.ks, c.table, i32(total), w, cu_lens=offsets([new, new]), rotate=False)
+    assert bool(torch.isfinite(w).all())
+
+
 def test_weights_sum_to_the_rows():
     """With the lse of the attention itself each row's weights add up to 1."""
     new, total = [70, 1], [400, 90]
