@@ -37,6 +37,10 @@ constexpr float A8_NONE = -1e30f; // reference of nothing
 constexpr float A8_LAG = 15.f;    // log2 of the largest weight (fp16 holds it)
 constexpr float A8_HEAD = 8.f;    // log2 of a maximum's weight when it becomes the reference
 
+// What a kernel is built for: causal rows, the same with their lse, trees (with theirs, where it is wanted).
+// (Kernels of their own: what an lse needs beside the outputs would cost the causal ones registers.)
+enum { A8_CAUSAL, A8_LSE, A8_TREE };
+
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef int v2i __attribute__((ext_vector_type(2)));
@@ -267,6 +271,7 @@ __device__ __forceinline__ void note_pair(const AttnArgs& p, const Span& w, cons
 }
 
 // Rows in front of the first sequence and behind the last are zeros (the logarithm of their sums -inf).
+template <bool LSE>
 __device__ __forceinline__ void zero_rest(const AttnArgs& p, const Item& it, int D) {
   const int64_t n = it.begin + p.s.T - it.end;
   if (n == 0) return;
@@ -275,7 +280,7 @@ __device__ __forceinline__ void zero_rest(const AttnArgs& p, const Item& it, int
   for (int64_t i = blockIdx.x; i < n; i += gridDim.x) {
     const int64_t t = i < it.begin ? i : it.end + i - it.begin;
     for (int64_t c = threadIdx.x; c < chunks; c += blockDim.x) o[t * chunks + c] = make_uint4(0, 0, 0, 0);
-    if (p.lse)
+    if (LSE && p.lse)
       for (int64_t h = threadIdx.x; h < p.Hq; h += blockDim.x) p.lse[t * p.Hq + h] = -INFINITY;
   }
 }
@@ -570,8 +575,9 @@ template <int D> __device__ __forceinline__ int v_swizzle(int key) {
   else return (key & 7) | ((key >> 4) & 1) << 3;
 }
 
-template <int DT, int D, int RT, bool TREE>
+template <int DT, int D, int RT, int MODE>
 __global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const AttnArgs p) {
+  constexpr bool TREE = MODE == A8_TREE, LSE = MODE != A8_CAUSAL;
   constexpr int ROWS = 16 * RT, KT = stream_keys<D>(), NG = KT / 16, KS = D / 64, DTL = D / 16;
   constexpr int TPM = 64 / NG;  // tiles whose groups the lanes hold
   constexpr int PARTS = DT == SL8_DTYPE_F16 && RT == 1 ? 2 : 1;  // of a weight
@@ -586,7 +592,7 @@ __global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const
   const int col = lane & 15, g4 = lane >> 4;
 
   const Item it = find_item<ROWS, TREE>(p, lane, blockIdx.x);
-  zero_rest(p, it, D);
+  zero_rest<LSE>(p, it, D);
   if (!it.live) return;
   const Span w = item_span<ROWS, TREE>(p, it);
   // places: K's lane in a group, the copies' lanes (16-byte chunk of the row that goes to the
@@ -762,7 +768,7 @@ __global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const
       const int64_t to = row_at(p, w, it.kvh, r, D) + d;
 #pragma unroll
       for (int e = 0; e < 4; ++e) st_out<DT>(p.out, to + e, a[e]);
-      if (p.lse && d == 0) p.lse[to / D] = row_lse(mm, den);
+      if (LSE && p.lse && d == 0) p.lse[to / D] = row_lse(mm, den);
     } else {
       const int64_t row = (int64_t)blockIdx.x * ROWS + r;
       *reinterpret_cast<v4f*>(p.part + row * D + d) = a;
@@ -802,8 +808,9 @@ template <int D> __device__ __forceinline__ int v16_swizzle(int key) {  // 32-by
   else return key & 7;
 }
 
-template <int DT, int D, int RT, int NW, bool TREE>
+template <int DT, int D, int RT, int NW, int MODE>
 __global__ void __launch_bounds__(64 * NW, 2) attn_block8_tile_kernel(const AttnArgs p) {
+  constexpr bool TREE = MODE == A8_TREE, LSE = MODE != A8_CAUSAL;
   constexpr int THREADS = 64 * NW, ROWS = 16 * RT * NW, KT = tile_keys<D>(), NG = KT / 16;
   constexpr int KS = D / 64, DTL = D / 16, CPR = D / 16;
   constexpr int TPM = 64 / NG;
@@ -812,6 +819,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_block8_tile_kernel(const Attn
   __shared__ __attribute__((aligned(16))) int8_t k0_s[KT * D], k1_s[KT * D];
   __shared__ __attribute__((aligned(16))) uint16_t v0_s[KT * D], v1_s[KT * D];
   __shared__ float qs_s[ROWS];
+  __shared__ float2 ml_s[LSE ? ROWS : 1];
   __shared__ uint64_t tree_s[TREE ? ROWS * TREE_ROW : 1];
   static_assert(ROWS <= 4 * KT, "the rows' codes fit where V will be");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -820,7 +828,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_block8_tile_kernel(const Attn
   typedef short v8s __attribute__((ext_vector_type(8)));
 
   const Item it = find_item<ROWS, TREE>(p, lane, blockIdx.x);
-  zero_rest(p, it, D);
+  zero_rest<LSE>(p, it, D);
   if (!it.live) return;
   const Span w = item_span<ROWS, TREE>(p, it);
 
@@ -963,12 +971,13 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_block8_tile_kernel(const Attn
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
     const int r = 16 * (RT * wave + rt) + col;
+    if constexpr (LSE) {
+      if (g4 == 0) ml_s[r] = make_float2(st.m[rt], l);
+    }
     if (r >= w.cnt) continue;
     if (it.splits == 1) {
       const float inv = l > 0.f ? 1.f / l : 0.f;
-      const int64_t at = row_at(p, w, it.kvh, r, D);
-      if (p.lse && g4 == 0) p.lse[at / D] = row_lse(st.m[rt], l);
-      uint16_t* to = static_cast<uint16_t*>(p.out) + at + 4 * g4;
+      uint16_t* to = static_cast<uint16_t*>(p.out) + row_at(p, w, it.kvh, r, D) + 4 * g4;
 #pragma unroll
       for (int d = 0; d < DTL; ++d) {
         const v4f a = st.o[rt][d] * inv;
@@ -980,6 +989,12 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_block8_tile_kernel(const Attn
       for (int d = 0; d < DTL; ++d) *reinterpret_cast<v4f*>(p.part + row * D + 16 * d + 4 * g4) = st.o[rt][d];
       if (g4 == 0) p.ml[row] = make_float2(st.m[rt], l);
     }
+  }
+  if constexpr (LSE) {
+    // (through LDS: the logarithm next to the outputs takes up to 20 registers more, at D = 64 a wave a SIMD, and
+    // spills 150 at D = 256: prompts with a window, D = 64, 58 for 45 us)
+    __syncthreads();
+    if (p.lse && it.splits == 1 && tid < w.cnt) p.lse[row_at(p, w, it.kvh, tid, 1)] = row_lse(ml_s[tid].x, ml_s[tid].y);
   }
   if (p.slots && it.split == 0 && tid == 0) note_pair(p, w, it);
 }
@@ -1043,17 +1058,16 @@ __global__ void __launch_bounds__(64 * JOIN_ROWS) attn_block8_join_kernel(const 
 template <int D_, int RT_, int NW_> struct Shape {
   static constexpr int D = D_, RT = RT_, NW = NW_, ROWS = 16 * RT_ * (NW_ ? NW_ : 1);
   static constexpr int THREADS = NW_ ? 64 * NW_ : A8_THREADS;
-  template <int DT, bool TREE> static auto kernel() {
-    static_assert(!TREE || !NW_ || RT_ == 1, "trees go to tiles of 64 rows");
-    if constexpr (NW_) return attn_block8_tile_kernel<DT, D, RT, NW, TREE>;
-    else return attn_block8_stream_kernel<DT, D, RT, TREE>;
+  template <int DT, int MODE> static auto kernel() {
+    if constexpr (NW_) return attn_block8_tile_kernel<DT, D, RT, NW, MODE>;
+    else return attn_block8_stream_kernel<DT, D, RT, MODE>;
   }
   // workgroups resident on one CU (asked once)
   static int wgs_per_cu() {
     static std::atomic<int> n{0};
     int v = n.load(std::memory_order_relaxed);
     if (v == 0) {
-      if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&v, reinterpret_cast<const void*>(kernel<0, false>()), THREADS, 0) !=
+      if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&v, reinterpret_cast<const void*>(kernel<0, A8_CAUSAL>()), THREADS, 0) !=
               hipSuccess || v < 1) {
         (void)hipGetLastError();
         return 2;  // no device: any figure (nothing is launched)
@@ -1072,9 +1086,10 @@ template <int D_, int RT_, int NW_> struct Shape {
 // rows (the drafts above) take 57 in tiles, 88 streamed as two units. 32 streamed rows at D = 128 need more
 // than the 256 registers of two waves a SIMD: 27 spill (96 to 112 bytes a lane) and come back in the loop
 // over keys; 16 rows at D = 256 spill 2, and 32 rows there, whose sums take 128, are not built.
-// Trees go to tiles of 64 rows: their rows fill 128 badly, and the masks' registers are theirs. 16 trees of 31 to 60
-// tokens (124 to 240 rows) on 1024 to 8191 keys: 107 us, 116 in tiles of 128; D = 256, 4 of 66 to 129 (8 heads to a
-// KV head) on 513 to 4096: 55, 111.
+// Trees of up to 128 rows, and all at D = 256, go to tiles of 64, which several workgroups of a CU hold: 8 trees of 14
+// to 26 tokens (32 / 8 heads, D = 128) on 500 to 4000 keys 37 us, 40 in tiles of 128; D = 256, 4 of 66 to 129 (8 heads to a
+// KV head) on 130 to 1024 36 and 45, on 513 to 4096 53 and 57. With more rows those of 128 win: 16 of 31 to 60 tokens on
+// 512 to 4096 keys 63 us, 69 in tiles of 64, on 2048 to 16384 160 and 175; D = 64, 2 of 101 to 200 on 20000 67 and 75.
 template <typename F>
 auto with_shape(int64_t D, int64_t rows, bool tree, F&& f) {
   auto by_rows = [&](auto d) {
@@ -1083,7 +1098,7 @@ auto with_shape(int64_t D, int64_t rows, bool tree, F&& f) {
     if constexpr (DD < 256) {
       if (rows <= 32) return f(Shape<DD, 2, 0>{});
     }
-    if (rows <= 64 || tree) return f(Shape<DD, 1, 4>{});
+    if (rows <= 64 || (tree && (rows <= 128 || DD == 256))) return f(Shape<DD, 1, 4>{});
     return f(Shape<DD, 2, 4>{});
   };
   if (D == 64) return by_rows(std::integral_constant<int, 64>{});
@@ -1216,10 +1231,11 @@ int attn_paged(const char* tag, const void* q, int dtype, int rotate, float q_sc
     }
     auto go = [&](auto dt) {
       constexpr int DT = decltype(dt)::value;
-      if constexpr (!S::NW || S::RT == 1) {
-        if (tree_mask) S::template kernel<DT, true>()<<<grid, S::THREADS, 0, st>>>(p);
+      if constexpr (!S::NW || S::RT == 1 || S::D < 256) {
+        if (tree_mask) S::template kernel<DT, A8_TREE>()<<<grid, S::THREADS, 0, st>>>(p);
       }
-      if (!tree_mask) S::template kernel<DT, false>()<<<grid, S::THREADS, 0, st>>>(p);
+      if (!tree_mask && lse) S::template kernel<DT, A8_LSE>()<<<grid, S::THREADS, 0, st>>>(p);
+      if (!tree_mask && !lse) S::template kernel<DT, A8_CAUSAL>()<<<grid, S::THREADS, 0, st>>>(p);
       if (plan.slots)
         attn_block8_join_kernel<DT, S::D, S::ROWS>
             <<<dim3((unsigned)plan.pairs, S::ROWS / JOIN_ROWS), 64 * JOIN_ROWS, 0, st>>>(p);
