@@ -465,9 +465,10 @@ int sl8_attn_paged_block8_tree(const void* q, int dtype, int rotate, float q_sca
  *              group's heads of e^(score_ij - lse_i),   j < context_lens[b]; others are left alone.
  * q (rows as codes; rotate, window_left, cu_lens as in sl8_attn_paged_block8, causal rows) 16-byte aligned;
  * lse fp32 [T,Hq] of the same rows, as sl8_attn_paged_block8_tree gives it (-inf: the row adds nothing).
- * Keys in blocks outside the pool get nothing added. workspace: sl8_attn_weights_block8_workspace() bytes,
- * uninitialised, 16-byte aligned. */
-size_t sl8_attn_weights_block8_workspace(int64_t T, int64_t Hq, int64_t D);
+ * Keys in blocks outside the pool get nothing added. workspace: sl8_attn_weights_block8_workspace() bytes
+ * (current device; max_context_len = max_blocks_per_seq * block_size), uninitialised, 16-byte aligned. */
+size_t sl8_attn_weights_block8_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                         int64_t max_context_len);
 int sl8_attn_weights_block8(const void* q, int dtype, int rotate, float q_scale_mul, const float* lse,
                             const int8_t* k_cache, const float* k_scale, const int32_t* cu_lens,
                             const int32_t* context_lens, const int32_t* block_table, float* weights,

@@ -1046,7 +1046,7 @@ def attn_weights_block8(q, q_mul, rotate, lse, k_cache, k_scale, block_table, co
         _fail(f"{tag}: decay must be finite, got {decay}")
     if B and maxb:
         with on_device(q):
-            ws_bytes = _lib.load().sl8_attn_weights_block8_workspace(T, Hq, D)
+            ws_bytes = _lib.load().sl8_attn_weights_block8_workspace(T, B, Hq, Hkv, D, maxb * bs)
             ws = q.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
             call("sl8_attn_weights_block8", q.data_ptr(), dtype_code(q.dtype), int(bool(rotate)),
                  float(q_mul), lse.data_ptr(), k_cache.data_ptr(), k_scale.data_ptr(), _lib.ptr(cu_lens),

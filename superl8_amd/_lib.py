@@ -83,7 +83,7 @@ SIGNATURES = {
     "sl8_attn_paged_block8": (_I, [_P, _I, _I, _F] + [_P] * 8 + [_I64] * 9 + [_P, _SZ, _P]),
     "sl8_attn_paged_block8_tree": (_I, [_P, _I, _I, _F] + [_P] * 8 + [_I64, _P, _P] + [_I64] * 9 + [_P, _SZ, _P]),
     "sl8_attn_paged_block8_tree_workspace": (_SZ, [_I64] * 6),
-    "sl8_attn_weights_block8_workspace": (_SZ, [_I64] * 3),
+    "sl8_attn_weights_block8_workspace": (_SZ, [_I64] * 6),
     "sl8_attn_weights_block8": (_I, [_P, _I, _I, _F] + [_P] * 7 + [_I64] * 2 + [_F] + [_I64] * 9 + [_P, _SZ, _P]),
     "sl8_kv_evict_block8": (_I, [_P] * 7 + [_I64] * 2 + [_P] * 3 + [_I64] * 10 + [_P]),
     "sl8_linear_w8a8_workspace": (_SZ, [_I64] * 3),

@@ -31,6 +31,9 @@ struct WeightArgs {
   bool rotate;
   int8_t* codes;  // [Hkv][T * G][D]
   float2* rows;   // [Hkv][T * G]: scale * q_mul, lse * log2 e
+  int parts;      // of an item's rows
+  int items;      // at most
+  float* part;    // [parts][items][64], parts > 1
 };
 
 // The rows as codes, KV head by KV head.
@@ -117,9 +120,28 @@ __device__ __forceinline__ KeyTile key_tile(const WeightArgs& p, int lane, int l
   return k;
 }
 
+// The rows that see any of an item's keys, (token, head of the group) in order, and whether there is nothing to do.
+struct Rows {
+  int r0, r1;
+  bool stay;  // behind every window, and no fading
+};
+__device__ __forceinline__ Rows rows_of(const WeightArgs& p, const KeyTile& it) {
+  const int64_t t0 = max(0, it.key0 - it.pos0);
+  const int64_t t1 = p.window < 0 ? it.n : min((int64_t)it.n, (int64_t)it.key0 + AW_KEYS - 1 + p.window - it.pos0);
+  const int r0 = (int)min(t0, (int64_t)it.n) * p.G, r1 = (int)max(t1, (int64_t)0) * p.G;
+  return {r0, r1, r0 >= r1 && p.decay == 1.f && min(it.key0 + AW_KEYS, it.len) <= it.pos0};
+}
+// The key that a lane puts out: lane (g4, col) key 16 (col / 4) + 4 g4 + col % 4.
+__device__ __forceinline__ int key_of(const KeyTile& it, int lane) {
+  return it.key0 + 16 * ((lane & 15) >> 2) + 4 * (lane >> 4) + (lane & 3);
+}
+__device__ __forceinline__ void put(const WeightArgs& p, const KeyTile& it, int key, float was, float sum) {
+  if (key < it.len) p.w[it.b * p.wb + it.kvh * p.wh + key] = key < it.pos0 ? fmaf(was, p.decay, sum) : sum;
+}
+
 // 64 keys an item. WAVES 1: each wave for itself, its keys' loads being what counts; else the waves of a
-// workgroup share the rows and their sums meet in LDS. Keys are A operands in registers (v_mfma_i32_16x16x64_i8),
-// 16 rows at a time the B operands; lane (g4, col) then has keys 16 g + 4 g4 + i for row col.
+// workgroup share the rows (of part blockIdx.y of them) and their sums meet in LDS. Keys are A operands in registers
+// (v_mfma_i32_16x16x64_i8), 16 rows at a time the B operands; lane (g4, col) then has keys 16 g + 4 g4 + i for row col.
 template <int D, int WAVES>
 __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) weights_kernel(const WeightArgs p) {
   constexpr int KS = D / 64, KG = AW_KEYS / 16;
@@ -128,18 +150,18 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) weights_kernel(
   const int col = lane & 15, g4 = lane >> 4;
   const int first = WAVES == 1 ? blockIdx.x * 4 + wave : blockIdx.x, step = WAVES == 1 ? gridDim.x * 4 : gridDim.x;
   const int lens = lane < p.s.B ? p.s.lens[lane] : 0;
-  int id = first;
-  for (KeyTile it = key_tile(p, lane, lens, id), next; it.b >= 0; it = next) {
-    const int key0 = it.key0, len = it.len, n = it.n, pos0 = it.pos0;
-    // the rows that see any of the keys: (token, head of the group) in order
-    const int64_t t0 = max(0, key0 - pos0);
-    const int64_t t1 = p.window < 0 ? n : min((int64_t)n, (int64_t)key0 + AW_KEYS - 1 + p.window - pos0);
-    const int r0 = (int)min(t0, (int64_t)n) * p.G, r1 = (int)max(t1, (int64_t)0) * p.G;
-    if (r0 >= r1 && p.decay == 1.f && min(key0 + AW_KEYS, len) <= pos0) {  // (behind every window) nothing changes
-      id += step;
-      next = key_tile(p, lane, lens, id);
-      continue;
+  for (int id = first;; id += step) {
+    const KeyTile it = key_tile(p, lane, lens, id);
+    if (it.b < 0) return;
+    const Rows all = rows_of(p, it);
+    if (all.stay) continue;
+    int r0 = all.r0, r1 = all.r1;
+    if (WAVES > 1 && p.parts > 1) {
+      const int per = ((r1 - r0 + 15) / 16 + p.parts - 1) / p.parts * 16;
+      r0 = min(r0 + (int)blockIdx.y * per, r1);
+      r1 = min(r0 + per, r1);
     }
+    const int key0 = it.key0, pos0 = it.pos0;
     v4i ka[KG][KS];
 #pragma unroll
     for (int g = 0; g < KG; ++g) {
@@ -147,11 +169,8 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) weights_kernel(
 #pragma unroll
       for (int s = 0; s < KS; ++s) ka[g][s] = *reinterpret_cast<const v4i*>(from + 64 * s);
     }
-    const int key = key0 + 16 * (col >> 2) + 4 * g4 + (col & 3);  // the one that this lane writes
-    float* w = p.w + it.b * p.wb + it.kvh * p.wh;
-    const float was = w[min(key, len - 1)];
-    id += step;
-    next = key_tile(p, lane, lens, id);
+    const int key = key_of(it, lane);
+    const float was = p.w[it.b * p.wb + it.kvh * p.wh + min(key, it.len - 1)];
     const int8_t* codes = p.codes + ((int64_t)it.kvh * p.s.T + it.row0) * p.G * D;
     const float2* rows = p.rows + ((int64_t)it.kvh * p.s.T + it.row0) * p.G;
     float acc[KG][4] = {};
@@ -222,27 +241,69 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) weights_kernel(
     if constexpr (WAVES > 1) {
       sum_s[wave][lane] = sum;
       __syncthreads();
-      sum = 0.f;
       if (wave == 0) {
+        sum = 0.f;
 #pragma unroll
         for (int x = 0; x < WAVES; ++x) sum += sum_s[x][lane];
+        if (p.parts > 1) p.part[((int64_t)blockIdx.y * p.items + id) * AW_KEYS + lane] = sum;
+        else put(p, it, key, was, sum);
       }
+      __syncthreads();  // (the next item's sums go to the same place)
+    } else {
+      put(p, it, key, was, sum);
     }
-    if (key < len && (WAVES == 1 || wave == 0)) w[key] = key < pos0 ? fmaf(was, p.decay, sum) : sum;
-    if constexpr (WAVES > 1) __syncthreads();  // (the next item's sums go to the same place)
   }
 }
 
-size_t weights_bytes(int64_t T, int64_t Hq, int64_t D) { return (size_t)(T * Hq) * (D + sizeof(float2)); }
+// The parts of the rows added up, in their order: a wave an item.
+__global__ void __launch_bounds__(256) weights_join_kernel(const WeightArgs p) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lens = lane < p.s.B ? p.s.lens[lane] : 0;
+  const KeyTile it = key_tile(p, lane, lens, blockIdx.x * 4 + wave);
+  if (it.b < 0 || rows_of(p, it).stay) return;
+  const int key = key_of(it, lane);
+  const float was = p.w[it.b * p.wb + it.kvh * p.wh + min(key, it.len - 1)];
+  float sum = 0.f;
+#pragma unroll 8
+  for (int s = 0; s < p.parts; ++s) sum += p.part[((int64_t)s * p.items + blockIdx.x * 4 + wave) * AW_KEYS + lane];
+  put(p, it, key, was, sum);
+}
+
+// How a call runs: rows of a sequence and KV head on average, items at most, and in how many parts the rows of an
+// item go to workgroups of their own: where items are few, and of as many rows that a part has 16 for each of its
+// waves four times. Items differ (those of a causal prompt's end are seen by few of its rows), so there are several
+// for each workgroup that is resident.
+struct WeightPlan {
+  int64_t rows, items, parts;
+  size_t rows_at, part_at, bytes;
+};
+constexpr int AW_WAVES = 4;
+WeightPlan weights_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t cap) {
+  WeightPlan a{};
+  a.rows = T * (Hq / Hkv) / B;
+  a.items = B * Hkv * ((cap + AW_KEYS - 1) / AW_KEYS);
+  a.parts = 1;
+  if (a.rows > 32 && a.items > 0) {
+    const int64_t want = (int64_t)cu_count() * 12 / a.items;
+    a.parts = std::max<int64_t>(1, std::min<int64_t>({want, a.rows / (64 * AW_WAVES), 64}));
+  }
+  a.rows_at = (size_t)(T * Hq) * D;
+  a.part_at = a.rows_at + (size_t)(T * Hq) * sizeof(float2);
+  a.bytes = a.part_at + (a.parts > 1 ? (size_t)(a.parts * a.items) * AW_KEYS * sizeof(float) : 0);
+  return a;
+}
 
 }  // namespace
 }  // namespace sl8
 
 using namespace sl8;
 
-extern "C" size_t sl8_attn_weights_block8_workspace(int64_t T, int64_t Hq, int64_t D) {
-  if (T <= 0 || Hq <= 0 || D <= 0 || T >= (1LL << 28) || Hq >= (1 << 16) || D > 256) return 0;
-  return weights_bytes(T, Hq, D);
+extern "C" size_t sl8_attn_weights_block8_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                                    int64_t max_context_len) {
+  if (T <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || T >= (1LL << 28) || B >= (1 << 24) || Hq >= (1 << 16)) return 0;
+  if ((D != 64 && D != 128 && D != 256) || Hq % Hkv || max_context_len < 0 || max_context_len >= (1LL << 30)) return 0;
+  if (B * Hkv * (max_context_len / AW_KEYS + 1) >= (1LL << 30)) return 0;
+  return weights_plan(T, B, Hq, Hkv, D, max_context_len).bytes;
 }
 
 extern "C" int sl8_attn_weights_block8(const void* q, int dtype, int rotate, float q_scale_mul, const float* lse,
@@ -271,8 +332,11 @@ extern "C" int sl8_attn_weights_block8(const void* q, int dtype, int rotate, flo
                     (T == 0 || (q && lse)),
                 "fni8 %s: null pointer", tag);
   SL8_CHECK_ARG(aligned(q, 16) && aligned(k_cache, 16), "fni8 %s: q/k_cache must be 16-byte aligned", tag);
-  SL8_CHECK_ARG(T == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= weights_bytes(T, Hq, D)),
-                "fni8 %s: workspace needs %zu bytes", tag, weights_bytes(T, Hq, D));
+  const int64_t cap = max_blocks_per_seq * block_size;
+  SL8_CHECK_ARG(B * Hkv * (cap / AW_KEYS + 1) < (1LL << 30), "fni8 %s: shape too large", tag);
+  const WeightPlan plan = weights_plan(T, B, Hq, Hkv, D, cap);
+  SL8_CHECK_ARG(T == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= plan.bytes),
+                "fni8 %s: workspace needs %zu bytes", tag, plan.bytes);
   p.q = static_cast<const uint16_t*>(q);
   p.lse = lse;
   p.k = k_cache; p.ks = k_scale;
@@ -283,11 +347,11 @@ extern "C" int sl8_attn_weights_block8(const void* q, int dtype, int rotate, flo
   p.rotate = rotate != 0;
   p.window = window_left < 0 ? -1 : (int)(window_left < (1 << 30) ? window_left : (1 << 30));
   p.codes = static_cast<int8_t*>(workspace);
-  p.rows = reinterpret_cast<float2*>(p.codes + T * Hq * D);
+  p.rows = reinterpret_cast<float2*>(p.codes + plan.rows_at);
+  p.part = reinterpret_cast<float*>(p.codes + plan.part_at);
+  p.parts = (int)plan.parts;
+  p.items = (int)plan.items;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  const int64_t most = B * Hkv * ((max_blocks_per_seq * block_size + AW_KEYS - 1) / AW_KEYS);
-  SL8_CHECK_ARG(most < (1LL << 30), "fni8 %s: shape too large", tag);
-  const int64_t mean = T * p.G / B;  // of a sequence and KV head on average
   auto by_d = [&](auto d) {
     constexpr int DD = decltype(d)::value;
     constexpr int RPB = AW_THREADS / row_lanes(DD);
@@ -296,14 +360,14 @@ extern "C" int sl8_attn_weights_block8(const void* q, int dtype, int rotate, flo
       if (dtype == SL8_DTYPE_F16) weights_rows_kernel<SL8_DTYPE_F16, DD><<<pre, AW_THREADS, 0, st>>>(p);
       else weights_rows_kernel<SL8_DTYPE_BF16, DD><<<pre, AW_THREADS, 0, st>>>(p);
     }
-    auto go = [&](auto waves, int64_t items, int64_t per_cu) {
-      constexpr int WAVES = decltype(waves)::value;
-      weights_kernel<DD, WAVES><<<(unsigned)std::min((most + items - 1) / items, cu_count() * per_cu),
-                                  WAVES == 1 ? 256 : 64 * WAVES, 0, st>>>(p);
-    };
-    if (mean <= 32) go(std::integral_constant<int, 1>{}, 4, 8);
-    else if (mean <= 512) go(std::integral_constant<int, 4>{}, 1, 8);
-    else go(std::integral_constant<int, 16>{}, 1, 2);
+    const int64_t cus = cu_count();
+    if (plan.rows <= 32) {
+      weights_kernel<DD, 1><<<(unsigned)std::min((plan.items + 3) / 4, cus * 8), 256, 0, st>>>(p);
+    } else {
+      const dim3 grid((unsigned)std::min(plan.items, cus * 12), (unsigned)plan.parts);
+      weights_kernel<DD, AW_WAVES><<<grid, 64 * AW_WAVES, 0, st>>>(p);
+      if (plan.parts > 1) weights_join_kernel<<<(unsigned)((plan.items + 3) / 4), 256, 0, st>>>(p);
+    }
   };
   if (D == 64) by_d(std::integral_constant<int, 64>{});
   else if (D == 128) by_d(std::integral_constant<int, 128>{});

@@ -66,8 +66,10 @@ def test_nothing_to_do():
 
 def test_workspaces():
     lib = _lib.load()
-    assert lib.sl8_attn_weights_block8_workspace(10, 8, 128) >= 80 * 128
-    for bad in ((0, 8, 128), (10, 0, 128), (10, 8, 0), (-1, 8, 64), (1 << 40, 8, 64)):
+    assert lib.sl8_attn_weights_block8_workspace(10, 2, 8, 4, 128, 400) >= 80 * 128
+    for bad in ((0, 2, 8, 4, 128, 400), (10, 0, 8, 4, 128, 400), (10, 2, 0, 4, 128, 400), (10, 2, 8, 0, 128, 400),
+                (10, 2, 8, 3, 128, 400), (10, 2, 8, 4, 0, 400), (-1, 2, 8, 4, 64, 400), (1 << 40, 2, 8, 4, 64, 400),
+                (10, 2, 8, 4, 64, 1 << 40), (10, 1 << 20, 8, 4, 64, 1 << 25)):
         assert lib.sl8_attn_weights_block8_workspace(*bad) == 0
     assert lib.sl8_linear_w8a8_workspace(17, 100, 100) >= 32 * 128
     for bad in ((0, 8, 64), (8, 0, 64), (8, 8, 8), (1 << 40, 8, 64), (8, 8, 1 << 20)):
