@@ -442,7 +442,8 @@ int sl8_attn_paged_block8(const void* q, int dtype, int rotate, float q_scale_mu
 
 /* The same with a tree of drafted tokens, and with the sums' logarithms. tree_mask (NULL: as above)
  * int64 [T][mask_words] (1 .. 4 words, 8-byte aligned): row i of a sequence sees the tokens in front of
- * the new ones, and new token t < 64 * mask_words where bit t % 64 of word t / 64 of its mask is set. A window
+ * the new ones, and new token t < 64 * mask_words where bit t % 64 of word t / 64 of its mask is set (bits of
+ * tokens that its sequence does not have count for nothing). A window
  * keeps the last window_left of those: the marked ones, all of them, and of the tokens in front the last
  * max(0, window_left - marked). lse (NULL: not wanted) fp32 [T,Hq]: ln of the row's sum of e^score,
  * -inf for a row that sees nothing or of no sequence. Workspace, with a mask:

@@ -334,20 +334,23 @@ __device__ __forceinline__ void quant_rows(const AttnArgs& p, const Span& w, int
   }
 }
 
-// The masks of a unit's rows in LDS (rows past the last: as the last), zeros behind the last word.
-constexpr int TREE_MAX = 4, TREE_ROW = TREE_MAX + 1;  // words of 64 bits
-template <int ROWS, int THREADS>
-__device__ __forceinline__ void load_tree(const AttnArgs& p, const Span& w, uint64_t* tree_s) {
-  for (int i = threadIdx.x; i < ROWS * TREE_ROW; i += THREADS) {
-    const int r = i / TREE_ROW, x = i % TREE_ROW;
-    tree_s[i] = x < p.words ? p.tree[(w.row0 + token_of(w, min(r, w.cnt - 1))) * p.words + x] : 0;
-  }
-}
 // Bits [a, b) of 64.
 __device__ __forceinline__ uint64_t bit_range(int a, int b) {
   a = max(a, 0);
   b = min(b, 64);
   return a < b ? ~0ull >> (64 - (b - a)) << a : 0;
+}
+
+// The masks of a unit's rows in LDS (rows past the last: as the last), zeros behind the last word and for tokens
+// that the sequence does not have: a window counts the bits.
+constexpr int TREE_MAX = 4, TREE_ROW = TREE_MAX + 1;  // words of 64 bits
+template <int ROWS, int THREADS>
+__device__ __forceinline__ void load_tree(const AttnArgs& p, const Span& w, int n, uint64_t* tree_s) {
+  for (int i = threadIdx.x; i < ROWS * TREE_ROW; i += THREADS) {
+    const int r = i / TREE_ROW, x = i % TREE_ROW;
+    const uint64_t m = x < p.words ? p.tree[(w.row0 + token_of(w, min(r, w.cnt - 1))) * p.words + x] : 0;
+    tree_s[i] = m & bit_range(0, n - 64 * x);
+  }
 }
 
 // The logarithm of a row's sum l of weights under reference m (log2).
@@ -641,7 +644,7 @@ __global__ void __launch_bounds__(A8_THREADS, 2) attn_block8_stream_kernel(const
   if (ntiles) load(cur, 0, v0_s);
 
   quant_rows<DT, D, ROWS, A8_THREADS, TREE>(p, w, it.kvh, [&](int r) { return q_s + r * D; }, qs_s);
-  if constexpr (TREE) load_tree<ROWS, A8_THREADS>(p, w, tree_s);
+  if constexpr (TREE) load_tree<ROWS, A8_THREADS>(p, w, it.n, tree_s);
   __syncthreads();
 
   v4i qb[RT][KS];
@@ -875,7 +878,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_block8_tile_kernel(const Attn
     return r < FIT ? reinterpret_cast<int8_t*>(v0_s) + r * D : reinterpret_cast<int8_t*>(v1_s) + (r - FIT) * D;
   };
   quant_rows<DT, D, ROWS, THREADS, TREE>(p, w, it.kvh, q_place, qs_s);
-  if constexpr (TREE) load_tree<ROWS, THREADS>(p, w, tree_s);
+  if constexpr (TREE) load_tree<ROWS, THREADS>(p, w, it.n, tree_s);
   __syncthreads();
   v4i qb[RT][KS];
 #pragma unroll

@@ -397,3 +397,21 @@ def test_refusals():
             sl8.tree_mask(bad)
     with pytest.raises(ValueError, match="words"):
         sl8.tree_mask(torch.zeros(2, dtype=torch.int32), words=5)
+
+
+@pytest.mark.parametrize("window", [-1, 30])
+@pytest.mark.parametrize("n", [1, 5, 64, 90])
+def test_bits_of_tokens_that_are_not_there(n, window):
+    """They count for nothing, for a window either."""
+    c = Cache([n + 200, n], 2, 128, 16)
+    q = coded_queries(2 * n, 8, 128, F16, False)
+    bits = masks([n, n], 3)
+    clean = packed(bits, 3)
+    stray = clean.clone()
+    for w in range(3):
+        there = max(0, min(64, n - 64 * w))
+        stray[:, w] |= 0 if there == 64 else -1 << there
+    args = dict(cu_lens=offsets([n, n]), rotate=False, window_left=window, return_lse=True)
+    want = sl8.attn_paged_block8(q, *c.args(), i32([n + 200, n]), tree_mask=clean, **args)
+    got = sl8.attn_paged_block8(q, *c.args(), i32([n + 200, n]), tree_mask=stray, **args)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
