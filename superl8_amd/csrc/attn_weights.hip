@@ -270,9 +270,13 @@ __global__ void __launch_bounds__(256) weights_join_kernel(const WeightArgs p) {
 }
 
 // How a call runs: rows of a sequence and KV head on average, items at most, and in how many parts the rows of an
-// item go to workgroups of their own: where items are few, and of as many rows that a part has 16 for each of its
-// waves four times. Items differ (those of a causal prompt's end are seen by few of its rows), so there are several
-// for each workgroup that is resident.
+// item go to workgroups of their own: where items are few, so that there are two for each CU, and four where new rows
+// are a good part of the context (a causal prompt's last keys are seen by few of its rows, so items differ); parts
+// large enough to pay for the join. Whole and in parts (us): 2000 rows behind 100 keys, 8 heads to a KV head, D = 256, 134
+// and 44; 4000 behind 100, 8 / 2 heads, D = 128, 134 and 52; 2048 behind 2048, 32 / 8 heads, 101 and 92 (6 parts for 2:
+// 105); 700 behind 30000, 8 / 1 heads, 60 whole, 84 in two.
+// A wave an item for up to 32 rows, else four: one row, 32 sequences 35 and 96; 16 tokens of 4 heads, D = 64, 18.8 and 20.3;
+// 300 of 4 heads, D = 128, 47 and 24.
 struct WeightPlan {
   int64_t rows, items, parts;
   size_t rows_at, part_at, bytes;
@@ -284,8 +288,9 @@ WeightPlan weights_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D
   a.items = B * Hkv * ((cap + AW_KEYS - 1) / AW_KEYS);
   a.parts = 1;
   if (a.rows > 32 && a.items > 0) {
-    const int64_t want = (int64_t)cu_count() * 12 / a.items;
-    a.parts = std::max<int64_t>(1, std::min<int64_t>({want, a.rows / (64 * AW_WAVES), 64}));
+    const bool uneven = T / B * 4 >= cap;
+    const int64_t want = (int64_t)cu_count() * (uneven ? 4 : 2) / a.items;
+    a.parts = std::max<int64_t>(1, std::min<int64_t>({want, a.rows / (uneven ? 1024 : 512), 64}));
   }
   a.rows_at = (size_t)(T * Hq) * D;
   a.part_at = a.rows_at + (size_t)(T * Hq) * sizeof(float2);
