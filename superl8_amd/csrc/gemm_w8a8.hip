@@ -50,6 +50,12 @@ __device__ __forceinline__ void w8_ld4(const void* x, int64_t i, float* f) {
   }
 }
 
+// The larger magnitude, by its bits: infinity above all numbers and NaN above that, so that rows which hold one
+// come out as such (their scale is not finite) and not as the rest of the row.
+__device__ __forceinline__ float w8_top(float amax, float x) {
+  return __uint_as_float(max(__float_as_uint(amax), __float_as_uint(x) & 0x7FFFFFFFu));
+}
+
 // Chunk c of a row, as above.
 template <int DT>
 __device__ __forceinline__ void w8_chunk(const W8Args& p, int64_t row, int c, float* f) {
@@ -83,7 +89,7 @@ __global__ void __launch_bounds__(256) w8_quant_kernel(const W8Args p) {
   float f[NV ? NV : 1][16], amax = 0.f;
   auto top = [&](const float* x) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) amax = fmaxf(amax, fabsf(x[e]));
+    for (int e = 0; e < 16; ++e) amax = w8_top(amax, x[e]);
   };
   if constexpr (NV > 0) {
 #pragma unroll
@@ -99,7 +105,7 @@ __global__ void __launch_bounds__(256) w8_quant_kernel(const W8Args p) {
   amax = lane_group_max<64>(amax);
   if ((threadIdx.x & 63) == 0) amax_s[threadIdx.x >> 6] = amax;
   __syncthreads();
-  amax = fmaxf(fmaxf(amax_s[0], amax_s[1]), fmaxf(amax_s[2], amax_s[3]));
+  amax = w8_top(w8_top(amax_s[0], amax_s[1]), w8_top(amax_s[2], amax_s[3]));
   const float s = amax * (1.0f / 127.0f), safe = s == 0.f ? 1.f : s;
   if (threadIdx.x == 0) p.xs[row] = safe;
   auto put = [&](int c, const float* x) {
@@ -161,7 +167,7 @@ template <int ODT>
 __device__ __forceinline__ void w8_out4(const W8Args& p, v4i y, float xs, int m, int n) {
   float z[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) z[e] = (float)y[e] * xs * p.ws[min(n + e, p.N - 1)] + w8_bias(p, min(n + e, p.N - 1));
+  for (int e = 0; e < 4; ++e) z[e] = fmaf((float)y[e] * xs, p.ws[min(n + e, p.N - 1)], w8_bias(p, min(n + e, p.N - 1)));
   const int64_t to = (int64_t)m * p.N + n;
   if (p.N % 4 == 0) {
     w8_st4<ODT>(p.out, to, z);
@@ -213,17 +219,17 @@ __global__ void __launch_bounds__(64 * W8_WAVES) w8_stream_kernel(const W8Args p
         float f[16];
         values(raw[u][i], f);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) amax = fmaxf(amax, fabsf(f[e]));
+        for (int e = 0; e < 16; ++e) amax = w8_top(amax, f[e]);
       }
-    amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
-    amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
+    amax = w8_top(amax, __shfl_xor(amax, 16, 64));
+    amax = w8_top(amax, __shfl_xor(amax, 32, 64));
     if (g4 == 0) amax_s[wave][col] = amax;
     w8_barrier<63>();
     float mine = 0.f;
 #pragma unroll
     for (int x = 0; x < W8_WAVES; ++x) {
-      amax = fmaxf(amax, amax_s[x][col]);
-      mine = fmaxf(mine, amax_s[x][lane >> 2]);
+      amax = w8_top(amax, amax_s[x][col]);
+      mine = w8_top(mine, amax_s[x][lane >> 2]);
     }
     auto scale = [](float a) { return a * (1.0f / 127.0f) == 0.f ? 1.f : a * (1.0f / 127.0f); };
     const float safe = scale(amax);
@@ -329,7 +335,7 @@ __device__ __forceinline__ void w8_store(const W8Args& p, const v16i (&acc)[S::N
       for (int q = 0; q < 4; ++q) {
         float y[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = (float)acc[nb][mb][4 * q + e] * xs * ws[nb][4 * q + e] + bias[nb][4 * q + e];
+        for (int e = 0; e < 4; ++e) y[e] = fmaf((float)acc[nb][mb][4 * q + e] * xs, ws[nb][4 * q + e], bias[nb][4 * q + e]);
         const int at = (32 * nb + 8 * q + 4 * h) * OS;  // bytes into the row
         if constexpr (OS == 4) {
           *reinterpret_cast<float4*>(place(l32, at / 16)) = make_float4(y[0], y[1], y[2], y[3]);
@@ -535,10 +541,14 @@ struct W8Plan {
   size_t code_bytes, bytes;
 };
 
-// What takes the least time: streaming, or a tile and the parts in which the last round's tiles are cut along K.
+// What takes the least time (us): streaming, or a tile and the parts in which the last round's tiles are cut along K.
 // Tiles: rounds of the workgroups that are resident at once, each of as many stages as K has, a stage taking
 // one_us where a CU has one workgroup, up to full_us where it has per_cu; a join costs its launch and its
-// partial sums. Neither is faster than the weights' bytes.
+// partial sums. Neither is faster than the weights' bytes; launches and the rows' codes are the constants.
+// Both sides, calls on one stream: 1 row, 5120 x 5120 streamed 13.0, tiles of 32 rows 15.0; 17408 x 5120 24.7 and 27.1; 16 rows,
+// 4096 x 4096 13.0 and 14.9, 30000 x 4096 36.6 and 34.2. Tiles of 32, 64, 128 and 256 rows: 64 rows, 17408 x 5120 42.7, 31.9,
+// 37.9, 48.1; 512 rows, 4096 x 4096 23.3, 20.7, 27.1, 30.7 and 17408 x 5120 125, 90.8, 76.7, 74.2; 2048 rows, 4096 x 4096
+// 72.2, 55.6, 49.1, 67.2.
 W8Plan w8_plan(int64_t M, int64_t N, int64_t K) {
   struct Shape { int bm, bn, per_cu; double one_us, full_us; };
   static const Shape shapes[] = {{256, 256, 1, 1.7, 1.7}, {128, 128, 2, 0.9, 1.2}, {64, 128, 2, 0.6, 0.95}, {32, 128, 2, 0.45, 0.8}};
@@ -548,7 +558,7 @@ W8Plan w8_plan(int64_t M, int64_t N, int64_t K) {
   a.splits = 1;
   const double stages = (double)w8_padded(K) / W8_BK, cus = cu_count();
   double best = 1e30;
-  if (M <= W8_STREAM_ROWS && K <= W8_STREAM_K) best = 3. + (double)N * K / 4e6;
+  if (M <= W8_STREAM_ROWS && K <= W8_STREAM_K) best = M <= W8_FUSED_ROWS ? 3.5 + (double)N * K / 4.6e6 : 6. + (double)N * K / 4.2e6;
   for (const Shape& s : shapes) {
     const int64_t nt_m = (M + s.bm - 1) / s.bm, nt_n = (N + s.bn - 1) / s.bn, n = nt_m * nt_n;
     const int64_t slots = (int64_t)cus * s.per_cu, rest = n % slots, most = n - rest;
@@ -556,7 +566,7 @@ W8Plan w8_plan(int64_t M, int64_t N, int64_t K) {
       if (S > 1 && (rest == 0 || stages < 4 * S || rest * S > slots)) break;
       const double more = std::ceil((double)rest * S / cus) - 1.;
       const double part = rest ? std::ceil(stages / S) * (s.one_us + (s.full_us - s.one_us) * more / std::max(1, s.per_cu - 1)) : 0.;
-      double us = std::max((double)(most / slots) * stages * s.full_us + part, (double)N * K / 4.8e6) + 3.;
+      double us = std::max((double)(most / slots) * stages * s.full_us + part, (double)N * K / 4.8e6) + 6.;
       if (S > 1) us += 3.5 + (double)rest * S * s.bm * s.bn * 5 / 4e6;
       if (us >= best) continue;
       best = us;
@@ -628,7 +638,9 @@ extern "C" int sl8_linear_w8a8(const void* x, int x_dtype, const int8_t* w, cons
   auto go = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     if (plan.tile == 0) {
-      const unsigned wgs = (unsigned)std::min<int64_t>((N + 15) / 16, 2 * cu_count());
+      // (as many as are resident: a wave's codes and two groups of weights take up to 245 registers. With twice as
+      // many 5120 x 5120 takes 18.4 for 13.0 us)
+      const unsigned wgs = (unsigned)std::min<int64_t>((N + 15) / 16, (int64_t)cu_count() * (K <= 2048 ? 2 : 1));
       auto stream = [&](auto xdt) {
         constexpr int XDT = decltype(xdt)::value;
         if (K <= 2048) w8_stream_kernel<DT, 2, XDT><<<wgs, 64 * W8_WAVES, 0, st>>>(p);

@@ -412,8 +412,8 @@ def attn_paged_block8(q: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.Ten
 
     tree_mask int64 [T] or [T,1..4] (see tree_mask): drafted tokens in a tree. A row sees its
     sequence's tokens in front of the new ones, and of those the j-th where bit j of its mask is set
-    (bits stand for the first 64 to 256; itself too only if marked); a window counts the marked ones
-    first and takes what is left of it in front. return_lse: (out, lse fp32 [T,Hq]), the logarithm
+    (bits stand for the first 64 to 256; itself too only if marked; bits of tokens that are not there
+    count for nothing); a window counts the marked ones first and takes what is left of it in front. return_lse: (out, lse fp32 [T,Hq]), the logarithm
     of each row's sum of e^score, -inf where it sees nothing."""
     softmax_scale = (1.0 / (q.shape[-1] ** 0.5)) if scale is None else scale
     q = q.contiguous()
@@ -570,7 +570,8 @@ def linear_w8a8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *,
     """Linear layer of int8 weights: x [..., K] fp16/bf16/fp32, each row quantised as by
     quantize_i8_rowwise; w int8 [N,K] with w_scale fp32 [N] (a scale per output channel: the
     per_row_i8 QTensor) -> [..., N] of out_dtype. K a multiple of 4, at least 16. The integer sums are
-    exact; scales and bias are applied in fp32 and the result is rounded once."""
+    exact; scales and bias are applied in fp32 and the result is rounded once. A row of x that holds
+    NaN or infinity gives no finite output; the other rows are as without it."""
     if x.dim() == 2:
         return _C.linear_w8a8(x.contiguous(), w.contiguous(), w_scale.contiguous(), bias, out_dtype)
     *lead, K = x.shape

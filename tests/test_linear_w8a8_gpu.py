@@ -138,3 +138,28 @@ def test_refusals():
                    dict(x=torch.zeros(1, 131072, device=DEV, dtype=F16), w=torch.zeros(32, 131072, device=DEV, dtype=torch.int8))]:
         with pytest.raises(RuntimeError, match="fni8"):
             _C.linear_w8a8(**base | change)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("M,N,K", [(3, 40, 512), (16, 40, 5120), (33, 257, 1028), (700, 300, 20000)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_rows_that_are_not_finite(M, N, K, dtype, bad):
+    """A row with NaN or infinity has no finite output; the others do not change."""
+    x, w, ws, b = inputs(M, N, K, dtype, F32)
+    rows = [1, M - 1]
+    x[rows[0], K - 1] = bad
+    x[rows[1], K // 3] = bad
+    y = sl8.linear_w8a8(x, w, ws, bias=b)
+    assert not bool(y[rows].isfinite().any())
+    x[rows] = 0
+    rest = [i for i in range(M) if i not in rows]
+    assert torch.equal(y[rest], sl8.linear_w8a8(x, w, ws, bias=b)[rest])
+
+
+@pytest.mark.parametrize("N,K", [(300, 1024), (4099, 2052), (1000, 20000)])
+def test_rows_do_not_depend_on_the_batch(N, K):
+    """Streamed, in tiles, in parts of K: a row's outputs are the same bits."""
+    x, w, ws, b = inputs(1500, N, K, BF16, F16)
+    y = sl8.linear_w8a8(x, w, ws, bias=b, out_dtype=F32)
+    for M in (1, 3, 7, 16, 40, 100, 400):
+        assert torch.equal(sl8.linear_w8a8(x[:M], w, ws, bias=b, out_dtype=F32), y[:M])
