@@ -7,6 +7,10 @@
 // sequences share are only read. A block takes
 //   s' = max(scales of the blocks that its rows come from, 2^-60), codes c' = rint(c * (s / s')),
 // so rows that stay together, or come from blocks of one scale, are copied as they are.
+//
+// Bound by the counting, which has a workgroup for each sequence and head, and by the kept rows' bytes, K and V, in
+// and out. Kernels (us): 4 sequences of 733 to 1100 tokens to 1024, 8 heads, D = 128, select 7.6, move 7 (the 17 MB
+// of rows come from and go to caches); 8 of 21845 to 32768 to 4096 select 27, move 31 (134 MB, 26 at the rate of a copy).
 #include <algorithm>
 
 #include "block8.hpp"
@@ -57,7 +61,7 @@ __device__ __forceinline__ int2 over_waves(int mine, int wave, int* sums) {
 // range that the weights take (by their bits as whole numbers: a bin's count rarely meets another's atomics there,
 // as the highest byte's would), then over the bin that holds it, three times at most. Which stay then follows in
 // order from the counts of each 64. VPT weights a thread are kept in registers; 0: longer contexts are read again
-// for each count.
+// for each count (32768 tokens so: 67 us for 27).
 template <int VPT>
 __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictArgs p) {
   constexpr int BINS = 2048, ROWS = VPT ? VPT : 1;

@@ -3,6 +3,12 @@
 //   xs[m] = amax|x[m]| * fp32(1/127) (1 for a row of zeros), c = clamp(rint(x / xs), -127, 127),
 //   y[m,n] = xs[m] * ws[n] * sum_k c[m,k] w[n,k] + bias[n], rounded once.
 // The sums are exact integers (K < 2^17).
+//
+// Up to some tens of rows are bound by the weights' bytes, more by the matrix instructions. A call among others (us; a
+// copy's 5.16 TB/s and a large int8 product's 2.10 POP/s give the floor): 1 row, 4096 x 4096 9.1 (floor 3.3; kernel
+// 8.6 to 9.3, most of it the way to the first weights and the waves' sums); 16 rows, 17408 x 5120 23.5 (17.4;
+// codes 4.2, tiles of 32 rows 16.6, 5.4 TB/s); 333 rows, 5003 x 2052, 19.4 (3.6; codes 4.1, tiles of 64 rows 16.4: a chain
+// of 17 stages); 4096 rows, 17408 x 5120 370 (348; codes 20, tiles of 256 rows 334 to 362, join 16).
 #include <algorithm>
 #include <cmath>
 
@@ -156,7 +162,7 @@ __device__ __forceinline__ void w8_st4(void* out, int64_t i, const float* y) {
 // ---------------------------------------------------------------------------
 // Up to 16 rows: 16 channels at a time, each wave with its part of K: weights straight from memory into A operands
 // of v_mfma_i32_16x16x64_i8 (lane (g4, col): 16 bytes of row col), the codes as B operands. The waves' sums
-// meet in LDS. Bound by the weights' bytes. The codes of a wave's part stay in registers while the workgroup goes
+// meet in LDS. Bound by the weights' bytes (17408 x 5120: 3.6 TB/s). The codes of a wave's part stay in registers while the workgroup goes
 // through its groups of channels, a group's weights on their way while the one before is multiplied; the two
 // halves of a line are read next to each other (U units of 128 bytes a wave).
 // ---------------------------------------------------------------------------
@@ -283,9 +289,12 @@ __global__ void __launch_bounds__(64 * W8_WAVES) w8_stream_kernel(const W8Args p
 
 // ---------------------------------------------------------------------------
 // Many rows: BN x BM output tiles (channels x rows), MW waves along the rows and NW along the channels, each
-// with 32 NB x 32 MB of them on v_mfma_i32_32x32x32_i8. Stages of 128 bytes of K (whole lines) go through two places
-// in LDS by direct copies, a stage ahead; 16-byte chunks of a row are placed by an xor of the row, so that
-// 16 rows of a read lie in different banks.
+// with 32 NB x 32 MB of them on v_mfma_i32_32x32x32_i8. Stages of 128 bytes of K (whole lines; with 64 bytes
+// 512 x 17408 x 5120 took 100 us, 77 now) go through RING places in LDS by direct copies, RING - 1
+// ahead of the products, one barrier a stage; 16-byte chunks of a row are placed by an xor of the row, so that
+// 16 rows of a read lie in different banks. Bound by the matrix pipe's power in large tiles (4096 x 17408 x 5120: it is busy
+// in 54 % of the cycles, at 1.55 to 1.6 GHz, as the library's product of that size, 385 us, is), by the copies in
+// tiles of 32 and 64 rows, whose rings are longer for that.
 // ---------------------------------------------------------------------------
 template <int BM_, int BN_, int MW_, int NW_, int RING_> struct W8Tile {
   static constexpr int RING = RING_;  // stages in LDS
@@ -456,7 +465,7 @@ __global__ void __launch_bounds__(S::THREADS, 2) w8_tile_kernel(const W8Args p) 
           acc[nb][mb] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[nb], b[mb], acc[nb][mb], 0, 0, 0);
     }
   };
-  // the other stage's place is free behind the barrier
+  // (the place of the stage before is free behind the barrier)
   auto step = [&](int kt, const int8_t* st, int8_t* to) __attribute__((always_inline)) {
     w8_barrier<(S::RING - 2) * (WCOP + XCOP)>();
     load(kt + S::RING - 1, to);

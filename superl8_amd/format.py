@@ -3,8 +3,9 @@
 QTensor (reference superl8/format.py:219-303) describes a stored weight; the
 schemes this hot path computes on are ``gguf_kquant`` (native GGUF k-quant
 bytes kept resident, byte-identical to the GGUF file; the sub-block scales
-live inside the bytes) for the Q4_K / Q5_K / Q6_K kernels and ``raw`` (a
-tensor used as is). ``per_row_i8`` / ``per_chan_i8`` (int8 + fp32 scale) are
+live inside the bytes) for the Q4_K / Q5_K / Q6_K kernels, ``per_row_i8``
+(int8 + a fp32 scale per output channel, not rotated) for the int8 linear and
+``raw`` (a tensor used as is). Rotated ``per_row_i8`` and ``per_chan_i8`` are
 carried by the file format so checkpoints holding them load, but no kernel of
 this path consumes them.
 
