@@ -157,7 +157,7 @@ def test_rows_that_are_not_finite(M, N, K, dtype, bad):
 
 
 @pytest.mark.parametrize("N,K", [(300, 1024), (4099, 2052), (1000, 20000)])
-def test_rows_do_not_depend_on_the_batch(N, K):
+def test_bits_of_a_row_in_any_batch(N, K):
     """Streamed, in tiles, in parts of K: a row's outputs are the same bits."""
     x, w, ws, b = inputs(1500, N, K, BF16, F16)
     y = sl8.linear_w8a8(x, w, ws, bias=b, out_dtype=F32)

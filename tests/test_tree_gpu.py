@@ -415,3 +415,13 @@ def test_bits_of_tokens_that_are_not_there(n, window):
     want = sl8.attn_paged_block8(q, *c.args(), i32([n + 200, n]), tree_mask=clean, **args)
     got = sl8.attn_paged_block8(q, *c.args(), i32([n + 200, n]), tree_mask=stray, **args)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("new,old,Hkv,window", [([130], [3000], 1, -1), ([300, 20], [40, 5000], 2, -1), ([600], [0], 1, -1),
+                                                ([260], [1500], 1, 100), ([140, 0, 140], [700, 9, 80], 1, -1)])
+def test_weights_of_rows_in_parts(new, old, Hkv, window):
+    """Few items of many rows: behind long and short contexts, where parts end inside a token's heads or hold none."""
+    total = [n + o for n, o in zip(new, old)]
+    c = Cache(total, Hkv, 64, 16)
+    q = coded_queries(sum(new), 10 * Hkv, 64, F16, False)
+    weights_and_check(c, q, new, total, window=window, decay=0.5)
