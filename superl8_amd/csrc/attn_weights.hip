@@ -6,11 +6,12 @@
 //   w_j <- (j < len - n ? decay * w_j : 0) + sum over the n new rows i that see j, over the group's
 //          heads, of 2^(s_ij - lse_i log2 e)
 // for each KV head. Bound by the bytes of K for few rows, by the exponentials (VALU, a quarter of the rate of other
-// instructions) for many. A call among others (us): 32 x 1 token behind 1024 to 8191, 32 / 8 heads, D = 128, 35 to 38 (rows 4.8,
-// keys 31 of which 24 are K's 122 MB at the rate of a copy); 6 x 20 to 33 tokens behind up to 3001 with a window, D = 64, 16 (rows 3, keys 8,
-// else the call); 2048 tokens behind 2048 keys, 32 / 8 heads, 81 (51 G operations, 24 at the rate of a large int8 product;
-// 201 million exponentials, 25 at theirs).
+// instructions) for many. A call among others (us): 32 x 1 token behind 1024 to 8191, 32 / 8 heads, D = 128, 35 (rows 4,
+// keys 28 of which 24 are K's 122 MB at the rate of a copy); 6 x 20 to 33 tokens behind up to 3001 with a window, D = 64, 16 (rows 3, keys 8,
+// else the call); 2048 tokens behind 2048 keys, 32 / 8 heads, 77 (51 G operations, 24 at the rate of a large int8 product;
+// 201 million exponentials, 23 at theirs; beside each a conversion, a product and a sum).
 #include <algorithm>
+#include <climits>
 
 #include "attn_common.hpp"
 #include "block8.hpp"
@@ -147,7 +148,7 @@ __device__ __forceinline__ void put(const WeightArgs& p, const KeyTile& it, int 
 // workgroup share the rows (of part blockIdx.y of them) and their sums meet in LDS. Keys are A operands in registers
 // (v_mfma_i32_16x16x64_i8), 16 rows at a time the B operands; lane (g4, col) then has keys 16 g + 4 g4 + i for row col.
 template <int D, int WAVES>
-__global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) weights_kernel(const WeightArgs p) {
+__global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, 2) weights_kernel(const WeightArgs p) {
   constexpr int KS = D / 64, KG = AW_KEYS / 16;
   __shared__ float sum_s[WAVES == 1 ? 1 : WAVES][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -177,25 +178,30 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) weights_kernel(
     const float was = p.w[it.b * p.wb + it.kvh * p.wh + min(key, it.len - 1)];
     const int8_t* codes = p.codes + ((int64_t)it.kvh * p.s.T + it.row0) * p.G * D;
     const float2* rows = p.rows + ((int64_t)it.kvh * p.s.T + it.row0) * p.G;
+    // rows from `seen` on see all of the keys, up to `until` (row units; a window's side)
+    const int seen = (int)min((int64_t)max(key0 + AW_KEYS - 1 - pos0, 0) * p.G, (int64_t)INT_MAX);
+    const int until = p.window < 0 ? INT_MAX
+                                   : (int)min(max(((int64_t)key0 - pos0 + p.window) * p.G, (int64_t)0), (int64_t)INT_MAX);
     float acc[KG][4] = {};
     const int rw = r0 + (WAVES == 1 ? 0 : 16 * wave);
-    v4i qb[KS], qn[KS];
-    float2 y, yn;
+    v4i q0[KS], q1[KS];
+    float2 y0, y1;
     auto load = [&](int r, v4i (&q)[KS], float2& s) __attribute__((always_inline)) {
-      const int row = min(r + col, r1 - 1);
+      r = min(r, r1 - 1);  // (past the last: as the last)
+      const uint32_t row = min(col, r1 - 1 - r);
+      const int8_t* from = codes + (int64_t)r * D;
 #pragma unroll
-      for (int i = 0; i < KS; ++i) q[i] = *reinterpret_cast<const v4i*>(codes + (int64_t)row * D + 64 * i + 16 * g4);
-      s = rows[row];
+      for (int i = 0; i < KS; ++i) q[i] = *reinterpret_cast<const v4i*>(from + (row * D + 64 * i + 16 * g4));
+      s = (rows + r)[row];
     };
-    if (rw < r1) load(rw, qb, y);
-    for (int r = rw; r < r1; r += 16 * WAVES) {
-      load(r + 16 * WAVES, qn, yn);  // (past the last: as the last)
+    auto pass = [&](int r, const v4i (&q)[KS], float2 y, v4i (&next)[KS], float2& yn) __attribute__((always_inline)) {
+      load(r + 16 * WAVES, next, yn);
       v4i sc[KG];
 #pragma unroll
       for (int g = 0; g < KG; ++g) {
         sc[g] = v4i{0, 0, 0, 0};
 #pragma unroll
-        for (int s = 0; s < KS; ++s) sc[g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(ka[g][s], qb[s], sc[g], 0, 0, 0);
+        for (int s = 0; s < KS; ++s) sc[g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(ka[g][s], q[s], sc[g], 0, 0, 0);
       }
       float e[KG][4];
 #pragma unroll
@@ -204,9 +210,7 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) weights_kernel(
 #pragma unroll
         for (int i = 0; i < 4; ++i) e[g][i] = __builtin_amdgcn_exp2f(fmaf((float)sc[g][i], a, c));
       }
-      // all rows see all keys, or each its own
-      const int p0 = pos0 + r / p.G, p1 = pos0 + (r + 15) / p.G;
-      if (!(r + 16 <= r1 && key0 + AW_KEYS - 1 <= p0 && (p.window < 0 || key0 > p1 - p.window))) {
+      if (!(r >= seen && r + 15 < until && r + 16 <= r1)) {  // each row its own
         const int pos = pos0 + (r + col) / p.G, lim = r + col < r1 ? pos + 1 : 0;
         const int low = p.window >= 0 ? pos - p.window + 1 : 0;
 #pragma unroll
@@ -221,9 +225,20 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) weights_kernel(
       for (int g = 0; g < KG; ++g)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[g][i] += e[g][i];
+    };
+    if (rw < r1) load(rw, q0, y0);
+    if constexpr (WAVES > 1) {
+      for (int r = rw; r < r1; r += 32 * WAVES) {
+        pass(r, q0, y0, q1, y1);
+        if (r + 16 * WAVES < r1) pass(r + 16 * WAVES, q1, y1, q0, y0);
+      }
+    } else {  // (one pass for the most part: fewer registers, a wave a SIMD more at D = 128)
+      for (int r = rw; r < r1; r += 16) {
+        pass(r, q0, y0, q1, y1);
 #pragma unroll
-      for (int s = 0; s < KS; ++s) qb[s] = qn[s];
-      y = yn;
+        for (int i = 0; i < KS; ++i) q0[i] = q1[i];
+        y0 = y1;
+      }
     }
     // over the 16 rows of a lane group; lane (g4, col) keeps key 16 (col / 4) + 4 g4 + col % 4
     float sum = 0.f;
@@ -277,9 +292,9 @@ __global__ void __launch_bounds__(256) weights_join_kernel(const WeightArgs p) {
 // item go to workgroups of their own: where items are few, so that there are two for each CU, and four where new rows
 // are a good part of the context (a causal prompt's last keys are seen by few of its rows, so items differ); parts
 // large enough to pay for the join. Whole and in parts (us): 2000 rows behind 100 keys, 8 heads to a KV head, D = 256, 134
-// and 44; 4000 behind 100, 8 / 2 heads, D = 128, 134 and 52; 2048 behind 2048, 32 / 8 heads, 101 and 92 (6 parts for 2:
+// and 40; 4000 behind 100, 8 / 2 heads, D = 128, 134 and 52; 2048 behind 2048, 32 / 8 heads, 101 and 92 (6 parts for 2:
 // 105); 700 behind 30000, 8 / 1 heads, 60 whole, 84 in two.
-// A wave an item for up to 32 rows, else four: one row, 32 sequences 35 and 96; 16 tokens of 4 heads, D = 64, 18.8 and 20.3;
+// A wave an item for up to 32 rows, else four: one row, 32 sequences 32 and 96; 16 tokens of 4 heads, D = 64, 18.8 and 20.3;
 // 300 of 4 heads, D = 128, 47 and 24.
 struct WeightPlan {
   int64_t rows, items, parts;

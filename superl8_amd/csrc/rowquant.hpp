@@ -284,21 +284,27 @@ __device__ __forceinline__ uint2 row_codes_wide(const float* f, int lane, bool r
         const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
         return (uint32_t)((lane & 16) ? r[0] : r[1]);
       });
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] *= 1.0 / __builtin_sqrt((double)D);
   }
+  const double norm = rotate ? 1.0 / __builtin_sqrt((double)D) : 1.0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) top = fmax(top, fabs(x[e]));
-  const float amax = lane_group_max<LPR>((float)top);  // (rounding keeps the order)
+  const float amax = lane_group_max<LPR>((float)(top * norm));  // (rounding keeps the order)
   const float s = amax * (1.0f / 127.0f);
   safe = s == 0.f ? 1.f : s;
-  const double inv = 1.0 / (double)safe;  // (the product is within 2^-52 of the quotient, its rounding to fp32 the same but for 2^-27)
-  uint32_t c[2] = {0, 0};
+  // 1 / safe by Newton's steps; the product is within 2^-51 of the quotient, its rounding to fp32 the same but for 2^-26
+  const double d = (double)safe;
+  double inv = __builtin_amdgcn_rcp(d);
+  inv = fma(inv, fma(-d, inv, 1.0), inv);
+  inv = fma(inv, fma(-d, inv, 1.0), inv) * norm;
+  uint32_t t[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float r = fminf(fmaxf(rintf((float)(x[e] * inv)), -127.f), 127.f);
-    c[e / 4] |= (uint32_t)(uint8_t)(int8_t)r << (8 * (e % 4));
-  }
+  for (int e = 0; e < 8; ++e)  // (the low byte of 1.5 * 2^23 + r is r, rounded to a whole number)
+    t[e] = __float_as_uint(__builtin_amdgcn_fmed3f((float)(x[e] * inv), -127.f, 127.f) + 12582912.f);
+  uint32_t c[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)  // (bytes as in codes8_each)
+    c[i] = __builtin_amdgcn_perm(t[4 * i + 1], t[4 * i], 0x0c0c0400u) |
+           __builtin_amdgcn_perm(t[4 * i + 3], t[4 * i + 2], 0x04000c0cu);
   return make_uint2(c[0], c[1]);
 }
 
