@@ -8,7 +8,7 @@
 // for each KV head. Bound by the bytes of K for few rows, by the exponentials (VALU, a quarter of the rate of other
 // instructions) for many. A call among others (us): 32 x 1 token behind 1024 to 8191, 32 / 8 heads, D = 128, 35 (rows 4,
 // keys 28 of which 24 are K's 122 MB at the rate of a copy); 6 x 20 to 33 tokens behind up to 3001 with a window, D = 64, 16 (rows 3, keys 8,
-// else the call); 2048 tokens behind 2048 keys, 32 / 8 heads, 77 (51 G operations, 24 at the rate of a large int8 product;
+// else the call); 2048 tokens behind 2048 keys, 32 / 8 heads, 75 (51 G operations, 24 at the rate of a large int8 product;
 // 201 million exponentials, 23 at theirs; beside each a conversion, a product and a sum).
 #include <algorithm>
 #include <climits>
@@ -147,15 +147,19 @@ __device__ __forceinline__ void put(const WeightArgs& p, const KeyTile& it, int 
 // 64 keys an item. WAVES 1: each wave for itself, its keys' loads being what counts; else the waves of a
 // workgroup share the rows (of part blockIdx.y of them) and their sums meet in LDS. Keys are A operands in registers
 // (v_mfma_i32_16x16x64_i8), 16 rows at a time the B operands; lane (g4, col) then has keys 16 g + 4 g4 + i for row col.
+// (Two waves a SIMD as the least: with one the products go to accumulation registers and are copied back. Four waves a
+// SIMD instead of three, or rows in 24 parts for waves of a tile each, take a prompt's 75 us to 87 and 105.)
 template <int D, int WAVES>
 __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, 2) weights_kernel(const WeightArgs p) {
   constexpr int KS = D / 64, KG = AW_KEYS / 16;
   __shared__ float sum_s[WAVES == 1 ? 1 : WAVES][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g4 = lane >> 4;
-  const int first = WAVES == 1 ? blockIdx.x * 4 + wave : blockIdx.x, step = WAVES == 1 ? gridDim.x * 4 : gridDim.x;
   const int lens = lane < p.s.B ? p.s.lens[lane] : 0;
-  for (int id = first;; id += step) {
+  // every other part begins from the end: the tiles of a causal prompt are seen by fewer rows the later they are
+  for (int x = blockIdx.y & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x;; x += gridDim.x) {
+    // WAVES 1: four tiles of a head next to each other (32 x 1 token 34.5 us, 35 where they are of four heads)
+    const int id = WAVES == 1 ? (x / p.Hkv * 4 + wave) * p.Hkv + x % p.Hkv : x;
     const KeyTile it = key_tile(p, lane, lens, id);
     if (it.b < 0) return;
     const Rows all = rows_of(p, it);
@@ -386,7 +390,8 @@ extern "C" int sl8_attn_weights_block8(const void* q, int dtype, int rotate, flo
     }
     const int64_t cus = cu_count();
     if (plan.rows <= 32) {
-      weights_kernel<DD, 1><<<(unsigned)std::min((plan.items + 3) / 4, cus * 8), 256, 0, st>>>(p);
+      const int64_t groups = (B * ((cap + AW_KEYS - 1) / AW_KEYS) + 3) / 4 * Hkv;
+      weights_kernel<DD, 1><<<(unsigned)std::min(groups, cus * 8), 256, 0, st>>>(p);
     } else {
       const dim3 grid((unsigned)std::min(plan.items, cus * 12), (unsigned)plan.parts);
       weights_kernel<DD, AW_WAVES><<<grid, 64 * AW_WAVES, 0, st>>>(p);
