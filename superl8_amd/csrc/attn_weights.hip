@@ -8,7 +8,7 @@
 // for each KV head. Bound by the bytes of K for few rows, by the exponentials (VALU, a quarter of the rate of other
 // instructions) for many. A call among others (us): 32 x 1 token behind 1024 to 8191, 32 / 8 heads, D = 128, 35 (rows 4,
 // keys 28 of which 24 are K's 122 MB at the rate of a copy); 6 x 20 to 33 tokens behind up to 3001 with a window, D = 64, 16 (rows 3, keys 8,
-// else the call); 2048 tokens behind 2048 keys, 32 / 8 heads, 75 (51 G operations, 24 at the rate of a large int8 product;
+// else the call); 2048 tokens behind 2048 keys, 32 / 8 heads, 66 (51 G operations, 24 at the rate of a large int8 product;
 // 201 million exponentials, 23 at theirs; beside each a conversion, a product and a sum).
 #include <algorithm>
 #include <climits>
@@ -34,7 +34,7 @@ struct WeightArgs {
   float q_mul, decay;
   int window;
   bool rotate;
-  int8_t* codes;  // [Hkv][T * G][D]
+  int8_t* codes;  // [Hkv][D / 64][T * G][64]: a load's 16 rows next to each other (below)
   float2* rows;   // [Hkv][T * G]: scale * q_mul, lse * log2 e
   int parts;      // of an item's rows
   int items;      // at most
@@ -54,8 +54,8 @@ __global__ void __launch_bounds__(AW_THREADS) weights_rows_kernel(const WeightAr
   float safe;
   const uint2 c = row_codes_wide<D>(f, lane, p.rotate, safe);
   if (i >= n) return;
-  const int64_t to = ((int64_t)kvh * p.s.T + t) * p.G + h - kvh * p.G;
-  reinterpret_cast<uint2*>(p.codes + to * D)[lane] = c;
+  const int64_t R = p.s.T * p.G, at = (int64_t)t * p.G + h - kvh * p.G, to = kvh * R + at;
+  *reinterpret_cast<uint2*>(p.codes + kvh * R * D + ((lane >> 3) * R + at) * 64 + 8 * (lane & 7)) = c;
   if (lane == 0) {
     const float l = p.lse[row];
     // (a row that sees nothing: no weights)
@@ -147,8 +147,9 @@ __device__ __forceinline__ void put(const WeightArgs& p, const KeyTile& it, int 
 // 64 keys an item. WAVES 1: each wave for itself, its keys' loads being what counts; else the waves of a
 // workgroup share the rows (of part blockIdx.y of them) and their sums meet in LDS. Keys are A operands in registers
 // (v_mfma_i32_16x16x64_i8), 16 rows at a time the B operands; lane (g4, col) then has keys 16 g + 4 g4 + i for row col.
-// (Two waves a SIMD as the least: with one the products go to accumulation registers and are copied back. Four waves a
-// SIMD instead of three, or rows in 24 parts for waves of a tile each, take a prompt's 75 us to 87 and 105.)
+// (Two waves a SIMD as the least: with one the products go to accumulation registers and are copied back. Rows of
+// codes lie 64 bytes at a time, so that a load's 16 are whole lines: in rows of D bytes, two loads to each line, waves
+// waited for them in 55 % of their cycles, 19 % now, and 8000 tokens behind 100 keys took 332 us, 280 now.)
 template <int D, int WAVES>
 __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, 2) weights_kernel(const WeightArgs p) {
   constexpr int KS = D / 64, KG = AW_KEYS / 16;
@@ -180,7 +181,8 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, 2) weights_kern
     }
     const int key = key_of(it, lane);
     const float was = p.w[it.b * p.wb + it.kvh * p.wh + min(key, it.len - 1)];
-    const int8_t* codes = p.codes + ((int64_t)it.kvh * p.s.T + it.row0) * p.G * D;
+    const int64_t R = p.s.T * p.G;
+    const int8_t* codes = p.codes + it.kvh * R * D + it.row0 * p.G * 64;
     const float2* rows = p.rows + ((int64_t)it.kvh * p.s.T + it.row0) * p.G;
     // rows from `seen` on see all of the keys, up to `until` (row units; a window's side)
     const int seen = (int)min((int64_t)max(key0 + AW_KEYS - 1 - pos0, 0) * p.G, (int64_t)INT_MAX);
@@ -193,9 +195,8 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, 2) weights_kern
     auto load = [&](int r, v4i (&q)[KS], float2& s) __attribute__((always_inline)) {
       r = min(r, r1 - 1);  // (past the last: as the last)
       const uint32_t row = min(col, r1 - 1 - r);
-      const int8_t* from = codes + (int64_t)r * D;
 #pragma unroll
-      for (int i = 0; i < KS; ++i) q[i] = *reinterpret_cast<const v4i*>(from + (row * D + 64 * i + 16 * g4));
+      for (int i = 0; i < KS; ++i) q[i] = *reinterpret_cast<const v4i*>(codes + (i * R + r) * 64 + (64 * row + 16 * g4));
       s = (rows + r)[row];
     };
     auto pass = [&](int r, const v4i (&q)[KS], float2 y, v4i (&next)[KS], float2& yn) __attribute__((always_inline)) {
@@ -215,15 +216,14 @@ __global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, 2) weights_kern
         for (int i = 0; i < 4; ++i) e[g][i] = __builtin_amdgcn_exp2f(fmaf((float)sc[g][i], a, c));
       }
       if (!(r >= seen && r + 15 < until && r + 16 <= r1)) {  // each row its own
-        const int pos = pos0 + (r + col) / p.G, lim = r + col < r1 ? pos + 1 : 0;
+        // (places counted from the lane's first key)
+        const int pos = pos0 + (r + col) / p.G - key0 - 4 * g4, lim = r + col < r1 ? pos + 1 : 0;
         const int low = p.window >= 0 ? pos - p.window + 1 : 0;
 #pragma unroll
         for (int g = 0; g < KG; ++g)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int k = key0 + 16 * g + 4 * g4 + i;
-            if (k >= lim || k < low) e[g][i] = 0.f;
-          }
+          for (int i = 0; i < 4; ++i)
+            if (16 * g + i >= lim || 16 * g + i < low) e[g][i] = 0.f;
       }
 #pragma unroll
       for (int g = 0; g < KG; ++g)
@@ -296,8 +296,8 @@ __global__ void __launch_bounds__(256) weights_join_kernel(const WeightArgs p) {
 // item go to workgroups of their own: where items are few, so that there are two for each CU, and four where new rows
 // are a good part of the context (a causal prompt's last keys are seen by few of its rows, so items differ); parts
 // large enough to pay for the join. Whole and in parts (us): 2000 rows behind 100 keys, 8 heads to a KV head, D = 256, 134
-// and 40; 4000 behind 100, 8 / 2 heads, D = 128, 134 and 52; 2048 behind 2048, 32 / 8 heads, 101 and 92 (6 parts for 2:
-// 105); 700 behind 30000, 8 / 1 heads, 60 whole, 84 in two.
+// and 35; 4000 behind 100, 8 / 2 heads, D = 128, 134 and 51; 2048 behind 2048, 32 / 8 heads, 101 and 92, later 75 (6 parts
+// for 2: 87); 700 behind 30000, 8 / 1 heads, 60 whole, 84 in two.
 // A wave an item for up to 32 rows, else four: one row, 32 sequences 32 and 96; 16 tokens of 4 heads, D = 64, 18.8 and 20.3;
 // 300 of 4 heads, D = 128, 47 and 24.
 struct WeightPlan {
