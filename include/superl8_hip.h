@@ -498,7 +498,7 @@ int sl8_kv_evict_block8(int8_t* k_cache, float* k_scale, int8_t* v_cache, float*
  * Linear layer of int8 weights with a scale per output channel: x [M,K] f16 / bf16 / f32, each row
  * quantised to int8 as sl8_quantize_i8_rowwise; w int8 [N,K]; w_scale fp32 [N]; bias [N] (f16 / bf16 /
  * f32; NULL: none) -> out [M,N] = x_scale[m] * w_scale[n] * sum_k x_i8 w + bias[n], the sums exact, rounded
- * once. K a multiple of 4, 16 to 131068; w 16-byte aligned (4 where K % 16 != 0). workspace:
+ * once; a row with NaN or infinity has no finite output. K a multiple of 4, 16 to 131068; w 16-byte aligned (4 where K % 16 != 0). workspace:
  * sl8_linear_w8a8_workspace() bytes, uninitialised, 16-byte aligned.
  * ---------------------------------------------------------------------- */
 size_t sl8_linear_w8a8_workspace(int64_t M, int64_t N, int64_t K);
