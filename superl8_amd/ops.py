@@ -447,7 +447,8 @@ def tree_mask(parents: torch.Tensor, cu_lens: torch.Tensor | None = None, *, wor
     up = torch.where(parents >= 0, first + parents.long(), T)
     up = torch.where((up >= first) & (up < end), up, T)
     none = mask.new_zeros(1, words)
-    for _ in range((64 * words - 1).bit_length()):  # the masks of twice as many levels, each time
+    # the masks of twice as many levels, each time; a path may be as long as the list, whatever has bits
+    for _ in range(max(T - 1, 1).bit_length()):
         mask = mask | torch.cat([mask, none])[up]
         up = torch.cat([up, up.new_full((1,), T)])[up]
     return mask

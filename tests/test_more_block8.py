@@ -109,3 +109,18 @@ def test_masks_of_random_trees():
         for r, a in zip(got.tolist(), want):
             assert sum((x & (1 << 64) - 1) << (64 * k) for k, x in enumerate(r)) == a
     assert sl8.tree_mask(torch.zeros(0, dtype=torch.int32)).shape == (0, 1)
+
+
+@pytest.mark.parametrize("n,words", [(65, 1), (100, 1), (128, 1), (129, 1), (200, 2), (300, 4), (700, 4)])
+def test_masks_of_paths_longer_than_their_words(n, words):
+    """A token behind the last bit still has the bits of all above it: chains, chains whose parents stand behind
+    their children, and one beside a sequence of its own."""
+    full = (1 << 64 * words) - 1
+    whole = lambda r: sum((x & (1 << 64) - 1) << (64 * k) for k, x in enumerate(r))
+    down = sl8.tree_mask(torch.arange(-1, n - 1), words=words)
+    assert [whole(r) for r in down.tolist()] == [(1 << i + 1) - 1 & full for i in range(n)]
+    up = sl8.tree_mask(torch.arange(1, n + 1), words=words)  # (the last one's parent is not there)
+    assert [whole(r) for r in up.tolist()] == [(1 << n) - (1 << i) & full for i in range(n)]
+    two = sl8.tree_mask(torch.cat([torch.arange(-1, 2), torch.arange(-1, n - 1)]).int(),
+                        torch.tensor([0, 3, 3 + n], dtype=torch.int32), words=words)
+    assert [whole(r) for r in two.tolist()] == [(1 << i + 1) - 1 & full for i in [*range(3), *range(n)]]
