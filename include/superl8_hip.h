@@ -481,11 +481,12 @@ int sl8_attn_weights_block8(const void* q, int dtype, int rotate, float q_scale_
 /* Eviction: of each sequence and KV head min(context_lens, budget) tokens stay, the first `sinks`, the last
  * `recent` (sinks + recent <= budget) and between them those of the largest weights (as above; no NaN), ties
  * to the lowest index. They move, in their order, into the blocks of new_table int32 [B][new_max_blocks]
- * (blocks that no row of block_table in the call holds), the j-th into slot j: a block and head takes
- * scale' = max(scales of the blocks that its rows come from, 2^-60), codes rint(c * (scale / scale')). Rows
- * behind the last one stay as they are, blocks of block_table too. new_lens int32 [B] = min(context_lens,
- * budget); kept int32 [B][Hkv][budget]: the tokens' old indexes, -1 behind the last; weights of the kept are
- * packed to the front, those behind stay. Tokens in blocks outside the pool are zeros where they arrive. */
+ * (each in one row of it only, and in no row of block_table in the call), the j-th into slot j: a block and
+ * head takes scale' = max(scales of the blocks that its rows come from, 2^-60), codes rint(c * (scale /
+ * scale')). Rows behind the last one stay as they are, blocks of block_table too. new_lens int32 [B] =
+ * min(context_lens, budget), of memory that is not context_lens'; kept int32 [B][Hkv][budget]: the tokens'
+ * old indexes, -1 behind the last; weights of the kept are packed to the front, those behind stay. Tokens in
+ * blocks outside the pool are zeros where they arrive. */
 int sl8_kv_evict_block8(int8_t* k_cache, float* k_scale, int8_t* v_cache, float* v_scale,
                         const int32_t* context_lens, const int32_t* block_table, float* weights,
                         int64_t weights_stride_b, int64_t weights_stride_h, const int32_t* new_table,

@@ -315,6 +315,9 @@ extern "C" int sl8_kv_evict_block8(int8_t* k_cache, float* k_scale, int8_t* v_ca
   SL8_CHECK_ARG(aligned(k_cache, 16) && aligned(v_cache, 16), "fni8 %s: caches must be 16-byte aligned", tag);
   SL8_CHECK_ARG(B * Hkv < (1LL << 32) / EV_THREADS && B * Hkv * blocks < (1LL << 32) / 256,
                 "fni8 %s: shape too large", tag);
+  // (a sequence's heads are workgroups of their own, and the first one writes its new length)
+  SL8_CHECK_ARG(new_lens + B <= context_lens || context_lens + B <= new_lens,
+                "fni8 %s: new_lens must not overlap context_lens", tag);
   p.k = k_cache; p.v = v_cache; p.ks = k_scale; p.vs = v_scale;
   p.w = weights; p.wb = weights_stride_b; p.wh = weights_stride_h;
   p.to = new_table;

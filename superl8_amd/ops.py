@@ -485,8 +485,8 @@ def kv_evict_block8(k_cache: torch.Tensor, k_scale: torch.Tensor, v_cache: torch
     ties to the lowest index, no NaN); heads keep different ones. Shorter sequences keep all.
 
     The kept tokens move in order into the blocks of new_table int32 [B,blocks], which no row of
-    block_table in the call may hold: from then on that is the sequence's table (the old blocks are
-    only read: shared prefixes stay whole). A block takes the largest scale of those its rows come
+    block_table in the call and no two of new_table may hold: from then on that is the sequence's table
+    (the old blocks are only read: shared prefixes stay whole). A block takes the largest scale of those its rows come
     from; rows of others are rounded again, rows of the same are copied. weights [B,Hkv,tokens] of the
     kept tokens move to the front, in place. Returns (lengths int32 [B], kept int32 [B,Hkv,budget]: the
     tokens' old places, -1 behind the last). Nothing is read on the host."""

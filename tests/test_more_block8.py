@@ -124,3 +124,10 @@ def test_masks_of_paths_longer_than_their_words(n, words):
     two = sl8.tree_mask(torch.cat([torch.arange(-1, 2), torch.arange(-1, n - 1)]).int(),
                         torch.tensor([0, 3, 3 + n], dtype=torch.int32), words=words)
     assert [whole(r) for r in two.tolist()] == [(1 << i + 1) - 1 & full for i in [*range(3), *range(n)]]
+
+
+@pytest.mark.parametrize("lens,new", [(4096, 4096), (4096, 4100), (4100, 4096)])
+def test_lengths_are_not_written_where_they_are_read(lens, new):
+    """Heads of a sequence read its length while another one's workgroup writes the new one."""
+    assert evict(lens=lens, new=new) == -1
+    assert b"new_lens" in _lib.load().sl8_last_error()
