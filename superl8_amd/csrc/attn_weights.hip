@@ -305,6 +305,12 @@ struct WeightPlan {
   size_t rows_at, part_at, bytes;
 };
 constexpr int AW_WAVES = 4;
+// Workgroups of the pass over the rows, and whether a launch (below 2^32 threads) holds them.
+int64_t rows_wgs(int64_t rows, int64_t D) {
+  const int64_t per = AW_THREADS / row_lanes((int)D);
+  return (rows + per - 1) / per;
+}
+bool rows_fit(int64_t rows, int64_t D) { return rows < (1LL << 30) && rows_wgs(rows, D) < (1LL << 32) / AW_THREADS; }
 WeightPlan weights_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t cap) {
   WeightPlan a{};
   a.rows = T * (Hq / Hkv) / B;
@@ -330,7 +336,7 @@ extern "C" size_t sl8_attn_weights_block8_workspace(int64_t T, int64_t B, int64_
                                                     int64_t max_context_len) {
   if (T <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || T >= (1LL << 28) || B >= (1 << 24) || Hq >= (1 << 16)) return 0;
   if ((D != 64 && D != 128 && D != 256) || Hq % Hkv || max_context_len < 0 || max_context_len >= (1LL << 30)) return 0;
-  if (B * Hkv * (max_context_len / AW_KEYS + 1) >= (1LL << 30)) return 0;
+  if (B * Hkv * (max_context_len / AW_KEYS + 1) >= (1LL << 30) || !rows_fit(T * Hq, D)) return 0;
   return weights_plan(T, B, Hq, Hkv, D, max_context_len).bytes;
 }
 
@@ -353,7 +359,7 @@ extern "C" int sl8_attn_weights_block8(const void* q, int dtype, int rotate, flo
                    (int)block_size};
   if (const int rc = block8_check(tag, p.s, Hkv, D)) return rc;
   SL8_CHECK_ARG(Hq > 0 && Hq % Hkv == 0, "fni8 %s: H_q must be divisible by H_kv (GQA)", tag);
-  SL8_CHECK_ARG(T * Hq < (1LL << 30), "fni8 %s: shape too large", tag);
+  SL8_CHECK_ARG(rows_fit(T * Hq, D), "fni8 %s: shape too large", tag);
   if (B == 0 || max_blocks_per_seq == 0) return SL8_OK;
   SL8_CHECK_ARG(num_blocks > 0, "fni8 %s: the cache has no blocks", tag);
   SL8_CHECK_ARG(context_lens && block_table && weights && k_cache && k_scale &&
@@ -382,8 +388,7 @@ extern "C" int sl8_attn_weights_block8(const void* q, int dtype, int rotate, flo
   const hipStream_t st = static_cast<hipStream_t>(stream);
   auto by_d = [&](auto d) {
     constexpr int DD = decltype(d)::value;
-    constexpr int RPB = AW_THREADS / row_lanes(DD);
-    const unsigned pre = (unsigned)((T * Hq + RPB - 1) / RPB);
+    const unsigned pre = (unsigned)rows_wgs(T * Hq, DD);
     if (T) {
       if (dtype == SL8_DTYPE_F16) weights_rows_kernel<SL8_DTYPE_F16, DD><<<pre, AW_THREADS, 0, st>>>(p);
       else weights_rows_kernel<SL8_DTYPE_BF16, DD><<<pre, AW_THREADS, 0, st>>>(p);

@@ -131,3 +131,13 @@ def test_lengths_are_not_written_where_they_are_read(lens, new):
     """Heads of a sequence read its length while another one's workgroup writes the new one."""
     assert evict(lens=lens, new=new) == -1
     assert b"new_lens" in _lib.load().sl8_last_error()
+
+
+@pytest.mark.parametrize("change", [dict(T=1 << 27, B=1, Hq=1, D=256, cu=16), dict(T=1 << 24, B=2, Hq=8, Hkv=8, D=256, cu=16),
+                                    dict(T=1 << 27, B=1, Hq=2, D=128, cu=16), dict(T=(1 << 27) + 1, B=1, Hq=4, Hkv=4, D=64, cu=16)])
+def test_rows_that_a_launch_cannot_hold(change):
+    """The pass over the rows has a workgroup of 256 threads for 2048 elements, and a launch below 2^32 threads."""
+    assert weights(**change) == -1
+    assert b"large" in _lib.load().sl8_last_error()
+    c = dict(Hkv=1) | change
+    assert _lib.load().sl8_attn_weights_block8_workspace(c["T"], c["B"], c["Hq"], c["Hkv"], c["D"], 64) == 0
