@@ -446,7 +446,8 @@ int sl8_attn_paged_block8(const void* q, int dtype, int rotate, float q_scale_mu
  * tokens that its sequence does not have count for nothing). A window
  * keeps the last window_left of those: the marked ones, all of them, and of the tokens in front the last
  * max(0, window_left - marked). lse (NULL: not wanted) fp32 [T,Hq]: ln of the row's sum of e^score,
- * -inf for a row that sees nothing or of no sequence. Workspace, with a mask:
+ * -inf for a row that sees nothing or of no sequence. With a mask or lse rows are rotated in 64 bits (their
+ * codes are sl8_attn_weights_block8's; few differ from those of 32 bits). Workspace, with a mask:
  * sl8_attn_paged_block8_tree_workspace() bytes, else as above. */
 size_t sl8_attn_paged_block8_tree_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
                                             int64_t max_context_len);

@@ -1,8 +1,9 @@
 // The softmax weights of cached keys, gathered for the block-scaled paged int8 cache (block8.hpp): what a
 // cache that is kept within a budget decides by. No counterpart in the reference.
 //
-// Rows are quantised and scores taken as by the attention (attn_block8.hip); with the logarithm of a row's
-// sum, which that attention gives, a key's weight in the row is known without a second look at the keys:
+// Rows are quantised and scores taken as by the attention where it gives the logarithms of the rows' sums
+// (attn_block8.hip; rotations in 64 bits, so that both find the same codes); with a row's, a key's weight in it is
+// known without a second look at the keys:
 //   w_j <- (j < len - n ? decay * w_j : 0) + sum over the n new rows i that see j, over the group's
 //          heads, of 2^(s_ij - lse_i log2 e)
 // for each KV head. Bound by the bytes of K for few rows, by the exponentials (VALU, a quarter of the rate of other

@@ -413,8 +413,10 @@ def attn_paged_block8(q: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.Ten
     tree_mask int64 [T] or [T,1..4] (see tree_mask): drafted tokens in a tree. A row sees its
     sequence's tokens in front of the new ones, and of those the j-th where bit j of its mask is set
     (bits stand for the first 64 to 256; itself too only if marked; bits of tokens that are not there
-    count for nothing); a window counts the marked ones first and takes what is left of it in front. return_lse: (out, lse fp32 [T,Hq]), the logarithm
-    of each row's sum of e^score, -inf where it sees nothing."""
+    count for nothing); a window counts the marked ones first and takes what is left of it in front.
+    return_lse: (out, lse fp32 [T,Hq]), the logarithm of each row's sum of e^score, -inf where it sees
+    nothing. With either, rows are rotated in 64 bits, as attn_weights_block8 does: a code next to a
+    half may then be the next one to that of a call with neither."""
     softmax_scale = (1.0 / (q.shape[-1] ** 0.5)) if scale is None else scale
     q = q.contiguous()
     if q.data_ptr() % 16:

@@ -425,3 +425,54 @@ def test_weights_of_rows_in_parts(new, old, Hkv, window):
     c = Cache(total, Hkv, 64, 16)
     q = coded_queries(sum(new), 10 * Hkv, 64, F16, False)
     weights_and_check(c, q, new, total, window=window, decay=0.5)
+
+
+# ---------------------------------------------------------------------------
+# each row's weights alone
+# ---------------------------------------------------------------------------
+def row_sums(c, q, lens, rotate, window=-1, lse=None):
+    """What each row's weights add up to, heads apart (as many query heads as KV heads, a row a sequence)."""
+    B, H, _ = q.shape
+    if lse is None:
+        _, lse = sl8.attn_paged_block8(q, *c.args(), lens, rotate=rotate, window_left=window, return_lse=True)
+    w = torch.zeros(B, H, c.table.shape[1] * c.bs, device=DEV)
+    sl8.attn_weights_block8(q, lse, c.k, c.ks, c.table, lens, w, rotate=rotate, window_left=window, decay=0.0)
+    return w.double().sum(-1), lse
+
+
+def sums_are_one(sums, lse, N):
+    """The same codes and exact products on both sides; each score rounds 4 times at up to 2^7 in base 2 (2^-15, and
+    again in the sum that lse is of), exp2 on both sides and N additions (N * 2^-24 each), lse itself and its
+    product 2^-23 of its size."""
+    lim = 2 * 2.0 ** -15 + 2 * N * 2.0 ** -24 + lse.double().abs() * 2.0 ** -22
+    off = (sums - 1).abs()
+    assert bool((off <= lim).all()), (float(off.max()), int((off > lim).sum()))
+
+
+@pytest.mark.parametrize("rotate", [True, False])
+@pytest.mark.parametrize("D,H", [(64, 32), (128, 16), (256, 8)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_weights_of_each_row_sum_to_one(D, H, dtype, rotate):
+    """Single tokens of a thousand sequences on shared blocks: the codes of every row are those that its lse is of."""
+    c = Cache([90, 33], H, D, 16)
+    B = 1024
+    c.table = c.table[torch.arange(B, device=DEV) % 2].contiguous()
+    lens = torch.where(torch.arange(B, device=DEV) % 2 == 0, 90, 33).int()
+    q = torch.randn(B, H, D, device=DEV).to(dtype)
+    sums_are_one(*row_sums(c, q, lens, rotate), 90)
+
+
+@pytest.mark.parametrize("D,G,n,window", [(64, 4, 300, -1), (128, 1, 700, -1), (128, 8, 260, 70), (256, 2, 300, -1),
+                                          (256, 1, 40, -1)])
+def test_weights_of_a_prompt_sum_to_one(D, G, n, window):
+    """A prompt's rows in tiles, then each alone behind what it sees."""
+    H, total = 8, n + 50
+    c = Cache([total], H // G, D, 16)
+    q = torch.randn(n, H, D, device=DEV).to(F16)
+    _, lse = sl8.attn_paged_block8(q, *c.args(), i32([total]), cu_lens=offsets([n]), window_left=window, return_lse=True)
+    d = c.copy()  # the KV head of each query head, as one of its own
+    for name in ("k", "ks", "v", "vs"):
+        setattr(d, name, getattr(c, name).repeat_interleave(G, 1).contiguous())
+    d.table = c.table.expand(n, -1).contiguous()
+    lens = torch.arange(total - n + 1, total + 1, device=DEV, dtype=torch.int32)
+    sums_are_one(*row_sums(d, q, lens, True, window, lse), total)
