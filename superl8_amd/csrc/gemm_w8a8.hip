@@ -147,6 +147,14 @@ __device__ __forceinline__ float w8_bias(const W8Args& p, int n) {
   return p.bias_dt == SL8_DTYPE_F16 ? h2f(b) : bf2f(b);
 }
 
+// An output in fp32. (A value of its own: where the compiler joins the fma with the conversion to fp16, as it did for
+// some elements of the tiles, that rounds once and not twice, and a row's bits went by how the call was cut.)
+__device__ __forceinline__ float w8_value(int y, float xs, float ws, float bias) {
+  float z = fmaf((float)y * xs, ws, bias);
+  asm("" : "+v"(z));
+  return z;
+}
+
 template <int ODT>
 __device__ __forceinline__ void w8_st4(void* out, int64_t i, const float* y) {
   if constexpr (ODT == SL8_DTYPE_F32) {
@@ -173,7 +181,7 @@ template <int ODT>
 __device__ __forceinline__ void w8_out4(const W8Args& p, v4i y, float xs, int m, int n) {
   float z[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) z[e] = fmaf((float)y[e] * xs, p.ws[min(n + e, p.N - 1)], w8_bias(p, min(n + e, p.N - 1)));
+  for (int e = 0; e < 4; ++e) z[e] = w8_value(y[e], xs, p.ws[min(n + e, p.N - 1)], w8_bias(p, min(n + e, p.N - 1)));
   const int64_t to = (int64_t)m * p.N + n;
   if (p.N % 4 == 0) {
     w8_st4<ODT>(p.out, to, z);
@@ -344,7 +352,7 @@ __device__ __forceinline__ void w8_store(const W8Args& p, const v16i (&acc)[S::N
       for (int q = 0; q < 4; ++q) {
         float y[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = fmaf((float)acc[nb][mb][4 * q + e] * xs, ws[nb][4 * q + e], bias[nb][4 * q + e]);
+        for (int e = 0; e < 4; ++e) y[e] = w8_value(acc[nb][mb][4 * q + e], xs, ws[nb][4 * q + e], bias[nb][4 * q + e]);
         const int at = (32 * nb + 8 * q + 4 * h) * OS;  // bytes into the row
         if constexpr (OS == 4) {
           *reinterpret_cast<float4*>(place(l32, at / 16)) = make_float4(y[0], y[1], y[2], y[3]);

@@ -163,3 +163,18 @@ def test_bits_of_a_row_in_any_batch(N, K):
     y = sl8.linear_w8a8(x, w, ws, bias=b, out_dtype=F32)
     for M in (1, 3, 7, 16, 40, 100, 400):
         assert torch.equal(sl8.linear_w8a8(x[:M], w, ws, bias=b, out_dtype=F32), y[:M])
+
+
+@pytest.mark.parametrize("out", [F16, BF16])
+@pytest.mark.parametrize("N,K,most", [(60000, 512, 300), (30000, 4096, 40), (4099, 2052, 1500), (20000, 5120, 100)])
+@pytest.mark.parametrize("bias", [None, F16])
+def test_roundings_do_not_go_by_the_batch(N, K, most, out, bias):
+    """16-bit outputs too are the same bits streamed, in tiles and in parts of K: some of so many lie next to the
+    middle of two neighbours, where one rounding and two give different ones."""
+    x, w, ws, b = inputs(most, N, K, out, bias)
+    y = sl8.linear_w8a8(x, w, ws, bias=b, out_dtype=out)
+    exact = sl8.linear_w8a8(x, w, ws, bias=b, out_dtype=F32)
+    assert torch.equal(y, exact.to(out))
+    for M in (1, 4, 7, 16, 33, 100, 300, 700):
+        if M < most:
+            assert torch.equal(sl8.linear_w8a8(x[:M], w, ws, bias=b, out_dtype=out), y[:M]), M
