@@ -565,7 +565,9 @@ struct W8Plan {
 // Both sides, calls on one stream: 1 row, 5120 x 5120 streamed 13.0, tiles of 32 rows 15.0; 17408 x 5120 24.7 and 27.1; 16 rows,
 // 4096 x 4096 13.0 and 14.9, 30000 x 4096 36.6 and 34.2. Tiles of 32, 64, 128 and 256 rows: 64 rows, 17408 x 5120 42.7, 31.9,
 // 37.9, 48.1; 512 rows, 4096 x 4096 23.3, 20.7, 27.1, 30.7 and 17408 x 5120 125, 90.8, 76.7, 74.2; 2048 rows, 4096 x 4096
-// 72.2, 55.6, 49.1, 67.2.
+// 72.2, 55.6, 49.1, 67.2. Where all tiles come to the weights' bytes those of fewer rows are nearer to them: N = 128256,
+// K = 4096, 1 row streamed 96.6, tiles 101, 98.5, 111, 124 (so rows that half a tile holds do not go to it); 64 rows 136, 112, 122, 140;
+// 57344 x 8192, 8 rows 92.8, 90.8, 102, 117.
 W8Plan w8_plan(int64_t M, int64_t N, int64_t K) {
   struct Shape { int bm, bn, per_cu; double one_us, full_us; };
   static const Shape shapes[] = {{256, 256, 1, 1.7, 1.7}, {128, 128, 2, 0.9, 1.2}, {64, 128, 2, 0.6, 0.95}, {32, 128, 2, 0.45, 0.8}};
@@ -577,6 +579,7 @@ W8Plan w8_plan(int64_t M, int64_t N, int64_t K) {
   double best = 1e30;
   if (M <= W8_STREAM_ROWS && K <= W8_STREAM_K) best = M <= W8_FUSED_ROWS ? 3.5 + (double)N * K / 4.6e6 : 6. + (double)N * K / 4.2e6;
   for (const Shape& s : shapes) {
+    if (s.bm > 32 && 2 * M <= s.bm) continue;  // a tile of half the rows holds them all
     const int64_t nt_m = (M + s.bm - 1) / s.bm, nt_n = (N + s.bn - 1) / s.bn, n = nt_m * nt_n;
     const int64_t slots = (int64_t)cus * s.per_cu, rest = n % slots, most = n - rest;
     for (int S = 1; S <= 8; ++S) {

@@ -178,3 +178,11 @@ def test_roundings_do_not_go_by_the_batch(N, K, most, out, bias):
     for M in (1, 4, 7, 16, 33, 100, 300, 700):
         if M < most:
             assert torch.equal(sl8.linear_w8a8(x[:M], w, ws, bias=b, out_dtype=out), y[:M]), M
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 128256, 4096), (16, 128256, 4096), (33, 128256, 4096), (64, 128256, 4096),
+                                   (100, 128256, 4096), (1, 151936, 5120), (4, 57344, 8192), (3, 58591, 5148), (9, 48000, 10212),
+                                   (120, 65381, 2048)])
+def test_few_rows_of_many_channels(M, N, K):
+    """Where every tile comes to the time of the weights' bytes."""
+    check(*inputs(M, N, K, F16, BF16), F16)
