@@ -186,3 +186,11 @@ def test_roundings_do_not_go_by_the_batch(N, K, most, out, bias):
 def test_few_rows_of_many_channels(M, N, K):
     """Where every tile comes to the time of the weights' bytes."""
     check(*inputs(M, N, K, F16, BF16), F16)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 14336, 4096), (1, 17408, 5120), (4, 30000, 4096), (16, 12288, 4096), (2, 20011, 2052),
+                                   (16, 9001, 4100), (7, 40000, 1024)])
+@pytest.mark.parametrize("out", [F16, F32])
+def test_many_turns_of_the_streaming_kernel(M, N, K, out):
+    """3 to 8 groups of channels a workgroup: the places of the waves' sums are written again, other waves put them out."""
+    check(*inputs(M, N, K, BF16, F16), out)

@@ -476,3 +476,33 @@ def test_weights_of_a_prompt_sum_to_one(D, G, n, window):
     d.table = c.table.expand(n, -1).contiguous()
     lens = torch.arange(total - n + 1, total + 1, device=DEV, dtype=torch.int32)
     sums_are_one(*row_sums(d, q, lens, True, window, lse), total)
+
+
+@pytest.mark.parametrize("cu", [False, True])
+@pytest.mark.parametrize("decay,window", [(0.9, -1), (1.0, 100)])
+def test_weights_of_more_items_than_are_resident(decay, window, cu):
+    """Single tokens, a wave an item: each wave takes several, and with a window skips some."""
+    total = [1 + 1500 + 401 * i % 700 for i in range(130)]
+    c = Cache(total, 8, 64, 32)
+    q = coded_queries(130, 8, 64, F16, False)
+    weights_and_check(c, q, [1] * 130, total, window=window, decay=decay, cu=cu)
+
+
+@pytest.mark.parametrize("decay,window", [(0.9, -1), (1.0, 100)])
+@pytest.mark.parametrize("n", [44, 70])
+def test_weights_of_more_shared_items_than_are_resident(n, decay, window):
+    """The same with four waves an item, sequences without new rows and with few among the others."""
+    new = [(n, n - 3, 2 * n, n, 0, n, 1)[i % 7] for i in range(70)]
+    total = [m + 300 + 401 * i % 700 for i, m in enumerate(new)]
+    c = Cache(total, 8, 64, 32)
+    q = coded_queries(sum(new), 8, 64, F16, False)
+    weights_and_check(c, q, new, total, window=window, decay=decay)
+
+
+@pytest.mark.parametrize("new,old", [([1200] + [1] * 66, 100), ([1] * 40 + [300] + [1] * 200, 60)])
+def test_weights_of_a_prompt_beside_single_tokens(new, old):
+    """On average many rows a sequence (four waves an item), and few (one)."""
+    total = [n + old + 37 * i % 900 for i, n in enumerate(new)]
+    c = Cache(total, 2, 128, 16)
+    q = coded_queries(sum(new), 8, 128, F16, False)
+    weights_and_check(c, q, new, total, decay=0.5)
