@@ -442,13 +442,12 @@ int sl8_attn_paged_block8(const void* q, int dtype, int rotate, float q_scale_mu
 
 /* The same with a tree of drafted tokens, and with the sums' logarithms. tree_mask (NULL: as above)
  * int64 [T][mask_words] (1 .. 4 words, 8-byte aligned): row i of a sequence sees the tokens in front of
- * the new ones, and new token t < 64 * mask_words where bit t % 64 of word t / 64 of its mask is set (bits of
- * tokens that its sequence does not have count for nothing). A window
- * keeps the last window_left of those: the marked ones, all of them, and of the tokens in front the last
- * max(0, window_left - marked). lse (NULL: not wanted) fp32 [T,Hq]: ln of the row's sum of e^score,
- * -inf for a row that sees nothing or of no sequence. With a mask or lse rows are rotated in 64 bits (their
- * codes are sl8_attn_weights_block8's; few differ from those of 32 bits). Workspace, with a mask:
- * sl8_attn_paged_block8_tree_workspace() bytes, else as above. */
+ * the new ones, and new token t < 64 * mask_words where bit t % 64 of word t / 64 of its mask is set (bits
+ * of tokens that its sequence does not have count for nothing). A window keeps the last window_left of those:
+ * the marked ones, all of them, and of the tokens in front the last max(0, window_left - marked). lse (NULL:
+ * not wanted) fp32 [T,Hq]: ln of the row's sum of e^score, -inf for a row that sees nothing or of no sequence.
+ * With a mask or lse rows are rotated in 64 bits (their codes are sl8_attn_weights_block8's; few differ from
+ * those of 32 bits). Workspace, with a mask: sl8_attn_paged_block8_tree_workspace() bytes, else as above. */
 size_t sl8_attn_paged_block8_tree_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
                                             int64_t max_context_len);
 int sl8_attn_paged_block8_tree(const void* q, int dtype, int rotate, float q_scale_mul,
@@ -499,8 +498,9 @@ int sl8_kv_evict_block8(int8_t* k_cache, float* k_scale, int8_t* v_cache, float*
 /* ------------------------------------------------------------------------
  * Linear layer of int8 weights with a scale per output channel: x [M,K] f16 / bf16 / f32, each row
  * quantised to int8 as sl8_quantize_i8_rowwise; w int8 [N,K]; w_scale fp32 [N]; bias [N] (f16 / bf16 /
- * f32; NULL: none) -> out [M,N] = x_scale[m] * w_scale[n] * sum_k x_i8 w + bias[n], the sums exact, rounded
- * once; a row with NaN or infinity has no finite output. K a multiple of 4, 16 to 131068; w 16-byte aligned (4 where K % 16 != 0). workspace:
+ * f32; NULL: none) -> out [M,N] = x_scale[m] * w_scale[n] * sum_k x_i8 w + bias[n], the sums exact, the rest
+ * in fp32, rounded to out's type: the same bits for a row in any batch. A row with NaN or infinity has no
+ * finite output. K a multiple of 4, 16 to 131068; w 16-byte aligned (4 where K % 16 != 0). workspace:
  * sl8_linear_w8a8_workspace() bytes, uninitialised, 16-byte aligned.
  * ---------------------------------------------------------------------- */
 size_t sl8_linear_w8a8_workspace(int64_t M, int64_t N, int64_t K);

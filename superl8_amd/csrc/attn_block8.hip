@@ -294,9 +294,10 @@ __device__ __forceinline__ int64_t row_at(const AttnArgs& p, const Span& w, int 
 // The unit's rows as int8 codes in LDS (row r at place(r)) with their scales (times q_mul); rows past
 // the last are zeros. WIDE: as row_codes_wide has them, wherever a row's lse leaves the call: it goes to callers in
 // 32 bits, the weights of the keys (attn_weights.hip) are taken against it by codes of their own, and a code that
-// another one stands for moves a row's sum by up to 4 * 10^-3 (D = 128, one row in some thousands in 32 bits).
-// Causal rows with their lse take 62.8 us so for 58.6 in 32 bits (700 tokens behind 300, 16 / 2 heads, D = 256), 42.4
-// for 41.2 (5 tokens of 16 sequences, 32 / 8 heads, D = 128), 114.4 for 113.8 (2048 behind 2048), 57.3 for 57.2 (32 x 1).
+// another one stands for moves a row's sum by up to 7 * 10^-3 (D = 128, one row in 6000 in 32 bits).
+// Causal rows with their lse take 62.8 us so for 58.6 in 32 bits (700 tokens behind 300, 16 / 2 heads, D = 256),
+// 42.4 for 41.2 (5 tokens of 16 sequences behind 1024 to 8074, 32 / 8 heads, D = 128), 114.4 for 113.8 (2048 behind
+// 2048), 57.3 for 57.2 (32 x 1 behind 1024 to 8185).
 template <int DT, int D, int ROWS, int THREADS, bool WIDE, typename F>
 __device__ __forceinline__ void quant_rows(const AttnArgs& p, const Span& w, int kvh, F place, float* qs_s) {
   constexpr int LPR = row_lanes(D), RPB = THREADS / LPR;
@@ -1068,7 +1069,8 @@ template <int D_, int RT_, int NW_> struct Shape {
     if constexpr (NW_) return attn_block8_tile_kernel<DT, D, RT, NW, MODE>;
     else return attn_block8_stream_kernel<DT, D, RT, MODE>;
   }
-  // workgroups resident on one CU (asked once)
+  // workgroups resident on one CU (asked once, of the causal kernel: a workspace is asked for before it is known whether
+  // an lse is wanted. All three hold as many; were they fewer, splits would wait for a place)
   static int wgs_per_cu() {
     static std::atomic<int> n{0};
     int v = n.load(std::memory_order_relaxed);
@@ -1093,9 +1095,10 @@ template <int D_, int RT_, int NW_> struct Shape {
 // than the 256 registers of two waves a SIMD: 27 spill (96 to 112 bytes a lane) and come back in the loop
 // over keys; 16 rows at D = 256 spill 2, and 32 rows there, whose sums take 128, are not built.
 // Trees of up to 128 rows, and all at D = 256, go to tiles of 64, which several workgroups of a CU hold: 8 trees of 14
-// to 26 tokens (32 / 8 heads, D = 128) on 500 to 4000 keys 37 us, 40 in tiles of 128; D = 256, 4 of 66 to 129 (8 heads to a
-// KV head) on 130 to 1024 36 and 45, on 513 to 4096 53 and 57. With more rows those of 128 win: 16 of 31 to 60 tokens on
-// 512 to 4096 keys 63 us, 69 in tiles of 64, on 2048 to 16384 160 and 175; D = 64, 2 of 101 to 200 on 20000 67 and 75.
+// to 26 tokens (32 / 8 heads, D = 128) on 500 to 4000 keys 37 us, 40 in tiles of 128; D = 256, 4 of 66 to 129 (8 heads
+// to a KV head) on 130 to 1024 36 and 45, on 513 to 4096 53 and 57. With more rows those of 128 win: 16 of 31 to 60
+// tokens on 512 to 4096 keys 63 us, 69 in tiles of 64, on 2048 to 16384 160 and 175; D = 64, 2 of 101 to 200 on 20000
+// 67 and 75.
 template <typename F>
 auto with_shape(int64_t D, int64_t rows, bool tree, F&& f) {
   auto by_rows = [&](auto d) {

@@ -7,10 +7,11 @@
 //   w_j <- (j < len - n ? decay * w_j : 0) + sum over the n new rows i that see j, over the group's
 //          heads, of 2^(s_ij - lse_i log2 e)
 // for each KV head. Bound by the bytes of K for few rows, by the exponentials (VALU, a quarter of the rate of other
-// instructions) for many. A call among others (us): 32 x 1 token behind 1024 to 8191, 32 / 8 heads, D = 128, 35 (rows 4,
-// keys 28 of which 24 are K's 122 MB at the rate of a copy); 6 x 20 to 33 tokens behind up to 3001 with a window, D = 64, 16 (rows 3, keys 8,
-// else the call); 2048 tokens behind 2048 keys, 32 / 8 heads, 66 (51 G operations, 24 at the rate of a large int8 product;
-// 201 million exponentials, 23 at theirs; beside each a conversion, a product and a sum).
+// instructions) for many. A call among others (us): 32 x 1 token behind 1024 to 8191, 32 / 8 heads, D = 128, 35 (K's
+// 122 MB take 24 at the rate of a copy); 6 x 20 to 33 tokens behind up to 3001 with a window, D = 64, 16, the host's
+// call; 2048 tokens behind 2048 keys, 32 / 8 heads, 65 (51 G operations, 24 at the rate of a large int8 product; 201
+// million exponentials, 23 at theirs; beside each a conversion, a product and a sum). Kernels in a trace of 30 calls, where
+// clocks are lower and launches apart (calls 40, 42 and 77): rows 4.0, keys 28; 3.0 and 7.5; 15, 58, join 5.
 #include <algorithm>
 #include <climits>
 
@@ -296,11 +297,11 @@ __global__ void __launch_bounds__(256) weights_join_kernel(const WeightArgs p) {
 // How a call runs: rows of a sequence and KV head on average, items at most, and in how many parts the rows of an
 // item go to workgroups of their own: where items are few, so that there are two for each CU, and four where new rows
 // are a good part of the context (a causal prompt's last keys are seen by few of its rows, so items differ); parts
-// large enough to pay for the join. Whole and in parts (us): 2000 rows behind 100 keys, 8 heads to a KV head, D = 256, 134
-// and 35; 4000 behind 100, 8 / 2 heads, D = 128, 134 and 51; 2048 behind 2048, 32 / 8 heads, 101 and 92, later 75 (6 parts
-// for 2: 87); 700 behind 30000, 8 / 1 heads, 60 whole, 84 in two.
-// A wave an item for up to 32 rows, else four: one row, 32 sequences 32 and 96; 16 tokens of 4 heads, D = 64, 18.8 and 20.3;
-// 300 of 4 heads, D = 128, 47 and 24.
+// large enough to pay for the join. Whole and in parts (us): 2000 rows behind 100 keys, 8 heads to a KV head, D = 256,
+// 134 and 35; 4000 behind 100, 8 / 2 heads, D = 128, 134 and 51; 2048 behind 2048, 32 / 8 heads, 101 and 92, later 75
+// (6 parts for 2: 87); 700 behind 30000, 8 / 1 heads, 60 whole, 84 in two.
+// A wave an item for up to 32 rows, else four: one row, 32 sequences 32 and 96; 16 tokens of 4 heads, D = 64, 18.8 and
+// 20.3; 300 of 4 heads, D = 128, 47 and 24. (By the batch's average: lengths are on the device.)
 struct WeightPlan {
   int64_t rows, items, parts;
   size_t rows_at, part_at, bytes;

@@ -9,8 +9,8 @@
 // so rows that stay together, or come from blocks of one scale, are copied as they are.
 //
 // Bound by the counting, which has a workgroup for each sequence and head, and by the kept rows' bytes, K and V, in
-// and out. Kernels (us): 4 sequences of 733 to 1100 tokens to 1024, 8 heads, D = 128, select 7.6, move 7 (the 17 MB
-// of rows come from and go to caches); 8 of 21845 to 32768 to 4096 select 27, move 31 (134 MB, 26 at the rate of a copy).
+// and out. Kernels (us): 4 sequences of 733 to 1100 tokens to 1024, 8 heads, D = 128, select 7.7, move 7.5 (the 17 MB
+// of rows come from and go to caches); 8 of 21845 to 32768 to 4096 select 26, move 31 (134 MB, 26 at a copy's rate).
 #include <algorithm>
 
 #include "block8.hpp"

@@ -1,14 +1,15 @@
 // Linear layer of int8 weights with a scale per output channel, activations quantised with a scale per
 // token (the per_row_i8 weights of the package's containers):
 //   xs[m] = amax|x[m]| * fp32(1/127) (1 for a row of zeros), c = clamp(rint(x / xs), -127, 127),
-//   y[m,n] = xs[m] * ws[n] * sum_k c[m,k] w[n,k] + bias[n], rounded once.
-// The sums are exact integers (K < 2^17).
+//   y[m,n] = xs[m] * ws[n] * sum_k c[m,k] w[n,k] + bias[n].
+// The sums are exact integers (K < 2^17); scales and bias are applied in fp32, and that is rounded to y's type.
 //
 // Up to some tens of rows are bound by the weights' bytes, more by the matrix instructions. A call among others (us; a
-// copy's 5.16 TB/s and a large int8 product's 2.10 POP/s give the floor): 1 row, 4096 x 4096 9.1 (floor 3.3; kernel
-// 8.6 to 9.3, most of it the way to the first weights and the waves' sums); 16 rows, 17408 x 5120 23.5 (17.4;
-// codes 4.2, tiles of 32 rows 16.6, 5.4 TB/s); 333 rows, 5003 x 2052, 19.4 (3.6; codes 4.1, tiles of 64 rows 16.4: a chain
-// of 17 stages); 4096 rows, 17408 x 5120 370 (348; codes 20, tiles of 256 rows 334 to 362, join 16).
+// copy's 5.16 TB/s and a large int8 product's 2.10 POP/s give the floor): 1 row, 4096 x 4096 9.0 (floor 3.3; one
+// kernel); 16 rows, 17408 x 5120 24.4 (17.4); 333 rows, 5003 x 2052 19.4 (3.6: a chain of 17 stages); 4096 rows,
+// 17408 x 5120 368 (348). Their kernels in a trace of 30 calls, where clocks differ from those of a long run and a
+// kernel's time holds its own launch, so that they do not add up to a call: stream 8.8 to 9.1; codes 4.1, tiles of 32 rows
+// 16.2 (5.5 TB/s); codes 4.2, tiles of 64 rows 16.6; codes 19 to 22, tiles of 256 rows 331 to 362, join 16.
 #include <algorithm>
 #include <cmath>
 
@@ -170,9 +171,10 @@ __device__ __forceinline__ void w8_st4(void* out, int64_t i, const float* y) {
 // ---------------------------------------------------------------------------
 // Up to 16 rows: 16 channels at a time, each wave with its part of K: weights straight from memory into A operands
 // of v_mfma_i32_16x16x64_i8 (lane (g4, col): 16 bytes of row col), the codes as B operands. The waves' sums
-// meet in LDS. Bound by the weights' bytes (17408 x 5120: 3.6 TB/s). The codes of a wave's part stay in registers while the workgroup goes
-// through its groups of channels, a group's weights on their way while the one before is multiplied; the two
-// halves of a line are read next to each other (U units of 128 bytes a wave).
+// meet in LDS. Bound by the weights' bytes where a workgroup has many groups of channels (128256 x 4096: 5.4 TB/s;
+// 17408 x 5120 in 4.25 rounds, 3.5 to 4). The codes of a wave's part stay in registers while the workgroup goes through
+// its groups, a group's weights on their way while the one before is multiplied (behind the last group it reads that one
+// again); the two halves of a line are read next to each other (U units of 128 bytes a wave).
 // ---------------------------------------------------------------------------
 constexpr int W8_WAVES = 8;
 
@@ -298,11 +300,11 @@ __global__ void __launch_bounds__(64 * W8_WAVES) w8_stream_kernel(const W8Args p
 // ---------------------------------------------------------------------------
 // Many rows: BN x BM output tiles (channels x rows), MW waves along the rows and NW along the channels, each
 // with 32 NB x 32 MB of them on v_mfma_i32_32x32x32_i8. Stages of 128 bytes of K (whole lines; with 64 bytes
-// 512 x 17408 x 5120 took 100 us, 77 now) go through RING places in LDS by direct copies, RING - 1
-// ahead of the products, one barrier a stage; 16-byte chunks of a row are placed by an xor of the row, so that
-// 16 rows of a read lie in different banks. Bound by the matrix pipe's power in large tiles (4096 x 17408 x 5120: it is busy
-// in 54 % of the cycles, at 1.55 to 1.6 GHz, as the library's product of that size, 385 us, is), by the copies in
-// tiles of 32 and 64 rows, whose rings are longer for that.
+// 512 x 17408 x 5120 took 100 us, 77 now) go through RING places in LDS by direct copies, RING - 1 ahead of the
+// products, one barrier a stage; 16-byte chunks of a row are placed by an xor of the row, so that 16 rows of a read lie in
+// different banks. Bound by the matrix pipe's power in large tiles (4096 x 17408 x 5120: it is busy in 54 % of the
+// cycles, at 1.55 to 1.6 GHz, as the library's product of that size, 385 us, is), by the copies in tiles of 32 and 64
+// rows, whose rings are longer for that.
 // ---------------------------------------------------------------------------
 template <int BM_, int BN_, int MW_, int NW_, int RING_> struct W8Tile {
   static constexpr int RING = RING_;  // stages in LDS
@@ -562,12 +564,12 @@ struct W8Plan {
 // Tiles: rounds of the workgroups that are resident at once, each of as many stages as K has, a stage taking
 // one_us where a CU has one workgroup, up to full_us where it has per_cu; a join costs its launch and its
 // partial sums. Neither is faster than the weights' bytes; launches and the rows' codes are the constants.
-// Both sides, calls on one stream: 1 row, 5120 x 5120 streamed 13.0, tiles of 32 rows 15.0; 17408 x 5120 24.7 and 27.1; 16 rows,
-// 4096 x 4096 13.0 and 14.9, 30000 x 4096 36.6 and 34.2. Tiles of 32, 64, 128 and 256 rows: 64 rows, 17408 x 5120 42.7, 31.9,
-// 37.9, 48.1; 512 rows, 4096 x 4096 23.3, 20.7, 27.1, 30.7 and 17408 x 5120 125, 90.8, 76.7, 74.2; 2048 rows, 4096 x 4096
-// 72.2, 55.6, 49.1, 67.2. Where all tiles come to the weights' bytes those of fewer rows are nearer to them: N = 128256,
-// K = 4096, 1 row streamed 96.6, tiles 101, 98.5, 111, 124 (so rows that half a tile holds do not go to it); 64 rows 136, 112, 122, 140;
-// 57344 x 8192, 8 rows 92.8, 90.8, 102, 117.
+// Both sides, calls on one stream: 1 row, 5120 x 5120 streamed 13.0, tiles of 32 rows 15.0; 17408 x 5120 24.7 and 27.1;
+// 16 rows, 4096 x 4096 13.0 and 14.9, 30000 x 4096 36.6 and 34.2. Tiles of 32, 64, 128 and 256 rows: 64 rows,
+// 17408 x 5120 42.7, 31.9, 37.9, 48.1; 512 rows, 4096 x 4096 23.3, 20.7, 27.1, 30.7 and 17408 x 5120 125, 90.8, 76.7,
+// 74.2; 2048 rows, 4096 x 4096 72.2, 55.6, 49.1, 67.2. Where all tiles come to the weights' bytes those of few rows are
+// nearer to them, so rows that half a tile holds do not go to it: N = 128256, K = 4096, 1 row 101, 98.5, 111, 124
+// (streamed 96.6), 64 rows 136, 112, 122, 140; 57344 x 8192, 8 rows 92.8, 90.8, 102, 117.
 W8Plan w8_plan(int64_t M, int64_t N, int64_t K) {
   struct Shape { int bm, bn, per_cu; double one_us, full_us; };
   static const Shape shapes[] = {{256, 256, 1, 1.7, 1.7}, {128, 128, 2, 0.9, 1.2}, {64, 128, 2, 0.6, 0.95}, {32, 128, 2, 0.45, 0.8}};
