@@ -447,13 +447,14 @@ def tree_mask(parents: torch.Tensor, cu_lens: torch.Tensor | None = None, *, wor
     bit = torch.where((place >= 0) & (place < 64 * words), torch.ones_like(t) << (place % 64), 0)
     mask = torch.where(place[:, None] // 64 == torch.arange(words, device=t.device), bit[:, None], 0)
     up = torch.where(parents >= 0, first + parents.long(), T)
-    up = torch.where((up >= first) & (up < end), up, T)
-    none = mask.new_zeros(1, words)
+    # (a row T behind the others: no token, no bits, its own parent)
+    up = torch.cat([torch.where((up >= first) & (up < end), up, T), up.new_full((1,), T)])
+    mask = torch.cat([mask, mask.new_zeros(1, words)])
     # the masks of twice as many levels, each time; a path may be as long as the list, whatever has bits
     for _ in range(max(T - 1, 1).bit_length()):
-        mask = mask | torch.cat([mask, none])[up]
-        up = torch.cat([up, up.new_full((1,), T)])[up]
-    return mask
+        mask = mask | mask[up]
+        up = up[up]
+    return mask[:T]
 
 
 def attn_weights_block8(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.Tensor,
